@@ -14,5 +14,7 @@ from .binding import (  # noqa: F401
     Gpt2,
     Gpt2Config,
     Gpt2ParameterInfo,
+    PackedShape,
+    PagedShape,
     library_path,
 )

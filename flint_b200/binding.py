@@ -71,6 +71,20 @@ class AdamwTensor(ctypes.Structure):
     ]
 
 
+class PackedShape(ctypes.Structure):
+    """flint_b200_packed_shape."""
+
+    _fields_ = [(name, ctypes.c_size_t) for name in ("sequences", "rows", "heads", "kv_heads", "head_width",
+                                                     "q_stride", "kv_stride", "o_stride")]
+
+
+class PagedShape(ctypes.Structure):
+    """flint_b200_paged_shape."""
+
+    _fields_ = [*PackedShape._fields_,
+                *((name, ctypes.c_size_t) for name in ("pages", "page_size", "table_stride", "longest"))]
+
+
 class TrainerConfigC(ctypes.Structure):
     """flint_trainer_config."""
 
@@ -153,6 +167,8 @@ _C_TYPES = {
     "flint_trainer*": ctypes.c_void_p,
     "const flint_trainer*": ctypes.c_void_p,
     "flint_trainer**": ctypes.POINTER(ctypes.c_void_p),
+    "const flint_b200_packed_shape*": ctypes.POINTER(PackedShape),
+    "const flint_b200_paged_shape*": ctypes.POINTER(PagedShape),
     "const flint_trainer_config*": ctypes.POINTER(TrainerConfigC),
     "flint_trainer_status*": ctypes.POINTER(TrainerStatus),
     "const flint_trainer_status*": ctypes.POINTER(TrainerStatus),
@@ -490,6 +506,53 @@ class Flint:
                            head_width, scale, stream=None) -> None:
         self.call("flint_b200_attention_backward", dq, dk, dv, d_o, o, lse, delta, q, k, v,
                   batches, length, head_width, scale, stream=stream)
+
+    def packed_attention_workspace(self, shape) -> int:
+        return self._size_query("flint_b200_packed_attention_workspace", shape)
+
+    def packed_attention_forward(self, o, lse, q, k, v, starts, shape, scale, workspace=None,
+                                 workspace_bytes=None, stream=None) -> None:
+        """Causal attention over the sequences of a ragged batch; shape is a PackedShape."""
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_packed_attention_forward", o, lse, q, k, v, starts, shape, scale, workspace,
+                  workspace_bytes, stream=stream)
+
+    def packed_attention_backward_workspace(self, shape) -> int:
+        return self._size_query("flint_b200_packed_attention_backward_workspace", shape)
+
+    def packed_attention_backward(self, dq, dk, dv, d_o, o, lse, q, k, v, starts, shape, scale, workspace=None,
+                                  workspace_bytes=None, stream=None) -> None:
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_packed_attention_backward", dq, dk, dv, d_o, o, lse, q, k, v, starts, shape, scale,
+                  workspace, workspace_bytes, stream=stream)
+
+    def paged_store(self, k_pages, v_pages, k, v, starts, lengths, page_table, shape, stream=None) -> None:
+        """New tokens' keys and values into their pages; shape is a PagedShape."""
+        self.call("flint_b200_paged_store", k_pages, v_pages, k, v, starts, lengths, page_table, shape,
+                  stream=stream)
+
+    def paged_attention_workspace(self, shape) -> int:
+        return self._size_query("flint_b200_paged_attention_workspace", shape)
+
+    def paged_attention(self, o, lse, q, k_pages, v_pages, starts, lengths, page_table, shape, scale,
+                        workspace=None, workspace_bytes=None, stream=None) -> None:
+        """Attention of each sequence's new tokens over its pages, which hold their keys already."""
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_paged_attention", o, lse, q, k_pages, v_pages, starts, lengths, page_table, shape,
+                  scale, workspace, workspace_bytes, stream=stream)
+
+    def token_log_probs(self, log_probs, entropy, lse, top_log_probs, top_tokens, logits, targets, fp32_logits,
+                        rows, vocab, cols, top=0, stream=None) -> None:
+        self.call("flint_b200_token_log_probs", log_probs, entropy, lse, top_log_probs, top_tokens, logits, targets,
+                  bool(fp32_logits), rows, vocab, cols, top, stream=stream)
+
+    def token_log_probs_backward(self, dlogits, logits, targets, lse, entropy, d_log_probs, d_entropy, fp32_logits,
+                                 rows, vocab, cols, stream=None) -> None:
+        self.call("flint_b200_token_log_probs_backward", dlogits, logits, targets, lse, entropy, d_log_probs,
+                  d_entropy, bool(fp32_logits), rows, vocab, cols, stream=stream)
 
     def adamw(self, param, m, v, grad, half_copy, count, lr, beta1, beta2, eps, weight_decay,
               grad_scale, step, skip=None, stream=None) -> None:

@@ -17,6 +17,7 @@
 #include "device_utils.cuh"
 #include "flint/flint_b200.h"
 #include "attention.h"
+#include "packed.h"
 #include "gemm.h"
 
 namespace {
@@ -440,7 +441,9 @@ flint_status flint_b200_kernel_fault(int* raised) {
     FB_CUDA(fb::reductions_error_flag(&reductions, true));
     int rowwise = 0;
     FB_CUDA(fb::rowwise_error_flag(&rowwise, true));
-    *raised = (gemm != 0 || attention != 0 || reductions != 0 || rowwise != 0) ? 1 : 0;
+    int packed = 0;
+    FB_CUDA(fb::packed_error_flag(&packed, true));
+    *raised = (gemm != 0 || attention != 0 || reductions != 0 || rowwise != 0 || packed != 0) ? 1 : 0;
     return FLINT_OK;
 }
 

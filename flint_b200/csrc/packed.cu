@@ -1,0 +1,602 @@
+// Attention over sequences of different lengths, packed one behind the other or in the pages of a
+// cache, and the entry points of both (extensions: the reference has equal lengths only,
+// src/api/gpt2.cpp:495-530).
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+
+#include "common.h"
+#include "device_utils.cuh"
+#include "flint/flint_b200.h"
+#include "packed.h"
+
+namespace fb {
+namespace {
+
+constexpr int kHead = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ int g_packed_error = 0;
+
+__device__ __forceinline__ void report() { atomicExch(&g_packed_error, 1); }
+
+// A sequence's place in the rows and how many keys it has; values outside their ranges are
+// clamped and reported.
+struct Sequence {
+    int first, count, keys;
+};
+
+__device__ __forceinline__ Sequence sequence_at(const PackedArgs& p, int s) {
+    const int a = p.starts[s], b = p.starts[s + 1];
+    Sequence out;
+    out.first = min(max(a, 0), p.rows);
+    out.count = min(max(b, out.first), p.rows) - out.first;
+    bool good = out.first == a && out.first + out.count == b;
+    out.keys = out.count;
+    if (p.lengths != nullptr) {
+        const int given = p.lengths[s];
+        const long long most = static_cast<long long>(p.table_stride) * p.page_size;
+        out.keys = static_cast<int>(min(static_cast<long long>(max(given, 0)), most));
+        good = good && out.keys == given;
+    }
+    if (!good) {
+        report();
+    }
+    return out;
+}
+
+// The page that holds a key of sequence s, or -1 (reported) where the table names none.
+__device__ __forceinline__ long long page_of(const PackedArgs& p, int s, int key) {
+    const int page = p.table[static_cast<long long>(s) * p.table_stride + key / p.page_size];
+    if (page < 0 || page >= p.pages) {
+        report();
+        return -1;
+    }
+    return page;
+}
+
+// Where the row of 64 values of a key (in K or V) begins; negative for a page that is not there.
+__device__ __forceinline__ long long key_offset(const PackedArgs& p, const Sequence& q, int s, int key,
+                                                int kv_head) {
+    if (p.table == nullptr) {
+        return (q.first + static_cast<long long>(key)) * p.kv_stride + kv_head * kHead;
+    }
+    const long long page = page_of(p, s, key);
+    return page < 0 ? -1 : ((page * p.kv_heads + kv_head) * p.page_size + key % p.page_size) * kHead;
+}
+
+__device__ __forceinline__ float2 load_pair(const __half* row, int lane) {
+    return __half22float2(reinterpret_cast<const __half2*>(row)[lane]);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        v += __shfl_xor_sync(fb::kFullMask, v, off);
+    }
+    return v;
+}
+
+// One warp per (token, head), two of the 64 columns per lane.
+__global__ void __launch_bounds__(256) fb_packed_forward_rows(const PackedArgs p) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int lane = threadIdx.x % 32;
+    const int warp = blockIdx.x * 8 + threadIdx.x / 32;
+    const int warps = gridDim.x * 8;
+    const int group = p.heads / p.kv_heads;
+    for (int s = blockIdx.y; s < p.sequences; s += gridDim.y) {
+        const Sequence q = sequence_at(p, s);
+        for (long long item = warp; item < static_cast<long long>(q.count) * p.heads; item += warps) {
+            const int i = static_cast<int>(item / p.heads), head = static_cast<int>(item % p.heads);
+            const long long row = q.first + i;
+            const float2 x = load_pair(p.q + row * p.q_stride + head * kHead, lane);
+            const int visible = q.keys - q.count + i + 1;
+            float m = -INFINITY, l = 0.0f;
+            float2 acc = make_float2(0.0f, 0.0f);
+            for (int key = 0; key < visible; ++key) {
+                const long long at = key_offset(p, q, s, key, head / group);
+                if (at < 0) {
+                    continue;
+                }
+                const float2 kk = load_pair(p.k + at, lane);
+                const float score = warp_sum(x.x * kk.x + x.y * kk.y) * (p.scale * kLog2e);
+                if (score == -INFINITY) {
+                    continue;   // weighs nothing
+                }
+                const float top = score > m || score != score ? score : m;
+                const float keep = exp2f(m - top), weight = exp2f(score - top);
+                const float2 vv = load_pair(p.v + at, lane);
+                m = top;
+                l = l * keep + weight;
+                acc.x = acc.x * keep + weight * vv.x;
+                acc.y = acc.y * keep + weight * vv.y;
+            }
+            // No key at all gives zeros; keys that all weigh nothing give 0 / 0.
+            const float inv = visible > 0 ? 1.0f / l : 0.0f;
+            reinterpret_cast<__half2*>(p.o + row * p.o_stride + head * kHead)[lane] =
+                visible > 0 ? __floats2half2_rn(acc.x / l, acc.y / l) : __floats2half2_rn(inv, inv);
+            if (p.lse != nullptr && lane == 0) {
+                p.lse[static_cast<long long>(head) * p.rows + row] = l > 0.0f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float pair_dot(float2 a, float2 b) { return warp_sum(a.x * b.x + a.y * b.y); }
+
+// One warp per (token, head) for dq, then one per (token, K/V head) for dk and dv.
+__global__ void __launch_bounds__(256) fb_packed_backward_rows(const PackedArgs p, const PackedGradients g) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int lane = threadIdx.x % 32;
+    const int warp = blockIdx.x * 8 + threadIdx.x / 32;
+    const int warps = gridDim.x * 8;
+    const int group = p.heads / p.kv_heads;
+    const float scale2 = p.scale * kLog2e;
+    for (int s = blockIdx.y; s < p.sequences; s += gridDim.y) {
+        const Sequence q = sequence_at(p, s);
+        auto delta_of = [&](long long row, int head, float2 grad) {
+            return pair_dot(grad, load_pair(p.o + row * p.o_stride + head * kHead, lane));
+        };
+        const long long queries = static_cast<long long>(q.count) * p.heads;
+        const long long keys = static_cast<long long>(q.count) * p.kv_heads;
+        for (long long item = warp; item < queries + keys; item += warps) {
+            if (item < queries) {
+                const int i = static_cast<int>(item / p.heads), head = static_cast<int>(item % p.heads);
+                const long long row = q.first + i;
+                const float2 x = load_pair(p.q + row * p.q_stride + head * kHead, lane);
+                const float2 grad = load_pair(g.d_o + row * p.o_stride + head * kHead, lane);
+                const float delta = delta_of(row, head, grad);
+                const float lse2 = p.lse[static_cast<long long>(head) * p.rows + row] * kLog2e;
+                float2 dq = make_float2(0.0f, 0.0f);
+                for (int key = 0; key <= i; ++key) {
+                    const long long at = key_offset(p, q, s, key, head / group);
+                    const float2 kk = load_pair(p.k + at, lane);
+                    const float weight = exp2f(pair_dot(x, kk) * scale2 - lse2);
+                    const float ds = weight * (pair_dot(grad, load_pair(p.v + at, lane)) - delta) * p.scale;
+                    dq.x += ds * kk.x;
+                    dq.y += ds * kk.y;
+                }
+                reinterpret_cast<__half2*>(g.dq + row * p.q_stride + head * kHead)[lane] =
+                    __floats2half2_rn(dq.x, dq.y);
+            } else {
+                const long long which = item - queries;
+                const int j = static_cast<int>(which / p.kv_heads), kv_head = static_cast<int>(which % p.kv_heads);
+                const long long at = key_offset(p, q, s, j, kv_head);
+                const float2 kk = load_pair(p.k + at, lane), vv = load_pair(p.v + at, lane);
+                float2 dk = make_float2(0.0f, 0.0f), dv = dk;
+                for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
+                    for (int i = j; i < q.count; ++i) {
+                        const long long row = q.first + i;
+                        const float2 x = load_pair(p.q + row * p.q_stride + head * kHead, lane);
+                        const float2 grad = load_pair(g.d_o + row * p.o_stride + head * kHead, lane);
+                        const float lse2 = p.lse[static_cast<long long>(head) * p.rows + row] * kLog2e;
+                        const float weight = exp2f(pair_dot(x, kk) * scale2 - lse2);
+                        const float ds = weight * (pair_dot(grad, vv) - delta_of(row, head, grad)) * p.scale;
+                        dv.x += weight * grad.x;
+                        dv.y += weight * grad.y;
+                        dk.x += ds * x.x;
+                        dk.y += ds * x.y;
+                    }
+                }
+                reinterpret_cast<__half2*>(g.dk + at)[lane] = __floats2half2_rn(dk.x, dk.y);
+                reinterpret_cast<__half2*>(g.dv + at)[lane] = __floats2half2_rn(dv.x, dv.y);
+            }
+        }
+    }
+}
+
+// Copies the new tokens' keys and values into their pages: eight lanes per row of 64 values.
+__global__ void __launch_bounds__(256)
+    fb_paged_store(const PackedArgs p, __half* k_pages, __half* v_pages) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int piece = threadIdx.x % 8;
+    const long long first = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / 8;
+    const long long stride = static_cast<long long>(gridDim.x) * 32;
+    for (int s = blockIdx.y; s < p.sequences; s += gridDim.y) {
+        const Sequence q = sequence_at(p, s);
+        for (long long item = first; item < static_cast<long long>(q.count) * p.kv_heads * 2; item += stride) {
+            const int which = static_cast<int>(item % 2);
+            const int head = static_cast<int>(item / 2 % p.kv_heads);
+            const int i = static_cast<int>(item / 2 / p.kv_heads);
+            const int key = q.keys - q.count + i;
+            if (key < 0) {
+                continue;
+            }
+            const long long page = page_of(p, s, key);
+            if (page < 0) {
+                continue;
+            }
+            const __half* from = (which == 0 ? p.k : p.v) + (q.first + static_cast<long long>(i)) * p.kv_stride +
+                                 head * kHead;
+            __half* to = (which == 0 ? k_pages : v_pages) +
+                         ((page * p.kv_heads + head) * p.page_size + key % p.page_size) * kHead;
+            reinterpret_cast<uint4*>(to)[piece] = reinterpret_cast<const uint4*>(from)[piece];
+        }
+    }
+}
+
+dim3 sequence_grid(const PackedArgs& p, int items_per_block, long long items, int sms) {
+    const long long per_sequence = (items / std::max(1, p.sequences) + items_per_block) / items_per_block;
+    const unsigned y = static_cast<unsigned>(std::min(p.sequences, 65535));
+    const long long most = std::max<long long>(1, 16LL * sms / y + 1);
+    return dim3(static_cast<unsigned>(std::min(std::max<long long>(1, 2 * per_sequence), most)), y);
+}
+
+}  // namespace
+
+cudaError_t packed_error_flag(int* value, bool reset) {
+    cudaError_t e = cudaMemcpyFromSymbol(value, g_packed_error, sizeof(int));
+    if (e == cudaSuccess && reset && *value != 0) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_packed_error, &zero, sizeof(int));
+    }
+    return e;
+}
+
+}  // namespace fb
+
+// ---- entry points ------------------------------------------------------------------------------
+
+namespace {
+
+constexpr flint_status kBad = FLINT_ERROR_INVALID_ARGUMENT;
+constexpr size_t kMostSequences = 65535;
+constexpr size_t kMostRows = size_t{1} << 24;
+constexpr size_t kMostHeads = 1024;
+constexpr size_t kMostGroup = 128;
+constexpr size_t kMostStride = size_t{1} << 24;
+
+flint_status check_rows(const char* name, size_t sequences, size_t rows, size_t heads, size_t kv_heads,
+                        size_t head_width, size_t q_stride, size_t kv_stride, size_t o_stride) {
+    if (sequences > kMostSequences || rows > kMostRows) {
+        return fb::fail(kBad, "%s: sequences (%zu) can be up to %zu, and rows (%zu) up to %zu", name, sequences,
+                        kMostSequences, rows, kMostRows);
+    }
+    if (kv_heads == 0 || heads == 0 || heads > kMostHeads || heads % kv_heads != 0 || heads / kv_heads > kMostGroup) {
+        return fb::fail(kBad,
+                        "%s: heads (%zu) must be from 1 to %zu and a multiple of kv_heads (%zu), up to %zu times it",
+                        name, heads, kMostHeads, kv_heads, kMostGroup);
+    }
+    if (head_width != 64) {
+        return fb::fail(kBad, "%s: head_width (%zu) must be 64", name, head_width);
+    }
+    const struct {
+        const char* name;
+        size_t value, least;
+    } strides[] = {{"q_stride", q_stride, heads * 64}, {"kv_stride", kv_stride, kv_heads * 64},
+                   {"o_stride", o_stride, heads * 64}};
+    for (const auto& s : strides) {
+        if (s.value % 8 != 0 || s.value < s.least || s.value > kMostStride) {
+            return fb::fail(kBad, "%s: %s (%zu) must be a multiple of 8 from %zu to %zu", name, s.name, s.value,
+                            s.least, kMostStride);
+        }
+    }
+    return FLINT_OK;
+}
+
+flint_status check_scale(const char* name, float scale) {
+    if (!std::isfinite(scale) || scale <= 0.0f) {
+        return fb::fail(kBad, "%s: scale (%g) must be finite and positive", name, static_cast<double>(scale));
+    }
+    return FLINT_OK;
+}
+
+// A matrix of `rows` rows of `width` bytes, `stride` bytes apart; a contiguous array is one row.
+struct Rows {
+    const char* name;
+    const void* pointer;
+    size_t rows, width, stride;
+    size_t bytes() const { return rows == 0 ? 0 : (rows - 1) * stride + width; }
+};
+
+bool rows_overlap(const Rows& a, const Rows& b) {
+    if (!fb::overlap(a.pointer, a.bytes(), b.pointer, b.bytes())) {
+        return false;
+    }
+    if (a.rows < 2 || b.rows < 2 || a.stride != b.stride) {
+        return true;
+    }
+    // Columns of one matrix of rows do not touch each other although their ranges interleave.
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.pointer), y = reinterpret_cast<uintptr_t>(b.pointer);
+    const size_t gap = y >= x ? (y - x) % a.stride : (a.stride - (x - y) % a.stride) % a.stride;
+    return gap < a.width || gap + b.width > a.stride;
+}
+
+// As fb::check_spans, for rows with gaps between them.
+template <size_t N>
+flint_status check_all(const char* name, const Rows (&list)[N], size_t outputs) {
+    fb::Span spans[N];
+    for (size_t i = 0; i < N; ++i) {
+        spans[i] = fb::Span{list[i].name, list[i].pointer, list[i].bytes()};
+    }
+    FB_TRY(fb::check_spans(name, spans, N, 0));
+    for (size_t i = 0; i < outputs; ++i) {
+        for (size_t j = i + 1; j < N; ++j) {
+            if (rows_overlap(list[i], list[j])) {
+                return fb::fail(kBad, "%s: %s and %s overlap", name, list[i].name, list[j].name);
+            }
+        }
+    }
+    return FLINT_OK;
+}
+
+Rows flat(const char* name, const void* pointer, size_t bytes) { return Rows{name, pointer, 1, bytes, bytes}; }
+
+Rows token_rows(const char* name, const void* pointer, size_t rows, size_t heads, size_t stride) {
+    return Rows{name, pointer, rows, heads * 128, stride * 2};
+}
+
+// An array that may be left out stands in the list as something that overlaps nothing.
+Rows optional(const char* name, const void* pointer, size_t bytes, const void* instead) {
+    return pointer != nullptr ? flat(name, pointer, bytes) : flat(name, instead, 0);
+}
+
+flint_status check_workspace(const char* name, size_t needed, size_t given) {
+    if (given < needed) {
+        return fb::fail(kBad, "%s: needs %zu bytes of workspace, given %zu", name, needed, given);
+    }
+    return FLINT_OK;
+}
+
+flint_status check_shape(const char* name, const flint_b200_packed_shape* shape) {
+    if (shape == nullptr) {
+        return fb::fail(kBad, "%s: shape is null", name);
+    }
+    return check_rows(name, shape->sequences, shape->rows, shape->heads, shape->kv_heads, shape->head_width,
+                      shape->q_stride, shape->kv_stride, shape->o_stride);
+}
+
+flint_status check_shape(const char* name, const flint_b200_paged_shape* shape) {
+    if (shape == nullptr) {
+        return fb::fail(kBad, "%s: shape is null", name);
+    }
+    FB_TRY(check_rows(name, shape->sequences, shape->rows, shape->heads, shape->kv_heads, shape->head_width,
+                      shape->q_stride, shape->kv_stride, shape->o_stride));
+    const size_t size = shape->page_size;
+    if (size < 16 || size > 1024 || (size & (size - 1)) != 0) {
+        return fb::fail(kBad, "%s: page_size (%zu) must be a power of two from 16 to 1024", name, size);
+    }
+    constexpr size_t kMost = (size_t{1} << 31) - 1;
+    if (shape->pages == 0 || shape->pages > kMost / size / shape->kv_heads) {
+        return fb::fail(kBad, "%s: pages (%zu) must be from 1 to %zu", name, shape->pages,
+                        kMost / size / shape->kv_heads);
+    }
+    if (shape->table_stride == 0 || shape->table_stride > (size_t{1} << 26) / size) {
+        return fb::fail(kBad, "%s: table_stride (%zu) must be from 1 to %zu", name, shape->table_stride,
+                        (size_t{1} << 26) / size);
+    }
+    if (shape->longest == 0 || shape->longest > kMostRows) {
+        return fb::fail(kBad, "%s: longest (%zu) must be from 1 to %zu", name, shape->longest, kMostRows);
+    }
+    return FLINT_OK;
+}
+
+template <typename Shape>
+fb::PackedArgs base_args(const Shape& s, float scale) {
+    fb::PackedArgs p = {};
+    p.sequences = static_cast<int>(s.sequences);
+    p.rows = static_cast<int>(s.rows);
+    p.heads = static_cast<int>(s.heads);
+    p.kv_heads = static_cast<int>(s.kv_heads);
+    p.q_stride = static_cast<long long>(s.q_stride);
+    p.kv_stride = static_cast<long long>(s.kv_stride);
+    p.o_stride = static_cast<long long>(s.o_stride);
+    p.scale = scale;
+    return p;
+}
+
+fb::PackedArgs paged_args(const flint_b200_paged_shape& s, float scale) {
+    fb::PackedArgs p = base_args(s, scale);
+    p.pages = static_cast<long long>(s.pages);
+    p.page_size = static_cast<int>(s.page_size);
+    p.table_stride = static_cast<int>(s.table_stride);
+    return p;
+}
+
+template <typename Shape>
+bool nothing(const Shape& s) {
+    return s.sequences == 0 || s.rows == 0;
+}
+
+size_t cache_bytes(const flint_b200_paged_shape& s) { return s.pages * s.kv_heads * s.page_size * 128; }
+
+}  // namespace
+
+extern "C" {
+
+flint_status flint_b200_packed_attention_workspace(const flint_b200_packed_shape* shape, size_t* bytes) {
+    constexpr const char* name = "flint_b200_packed_attention_workspace";
+    FB_TRY(check_shape(name, shape));
+    if (bytes == nullptr) {
+        return fb::fail(kBad, "%s: bytes is null", name);
+    }
+    *bytes = 16;
+    return FLINT_OK;
+}
+
+flint_status flint_b200_packed_attention_forward(void* o, void* lse, const void* q, const void* k, const void* v,
+                                                 const void* starts, const flint_b200_packed_shape* shape,
+                                                 float scale, void* workspace, size_t workspace_bytes,
+                                                 flint_stream stream) {
+    constexpr const char* name = "flint_b200_packed_attention_forward";
+    FB_TRY(check_shape(name, shape));
+    FB_TRY(check_scale(name, scale));
+    if (nothing(*shape)) {
+        return FLINT_OK;
+    }
+    size_t needed = 0;
+    FB_TRY(flint_b200_packed_attention_workspace(shape, &needed));
+    FB_TRY(check_workspace(name, needed, workspace_bytes));
+    const size_t rows = shape->rows;
+    const Rows list[] = {
+        token_rows("o", o, rows, shape->heads, shape->o_stride),
+        optional("lse", lse, shape->heads * rows * 4, o),
+        flat("workspace", workspace, needed),
+        token_rows("q", q, rows, shape->heads, shape->q_stride),
+        token_rows("k", k, rows, shape->kv_heads, shape->kv_stride),
+        token_rows("v", v, rows, shape->kv_heads, shape->kv_stride),
+        flat("starts", starts, (shape->sequences + 1) * 4),
+    };
+    FB_TRY(check_all(name, list, 3));
+    fb::PackedArgs p = base_args(*shape, scale);
+    p.q = static_cast<const __half*>(q);
+    p.k = static_cast<const __half*>(k);
+    p.v = static_cast<const __half*>(v);
+    p.o = static_cast<__half*>(o);
+    p.lse = static_cast<float*>(lse);
+    p.starts = static_cast<const int*>(starts);
+    int sms = 148;
+    FB_CUDA(fb::sm_count(&sms));
+    FB_CUDA(fb::launch_dependent(fb::fb_packed_forward_rows,
+                                 fb::sequence_grid(p, 8, static_cast<long long>(rows) * p.heads, sms), dim3(256), 0,
+                                 stream, p));
+    return FLINT_OK;
+}
+
+flint_status flint_b200_packed_attention_backward_workspace(const flint_b200_packed_shape* shape, size_t* bytes) {
+    constexpr const char* name = "flint_b200_packed_attention_backward_workspace";
+    FB_TRY(check_shape(name, shape));
+    if (bytes == nullptr) {
+        return fb::fail(kBad, "%s: bytes is null", name);
+    }
+    *bytes = 16;
+    return FLINT_OK;
+}
+
+flint_status flint_b200_packed_attention_backward(void* dq, void* dk, void* dv, const void* d_o, const void* o,
+                                                  const void* lse, const void* q, const void* k, const void* v,
+                                                  const void* starts, const flint_b200_packed_shape* shape,
+                                                  float scale, void* workspace, size_t workspace_bytes,
+                                                  flint_stream stream) {
+    constexpr const char* name = "flint_b200_packed_attention_backward";
+    FB_TRY(check_shape(name, shape));
+    FB_TRY(check_scale(name, scale));
+    if (nothing(*shape)) {
+        return FLINT_OK;
+    }
+    size_t needed = 0;
+    FB_TRY(flint_b200_packed_attention_backward_workspace(shape, &needed));
+    FB_TRY(check_workspace(name, needed, workspace_bytes));
+    const size_t rows = shape->rows;
+    const Rows list[] = {
+        token_rows("dq", dq, rows, shape->heads, shape->q_stride),
+        token_rows("dk", dk, rows, shape->kv_heads, shape->kv_stride),
+        token_rows("dv", dv, rows, shape->kv_heads, shape->kv_stride),
+        flat("workspace", workspace, needed),
+        token_rows("d_o", d_o, rows, shape->heads, shape->o_stride),
+        token_rows("o", o, rows, shape->heads, shape->o_stride),
+        flat("lse", lse, shape->heads * rows * 4),
+        token_rows("q", q, rows, shape->heads, shape->q_stride),
+        token_rows("k", k, rows, shape->kv_heads, shape->kv_stride),
+        token_rows("v", v, rows, shape->kv_heads, shape->kv_stride),
+        flat("starts", starts, (shape->sequences + 1) * 4),
+    };
+    FB_TRY(check_all(name, list, 4));
+    fb::PackedArgs p = base_args(*shape, scale);
+    p.q = static_cast<const __half*>(q);
+    p.k = static_cast<const __half*>(k);
+    p.v = static_cast<const __half*>(v);
+    p.o = static_cast<__half*>(const_cast<void*>(o));
+    p.lse = static_cast<float*>(const_cast<void*>(lse));
+    p.starts = static_cast<const int*>(starts);
+    const fb::PackedGradients g{static_cast<__half*>(dq), static_cast<__half*>(dk), static_cast<__half*>(dv),
+                                static_cast<const __half*>(d_o)};
+    int sms = 148;
+    FB_CUDA(fb::sm_count(&sms));
+    FB_CUDA(fb::launch_dependent(fb::fb_packed_backward_rows,
+                                 fb::sequence_grid(p, 8, static_cast<long long>(rows) * (p.heads + p.kv_heads), sms),
+                                 dim3(256), 0, stream, p, g));
+    return FLINT_OK;
+}
+
+flint_status flint_b200_paged_store(void* k_pages, void* v_pages, const void* k, const void* v, const void* starts,
+                                    const void* lengths, const void* page_table, const flint_b200_paged_shape* shape,
+                                    flint_stream stream) {
+    constexpr const char* name = "flint_b200_paged_store";
+    FB_TRY(check_shape(name, shape));
+    if (nothing(*shape)) {
+        return FLINT_OK;
+    }
+    const Rows list[] = {
+        flat("k_pages", k_pages, cache_bytes(*shape)),
+        flat("v_pages", v_pages, cache_bytes(*shape)),
+        token_rows("k", k, shape->rows, shape->kv_heads, shape->kv_stride),
+        token_rows("v", v, shape->rows, shape->kv_heads, shape->kv_stride),
+        flat("starts", starts, (shape->sequences + 1) * 4),
+        flat("lengths", lengths, shape->sequences * 4),
+        flat("page_table", page_table, shape->sequences * shape->table_stride * 4),
+    };
+    FB_TRY(check_all(name, list, 2));
+    fb::PackedArgs p = paged_args(*shape, 1.0f);
+    p.k = static_cast<const __half*>(k);
+    p.v = static_cast<const __half*>(v);
+    p.starts = static_cast<const int*>(starts);
+    p.lengths = static_cast<const int*>(lengths);
+    p.table = static_cast<const int*>(page_table);
+    int sms = 148;
+    FB_CUDA(fb::sm_count(&sms));
+    FB_CUDA(fb::launch_dependent(fb::fb_paged_store,
+                                 fb::sequence_grid(p, 32, static_cast<long long>(p.rows) * p.kv_heads * 2, sms),
+                                 dim3(256), 0, stream, p, static_cast<__half*>(k_pages),
+                                 static_cast<__half*>(v_pages)));
+    return FLINT_OK;
+}
+
+flint_status flint_b200_paged_attention_workspace(const flint_b200_paged_shape* shape, size_t* bytes) {
+    constexpr const char* name = "flint_b200_paged_attention_workspace";
+    FB_TRY(check_shape(name, shape));
+    if (bytes == nullptr) {
+        return fb::fail(kBad, "%s: bytes is null", name);
+    }
+    *bytes = 16;
+    return FLINT_OK;
+}
+
+flint_status flint_b200_paged_attention(void* o, void* lse, const void* q, const void* k_pages, const void* v_pages,
+                                        const void* starts, const void* lengths, const void* page_table,
+                                        const flint_b200_paged_shape* shape, float scale, void* workspace,
+                                        size_t workspace_bytes, flint_stream stream) {
+    constexpr const char* name = "flint_b200_paged_attention";
+    FB_TRY(check_shape(name, shape));
+    FB_TRY(check_scale(name, scale));
+    if (nothing(*shape)) {
+        return FLINT_OK;
+    }
+    size_t needed = 0;
+    FB_TRY(flint_b200_paged_attention_workspace(shape, &needed));
+    FB_TRY(check_workspace(name, needed, workspace_bytes));
+    const Rows list[] = {
+        token_rows("o", o, shape->rows, shape->heads, shape->o_stride),
+        optional("lse", lse, shape->heads * shape->rows * 4, o),
+        flat("workspace", workspace, needed),
+        token_rows("q", q, shape->rows, shape->heads, shape->q_stride),
+        flat("k_pages", k_pages, cache_bytes(*shape)),
+        flat("v_pages", v_pages, cache_bytes(*shape)),
+        flat("starts", starts, (shape->sequences + 1) * 4),
+        flat("lengths", lengths, shape->sequences * 4),
+        flat("page_table", page_table, shape->sequences * shape->table_stride * 4),
+    };
+    FB_TRY(check_all(name, list, 3));
+    fb::PackedArgs p = paged_args(*shape, scale);
+    p.q = static_cast<const __half*>(q);
+    p.k = static_cast<const __half*>(k_pages);
+    p.v = static_cast<const __half*>(v_pages);
+    p.o = static_cast<__half*>(o);
+    p.lse = static_cast<float*>(lse);
+    p.starts = static_cast<const int*>(starts);
+    p.lengths = static_cast<const int*>(lengths);
+    p.table = static_cast<const int*>(page_table);
+    int sms = 148;
+    FB_CUDA(fb::sm_count(&sms));
+    FB_CUDA(fb::launch_dependent(fb::fb_packed_forward_rows,
+                                 fb::sequence_grid(p, 8, static_cast<long long>(p.rows) * p.heads, sms), dim3(256), 0,
+                                 stream, p));
+    return FLINT_OK;
+}
+
+}  // extern "C"

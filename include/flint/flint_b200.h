@@ -16,7 +16,8 @@ extern "C" {
 #endif
 
 /* 1 if a kernel (GEMM, attention, column sums, cross-entropy) gave up on a
- * bounded barrier wait since the last call (the flag is cleared), 0 otherwise.
+ * bounded barrier wait since the last call, or one that reads starts, lengths or page numbers
+ * met one out of range (the flag is cleared), 0 otherwise.
  * Synchronises the device; meant for tests. */
 FLINT_API flint_status flint_b200_kernel_fault(int* raised);
 
@@ -215,6 +216,133 @@ FLINT_API flint_status flint_b200_generator_logits(const flint_b200_generator* g
 FLINT_API flint_status flint_b200_generator_bytes_per_step(const flint_b200_generator* generator,
                                                            size_t* weight_bytes,
                                                            size_t* cache_bytes);
+
+/* ---- sequences of different lengths --------------------------------------------------------
+ *
+ * A batch is `rows` rows, one per token, in which the sequences lie one behind the other:
+ * `starts` (int32 [sequences + 1] on the device, non-decreasing, 0 .. rows) says where, sequence s
+ * having rows starts[s] .. starts[s + 1] - 1, which may be none; rows outside all sequences are
+ * left as they are. Heads of 64 FP16 values lie side by side in a row; rows of q (and dq) are q_stride
+ * elements apart, those of k, v (dk, dv) kv_stride, those of o (d_o) o_stride, so that the parts of
+ * a product's [q | k | v] rows can be given as they lie. Query head h reads head
+ * h / (heads / kv_heads) of k and v. lse is FP32 [heads, rows].
+ *
+ * Limits: sequences up to 65,535, rows up to 2^24, heads up to 1,024 and up to 128 times kv_heads,
+ * strides multiples of 8 up to 2^24, scale finite and positive. Pointers are 16-byte aligned and
+ * outputs overlap neither each other nor inputs (columns of one matrix do not overlap).
+ * What lies in device memory (starts, lengths, page numbers) is not known to the host: values
+ * outside their ranges are clamped by the kernels, which touch nothing outside the arrays, and
+ * reported by flint_b200_kernel_fault; the results are then undefined.
+ *
+ * A workspace is overwritten by every call and keeps nothing from one to the next; calls that can
+ * run at the same time need one each. Its size depends on the shape and on the GPU's SM count. */
+typedef struct {
+    size_t sequences;
+    size_t rows;
+    size_t heads;
+    size_t kv_heads;
+    size_t head_width;
+    size_t q_stride;
+    size_t kv_stride;
+    size_t o_stride;
+} flint_b200_packed_shape;
+
+FLINT_API flint_status flint_b200_packed_attention_workspace(const flint_b200_packed_shape* shape,
+                                                             size_t* bytes);
+
+/* Causal attention within each sequence: o_i = sum over j <= i of p_ij v_j with p the softmax of
+ * scale * q_i . k_j, and lse_i (may be null) the natural log of the scores' sum of exponentials. Keys whose
+ * score is minus infinity weigh nothing (a row of nothing else is NaN). Values of a sequence
+ * reach only that sequence, whatever they are; within it a value of v that is not finite may reach
+ * rows up to 127 before its own. */
+FLINT_API flint_status flint_b200_packed_attention_forward(
+    void* o, void* lse, const void* q, const void* k, const void* v, const void* starts,
+    const flint_b200_packed_shape* shape, float scale, void* workspace, size_t workspace_bytes,
+    flint_stream stream);
+
+FLINT_API flint_status flint_b200_packed_attention_backward_workspace(
+    const flint_b200_packed_shape* shape, size_t* bytes);
+
+/* Gradients of the above from d_o and the forward call's o and lse. dk and dv are sums over the
+ * query heads that share a head, taken in one fixed order: results repeat bit for bit. */
+FLINT_API flint_status flint_b200_packed_attention_backward(
+    void* dq, void* dk, void* dv, const void* d_o, const void* o, const void* lse, const void* q,
+    const void* k, const void* v, const void* starts, const flint_b200_packed_shape* shape,
+    float scale, void* workspace, size_t workspace_bytes, flint_stream stream);
+
+/* A cache of keys and values in pages, FP16 [pages, kv_heads, page_size, 64] each: page_size is a
+ * power of two from 16 to 1,024, pages * kv_heads * page_size below 2^31. Position t of sequence s
+ * is slot t % page_size of page page_table[s * table_stride + t / page_size] (int32 on the device,
+ * 0 .. pages - 1 where a position is used, anything elsewhere). `lengths` (int32 [sequences] on the
+ * device, up to table_stride * page_size) counts each sequence's positions, this call's new tokens
+ * among them: those are the last starts[s + 1] - starts[s] ones. `longest` says how many new tokens a
+ * sequence has at most; it chooses the kernel and bounds nothing. The other fields and limits are
+ * flint_b200_packed_shape's; kv_stride is that of the new tokens' k and v. */
+typedef struct {
+    size_t sequences;
+    size_t rows;
+    size_t heads;
+    size_t kv_heads;
+    size_t head_width;
+    size_t q_stride;
+    size_t kv_stride;
+    size_t o_stride;
+    size_t pages;
+    size_t page_size;
+    size_t table_stride;
+    size_t longest;
+} flint_b200_paged_shape;
+
+/* Copies the new tokens' keys and values into their positions of the cache. Two sequences that
+ * store into one page's same slot race; sequences may share pages that they only read. */
+FLINT_API flint_status flint_b200_paged_store(void* k_pages, void* v_pages, const void* k,
+                                              const void* v, const void* starts,
+                                              const void* lengths, const void* page_table,
+                                              const flint_b200_paged_shape* shape,
+                                              flint_stream stream);
+
+FLINT_API flint_status flint_b200_paged_attention_workspace(const flint_b200_paged_shape* shape,
+                                                            size_t* bytes);
+
+/* Attention of the new tokens over the cache, in which their own keys and values are already:
+ * each sees the positions up to its own. lse may be null. A token without any position
+ * (a sequence whose length is below its number of new tokens) gets zeros and an lse of minus infinity.
+ * Slots behind a sequence's last position may hold anything. */
+FLINT_API flint_status flint_b200_paged_attention(void* o, void* lse, const void* q,
+                                                  const void* k_pages, const void* v_pages,
+                                                  const void* starts, const void* lengths,
+                                                  const void* page_table,
+                                                  const flint_b200_paged_shape* shape, float scale,
+                                                  void* workspace, size_t workspace_bytes,
+                                                  flint_stream stream);
+
+/* ---- probabilities of tokens ----------------------------------------------------------------
+ *
+ * Over the first vocab columns of each row x of logits [rows, cols], FP16 or (fp32_logits not 0)
+ * FP32:  lse = log sum exp x,  log_probs = x[target] - lse,  entropy = -sum p log p with
+ * p = exp(x - lse), all FP32 [rows];  top_tokens (uint16 [rows, top]) the columns of the `top`
+ * largest logits in descending order, equal ones by ascending column, and top_log_probs (FP32
+ * [rows, top]) theirs. targets are uint16; one that is not below vocab marks a row that does not count: its
+ * log-probability is 0. log_probs (with targets), entropy and lse may be null, and with top 0 the top's arrays.
+ * A logit of minus infinity is a token that cannot come; a row of nothing else has an entropy of 0 and
+ * log-probabilities and an lse of minus infinity. A row with a NaN or plus infinity has NaNs
+ * (NaN sorts above all numbers). cols is a multiple of 8 from 8 to 65,536, top up to 32 and vocab, rows up to 2^31. */
+FLINT_API flint_status flint_b200_token_log_probs(void* log_probs, void* entropy, void* lse,
+                                                  void* top_log_probs, void* top_tokens,
+                                                  const void* logits, const void* targets,
+                                                  int fp32_logits, size_t rows, size_t vocab,
+                                                  size_t cols, size_t top, flint_stream stream);
+
+/* The logits' gradient for the gradients d_log_probs and d_entropy (FP32 [rows], one may be null) of
+ * the above's outputs, from its lse and entropy:
+ *   dlogits_c = d_log_probs ([c == target] - p_c) - d_entropy p_c (log p_c + entropy)
+ * in the logits' type, +0 in columns from vocab on; targets not below vocab count as
+ * d_log_probs = 0. A column of minus infinity gets 0, and so does a row of nothing else. dlogits may be
+ * logits itself. */
+FLINT_API flint_status flint_b200_token_log_probs_backward(
+    void* dlogits, const void* logits, const void* targets, const void* lse, const void* entropy,
+    const void* d_log_probs, const void* d_entropy, int fp32_logits, size_t rows, size_t vocab,
+    size_t cols, flint_stream stream);
 
 /* Sets *found_nonfinite (device int) to 1 if any of the count FP32 values is
  * inf or NaN; leaves it unchanged otherwise, so several calls can share it.
