@@ -40,6 +40,7 @@
 #include "device_utils.cuh"
 #include "flint/flint_b200.h"
 #include "sm100.cuh"
+#include "softmax.cuh"
 
 namespace fb {
 namespace {
@@ -86,48 +87,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
         : "memory");
 }
 
-// 2^x on the special-function unit (relative error about 2^-22, flushes denormals).
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// How far (in base-2 exponent units) a tile's maximum may exceed the reference exponent
-// before the forward kernel moves the reference and rescales its accumulator:
-// probabilities then stay below 2^8, well inside FP16.
-constexpr float kLazyShift = 8.0f;
-
-// The reference exponent of a row for which no key has counted so far: the least finite value, so that
-// keys of minus infinity (an infinity in K, or a mask) give probabilities of 2^-inf where -inf - -inf would be
-// NaN, and the first key that counts moves it.
-constexpr float kNoKey = -3.402823466e38f;
-
-// 2^x for two values at once on the FMA pipe, for the share of the forward kernel's
-// exponentials that the special-function unit has no time for: x = n + f with n the
-// nearest integer (taken from the low mantissa bits of x + 1.5 * 2^23), 2^f by a
-// degree-4 polynomial on [-0.5, 0.5] (relative error 2.7e-6, two orders below the FP16
-// rounding of the probabilities), n added into the exponent field. x must be at most
-// 127 - 1; anything below -120 counts as -120 (2^-120 is zero in FP16).
-__device__ __forceinline__ void exp2_pair_fma(fb::F2 x, float& lo, float& hi) {
-    float x0, x1;
-    fb::f2_unpack(x, x0, x1);
-    const fb::F2 clamped = fb::f2_pack(fmaxf(x0, -120.0f), fmaxf(x1, -120.0f));
-    const fb::F2 magic = fb::f2_pack(12582912.0f, 12582912.0f);
-    const fb::F2 z = fb::f2_add(clamped, magic);
-    const fb::F2 f = fb::f2_sub(clamped, fb::f2_sub(z, magic));
-    fb::F2 poly = fb::f2_fma(f, fb::f2_pack(0.009570090100169182f, 0.009570090100169182f),
-                             fb::f2_pack(0.05591785907745361f, 0.05591785907745361f));
-    poly = fb::f2_fma(poly, f, fb::f2_pack(0.2402474582195282f, 0.2402474582195282f));
-    poly = fb::f2_fma(poly, f, fb::f2_pack(0.6931217908859253f, 0.6931217908859253f));
-    poly = fb::f2_fma(poly, f, fb::f2_pack(0.9999992847442627f, 0.9999992847442627f));
-    float p0, p1, z0, z1;
-    fb::f2_unpack(poly, p0, p1);
-    fb::f2_unpack(z, z0, z1);
-    lo = __int_as_float(__float_as_int(p0) + (__float_as_int(z0) << 23));
-    hi = __int_as_float(__float_as_int(p1) + (__float_as_int(z1) << 23));
-}
-
 // Of every four pairs of exponentials in the forward kernel, how many take the FMA pipe.
 #ifndef FB_ATTN_FMA_EXP_OF_4
 #define FB_ATTN_FMA_EXP_OF_4 1
@@ -146,12 +105,6 @@ __device__ __forceinline__ void exp2_two(int pair, float x0, float x1, float& e0
     }
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 // Named barrier between the two warps that share a TMEM lane quadrant (the two
 // halves of the same 32 rows); barrier 0 is __syncthreads, 1..4 are the quadrants'.
 __device__ __forceinline__ void quadrant_sync(int quadrant) {
@@ -161,17 +114,6 @@ __device__ __forceinline__ void quadrant_sync(int quadrant) {
 // The four warps of a quadrant: both column halves of both tiles (barriers 9..12).
 __device__ __forceinline__ void item_sync(int quadrant) {
     asm volatile("bar.sync %0, 128;" ::"r"(quadrant + 9) : "memory");
-}
-
-// Descriptors for the three ways a tile is read.
-// K-major tile [128 rows][64 cols] (rows = M or N index): 16-column step = 32 bytes.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t tile, int kstep) {
-    return sm100::smem_desc_sw128(tile + kstep * 32, 16, 1024);
-}
-// MN-major view of the same memory: rows are the K index, 16 rows = 2,048 bytes;
-// 64-column blocks (panels) are `lbo` bytes apart.
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t tile, int kstep, uint32_t lbo) {
-    return sm100::smem_desc_sw128(tile + kstep * 2048, lbo, 1024);
 }
 
 constexpr uint32_t kIdescS = sm100::instr_desc_f16(128, 128, false, false);   // Q K^T, dO V^T

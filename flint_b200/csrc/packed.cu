@@ -9,53 +9,13 @@
 #include "common.h"
 #include "device_utils.cuh"
 #include "flint/flint_b200.h"
-#include "packed.h"
+#include "packed.cuh"
 
 namespace fb {
 namespace {
 
 constexpr int kHead = 64;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-__device__ int g_packed_error = 0;
-
-__device__ __forceinline__ void report() { atomicExch(&g_packed_error, 1); }
-
-// A sequence's place in the rows and how many keys it has; values outside their ranges are
-// clamped and reported.
-struct Sequence {
-    int first, count, keys;
-};
-
-__device__ __forceinline__ Sequence sequence_at(const PackedArgs& p, int s) {
-    const int a = p.starts[s], b = p.starts[s + 1];
-    Sequence out;
-    out.first = min(max(a, 0), p.rows);
-    out.count = min(max(b, out.first), p.rows) - out.first;
-    bool good = out.first == a && out.first + out.count == b;
-    out.keys = out.count;
-    if (p.lengths != nullptr) {
-        const int given = p.lengths[s];
-        const long long most = static_cast<long long>(p.table_stride) * p.page_size;
-        out.keys = static_cast<int>(min(static_cast<long long>(max(given, 0)), most));
-        good = good && out.keys == given;
-    }
-    if (!good) {
-        report();
-    }
-    return out;
-}
-
-// The page that holds a key of sequence s, or -1 (reported) where the table names none.
-__device__ __forceinline__ long long page_of(const PackedArgs& p, int s, int key) {
-    const int page = p.table[static_cast<long long>(s) * p.table_stride + key / p.page_size];
-    if (page < 0 || page >= p.pages) {
-        report();
-        return -1;
-    }
-    return page;
-}
 
 // Where the row of 64 values of a key (in K or V) begins; negative for a page that is not there.
 __device__ __forceinline__ long long key_offset(const PackedArgs& p, const Sequence& q, int s, int key,
@@ -77,52 +37,6 @@ __device__ __forceinline__ float warp_sum(float v) {
         v += __shfl_xor_sync(fb::kFullMask, v, off);
     }
     return v;
-}
-
-// One warp per (token, head), two of the 64 columns per lane.
-__global__ void __launch_bounds__(256) fb_packed_forward_rows(const PackedArgs p) {
-    fb::dependency_wait();
-    fb::dependency_release();
-    const int lane = threadIdx.x % 32;
-    const int warp = blockIdx.x * 8 + threadIdx.x / 32;
-    const int warps = gridDim.x * 8;
-    const int group = p.heads / p.kv_heads;
-    for (int s = blockIdx.y; s < p.sequences; s += gridDim.y) {
-        const Sequence q = sequence_at(p, s);
-        for (long long item = warp; item < static_cast<long long>(q.count) * p.heads; item += warps) {
-            const int i = static_cast<int>(item / p.heads), head = static_cast<int>(item % p.heads);
-            const long long row = q.first + i;
-            const float2 x = load_pair(p.q + row * p.q_stride + head * kHead, lane);
-            const int visible = q.keys - q.count + i + 1;
-            float m = -INFINITY, l = 0.0f;
-            float2 acc = make_float2(0.0f, 0.0f);
-            for (int key = 0; key < visible; ++key) {
-                const long long at = key_offset(p, q, s, key, head / group);
-                if (at < 0) {
-                    continue;
-                }
-                const float2 kk = load_pair(p.k + at, lane);
-                const float score = warp_sum(x.x * kk.x + x.y * kk.y) * (p.scale * kLog2e);
-                if (score == -INFINITY) {
-                    continue;   // weighs nothing
-                }
-                const float top = score > m || score != score ? score : m;
-                const float keep = exp2f(m - top), weight = exp2f(score - top);
-                const float2 vv = load_pair(p.v + at, lane);
-                m = top;
-                l = l * keep + weight;
-                acc.x = acc.x * keep + weight * vv.x;
-                acc.y = acc.y * keep + weight * vv.y;
-            }
-            // No key at all gives zeros; keys that all weigh nothing give 0 / 0.
-            const float inv = visible > 0 ? 1.0f / l : 0.0f;
-            reinterpret_cast<__half2*>(p.o + row * p.o_stride + head * kHead)[lane] =
-                visible > 0 ? __floats2half2_rn(acc.x / l, acc.y / l) : __floats2half2_rn(inv, inv);
-            if (p.lse != nullptr && lane == 0) {
-                p.lse[static_cast<long long>(head) * p.rows + row] = l > 0.0f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
-            }
-        }
-    }
 }
 
 __device__ __forceinline__ float pair_dot(float2 a, float2 b) { return warp_sum(a.x * b.x + a.y * b.y); }
@@ -230,11 +144,10 @@ dim3 sequence_grid(const PackedArgs& p, int items_per_block, long long items, in
 }  // namespace
 
 cudaError_t packed_error_flag(int* value, bool reset) {
-    cudaError_t e = cudaMemcpyFromSymbol(value, g_packed_error, sizeof(int));
-    if (e == cudaSuccess && reset && *value != 0) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_packed_error, &zero, sizeof(int));
-    }
+    int here = 0, forward = 0;
+    cudaError_t e = read_error_word(&here, reset);
+    if (e == cudaSuccess) e = packed_forward_error_flag(&forward, reset);
+    *value = here != 0 || forward != 0 ? 1 : 0;
     return e;
 }
 
@@ -415,7 +328,7 @@ flint_status flint_b200_packed_attention_workspace(const flint_b200_packed_shape
     if (bytes == nullptr) {
         return fb::fail(kBad, "%s: bytes is null", name);
     }
-    *bytes = 16;
+    FB_CUDA(fb::packed_forward_workspace(bytes));
     return FLINT_OK;
 }
 
@@ -450,11 +363,7 @@ flint_status flint_b200_packed_attention_forward(void* o, void* lse, const void*
     p.o = static_cast<__half*>(o);
     p.lse = static_cast<float*>(lse);
     p.starts = static_cast<const int*>(starts);
-    int sms = 148;
-    FB_CUDA(fb::sm_count(&sms));
-    FB_CUDA(fb::launch_dependent(fb::fb_packed_forward_rows,
-                                 fb::sequence_grid(p, 8, static_cast<long long>(rows) * p.heads, sms), dim3(256), 0,
-                                 stream, p));
+    FB_CUDA(fb::packed_forward(p, workspace, stream));
     return FLINT_OK;
 }
 
@@ -553,7 +462,7 @@ flint_status flint_b200_paged_attention_workspace(const flint_b200_paged_shape* 
     if (bytes == nullptr) {
         return fb::fail(kBad, "%s: bytes is null", name);
     }
-    *bytes = 16;
+    FB_CUDA(fb::packed_forward_workspace(bytes));
     return FLINT_OK;
 }
 
@@ -591,11 +500,7 @@ flint_status flint_b200_paged_attention(void* o, void* lse, const void* q, const
     p.starts = static_cast<const int*>(starts);
     p.lengths = static_cast<const int*>(lengths);
     p.table = static_cast<const int*>(page_table);
-    int sms = 148;
-    FB_CUDA(fb::sm_count(&sms));
-    FB_CUDA(fb::launch_dependent(fb::fb_packed_forward_rows,
-                                 fb::sequence_grid(p, 8, static_cast<long long>(p.rows) * p.heads, sms), dim3(256), 0,
-                                 stream, p));
+    FB_CUDA(fb::packed_forward(p, workspace, stream));
     return FLINT_OK;
 }
 

@@ -33,7 +33,12 @@ struct PackedGradients {
     const __half* d_o;      // rows as o's
 };
 
-// Device error word of this file's kernels: a wait that gave up, or starts, lengths or page
+// Forward, over packed or paged keys; the workspace's size depends on the GPU only.
+cudaError_t packed_forward(const PackedArgs& args, void* workspace, cudaStream_t stream);
+cudaError_t packed_forward_workspace(size_t* bytes);
+cudaError_t packed_forward_error_flag(int* value, bool reset);
+
+// Device error words of these kernels: a wait that gave up, or starts, lengths or page
 // numbers outside their ranges (which are clamped, so that nothing outside is touched).
 cudaError_t packed_error_flag(int* value, bool reset);
 
