@@ -421,57 +421,53 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     break;
                 }
                 sm100::tc_fence_after_sync();
-                uint32_t raw[128];
+                // The scores are read twice, 32 columns at a time and the next 32 on their way: a row's
+                // 128 at once left no registers (the kernel spilled 950 bytes and took three times as long).
+                uint32_t raw[2][32];
+                const int visible = position - j * kKeyTile;     // columns up to this one are seen
+                const bool masked = j * kKeyTile + kKeyTile - 1 > piece.position();
+                float alpha = 1.0f;
+                bool moved = false;
                 if (active) {
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    sm100::tmem_ld_32x32(tmem_s + lane_base, raw[0]);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        sm100::tmem_ld_32x32(tmem_s + lane_base + 32 * c, reinterpret_cast<uint32_t(&)[32]>(raw[32 * c]));
-                    }
-                    sm100::tmem_ld_wait();
-                }
-                sm100::tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) {
-                    sm100::mbar_arrive(bar.s_free());
-                }
-                if (active) {
-                    if (j * kKeyTile + kKeyTile - 1 > piece.position()) {
-                        const int visible = position - j * kKeyTile;
+                        sm100::tmem_ld_wait();
+                        sm100::tmem_ld_32x32(tmem_s + lane_base + 32 * ((c + 1) % 4), raw[(c + 1) & 1]);
+                        uint32_t (&now)[32] = raw[c & 1];
+                        if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) {
-                            raw[i] = i <= visible ? raw[i] : 0xff800000u;
+                            for (int i = 0; i < 32; ++i) {
+                                now[i] = 32 * c + i <= visible ? now[i] : 0xff800000u;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                top[t] = max3_nan(top[t], __uint_as_float(now[i + t]), __uint_as_float(now[i + 4 + t]));
+                            }
                         }
                     }
-                    float top[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        top[t] = max3_nan(__uint_as_float(raw[t]), __uint_as_float(raw[4 + t]), __uint_as_float(raw[8 + t]));
-                    }
-#pragma unroll
-                    for (int i = 12; i < 124; i += 8) {
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            top[t] = max3_nan(top[t], __uint_as_float(raw[i + t]), __uint_as_float(raw[i + 4 + t]));
-                        }
-                    }
-                    const float local = max3_nan(max3_nan(top[0], top[1], top[2]),
-                                                 max3_nan(top[3], __uint_as_float(raw[124]), __uint_as_float(raw[125])),
-                                                 max3_nan(__uint_as_float(raw[126]), __uint_as_float(raw[127]),
-                                                          __uint_as_float(raw[127])));
-                    const float mx = max3_nan(m, local * scale2, kNoKey);
-                    const bool moved = valid && !(mx - m <= kLazyShift);   // (a NaN moves it too)
-                    float alpha = 1.0f;
+                    // The scale is positive, so the maximum may be scaled after it is taken.
+                    const float local = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale2;
+                    const float mx = max3_nan(m, local, local);
+                    moved = valid && !(mx - m <= kLazyShift);   // (a NaN moves it too)
                     if (moved) {
                         alpha = fast_exp2(m - mx);
                         m = mx;
                         l = f2_mul(l, f2_pack(alpha, alpha));
                     }
+                }
+                // O is complete up to the step before, and P's columns are free.
+                if (n > 0 && !sm100::mbar_wait_warp(bar.pv_done(), (n - 1) & 1, abort)) {
+                    ok = false;
+                    break;
+                }
+                sm100::tc_fence_after_sync();
+                if (active) {
                     if (j > piece.from && __any_sync(kFullMask, moved)) {
-                        if (!sm100::mbar_wait_warp(bar.pv_done(), (n - 1) & 1, abort)) {
-                            ok = false;
-                            break;
-                        }
-                        sm100::tc_fence_after_sync();
                         const F2 a2 = f2_pack(alpha, alpha);
 #pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
@@ -491,12 +487,30 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     const F2 shift = f2_pack(-m, -m);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
+                        sm100::tmem_ld_wait();
+                        if (c < 3) {
+                            sm100::tmem_ld_32x32(tmem_s + lane_base + 32 * (c + 1), raw[(c + 1) & 1]);
+                        } else {
+                            // All scores are read: the next step's may come.
+                            sm100::tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) {
+                                sm100::mbar_arrive(bar.s_free());
+                            }
+                        }
+                        uint32_t (&now)[32] = raw[c & 1];
+                        if (masked) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                now[i] = 32 * c + i <= visible ? now[i] : 0xff800000u;
+                            }
+                        }
                         uint32_t packed[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float x, y;
-                            const F2 t = f2_fma(f2_pack(__uint_as_float(raw[32 * c + 2 * i]),
-                                                        __uint_as_float(raw[32 * c + 2 * i + 1])), scale_pair, shift);
+                            const F2 t = f2_fma(f2_pack(__uint_as_float(now[2 * i]), __uint_as_float(now[2 * i + 1])),
+                                                scale_pair, shift);
                             if ((i & 3) == 0) {
                                 exp2_pair_fma(t, x, y);
                             } else {
@@ -507,23 +521,14 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             l = f2_add(l, f2_pack(x, y));
                             packed[i] = pack2(x, y);
                         }
-                        if (c == 0 && n > 0) {
-                            // P's columns are free once the step before has read them.
-                            if (!sm100::mbar_wait_warp(bar.pv_done(), (n - 1) & 1, abort)) {
-                                ok = false;
-                                break;
-                            }
-                            sm100::tc_fence_after_sync();
-                        }
                         sm100::tmem_st_32x16(tmem_p + lane_base + c * 16, packed);
                     }
-                    if (!ok) {
-                        break;
-                    }
                     sm100::tmem_st_wait();
-                } else if (n > 0 && !sm100::mbar_wait_warp(bar.pv_done(), (n - 1) & 1, abort)) {
-                    ok = false;
-                    break;
+                } else {
+                    __syncwarp();
+                    if (lane == 0) {
+                        sm100::mbar_arrive(bar.s_free());
+                    }
                 }
                 sm100::tc_fence_before_sync();
                 __syncwarp();
@@ -547,32 +552,28 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             float* part = p.parts + (2 * size_t{blockIdx.x} + (piece.from == 0 ? 1 : 0)) * kPartFloats;
             const float inv = position < 0 ? 0.0f : 1.0f / total;   // no key at all gives zeros
             __half* out = p.a.o + at_row * p.a.o_stride + head * kHead;
+            uint32_t acc[64];
+            if (active) {
+                sm100::tmem_ld_32x32(tmem_o + lane_base, reinterpret_cast<uint32_t(&)[32]>(acc[0]));
+                sm100::tmem_ld_32x32(tmem_o + lane_base + 32, reinterpret_cast<uint32_t(&)[32]>(acc[32]));
+                sm100::tmem_ld_wait();
+            }
+            if (valid && whole) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t acc[32];
-                if (active) {
-                    sm100::tmem_ld_32x32(tmem_o + lane_base + 32 * c, acc);
-                    sm100::tmem_ld_wait();
-                }
-                if (!valid) {
-                    continue;
-                }
-                if (whole) {
+                for (int b = 0; b < 8; ++b) {
+                    float v[8];
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            v[i] = position < 0 ? 0.0f : __uint_as_float(acc[b * 8 + i]) * inv;
-                        }
-                        *reinterpret_cast<uint4*>(out + 32 * c + 8 * b) = pack8(v);
+                    for (int i = 0; i < 8; ++i) {
+                        v[i] = position < 0 ? 0.0f : __uint_as_float(acc[b * 8 + i]) * inv;
                     }
-                } else {
+                    *reinterpret_cast<uint4*>(out + 8 * b) = pack8(v);
+                }
+            }
+            if (valid && !whole) {
 #pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        reinterpret_cast<uint4*>(part)[(8 * c + b) * kRows + row] =
-                            make_uint4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
-                    }
+                for (int b = 0; b < 16; ++b) {
+                    reinterpret_cast<uint4*>(part)[b * kRows + row] =
+                        make_uint4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
                 }
             }
             sm100::tc_fence_before_sync();
