@@ -10,98 +10,12 @@
 #include "device_utils.cuh"
 #include "flint/flint_b200.h"
 #include "packed.cuh"
+#include "packed_maps.h"
 
 namespace fb {
 namespace {
 
 constexpr int kHead = 64;
-constexpr float kLog2e = 1.4426950408889634f;
-
-// Where the row of 64 values of a key (in K or V) begins; negative for a page that is not there.
-__device__ __forceinline__ long long key_offset(const PackedArgs& p, const Sequence& q, int s, int key,
-                                                int kv_head) {
-    if (p.table == nullptr) {
-        return (q.first + static_cast<long long>(key)) * p.kv_stride + kv_head * kHead;
-    }
-    const long long page = page_of(p, s, key);
-    return page < 0 ? -1 : ((page * p.kv_heads + kv_head) * p.page_size + key % p.page_size) * kHead;
-}
-
-__device__ __forceinline__ float2 load_pair(const __half* row, int lane) {
-    return __half22float2(reinterpret_cast<const __half2*>(row)[lane]);
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        v += __shfl_xor_sync(fb::kFullMask, v, off);
-    }
-    return v;
-}
-
-__device__ __forceinline__ float pair_dot(float2 a, float2 b) { return warp_sum(a.x * b.x + a.y * b.y); }
-
-// One warp per (token, head) for dq, then one per (token, K/V head) for dk and dv.
-__global__ void __launch_bounds__(256) fb_packed_backward_rows(const PackedArgs p, const PackedGradients g) {
-    fb::dependency_wait();
-    fb::dependency_release();
-    const int lane = threadIdx.x % 32;
-    const int warp = blockIdx.x * 8 + threadIdx.x / 32;
-    const int warps = gridDim.x * 8;
-    const int group = p.heads / p.kv_heads;
-    const float scale2 = p.scale * kLog2e;
-    for (int s = blockIdx.y; s < p.sequences; s += gridDim.y) {
-        const Sequence q = sequence_at(p, s);
-        auto delta_of = [&](long long row, int head, float2 grad) {
-            return pair_dot(grad, load_pair(p.o + row * p.o_stride + head * kHead, lane));
-        };
-        const long long queries = static_cast<long long>(q.count) * p.heads;
-        const long long keys = static_cast<long long>(q.count) * p.kv_heads;
-        for (long long item = warp; item < queries + keys; item += warps) {
-            if (item < queries) {
-                const int i = static_cast<int>(item / p.heads), head = static_cast<int>(item % p.heads);
-                const long long row = q.first + i;
-                const float2 x = load_pair(p.q + row * p.q_stride + head * kHead, lane);
-                const float2 grad = load_pair(g.d_o + row * p.o_stride + head * kHead, lane);
-                const float delta = delta_of(row, head, grad);
-                const float lse2 = p.lse[static_cast<long long>(head) * p.rows + row] * kLog2e;
-                float2 dq = make_float2(0.0f, 0.0f);
-                for (int key = 0; key <= i; ++key) {
-                    const long long at = key_offset(p, q, s, key, head / group);
-                    const float2 kk = load_pair(p.k + at, lane);
-                    const float weight = exp2f(pair_dot(x, kk) * scale2 - lse2);
-                    const float ds = weight * (pair_dot(grad, load_pair(p.v + at, lane)) - delta) * p.scale;
-                    dq.x += ds * kk.x;
-                    dq.y += ds * kk.y;
-                }
-                reinterpret_cast<__half2*>(g.dq + row * p.q_stride + head * kHead)[lane] =
-                    __floats2half2_rn(dq.x, dq.y);
-            } else {
-                const long long which = item - queries;
-                const int j = static_cast<int>(which / p.kv_heads), kv_head = static_cast<int>(which % p.kv_heads);
-                const long long at = key_offset(p, q, s, j, kv_head);
-                const float2 kk = load_pair(p.k + at, lane), vv = load_pair(p.v + at, lane);
-                float2 dk = make_float2(0.0f, 0.0f), dv = dk;
-                for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
-                    for (int i = j; i < q.count; ++i) {
-                        const long long row = q.first + i;
-                        const float2 x = load_pair(p.q + row * p.q_stride + head * kHead, lane);
-                        const float2 grad = load_pair(g.d_o + row * p.o_stride + head * kHead, lane);
-                        const float lse2 = p.lse[static_cast<long long>(head) * p.rows + row] * kLog2e;
-                        const float weight = exp2f(pair_dot(x, kk) * scale2 - lse2);
-                        const float ds = weight * (pair_dot(grad, vv) - delta_of(row, head, grad)) * p.scale;
-                        dv.x += weight * grad.x;
-                        dv.y += weight * grad.y;
-                        dk.x += ds * x.x;
-                        dk.y += ds * x.y;
-                    }
-                }
-                reinterpret_cast<__half2*>(g.dk + at)[lane] = __floats2half2_rn(dk.x, dk.y);
-                reinterpret_cast<__half2*>(g.dv + at)[lane] = __floats2half2_rn(dv.x, dv.y);
-            }
-        }
-    }
-}
 
 // Copies the new tokens' keys and values into their pages: eight lanes per row of 64 values.
 __global__ void __launch_bounds__(256)
@@ -143,11 +57,71 @@ dim3 sequence_grid(const PackedArgs& p, int items_per_block, long long items, in
 
 }  // namespace
 
+namespace {
+
+constexpr unsigned kHeadWidth = 64;
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+cudaError_t encode_fn(EncodeTiled* out) {
+    static std::atomic<EncodeTiled> cached{nullptr};
+    EncodeTiled found = cached.load(std::memory_order_relaxed);
+    if (found == nullptr) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult status;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &status);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        if (status != cudaDriverEntryPointSuccess || fn == nullptr) {
+            return cudaErrorNotSupported;
+        }
+        found = reinterpret_cast<EncodeTiled>(fn);
+        cached.store(found, std::memory_order_relaxed);
+    }
+    *out = found;
+    return cudaSuccess;
+}
+
+cudaError_t encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                   const cuuint32_t* box) {
+    EncodeTiled fn = nullptr;
+    const cudaError_t e = encode_fn(&fn);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
+                          dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t encode_rows(CUtensorMap* map, const __half* base, int heads, int rows, long long stride, int box_heads,
+                        int box_rows) {
+    const cuuint64_t dims[3] = {kHeadWidth, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[2] = {kHeadWidth * 2, static_cast<cuuint64_t>(stride) * 2};
+    const cuuint32_t box[3] = {kHeadWidth, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+    return encode(map, base, 3, dims, strides, box);
+}
+
+cudaError_t encode_pages(CUtensorMap* map, const __half* base, long long rows, int box_rows) {
+    const cuuint64_t dims[2] = {kHeadWidth, static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {kHeadWidth * 2};
+    const cuuint32_t box[2] = {kHeadWidth, static_cast<cuuint32_t>(box_rows)};
+    return encode(map, base, 2, dims, strides, box);
+}
+
 cudaError_t packed_error_flag(int* value, bool reset) {
-    int here = 0, forward = 0;
+    int here = 0, forward = 0, backward = 0;
     cudaError_t e = read_error_word(&here, reset);
     if (e == cudaSuccess) e = packed_forward_error_flag(&forward, reset);
-    *value = here != 0 || forward != 0 ? 1 : 0;
+    if (e == cudaSuccess) e = packed_backward_error_flag(&backward, reset);
+    *value = here != 0 || forward != 0 || backward != 0 ? 1 : 0;
     return e;
 }
 
@@ -373,7 +347,7 @@ flint_status flint_b200_packed_attention_backward_workspace(const flint_b200_pac
     if (bytes == nullptr) {
         return fb::fail(kBad, "%s: bytes is null", name);
     }
-    *bytes = 16;
+    *bytes = fb::packed_backward_workspace(shape->sequences, shape->rows, shape->heads);
     return FLINT_OK;
 }
 
@@ -415,11 +389,7 @@ flint_status flint_b200_packed_attention_backward(void* dq, void* dk, void* dv, 
     p.starts = static_cast<const int*>(starts);
     const fb::PackedGradients g{static_cast<__half*>(dq), static_cast<__half*>(dk), static_cast<__half*>(dv),
                                 static_cast<const __half*>(d_o)};
-    int sms = 148;
-    FB_CUDA(fb::sm_count(&sms));
-    FB_CUDA(fb::launch_dependent(fb::fb_packed_backward_rows,
-                                 fb::sequence_grid(p, 8, static_cast<long long>(rows) * (p.heads + p.kv_heads), sms),
-                                 dim3(256), 0, stream, p, g));
+    FB_CUDA(fb::packed_backward(p, g, workspace, stream));
     return FLINT_OK;
 }
 

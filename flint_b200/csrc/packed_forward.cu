@@ -25,6 +25,7 @@
 #include "common.h"
 #include "device_utils.cuh"
 #include "packed.cuh"
+#include "packed_maps.h"
 #include "sm100.cuh"
 #include "softmax.cuh"
 
@@ -676,60 +677,6 @@ __global__ void __launch_bounds__(256) fb_packed_join(const JoinParams p) {
 }
 
 // ---- host -------------------------------------------------------------------------------------------
-
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-cudaError_t encode_fn(EncodeTiled* out) {
-    static std::atomic<EncodeTiled> cached{nullptr};
-    EncodeTiled found = cached.load(std::memory_order_relaxed);
-    if (found == nullptr) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult status;
-        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &status);
-        if (e != cudaSuccess) {
-            return e;
-        }
-        if (status != cudaDriverEntryPointSuccess || fn == nullptr) {
-            return cudaErrorNotSupported;
-        }
-        found = reinterpret_cast<EncodeTiled>(fn);
-        cached.store(found, std::memory_order_relaxed);
-    }
-    *out = found;
-    return cudaSuccess;
-}
-
-cudaError_t encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
-                   const cuuint32_t* box) {
-    EncodeTiled fn = nullptr;
-    const cudaError_t e = encode_fn(&fn);
-    if (e != cudaSuccess) {
-        return e;
-    }
-    const cuuint32_t step[3] = {1, 1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
-                          dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
-// (column, head, row) of a matrix of token rows, boxes of `box_heads` heads of `box_rows` rows.
-cudaError_t encode_rows(CUtensorMap* map, const __half* base, int heads, int rows, long long stride, int box_heads,
-                        int box_rows) {
-    const cuuint64_t dims[3] = {kHead, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[2] = {kHead * 2, static_cast<cuuint64_t>(stride) * 2};
-    const cuuint32_t box[3] = {kHead, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
-    return encode(map, base, 3, dims, strides, box);
-}
-
-cudaError_t encode_pages(CUtensorMap* map, const __half* base, long long rows, int box_rows) {
-    const cuuint64_t dims[2] = {kHead, static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {kHead * 2};
-    const cuuint32_t box[2] = {kHead, static_cast<cuuint32_t>(box_rows)};
-    return encode(map, base, 2, dims, strides, box);
-}
 
 size_t records_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(Record) + 255) / 256 * 256; }
 
