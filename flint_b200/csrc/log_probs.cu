@@ -11,12 +11,18 @@
 #include "common.h"
 #include "device_utils.cuh"
 #include "flint/flint_b200.h"
+#include "sm100.cuh"
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kMostTop = 32;
+constexpr int kBins = 32;            // parts of a slice whose maxima bound the alternatives from below
+constexpr int kCandidates = 512;
+constexpr int kMostRanks = 8;        // CTAs of a cluster
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -200.0f;   // e^-200 is 0 in FP32, and 0 * -200 a number
+
+using Key = unsigned long long;
 
 struct LogProbArgs {
     float* log_probs;
@@ -28,99 +34,413 @@ struct LogProbArgs {
     const uint16_t* targets;
     size_t rows;
     int vocab, cols, top;
+    int slice;      // 16-byte words per CTA of a cluster
+    int ranks;      // CTAs of a cluster
 };
 
-__device__ __forceinline__ float value_at(const float* row, int c) { return row[c]; }
-__device__ __forceinline__ float value_at(const __half* row, int c) { return __half2float(row[c]); }
+// Eight FP16 or four FP32 logits: a 16-byte word.
+template <typename T>
+struct Word {
+    static constexpr int kValues = 16 / sizeof(T);
+    __device__ static float value(const T* row, int c);
+    __device__ static void unpack(float (&v)[kValues], const uint4& q);
+    __device__ static uint4 pack(const float (&v)[kValues]);
+};
+template <>
+__device__ __forceinline__ float Word<float>::value(const float* row, int c) {
+    return row[c];
+}
+template <>
+__device__ __forceinline__ float Word<__half>::value(const __half* row, int c) {
+    return __half2float(row[c]);
+}
+template <>
+__device__ __forceinline__ void Word<float>::unpack(float (&v)[4], const uint4& q) {
+    v[0] = __uint_as_float(q.x);
+    v[1] = __uint_as_float(q.y);
+    v[2] = __uint_as_float(q.z);
+    v[3] = __uint_as_float(q.w);
+}
+template <>
+__device__ __forceinline__ void Word<__half>::unpack(float (&v)[8], const uint4& q) {
+    fb::unpack8(v, q);
+}
+template <>
+__device__ __forceinline__ uint4 Word<float>::pack(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <>
+__device__ __forceinline__ uint4 Word<__half>::pack(const float (&v)[8]) {
+    return fb::pack8(v);
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The largest value of a word; a NaN among them gives NaN.
+__device__ __forceinline__ float word_max(const uint4& q, float) {
+    return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)),
+                   max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+__device__ __forceinline__ float word_max(const uint4& q, __half) {
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
+}
+
+// A word's values from the `count`-th on become minus infinity, which counts for nothing.
+__device__ __forceinline__ void cut_word(uint4& q, int count, float) {
+    unsigned* w = reinterpret_cast<unsigned*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = i < count ? w[i] : 0xff800000u;
+    }
+}
+__device__ __forceinline__ void cut_word(uint4& q, int count, __half) {
+    unsigned* w = reinterpret_cast<unsigned*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = 2 * i >= count ? 0xfc00fc00u : 2 * i + 1 >= count ? (w[i] & 0xffffu) | 0xfc000000u : w[i];
+    }
+}
 
 // A number that orders logits by value (both zeros alike, NaN above all) and equal ones by place,
-// the lowest first. No two columns have the same.
-__device__ __forceinline__ unsigned long long order_key(float v, int column) {
+// the lowest first. No two columns have the same; none has 0.
+__device__ __forceinline__ Key order_key(float v, int column) {
     const unsigned bits = __float_as_uint(__fadd_rn(v, 0.0f));
     const unsigned ordered = v != v ? 0xffffffffu : (bits & 0x80000000u) != 0 ? ~bits : bits | 0x80000000u;
-    return (static_cast<unsigned long long>(ordered) << 32) | (0xffffffffu - static_cast<unsigned>(column));
+    return (static_cast<Key>(ordered) << 32) | (0xffffffffu - static_cast<unsigned>(column));
+}
+__device__ __forceinline__ int key_column(Key key) {
+    return static_cast<int>(0xffffffffu - static_cast<unsigned>(key));
+}
+__device__ __forceinline__ float key_value(Key key) {
+    const unsigned ordered = static_cast<unsigned>(key >> 32);
+    return __uint_as_float((ordered & 0x80000000u) != 0 ? ordered ^ 0x80000000u : ~ordered);
 }
 
-__device__ __forceinline__ float combine(float a, float b) { return a + b; }
-__device__ __forceinline__ unsigned long long combine(unsigned long long a, unsigned long long b) {
-    return a > b ? a : b;
+__device__ __forceinline__ float fast_exp(float d) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * kLog2e));
+    return y;
 }
 
-// The block's sum (float) or maximum (keys), for every thread.
-template <typename Value>
-__device__ Value block_reduce(Value v, Value* scratch) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        v = combine(v, __shfl_xor_sync(fb::kFullMask, v, off));
-    }
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) {
-        scratch[threadIdx.x / 32] = v;
-    }
-    __syncthreads();
-    v = scratch[threadIdx.x % (kThreads / 32)];
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) {
-        v = combine(v, __shfl_xor_sync(fb::kFullMask, v, off));
-    }
-    return v;
-}
+// ---- forward ---------------------------------------------------------------------------------------
+//
+// With m the row's largest logit, d = x - m and S = sum e^d, D = sum d e^d:
+//   lse = m + log S,  log p = d - log S,  entropy = log S - D / S   (all terms of one sign: nothing cancels)
+// A thread holds its words of the row in registers: one pass finds the maxima, the second takes
+// the exponentials while it asks for the next row's words, so that memory never waits. Long
+// rows, and few of them, are divided over a cluster's CTAs: each takes sums against its own maximum, and the
+// first puts them together.
+// The alternatives: the slice falls into 32 bins of neighbouring lanes. The k-th largest of the bins' maxima
+// is a lower bound of the k-th largest logit; what is not below it (about k values) is collected in the
+// second pass and put in order by counting. Where too many qualify (rows of equal logits), or a NaN is among
+// them, the row is gone through once per alternative.
+constexpr int blocks_per_sm(int threads, int held) { return (threads == 128 ? 4 : 1) * (held > 4 ? 1 : 2); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) fb_token_log_probs_rows(const LogProbArgs p) {
-    __shared__ float sums[kThreads / 32];
-    __shared__ unsigned long long keys[kThreads / 32];
+template <typename T, int kThreads, int kHeld>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_token_log_probs(const LogProbArgs p) {
+    using W = Word<T>;
+    constexpr int kWarps = kThreads / 32;
+    constexpr int kLanes = kThreads / kBins;      // of a bin
+    __shared__ float bins[2][kBins];
+    __shared__ float maxima[2][kWarps];
+    __shared__ float sums[2][2 * kWarps];
+    __shared__ Key reduced[kWarps];
+    __shared__ int counts[2];
+    __shared__ Key candidates[2][kCandidates];
+    __shared__ float parts[2][kMostRanks][3];     // the first CTA's: every CTA's m, S, D
+    __shared__ Key best[2][kMostRanks * kMostTop];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
+    const int rank = p.ranks > 1 ? static_cast<int>(sm100::cluster_cta_rank()) : 0;
+    const size_t stride = gridDim.x / p.ranks;
+    const int row_words = p.cols / W::kValues;
+    const int all_words = (p.vocab + W::kValues - 1) / W::kValues;
+    const int first_word = rank * p.slice;
+    const int words = max(0, min(p.slice, all_words - first_word));
+    const int last_word = all_words - 1 - first_word;     // of the row, counted from the slice's first
+    const int last_count = p.vocab - (all_words - 1) * W::kValues;
+    const int top = p.top;
+
+    if (tid < 2) {
+        counts[tid] = 0;
+    }
     fb::dependency_wait();
-    fb::dependency_release();
-    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T* x = static_cast<const T*>(p.logits) + row * p.cols;
-        unsigned long long best = 0;
-        for (int c = threadIdx.x; c < p.vocab; c += kThreads) {
-            best = combine(best, order_key(value_at(x, c), c));
+    if (p.ranks > 1) {
+        sm100::cluster_sync_all();    // every CTA of the cluster runs before any writes to the first one's memory
+    } else {
+        __syncthreads();
+    }
+    if (tid == 0) {
+        fb::dependency_release();
+    }
+    auto row_of = [&](size_t row) { return static_cast<const uint4*>(p.logits) + row * row_words + first_word; };
+    size_t row = blockIdx.x / p.ranks;
+    if (row >= p.rows) {
+        return;     // (the whole cluster)
+    }
+    uint4 held[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int i = tid + j * kThreads;
+        if (i < words) {
+            held[j] = fb::load_input(row_of(row) + i);
         }
-        best = block_reduce(best, keys);
-        const float top = value_at(x, static_cast<int>(0xffffffffu - static_cast<unsigned>(best)));
-        float total = 0.0f, weighted = 0.0f;
-        for (int c = threadIdx.x; c < p.vocab && top != -INFINITY; c += kThreads) {
-            const float d = value_at(x, c) - top;
-            const float e = expf(d);
-            total += e;
-            weighted += e * (d < kLowest ? kLowest : d);
+    }
+    for (int parity = 0; row < p.rows; row += stride, parity ^= 1) {
+        const T* values = static_cast<const T*>(p.logits) + row * p.cols;
+        const size_t next = row + stride;
+        if (tid == 0 && next + stride < p.rows && words > 0) {
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row_of(next + stride)),
+                         "r"(static_cast<uint32_t>(words) * 16u)
+                         : "memory");
         }
-        total = block_reduce(total, sums);
-        weighted = block_reduce(weighted, sums);
-        const float log_total = logf(total);
-        const bool none = top == -INFINITY;
-        auto log_prob = [&](float v) { return none ? -INFINITY : (v - top) - log_total; };
-        if (threadIdx.x == 0) {
+        const int target = p.targets != nullptr && tid == 0 && rank == 0 ? p.targets[row] : 0;
+        const float target_value = tid == 0 && rank == 0 && target < p.vocab ? W::value(values, target) : 0.0f;
+
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = tid + j * kThreads;
+            if (i < words) {
+                if (i == last_word && last_count < W::kValues) {
+                    cut_word(held[j], last_count, T());
+                }
+                mx = max_nan(mx, word_max(held[j], T()));
+            }
+        }
+#pragma unroll
+        for (int off = 1; off < kLanes; off <<= 1) {
+            mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
+        }
+        if (tid % kLanes == 0) {
+            bins[parity][tid / kLanes] = mx;
+        }
+#pragma unroll
+        for (int off = kLanes; off < 32; off <<= 1) {
+            mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
+        }
+        if (lane == 0) {
+            maxima[parity][warp] = mx;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            counts[parity ^ 1] = 0;     // (of the row before, which everybody is done with)
+        }
+        mx = maxima[parity][lane % kWarps];
+#pragma unroll
+        for (int off = 1; off < kWarps; off <<= 1) {
+            mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
+        }
+        // Whether a value can be among the `top` largest of the slice.
+        float bound = INFINITY;
+        if (top > 0) {
+            const float mine = bins[parity][lane];
+            int larger = 0;
+#pragma unroll
+            for (int off = 1; off < 32; ++off) {
+                const int other_lane = (lane + off) % 32;
+                const float other = __shfl_sync(fb::kFullMask, mine, other_lane);
+                larger += other > mine || (other == mine && other_lane < lane) ? 1 : 0;
+            }
+            const unsigned holds = __ballot_sync(fb::kFullMask, larger == top - 1);
+            bound = __shfl_sync(fb::kFullMask, mine, holds != 0 ? __ffs(holds) - 1 : 0);
+        }
+
+        fb::F2 sum[2] = {0, 0}, weighted[2] = {0, 0};
+        const fb::F2 mx2 = fb::f2_pack(mx, mx), log2e = fb::f2_pack(kLog2e, kLog2e);
+        const bool none = mx == -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = tid + j * kThreads;
+            if (i < words) {
+                float v[W::kValues];
+                W::unpack(v, held[j]);
+                if (top > 0 && word_max(held[j], T()) >= bound) {
+#pragma unroll
+                    for (int c = 0; c < W::kValues; ++c) {
+                        if (v[c] >= bound && v[c] > -INFINITY) {
+                            const int at = atomicAdd(&counts[parity], 1);
+                            if (at < kCandidates) {
+                                candidates[parity][at] = order_key(v[c], (first_word + i) * W::kValues + c);
+                            }
+                        }
+                    }
+                }
+                if (next < p.rows) {
+                    held[j] = fb::load_input(row_of(next) + i);
+                }
+#pragma unroll
+                for (int c = 0; c < W::kValues; c += 2) {
+                    float y0, y1, e0, e1;
+                    fb::f2_unpack(fb::f2_sub(fb::f2_pack(v[c], v[c + 1]), mx2), y0, y1);
+                    const fb::F2 d = fb::f2_pack(max_nan(y0, kLowest), max_nan(y1, kLowest));
+                    fb::f2_unpack(fb::f2_mul(d, log2e), y0, y1);
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
+                    const fb::F2 e = fb::f2_pack(e0, e1);
+                    sum[c / 2 % 2] = fb::f2_add(sum[c / 2 % 2], e);
+                    weighted[c / 2 % 2] = fb::f2_fma(e, d, weighted[c / 2 % 2]);
+                }
+            }
+        }
+        float a, b, total, mean;
+        fb::f2_unpack(fb::f2_add(sum[0], sum[1]), a, b);
+        total = a + b;
+        fb::f2_unpack(fb::f2_add(weighted[0], weighted[1]), a, b);
+        mean = a + b;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            total += __shfl_xor_sync(fb::kFullMask, total, off);
+            mean += __shfl_xor_sync(fb::kFullMask, mean, off);
+        }
+        if (lane == 0) {
+            sums[parity][2 * warp] = total;
+            sums[parity][2 * warp + 1] = mean;
+        }
+        __syncthreads();
+        total = sums[parity][2 * (lane % kWarps)];
+        mean = sums[parity][2 * (lane % kWarps) + 1];
+#pragma unroll
+        for (int off = 1; off < kWarps; off <<= 1) {
+            total += __shfl_xor_sync(fb::kFullMask, total, off);
+            mean += __shfl_xor_sync(fb::kFullMask, mean, off);
+        }
+        if (none) {
+            total = mean = 0.0f;
+        }
+        float log_total = logf(total);
+        auto log_prob = [&](float v) { return mx == -INFINITY ? -INFINITY : (v - mx) - log_total; };
+        auto emit = [&](int place, Key key) {
+            p.top_tokens[row * top + place] = static_cast<uint16_t>(key_column(key));
+            p.top_log_probs[row * top + place] = log_prob(key_value(key));
+        };
+        // The slice's `top` largest: written out, or into the first CTA's memory.
+        auto place_key = [&](int place, Key key) {
+            if (p.ranks == 1) {
+                emit(place, key);
+            } else {
+                const uint32_t to = sm100::map_to_cta(sm100::smem_u32(&best[parity][rank * kMostTop + place]), 0);
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
+            }
+        };
+        if (top > 0) {
+            const int found = counts[parity];
+            if (found <= kCandidates && mx == mx) {
+                for (int c = tid; c < found; c += kThreads) {
+                    const Key key = candidates[parity][c];
+                    int larger = 0;
+                    for (int other = 0; other < found; ++other) {
+                        larger += candidates[parity][other] > key ? 1 : 0;
+                    }
+                    if (larger < top) {
+                        place_key(larger, key);
+                    }
+                }
+                if (found < top && warp == 0) {
+                    // Fewer than that are above minus infinity: the first columns that are not.
+                    int place = found;
+                    const int end = min((first_word + words) * W::kValues, p.vocab);
+                    for (int c = first_word * W::kValues; place < top && c < end; c += 32) {
+                        const bool mine = c + lane < end && W::value(values, c + lane) == -INFINITY;
+                        const unsigned those = __ballot_sync(fb::kFullMask, mine);
+                        const int at = place + __popc(those & ((1u << lane) - 1));
+                        if (mine && at < top) {
+                            place_key(at, order_key(-INFINITY, c + lane));
+                        }
+                        place += __popc(those);
+                    }
+                    for (int at = place + lane; at < top; at += 32) {
+                        place_key(at, 0);     // (the slice has no more columns; another CTA's has)
+                    }
+                }
+            } else {
+                Key before = ~Key{0};
+                for (int k = 0; k < top; ++k) {
+                    Key mine = 0;
+                    const int end = min((first_word + words) * W::kValues, p.vocab);
+                    for (int c = first_word * W::kValues + tid; c < end; c += kThreads) {
+                        const Key key = order_key(W::value(values, c), c);
+                        mine = key < before && key > mine ? key : mine;
+                    }
+#pragma unroll
+                    for (int off = 16; off > 0; off >>= 1) {
+                        const Key other = __shfl_xor_sync(fb::kFullMask, mine, off);
+                        mine = other > mine ? other : mine;
+                    }
+                    __syncthreads();
+                    if (lane == 0) {
+                        reduced[warp] = mine;
+                    }
+                    __syncthreads();
+                    for (int w = 0; w < kWarps; ++w) {
+                        mine = reduced[w] > mine ? reduced[w] : mine;
+                    }
+                    before = mine;
+                    if (tid == 0) {
+                        place_key(k, mine);
+                    }
+                }
+            }
+        }
+        if (p.ranks > 1) {
+            if (tid == 0) {
+                const float mine[3] = {mx, total, mean};
+                for (int i = 0; i < 3; ++i) {
+                    const uint32_t to = sm100::map_to_cta(sm100::smem_u32(&parts[parity][rank][i]), 0);
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(mine[i]) : "memory");
+                }
+            }
+            sm100::cluster_sync_all();
+            if (rank != 0) {
+                continue;
+            }
+            mx = -INFINITY;
+            for (int r = 0; r < p.ranks; ++r) {
+                mx = max_nan(mx, parts[parity][r][0]);
+            }
+            total = mean = 0.0f;
+            for (int r = 0; r < p.ranks; ++r) {
+                const float m = parts[parity][r][0];
+                if (m != -INFINITY) {
+                    const float shift = max_nan(m - mx, kLowest), weight = expf(shift);
+                    total = fmaf(weight, parts[parity][r][1], total);
+                    mean = fmaf(weight, fmaf(parts[parity][r][1], shift, parts[parity][r][2]), mean);
+                }
+            }
+            log_total = logf(total);
+            for (int c = tid; c < p.ranks * top; c += kThreads) {
+                const Key key = best[parity][c / top * kMostTop + c % top];
+                int larger = 0;
+                for (int r = 0; r < p.ranks; ++r) {
+                    for (int k = 0; k < top; ++k) {
+                        larger += best[parity][r * kMostTop + k] > key ? 1 : 0;
+                    }
+                }
+                if (key != 0 && larger < top) {
+                    emit(larger, key);
+                }
+            }
+        }
+        if (tid == 0) {
             if (p.log_probs != nullptr) {
-                const int target = p.targets[row];
-                p.log_probs[row] = target < p.vocab ? log_prob(value_at(x, target)) : 0.0f;
+                p.log_probs[row] = target < p.vocab ? log_prob(target_value) : 0.0f;
             }
             if (p.entropy != nullptr) {
-                p.entropy[row] = none ? 0.0f : log_total - weighted / total;
+                p.entropy[row] = mx == -INFINITY ? 0.0f : log_total - mean / total;
             }
             if (p.lse != nullptr) {
-                p.lse[row] = none ? -INFINITY : top + log_total;
-            }
-        }
-        for (int k = 0; k < p.top; ++k) {
-            const int column = static_cast<int>(0xffffffffu - static_cast<unsigned>(best));
-            if (threadIdx.x == 0) {
-                p.top_tokens[row * p.top + k] = static_cast<uint16_t>(column);
-                p.top_log_probs[row * p.top + k] = log_prob(value_at(x, column));
-            }
-            if (k + 1 < p.top) {
-                unsigned long long next = 0;
-                for (int c = threadIdx.x; c < p.vocab; c += kThreads) {
-                    const unsigned long long key = order_key(value_at(x, c), c);
-                    next = key < best ? combine(next, key) : next;
-                }
-                best = block_reduce(next, keys);
+                p.lse[row] = mx == -INFINITY ? -INFINITY : mx + log_total;
             }
         }
     }
 }
+
+// ---- backward --------------------------------------------------------------------------------------
 
 struct LogProbGradientArgs {
     void* dlogits;
@@ -132,32 +452,113 @@ struct LogProbGradientArgs {
     const float* d_entropy;
     size_t rows;
     int vocab, cols;
+    int chunk;          // words of a row, or of several rows, that a block takes at a time
+    int row_chunks;     // chunks of a row; 1 where a block takes several rows
+    int chunk_rows;     // rows that a block takes at a time
 };
 
-__device__ __forceinline__ void store_value(float* row, int c, float v) { row[c] = v; }
-__device__ __forceinline__ void store_value(__half* row, int c, float v) { row[c] = __float2half_rn(v); }
+// dx_c = a ([c = target] - p_c) - b p_c (log p_c + entropy) with log p_c = x_c - lse: one pass, bound by what it
+// reads and writes. A thread has four 16-byte words on their way at a time.
+constexpr int kGradientThreads = 512;
+constexpr int kGradientWords = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) fb_token_log_probs_backward_rows(const LogProbGradientArgs p) {
+__global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(const LogProbGradientArgs p) {
+    using W = Word<T>;
     fb::dependency_wait();
     fb::dependency_release();
-    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T* x = static_cast<const T*>(p.logits) + row * p.cols;
-        T* out = static_cast<T*>(p.dlogits) + row * p.cols;
-        const int target = p.targets != nullptr ? p.targets[row] : p.vocab;
-        const float a = p.d_log_probs != nullptr && target < p.vocab ? p.d_log_probs[row] : 0.0f;
-        const float b = p.d_entropy != nullptr ? p.d_entropy[row] : 0.0f;
-        const float lse = p.lse[row], entropy = p.d_entropy != nullptr ? p.entropy[row] : 0.0f;
-        for (int c = threadIdx.x; c < p.cols; c += kThreads) {
-            float grad = 0.0f;
-            if (c < p.vocab && lse != -INFINITY) {
-                const float d = value_at(x, c) - lse;
-                const float e = expf(d);
-                grad = (c == target ? a : 0.0f) - e * (a + b * ((d < kLowest ? kLowest : d) + entropy));
+    const int row_words = p.cols / W::kValues;
+    const int read_words = (p.vocab + W::kValues - 1) / W::kValues;
+    const size_t groups = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
+    for (size_t item = blockIdx.x; item < groups * p.row_chunks; item += gridDim.x) {
+        const size_t first_row = item / p.row_chunks * p.chunk_rows;
+        const int first_word = static_cast<int>(item % p.row_chunks) * p.chunk;
+        const int here = p.row_chunks > 1 ? min(p.chunk, row_words - first_word)
+                                          : static_cast<int>(min(static_cast<size_t>(p.chunk_rows), p.rows - first_row)) *
+                                                row_words;
+        uint4 held[kGradientWords];
+        size_t rows[kGradientWords];
+        int at[kGradientWords];
+#pragma unroll
+        for (int j = 0; j < kGradientWords; ++j) {
+            const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
+            const int r = p.row_chunks > 1 ? 0 : i / row_words;
+            rows[j] = first_row + r;
+            at[j] = first_word + i - r * row_words;
+            held[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < here && at[j] < read_words) {
+                held[j] = fb::load_input(static_cast<const uint4*>(p.logits) + rows[j] * row_words + at[j]);
             }
-            store_value(out, c, grad);
+        }
+#pragma unroll
+        for (int j = 0; j < kGradientWords; ++j) {
+            if (static_cast<int>(threadIdx.x) + j * kGradientThreads >= here) {
+                continue;
+            }
+            const size_t row = rows[j];
+            const int target = p.targets != nullptr ? p.targets[row] : p.vocab;
+            const float a = p.d_log_probs != nullptr && target < p.vocab ? p.d_log_probs[row] : 0.0f;
+            const float b = p.d_entropy != nullptr ? p.d_entropy[row] : 0.0f;
+            const float lse = p.lse[row], entropy = p.d_entropy != nullptr ? p.entropy[row] : 0.0f;
+            float v[W::kValues], out[W::kValues];
+            W::unpack(v, held[j]);
+            const int column = at[j] * W::kValues;
+#pragma unroll
+            for (int c = 0; c < W::kValues; ++c) {
+                const float d = max_nan(v[c] - lse, kLowest);
+                const float grad = -fast_exp(d) * fmaf(b, d + entropy, a);
+                out[c] = column + c < p.vocab && lse != -INFINITY ? grad + (column + c == target ? a : 0.0f) : 0.0f;
+            }
+            __stcs(static_cast<uint4*>(p.dlogits) + row * row_words + at[j], W::pack(out));
         }
     }
+}
+
+template <typename T, int kThreads, int kHeld>
+cudaError_t launch_form(LogProbArgs p, int ranks, int sms, cudaStream_t stream) {
+    const int words = (p.vocab + Word<T>::kValues - 1) / Word<T>::kValues;
+    p.ranks = ranks;
+    p.slice = (words + ranks - 1) / ranks;
+    const size_t resident = static_cast<size_t>(blocks_per_sm(kThreads, kHeld)) * sms;
+    const size_t clusters = std::max<size_t>(1, std::min(p.rows, resident / ranks));
+    const dim3 grid(static_cast<unsigned>(clusters * ranks));
+    if (ranks == 1) {
+        return fb::launch_dependent(fb_token_log_probs<T, kThreads, kHeld>, grid, dim3(kThreads), 0, stream, p);
+    }
+    return fb::launch_dependent_cluster(fb_token_log_probs<T, kThreads, kHeld>, grid, dim3(kThreads),
+                                        static_cast<unsigned>(ranks), 0, stream, p);
+}
+
+// Rows of up to 1,664 words (13,312 FP16 columns) take blocks of 128 threads, so that several rows are on an SM;
+// longer ones 512 threads, and as many CTAs of a cluster as hold them in registers. Few rows are
+// divided further, as long as the GPU has CTAs for it and each keeps 512 words.
+template <typename T>
+cudaError_t launch_forward(const LogProbArgs& p, int sms, cudaStream_t stream) {
+    const int words = (p.vocab + Word<T>::kValues - 1) / Word<T>::kValues;
+    if (words <= 4 * 128) {
+        return launch_form<T, 128, 4>(p, 1, sms, stream);
+    }
+    if (words <= 13 * 128 && p.rows * 2 > static_cast<size_t>(sms)) {
+        return launch_form<T, 128, 13>(p, 1, sms, stream);
+    }
+    int ranks = 1;
+    while ((words + ranks - 1) / ranks > 13 * 512 ||
+           (ranks < kMostRanks && p.rows * ranks * 2 <= static_cast<size_t>(sms) && words / ranks >= 2 * 512)) {
+        ranks *= 2;
+    }
+    return (words + ranks - 1) / ranks <= 4 * 512 ? launch_form<T, 512, 4>(p, ranks, sms, stream)
+                                                  : launch_form<T, 512, 13>(p, ranks, sms, stream);
+}
+
+template <typename T>
+cudaError_t launch_backward(LogProbGradientArgs p, int sms, cudaStream_t stream) {
+    const int words = p.cols / Word<T>::kValues;
+    p.chunk = kGradientThreads * kGradientWords;
+    p.row_chunks = words > p.chunk ? (words + p.chunk - 1) / p.chunk : 1;
+    p.chunk_rows = p.row_chunks > 1 ? 1 : p.chunk / words;
+    const size_t items = (p.rows + p.chunk_rows - 1) / p.chunk_rows * p.row_chunks;
+    const unsigned blocks = static_cast<unsigned>(std::min<size_t>(items, 4 * static_cast<size_t>(sms)));
+    return fb::launch_dependent(fb_token_log_probs_backward<T>, dim3(blocks), dim3(kGradientThreads), 0, stream, p);
 }
 
 constexpr flint_status kBad = FLINT_ERROR_INVALID_ARGUMENT;
@@ -230,9 +631,7 @@ flint_status flint_b200_token_log_probs(void* log_probs, void* entropy, void* ls
     p.top = static_cast<int>(top);
     int sms = 148;
     FB_CUDA(fb::sm_count(&sms));
-    const unsigned blocks = static_cast<unsigned>(std::min<size_t>(rows, 4 * static_cast<size_t>(sms)));
-    FB_CUDA(fb::launch_dependent(fp32_logits != 0 ? fb_token_log_probs_rows<float> : fb_token_log_probs_rows<__half>,
-                                 dim3(blocks), dim3(kThreads), 0, stream, p));
+    FB_CUDA(fp32_logits != 0 ? launch_forward<float>(p, sms, stream) : launch_forward<__half>(p, sms, stream));
     return FLINT_OK;
 }
 
@@ -280,10 +679,7 @@ flint_status flint_b200_token_log_probs_backward(void* dlogits, const void* logi
     p.cols = static_cast<int>(cols);
     int sms = 148;
     FB_CUDA(fb::sm_count(&sms));
-    const unsigned blocks = static_cast<unsigned>(std::min<size_t>(rows, 4 * static_cast<size_t>(sms)));
-    FB_CUDA(fb::launch_dependent(
-        fp32_logits != 0 ? fb_token_log_probs_backward_rows<float> : fb_token_log_probs_backward_rows<__half>,
-        dim3(blocks), dim3(kThreads), 0, stream, p));
+    FB_CUDA(fp32_logits != 0 ? launch_backward<float>(p, sms, stream) : launch_backward<__half>(p, sms, stream));
     return FLINT_OK;
 }
 
