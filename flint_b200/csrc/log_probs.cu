@@ -5,6 +5,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -20,6 +21,7 @@ constexpr int kBins = 32;            // parts of a slice whose maxima bound the 
 constexpr int kCandidates = 512;
 constexpr int kMostRanks = 8;        // CTAs of a cluster
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -200.0f;   // e^-200 is 0 in FP32, and 0 * -200 a number
 
 using Key = unsigned long long;
@@ -80,16 +82,85 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// The largest value of a word; a NaN among them gives NaN.
-__device__ __forceinline__ float word_max(const uint4& q, float) {
-    return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)),
-                   max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
-}
-__device__ __forceinline__ float word_max(const uint4& q, __half) {
-    const __half2* h = reinterpret_cast<const __half2*>(&q);
-    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return max_nan(__low2float(m), __high2float(m));
-}
+// The running maximum of words, whose NaN stays, and a word's, in which a NaN is passed over.
+struct MaxF {
+    float m = -INFINITY;
+    __device__ __forceinline__ void add(const uint4& q) {
+        m = max_nan(m, max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)),
+                               max_nan(__uint_as_float(q.z), __uint_as_float(q.w))));
+    }
+    __device__ __forceinline__ float value() const { return m; }
+    __device__ static __forceinline__ float word(const uint4& q) {
+        return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    }
+};
+struct MaxH {
+    __half2 m = __half2half2(__ushort_as_half(0xfc00));
+    __device__ __forceinline__ void add(const uint4& q) {
+        const __half2* h = reinterpret_cast<const __half2*>(&q);
+        m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    }
+    __device__ __forceinline__ float value() const { return max_nan(__low2float(m), __high2float(m)); }
+    __device__ static __forceinline__ float word(const uint4& q) {
+        const __half2* h = reinterpret_cast<const __half2*>(&q);
+        const __half2 w = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return __half2float(__hmax(__low2half(w), __high2half(w)));
+    }
+};
+template <typename T>
+using Max = typename std::conditional<sizeof(T) == 2, MaxH, MaxF>::type;
+
+// Sums of 2^y and of 2^y y with y = (x - m) log2 e, over the words given to add().
+struct SumsBase {
+    fb::F2 sum[2] = {0, 0}, weighted[2] = {0, 0};
+    __device__ __forceinline__ void pair(int i, fb::F2 y) {
+        float y0, y1, e0, e1;
+        fb::f2_unpack(y, y0, y1);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
+        const fb::F2 e = fb::f2_pack(e0, e1);
+        sum[i & 1] = fb::f2_add(sum[i & 1], e);
+        weighted[i & 1] = fb::f2_fma(e, y, weighted[i & 1]);
+    }
+    __device__ __forceinline__ void totals(float& total, float& mean) const {
+        float a, b;
+        fb::f2_unpack(fb::f2_add(sum[0], sum[1]), a, b);
+        total = a + b;
+        fb::f2_unpack(fb::f2_add(weighted[0], weighted[1]), a, b);
+        mean = a + b;
+    }
+};
+// (The difference first: it is exact near m, so that a row of one possible token has an entropy of exactly 0. One
+// instruction less, fma(x, log2 e, -m log2 e), is not.) 2^y y has to be a number for y of minus infinity.
+struct SumsF : SumsBase {
+    fb::F2 minus_m;
+    __device__ __forceinline__ explicit SumsF(float m) : minus_m(fb::f2_pack(-m, -m)) {}
+    __device__ __forceinline__ void add(const uint4& q) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float d0, d1;
+            fb::f2_unpack(fb::f2_add(fb::f2_pack(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])), minus_m), d0, d1);
+            pair(i, fb::f2_mul(fb::f2_pack(max_nan(d0, kLowest), max_nan(d1, kLowest)), fb::f2_pack(kLog2e, kLog2e)));
+        }
+    }
+};
+struct SumsH : SumsBase {
+    fb::F2 minus_m;
+    __device__ __forceinline__ explicit SumsH(float m) : minus_m(fb::f2_pack(-m, -m)) {}
+    __device__ __forceinline__ void add(const uint4& q) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // (The lowest finite value does for minus infinity.)
+            const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&w[i]), __half2half2(__ushort_as_half(0xfbff)));
+            const float2 x = __half22float2(h);
+            pair(i, fb::f2_mul(fb::f2_add(fb::f2_pack(x.x, x.y), minus_m), fb::f2_pack(kLog2e, kLog2e)));
+        }
+    }
+};
+template <typename T>
+using Sums = typename std::conditional<sizeof(T) == 2, SumsH, SumsF>::type;
 
 // A word's values from the `count`-th on become minus infinity, which counts for nothing.
 __device__ __forceinline__ void cut_word(uint4& q, int count, float) {
@@ -202,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         const int target = p.targets != nullptr && tid == 0 && rank == 0 ? p.targets[row] : 0;
         const float target_value = tid == 0 && rank == 0 && target < p.vocab ? W::value(values, target) : 0.0f;
 
-        float mx = -INFINITY;
+        Max<T> running;
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
             const int i = tid + j * kThreads;
@@ -210,9 +281,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                 if (i == last_word && last_count < W::kValues) {
                     cut_word(held[j], last_count, T());
                 }
-                mx = max_nan(mx, word_max(held[j], T()));
+                running.add(held[j]);
             }
         }
+        float mx = running.value();
+        const float my_max = mx;
 #pragma unroll
         for (int off = 1; off < kLanes; off <<= 1) {
             mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
@@ -251,16 +324,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             bound = __shfl_sync(fb::kFullMask, mine, holds != 0 ? __ffs(holds) - 1 : 0);
         }
 
-        fb::F2 sum[2] = {0, 0}, weighted[2] = {0, 0};
-        const fb::F2 mx2 = fb::f2_pack(mx, mx), log2e = fb::f2_pack(kLog2e, kLog2e);
         const bool none = mx == -INFINITY;
+        if (top > 0 && __any_sync(fb::kFullMask, my_max >= bound)) {
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < words) {
-                float v[W::kValues];
-                W::unpack(v, held[j]);
-                if (top > 0 && word_max(held[j], T()) >= bound) {
+            for (int j = 0; j < kHeld; ++j) {
+                const int i = tid + j * kThreads;
+                if (i < words && Max<T>::word(held[j]) >= bound) {
+                    float v[W::kValues];
+                    W::unpack(v, held[j]);
 #pragma unroll
                     for (int c = 0; c < W::kValues; ++c) {
                         if (v[c] >= bound && v[c] > -INFINITY) {
@@ -271,28 +342,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                         }
                     }
                 }
-                if (next < p.rows) {
-                    held[j] = fb::load_input(row_of(next) + i);
-                }
-#pragma unroll
-                for (int c = 0; c < W::kValues; c += 2) {
-                    float y0, y1, e0, e1;
-                    fb::f2_unpack(fb::f2_sub(fb::f2_pack(v[c], v[c + 1]), mx2), y0, y1);
-                    const fb::F2 d = fb::f2_pack(max_nan(y0, kLowest), max_nan(y1, kLowest));
-                    fb::f2_unpack(fb::f2_mul(d, log2e), y0, y1);
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
-                    const fb::F2 e = fb::f2_pack(e0, e1);
-                    sum[c / 2 % 2] = fb::f2_add(sum[c / 2 % 2], e);
-                    weighted[c / 2 % 2] = fb::f2_fma(e, d, weighted[c / 2 % 2]);
-                }
             }
         }
-        float a, b, total, mean;
-        fb::f2_unpack(fb::f2_add(sum[0], sum[1]), a, b);
-        total = a + b;
-        fb::f2_unpack(fb::f2_add(weighted[0], weighted[1]), a, b);
-        mean = a + b;
+        Sums<T> sums_of(mx);
+        const uint4* next_in = row_of(next < p.rows ? next : row);
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = tid + j * kThreads;
+            if (i < words) {
+                sums_of.add(held[j]);
+                held[j] = fb::load_input(next_in + i);
+            }
+        }
+        float total, mean;
+        sums_of.totals(total, mean);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
             total += __shfl_xor_sync(fb::kFullMask, total, off);
@@ -310,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             total += __shfl_xor_sync(fb::kFullMask, total, off);
             mean += __shfl_xor_sync(fb::kFullMask, mean, off);
         }
+        mean *= kLn2;
         if (none) {
             total = mean = 0.0f;
         }
@@ -407,9 +471,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             for (int r = 0; r < p.ranks; ++r) {
                 const float m = parts[parity][r][0];
                 if (m != -INFINITY) {
-                    const float shift = max_nan(m - mx, kLowest), weight = expf(shift);
+                    const float below = max_nan(m - mx, kLowest), weight = expf(below);
                     total = fmaf(weight, parts[parity][r][1], total);
-                    mean = fmaf(weight, fmaf(parts[parity][r][1], shift, parts[parity][r][2]), mean);
+                    mean = fmaf(weight, fmaf(parts[parity][r][1], below, parts[parity][r][2]), mean);
                 }
             }
             log_total = logf(total);
