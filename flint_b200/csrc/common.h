@@ -210,6 +210,8 @@ cudaError_t launch_bias_gradient(void* dbias, const void* dy, size_t rows, size_
 cudaError_t reductions_error_flag(int* value, bool reset);
 // The same for the cross-entropy kernel that stages whole rows by bulk copy.
 cudaError_t rowwise_error_flag(int* value, bool reset);
+// And for the log-probabilities' kernel, which does the same.
+cudaError_t log_probs_error_flag(int* value, bool reset);
 
 }  // namespace fb
 

@@ -26,6 +26,8 @@ constexpr float kLowest = -200.0f;   // e^-200 is 0 in FP32, and 0 * -200 a numb
 
 using Key = unsigned long long;
 
+__device__ int g_log_probs_error = 0;
+
 struct LogProbArgs {
     float* log_probs;
     float* entropy;
@@ -47,6 +49,10 @@ struct Word {
     __device__ static float value(const T* row, int c);
     __device__ static void unpack(float (&v)[kValues], const uint4& q);
     __device__ static uint4 pack(const float (&v)[kValues]);
+    // As unpack, but that FP16's minus infinity becomes the lowest finite value (its exponential is 0, and 0 times
+    // it a number); and for FP32, whose lowest value would not do, the same for differences.
+    __device__ static void unpack_finite(float (&v)[kValues], const uint4& q);
+    __device__ static fb::F2 clamp(fb::F2 d);
 };
 template <>
 __device__ __forceinline__ float Word<float>::value(const float* row, int c) {
@@ -76,10 +82,37 @@ __device__ __forceinline__ uint4 Word<__half>::pack(const float (&v)[8]) {
     return fb::pack8(v);
 }
 
+template <>
+__device__ __forceinline__ void Word<float>::unpack_finite(float (&v)[4], const uint4& q) {
+    unpack(v, q);
+}
+template <>
+__device__ __forceinline__ void Word<__half>::unpack_finite(float (&v)[8], const uint4& q) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2*>(&w[i]), __half2half2(__ushort_as_half(0xfbff)));
+        const float2 x = __half22float2(h);
+        v[2 * i] = x.x;
+        v[2 * i + 1] = x.y;
+    }
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
+}
+
+template <>
+__device__ __forceinline__ fb::F2 Word<float>::clamp(fb::F2 d) {
+    float a, b;
+    fb::f2_unpack(d, a, b);
+    return fb::f2_pack(max_nan(a, kLowest), max_nan(b, kLowest));
+}
+template <>
+__device__ __forceinline__ fb::F2 Word<__half>::clamp(fb::F2 d) {
+    return d;
 }
 
 // The running maximum of words, whose NaN stays, and a word's, in which a NaN is passed over.
@@ -111,23 +144,23 @@ template <typename T>
 using Max = typename std::conditional<sizeof(T) == 2, MaxH, MaxF>::type;
 
 // Sums of 2^y and of 2^y y with y = (x - m) log2 e, over the words given to add().
+// (One value at a time from the exponential on: packed sums cost as many moves into register pairs as they save.)
 struct SumsBase {
-    fb::F2 sum[2] = {0, 0}, weighted[2] = {0, 0};
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, weighted[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     __device__ __forceinline__ void pair(int i, fb::F2 y) {
         float y0, y1, e0, e1;
         fb::f2_unpack(y, y0, y1);
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
-        const fb::F2 e = fb::f2_pack(e0, e1);
-        sum[i & 1] = fb::f2_add(sum[i & 1], e);
-        weighted[i & 1] = fb::f2_fma(e, y, weighted[i & 1]);
+        const int at = 2 * (i & 1);
+        sum[at] += e0;
+        sum[at + 1] += e1;
+        weighted[at] = fmaf(e0, y0, weighted[at]);
+        weighted[at + 1] = fmaf(e1, y1, weighted[at + 1]);
     }
     __device__ __forceinline__ void totals(float& total, float& mean) const {
-        float a, b;
-        fb::f2_unpack(fb::f2_add(sum[0], sum[1]), a, b);
-        total = a + b;
-        fb::f2_unpack(fb::f2_add(weighted[0], weighted[1]), a, b);
-        mean = a + b;
+        total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        mean = (weighted[0] + weighted[1]) + (weighted[2] + weighted[3]);
     }
 };
 // (The difference first: it is exact near m, so that a row of one possible token has an entropy of exactly 0. One
@@ -193,12 +226,6 @@ __device__ __forceinline__ float key_value(Key key) {
     return __uint_as_float((ordered & 0x80000000u) != 0 ? ordered ^ 0x80000000u : ~ordered);
 }
 
-__device__ __forceinline__ float fast_exp(float d) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * kLog2e));
-    return y;
-}
-
 // ---- forward ---------------------------------------------------------------------------------------
 //
 // With m the row's largest logit, d = x - m and S = sum e^d, D = sum d e^d:
@@ -213,11 +240,18 @@ __device__ __forceinline__ float fast_exp(float d) {
 // them, the row is gone through once per alternative.
 constexpr int blocks_per_sm(int threads, int held) { return (threads == 128 ? 4 : 1) * (held > 4 ? 1 : 2); }
 
+constexpr int kChunks = 4;      // pieces in which a slice is copied into shared memory
+
+// kHeld > 0: a thread holds that many words of the row in registers, and asks for the next row's while it takes
+// the exponentials. kHeld == 0: the slice is copied into shared memory, and the CTA beside it on the SM computes
+// meanwhile.
 template <typename T, int kThreads, int kHeld>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_token_log_probs(const LogProbArgs p) {
     using W = Word<T>;
+    constexpr bool kStaged = kHeld == 0;
     constexpr int kWarps = kThreads / 32;
     constexpr int kLanes = kThreads / kBins;      // of a bin
+    extern __shared__ __align__(128) uint4 staged[];
     __shared__ float bins[2][kBins];
     __shared__ float maxima[2][kWarps];
     __shared__ float sums[2][2 * kWarps];
@@ -226,6 +260,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     __shared__ Key candidates[2][kCandidates];
     __shared__ float parts[2][kMostRanks][3];     // the first CTA's: every CTA's m, S, D
     __shared__ Key best[2][kMostRanks * kMostTop];
+    __shared__ alignas(8) unsigned long long barriers[kChunks];
+    __shared__ int abort_flag;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
     const int rank = p.ranks > 1 ? static_cast<int>(sm100::cluster_cta_rank()) : 0;
     const size_t stride = gridDim.x / p.ranks;
@@ -235,10 +271,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     const int words = max(0, min(p.slice, all_words - first_word));
     const int last_word = all_words - 1 - first_word;     // of the row, counted from the slice's first
     const int last_count = p.vocab - (all_words - 1) * W::kValues;
+    const int full = last_word == words - 1 && last_count < W::kValues ? words - 1 : words;   // words that count whole
     const int top = p.top;
 
     if (tid < 2) {
         counts[tid] = 0;
+    }
+    if (kStaged && tid == 0) {
+        abort_flag = 0;
+        for (int c = 0; c < kChunks; ++c) {
+            sm100::mbar_init(sm100::smem_u32(&barriers[c]), 1);
+        }
+        sm100::mbar_fence_init();
     }
     fb::dependency_wait();
     if (p.ranks > 1) {
@@ -254,19 +298,40 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     if (row >= p.rows) {
         return;     // (the whole cluster)
     }
-    uint4 held[kHeld];
+    const int chunk = ((words + kChunks - 1) / kChunks + kThreads - 1) / kThreads * kThreads;
+    auto copy_row = [&](size_t from) {     // thread 0
+        for (int c = 0; c < kChunks && c * chunk < words; ++c) {
+            const uint32_t bytes = static_cast<uint32_t>(min(chunk, words - c * chunk)) * 16u;
+            const uint32_t bar = sm100::smem_u32(&barriers[c]);
+            sm100::mbar_expect_tx(bar, bytes);
+            asm volatile(
+                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                ::"r"(sm100::smem_u32(staged + c * chunk)), "l"(row_of(from) + c * chunk), "r"(bytes), "r"(bar)
+                : "memory");
+        }
+    };
+    uint4 held[kStaged ? 1 : kHeld];
+    if constexpr (kStaged) {
+        if (tid == 0) {
+            copy_row(row);
+        }
+    } else {
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-        const int i = tid + j * kThreads;
-        if (i < words) {
-            held[j] = fb::load_input(row_of(row) + i);
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = tid + j * kThreads;
+            if (i < words) {
+                held[j] = fb::load_input(row_of(row) + i);
+            }
         }
     }
+    bool gave_up = false;
+    uint32_t phase = 0;
     for (int parity = 0; row < p.rows; row += stride, parity ^= 1) {
         const T* values = static_cast<const T*>(p.logits) + row * p.cols;
         const size_t next = row + stride;
-        if (tid == 0 && next + stride < p.rows && words > 0) {
-            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row_of(next + stride)),
+        const size_t soon = kStaged ? next : next + stride;
+        if (tid == 0 && soon < p.rows && words > 0) {
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row_of(soon)),
                          "r"(static_cast<uint32_t>(words) * 16u)
                          : "memory");
         }
@@ -274,14 +339,35 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         const float target_value = tid == 0 && rank == 0 && target < p.vocab ? W::value(values, target) : 0.0f;
 
         Max<T> running;
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < words) {
-                if (i == last_word && last_count < W::kValues) {
-                    cut_word(held[j], last_count, T());
+        bool there = true;
+        if constexpr (kStaged) {
+            for (int c = 0; c < kChunks && c * chunk < words; ++c) {
+                there = sm100::mbar_wait(sm100::smem_u32(&barriers[c]), phase, &abort_flag) && there;
+                const int end = min(full, (c + 1) * chunk);
+#pragma unroll 4
+                for (int i = c * chunk + tid; i < end; i += kThreads) {
+                    running.add(staged[i]);
                 }
-                running.add(held[j]);
+            }
+            phase ^= 1u;
+            if (full < words && tid == full % kThreads) {
+                // The last word, cut for good: this thread reads it again below.
+                uint4 q = staged[full];
+                cut_word(q, last_count, T());
+                staged[full] = q;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // ahead of the next row's copy
+                running.add(q);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                const int i = tid + j * kThreads;
+                if (i < words) {
+                    if (i >= full) {
+                        cut_word(held[j], last_count, T());
+                    }
+                    running.add(held[j]);
+                }
             }
         }
         float mx = running.value();
@@ -300,7 +386,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         if (lane == 0) {
             maxima[parity][warp] = mx;
         }
-        __syncthreads();
+        // One outcome for the whole CTA: who has seen its data must not wait for who has not. (A cluster's
+        // CTAs go on in step, to the end: the others still write into the first one's memory.)
+        if (kStaged ? __syncthreads_or(there ? 0 : 1) != 0 : (__syncthreads(), false)) {
+            gave_up = true;
+        }
         if (tid == 0) {
             counts[parity ^ 1] = 0;     // (of the row before, which everybody is done with)
         }
@@ -309,49 +399,68 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         for (int off = 1; off < kWarps; off <<= 1) {
             mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
         }
-        // Whether a value can be among the `top` largest of the slice.
+        // Whether a value can be among the `top` largest of the slice: the top-th largest of the bins' maxima, equal
+        // ones counted each.
         float bound = INFINITY;
         if (top > 0) {
             const float mine = bins[parity][lane];
-            int larger = 0;
-#pragma unroll
-            for (int off = 1; off < 32; ++off) {
-                const int other_lane = (lane + off) % 32;
-                const float other = __shfl_sync(fb::kFullMask, mine, other_lane);
-                larger += other > mine || (other == mine && other_lane < lane) ? 1 : 0;
+            unsigned ordered = static_cast<unsigned>(order_key(mine, 0) >> 32);
+            for (int left = top; left > 0;) {
+                const unsigned largest = __reduce_max_sync(fb::kFullMask, ordered);
+                const unsigned those = __ballot_sync(fb::kFullMask, ordered == largest);
+                bound = __shfl_sync(fb::kFullMask, mine, __ffs(those) - 1);
+                left -= __popc(those);
+                ordered = ordered == largest ? 0u : ordered;
             }
-            const unsigned holds = __ballot_sync(fb::kFullMask, larger == top - 1);
-            bound = __shfl_sync(fb::kFullMask, mine, holds != 0 ? __ffs(holds) - 1 : 0);
         }
-
         const bool none = mx == -INFINITY;
-        if (top > 0 && __any_sync(fb::kFullMask, my_max >= bound)) {
+        auto collect = [&](const uint4& q, int i) {
+            float v[W::kValues];
+            W::unpack(v, q);
 #pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int i = tid + j * kThreads;
-                if (i < words && Max<T>::word(held[j]) >= bound) {
-                    float v[W::kValues];
-                    W::unpack(v, held[j]);
-#pragma unroll
-                    for (int c = 0; c < W::kValues; ++c) {
-                        if (v[c] >= bound && v[c] > -INFINITY) {
-                            const int at = atomicAdd(&counts[parity], 1);
-                            if (at < kCandidates) {
-                                candidates[parity][at] = order_key(v[c], (first_word + i) * W::kValues + c);
-                            }
-                        }
+            for (int c = 0; c < W::kValues; ++c) {
+                if (v[c] >= bound && v[c] > -INFINITY) {
+                    const int at = atomicAdd(&counts[parity], 1);
+                    if (at < kCandidates) {
+                        candidates[parity][at] = order_key(v[c], (first_word + i) * W::kValues + c);
                     }
                 }
             }
-        }
+        };
+        const bool collects = top > 0 && __any_sync(fb::kFullMask, my_max >= bound);
         Sums<T> sums_of(mx);
-        const uint4* next_in = row_of(next < p.rows ? next : row);
+        if constexpr (kStaged) {
+            if (collects) {
+#pragma unroll 4
+                for (int i = tid; i < words; i += kThreads) {
+                    const uint4 q = staged[i];
+                    if (Max<T>::word(q) >= bound) {
+                        collect(q, i);
+                    }
+                }
+            }
+#pragma unroll 2
+            for (int i = tid; i < words; i += kThreads) {
+                sums_of.add(staged[i]);
+            }
+        } else {
+            if (collects) {
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < words) {
-                sums_of.add(held[j]);
-                held[j] = fb::load_input(next_in + i);
+                for (int j = 0; j < kHeld; ++j) {
+                    const int i = tid + j * kThreads;
+                    if (i < words && Max<T>::word(held[j]) >= bound) {
+                        collect(held[j], i);
+                    }
+                }
+            }
+            const uint4* next_in = row_of(next < p.rows ? next : row);
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                const int i = tid + j * kThreads;
+                if (i < words) {
+                    sums_of.add(held[j]);
+                    held[j] = fb::load_input(next_in + i);
+                }
             }
         }
         float total, mean;
@@ -366,6 +475,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             sums[parity][2 * warp + 1] = mean;
         }
         __syncthreads();
+        if (kStaged && tid == 0 && next < p.rows && !gave_up) {
+            copy_row(next);     // everybody has read this row's words
+        }
         total = sums[parity][2 * (lane % kWarps)];
         mean = sums[parity][2 * (lane % kWarps) + 1];
 #pragma unroll
@@ -502,6 +614,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             }
         }
     }
+    if (gave_up && tid == 0) {
+        // Copies that were started get a second, equally bounded chance to land before the memory goes.
+        atomicExch(&g_log_probs_error, 1);
+        const long long start = clock64();
+        while (clock64() - start < 2000000LL) {
+        }
+    }
 }
 
 // ---- backward --------------------------------------------------------------------------------------
@@ -564,38 +683,69 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
             const float a = p.d_log_probs != nullptr && target < p.vocab ? p.d_log_probs[row] : 0.0f;
             const float b = p.d_entropy != nullptr ? p.d_entropy[row] : 0.0f;
             const float lse = p.lse[row], entropy = p.d_entropy != nullptr ? p.entropy[row] : 0.0f;
+            // -p (a + b (d + entropy)) = e^d (-b d - (a + b entropy)); a row without tokens gives zeros.
+            const bool none = lse == -INFINITY;
+            const fb::F2 minus_lse = fb::f2_pack(none ? 0.0f : -lse, none ? 0.0f : -lse);
+            const float constant = none ? 0.0f : -fmaf(b, entropy, a);
+            const fb::F2 constant2 = fb::f2_pack(constant, constant);
+            const fb::F2 slope2 = fb::f2_pack(none ? 0.0f : -b, none ? 0.0f : -b);
             float v[W::kValues], out[W::kValues];
-            W::unpack(v, held[j]);
-            const int column = at[j] * W::kValues;
+            W::unpack_finite(v, held[j]);
 #pragma unroll
-            for (int c = 0; c < W::kValues; ++c) {
-                const float d = max_nan(v[c] - lse, kLowest);
-                const float grad = -fast_exp(d) * fmaf(b, d + entropy, a);
-                out[c] = column + c < p.vocab && lse != -INFINITY ? grad + (column + c == target ? a : 0.0f) : 0.0f;
+            for (int c = 0; c < W::kValues; c += 2) {
+                const fb::F2 d = W::clamp(fb::f2_add(fb::f2_pack(v[c], v[c + 1]), minus_lse));
+                float y0, y1, e0, e1;
+                fb::f2_unpack(fb::f2_mul(d, fb::f2_pack(kLog2e, kLog2e)), y0, y1);
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
+                fb::f2_unpack(fb::f2_mul(fb::f2_pack(e0, e1), fb::f2_fma(slope2, d, constant2)), out[c], out[c + 1]);
+            }
+            const int column = at[j] * W::kValues;
+            if (static_cast<unsigned>(target - column) < W::kValues && !none) {
+#pragma unroll
+                for (int c = 0; c < W::kValues; ++c) {
+                    out[c] += column + c == target ? a : 0.0f;
+                }
+            }
+            if (column + W::kValues > p.vocab) {
+#pragma unroll
+                for (int c = 0; c < W::kValues; ++c) {
+                    out[c] = column + c < p.vocab ? out[c] : 0.0f;
+                }
             }
             __stcs(static_cast<uint4*>(p.dlogits) + row * row_words + at[j], W::pack(out));
         }
     }
 }
 
+constexpr int kStagedWords = 6400;     // 100 KB: two CTAs per SM
+
 template <typename T, int kThreads, int kHeld>
 cudaError_t launch_form(LogProbArgs p, int ranks, int sms, cudaStream_t stream) {
     const int words = (p.vocab + Word<T>::kValues - 1) / Word<T>::kValues;
     p.ranks = ranks;
     p.slice = (words + ranks - 1) / ranks;
+    const size_t smem = kHeld == 0 ? static_cast<size_t>(p.slice) * 16 : 0;
+    if (kHeld == 0) {
+        static std::atomic<bool> configured[64] = {};
+        const cudaError_t e = fb::allow_shared_memory(fb_token_log_probs<T, kThreads, kHeld>, kStagedWords * 16, configured);
+        if (e != cudaSuccess) {
+            return e;
+        }
+    }
     const size_t resident = static_cast<size_t>(blocks_per_sm(kThreads, kHeld)) * sms;
     const size_t clusters = std::max<size_t>(1, std::min(p.rows, resident / ranks));
     const dim3 grid(static_cast<unsigned>(clusters * ranks));
     if (ranks == 1) {
-        return fb::launch_dependent(fb_token_log_probs<T, kThreads, kHeld>, grid, dim3(kThreads), 0, stream, p);
+        return fb::launch_dependent(fb_token_log_probs<T, kThreads, kHeld>, grid, dim3(kThreads), smem, stream, p);
     }
     return fb::launch_dependent_cluster(fb_token_log_probs<T, kThreads, kHeld>, grid, dim3(kThreads),
-                                        static_cast<unsigned>(ranks), 0, stream, p);
+                                        static_cast<unsigned>(ranks), smem, stream, p);
 }
 
 // Rows of up to 1,664 words (13,312 FP16 columns) take blocks of 128 threads, so that several rows are on an SM;
-// longer ones 512 threads, and as many CTAs of a cluster as hold them in registers. Few rows are
-// divided further, as long as the GPU has CTAs for it and each keeps 512 words.
+// longer ones 512 threads, and as many CTAs of a cluster as have room for them in half an SM's shared memory.
+// Few rows are divided further, as long as the GPU has CTAs for it and each keeps 512 words.
 template <typename T>
 cudaError_t launch_forward(const LogProbArgs& p, int sms, cudaStream_t stream) {
     const int words = (p.vocab + Word<T>::kValues - 1) / Word<T>::kValues;
@@ -606,12 +756,12 @@ cudaError_t launch_forward(const LogProbArgs& p, int sms, cudaStream_t stream) {
         return launch_form<T, 128, 13>(p, 1, sms, stream);
     }
     int ranks = 1;
-    while ((words + ranks - 1) / ranks > 13 * 512 ||
+    while ((words + ranks - 1) / ranks > kStagedWords ||
            (ranks < kMostRanks && p.rows * ranks * 2 <= static_cast<size_t>(sms) && words / ranks >= 2 * 512)) {
         ranks *= 2;
     }
     return (words + ranks - 1) / ranks <= 4 * 512 ? launch_form<T, 512, 4>(p, ranks, sms, stream)
-                                                  : launch_form<T, 512, 13>(p, ranks, sms, stream);
+                                                  : launch_form<T, 512, 0>(p, ranks, sms, stream);
 }
 
 template <typename T>
@@ -649,6 +799,19 @@ fb::Span span_or(const char* what, const void* pointer, size_t bytes, const void
 }
 
 }  // namespace
+
+namespace fb {
+
+cudaError_t log_probs_error_flag(int* value, bool reset) {
+    cudaError_t e = cudaMemcpyFromSymbol(value, g_log_probs_error, sizeof(int));
+    if (e == cudaSuccess && reset && *value != 0) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_log_probs_error, &zero, sizeof(int));
+    }
+    return e;
+}
+
+}  // namespace fb
 
 extern "C" {
 

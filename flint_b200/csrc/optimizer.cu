@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <iterator>
 #include <vector>
 
 #include <cuda_fp16.h>
@@ -443,7 +444,10 @@ flint_status flint_b200_kernel_fault(int* raised) {
     FB_CUDA(fb::rowwise_error_flag(&rowwise, true));
     int packed = 0;
     FB_CUDA(fb::packed_error_flag(&packed, true));
-    *raised = (gemm != 0 || attention != 0 || reductions != 0 || rowwise != 0 || packed != 0) ? 1 : 0;
+    int log_probs = 0;
+    FB_CUDA(fb::log_probs_error_flag(&log_probs, true));
+    const int all[] = {gemm, attention, reductions, rowwise, packed, log_probs};
+    *raised = std::any_of(std::begin(all), std::end(all), [](int flag) { return flag != 0; }) ? 1 : 0;
     return FLINT_OK;
 }
 
