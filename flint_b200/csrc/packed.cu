@@ -337,7 +337,7 @@ flint_status flint_b200_packed_attention_forward(void* o, void* lse, const void*
     p.o = static_cast<__half*>(o);
     p.lse = static_cast<float*>(lse);
     p.starts = static_cast<const int*>(starts);
-    FB_CUDA(fb::packed_forward(p, workspace, stream));
+    FB_CUDA(fb::packed_forward(p, p.rows, workspace, stream));
     return FLINT_OK;
 }
 
@@ -470,7 +470,7 @@ flint_status flint_b200_paged_attention(void* o, void* lse, const void* q, const
     p.starts = static_cast<const int*>(starts);
     p.lengths = static_cast<const int*>(lengths);
     p.table = static_cast<const int*>(page_table);
-    FB_CUDA(fb::packed_forward(p, workspace, stream));
+    FB_CUDA(fb::packed_forward(p, static_cast<int>(shape->longest), workspace, stream));
     return FLINT_OK;
 }
 

@@ -33,8 +33,9 @@ struct PackedGradients {
     const __half* d_o;      // rows as o's
 };
 
-// Forward, over packed or paged keys; the workspace's size depends on the GPU only.
-cudaError_t packed_forward(const PackedArgs& args, void* workspace, cudaStream_t stream);
+// Forward, over packed or paged keys; the workspace's size depends on the GPU only. `longest` is about how many new
+// tokens a sequence has at most (paged keys; it chooses the kernel's form).
+cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace, cudaStream_t stream);
 cudaError_t packed_forward_workspace(size_t* bytes);
 cudaError_t packed_forward_error_flag(int* value, bool reset);
 

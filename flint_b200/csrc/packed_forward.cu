@@ -41,7 +41,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 192;   // TMA warp, MMA warp, four softmax warps with a row per thread
 constexpr int kWarps = kThreads / 32;
 constexpr int kSlots = 4;       // ring of K and V tiles
-constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + 256;
+constexpr int kStagingBytes = 4 * 2048;
+constexpr int kPieces = 8;      // ring of piece descriptions
+constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
 constexpr int kLeastPart = 2;   // of the line of key tiles, per CTA
 
 constexpr size_t kPartFloats = size_t{kRows} * kHead + 2 * kRows;   // O [column / 4][row][4], maxima, sums
@@ -64,8 +66,10 @@ struct Barriers {
     __device__ uint32_t s_free() const { return base + 40; }
     __device__ uint32_t p_ready() const { return base + 48; }
     __device__ uint32_t pv_done() const { return base + 56; }
-    __device__ uint32_t slot_full(int s) const { return base + 64 + 8u * s; }
-    __device__ uint32_t slot_empty(int s) const { return base + 64 + 8u * (kSlots + s); }
+    __device__ uint32_t meeting() const { return base + 64; }
+    __device__ uint32_t piece_full(int i) const { return base + 72 + 8u * i; }
+    __device__ uint32_t slot_full(int s) const { return base + 72 + 8u * (kPieces + s); }
+    __device__ uint32_t slot_empty(int s) const { return base + 72 + 8u * (kPieces + kSlots + s); }
 };
 
 constexpr uint32_t kIdescS = sm100::instr_desc_f16(128, 128, false, false);
@@ -166,38 +170,49 @@ __device__ void locate(const TileParams& p, Cut (&cuts)[2], long long (&scan)[kW
     __syncthreads();
 }
 
-// A role's place in the CTA's sequence of key tiles.
-struct Steps {
-    Walk walk;
-    Piece piece;
-    int j, round;
-    bool valid;
-    __device__ __forceinline__ void begin(const TileParams& p, const Cut& lo, long long end) {
-        walk.begin(SequenceOf{p.a}, lo, end);
-        round = 0;
-        valid = walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
-        j = valid ? piece.from : 0;
-    }
-    __device__ __forceinline__ void advance(const TileParams& p) {
-        if (++j == piece.to) {
-            ++round;
-            valid = walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
-            j = valid ? piece.from : 0;
+// A piece as the TMA warp hands it to the others; `to` of 0 ends the list.
+struct PieceInfo {
+    int from, to, tiles;
+    int position;      // of the tile's first token
+    int tokens;        // in the tile
+    int first_row;     // of its first token
+    int head;          // K/V head
+    int keys;          // of the sequence
+};
+
+// Softmax warps that share rows meet here (bounded, like every wait).
+struct Meeting {
+    uint32_t bar;
+    uint32_t count;
+    volatile int* abort;
+    int lane;
+    __device__ __forceinline__ bool meet() {
+        __syncwarp();
+        if (lane == 0) {
+            sm100::mbar_arrive(bar);
         }
+        return sm100::mbar_wait_warp(bar, count++ & 1, abort);
     }
 };
 
-template <bool kPaged>
+// kSubsets > 1 (single tokens and few of them): a tile has 128 / kSubsets rows, which lie kSubsets times in the 128
+// lanes, and each copy takes its share of a key tile's columns (its other probabilities are zeros, written once),
+// with its own maxima and sums. A step's softmax then takes a kSubsets-th of the time, and all four warps
+// work where one would; the copies are put together at the end of a piece.
+template <bool kPaged, int kSubsets>
 __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __grid_constant__ TileParams p) {
     extern __shared__ unsigned char smem_raw[];
     const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_tiles = base;
     const uint32_t ring = base + 2 * kTileBytes;
-    const Barriers bar{ring + kSlots * kTileBytes};
+    const uint32_t staging = ring + kSlots * kTileBytes;      // 2 KB per softmax warp
+    const Barriers bar{staging + kStagingBytes};
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ Cut cuts[2];
     __shared__ long long scan[kWarps + 1];
+    __shared__ PieceInfo pieces[kPieces];
+    __shared__ float merge_max[4][32], merge_sum[4][32];
 
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x / 32), 0);
     const int lane = threadIdx.x % 32;
@@ -211,6 +226,10 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         sm100::mbar_init(bar.s_free(), 4);     // one arrival per softmax warp
         sm100::mbar_init(bar.p_ready(), 4);
         sm100::mbar_init(bar.pv_done(), 1);
+        sm100::mbar_init(bar.meeting(), 4);
+        for (int i = 0; i < kPieces; ++i) {
+            sm100::mbar_init(bar.piece_full(i), 1);
+        }
         for (int s = 0; s < kSlots; ++s) {
             sm100::mbar_init(bar.slot_full(s), 1);
             sm100::mbar_init(bar.slot_empty(s), 1);
@@ -230,17 +249,48 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
     sm100::tc_fence_after_sync();
     const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + 128, tmem_p = tmem_slot + 192;
     volatile int* abort = &abort_flag;
-    const Cut lo = cuts[0];
-    const long long end = cuts[1].at;
 
     if (warp == 0) {
-        Steps keys, values;     // the next K tile to fetch; the next V tile, one step behind
-        keys.begin(p, lo, end);
-        values.begin(p, lo, end);
+        Walk walk;
+        Piece piece;
+        walk.begin(SequenceOf{p.a}, cuts[0], cuts[1].at);
+        int round = 0;
+        bool more = walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
+        int j = more ? piece.from : 0;
         int slot = 0;
         uint32_t phase = 0;
         bool ok = true;
-        auto load = [&](const CUtensorMap* map, const Steps& at) {
+        // 32 of the sequence's page numbers, one per lane, and where each lane's part of the key tile at hand and of
+        // the one before lies.
+        int page_entries = 0, entries_from = -1, entries_of = -1;
+        int at_now = 0, head_now = 0, at_before = 0, head_before = 0;
+        auto find = [&]() {
+            at_before = at_now;
+            head_before = head_now;
+            head_now = piece.head;
+            if constexpr (kPaged) {
+                const int first = j * kKeyTile / p.a.page_size;     // page of the tile's first key
+                if (entries_of != piece.index || first < entries_from || first + p.boxes > entries_from + 32) {
+                    const int index = first + lane;
+                    entries_of = piece.index;
+                    entries_from = first;
+                    page_entries = -1;
+                    if (index < (piece.sequence.keys + p.a.page_size - 1) / p.a.page_size) {
+                        page_entries = static_cast<int>(page_of(p.a, piece.index, index * p.a.page_size));
+                    }
+                }
+                const int box = min(lane, p.boxes - 1);
+                const int page = __shfl_sync(kFullMask, page_entries, first - entries_from + box);
+                // A page that is not there is read from outside the cache, as zeros.
+                const int key = j * kKeyTile + box * p.box_rows;
+                at_now = page < 0 || key >= piece.sequence.keys
+                             ? static_cast<int>(p.a.pages * p.a.kv_heads * p.a.page_size)
+                             : (page * p.a.kv_heads + piece.head) * p.a.page_size + (key & (p.a.page_size - 1));
+            } else {
+                at_now = piece.sequence.first + j * kKeyTile;
+            }
+        };
+        auto load = [&](const CUtensorMap* map, int at, int head) {
             if (!sm100::mbar_wait_warp(bar.slot_empty(slot), phase ^ 1u, abort)) {
                 ok = false;
                 return;
@@ -252,16 +302,10 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             __syncwarp();
             if constexpr (kPaged) {
                 if (lane < p.boxes) {
-                    // A page that is not there is read from outside the cache, as zeros.
-                    const int key = at.j * kKeyTile + lane * p.box_rows;
-                    const long long page = key < at.piece.sequence.keys ? page_of(p.a, at.piece.index, key) : -1;
-                    const long long row = page < 0 ? p.a.pages * p.a.kv_heads * p.a.page_size
-                                                   : (page * p.a.kv_heads + at.piece.head) * p.a.page_size +
-                                                         key % p.a.page_size;
-                    sm100::tma_load_2d(dst + lane * p.box_rows * (kHead * 2), map, full, 0, static_cast<int>(row));
+                    sm100::tma_load_2d(dst + lane * p.box_rows * (kHead * 2), map, full, 0, at);
                 }
             } else if (lane == 0) {
-                sm100::tma_load_3d(dst, map, full, 0, at.piece.head, at.piece.sequence.first + at.j * kKeyTile);
+                sm100::tma_load_3d(dst, map, full, 0, head, at);
             }
             __syncwarp();
             if (++slot == kSlots) {
@@ -269,35 +313,62 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 phase ^= 1u;
             }
         };
-        auto load_keys = [&]() {
-            if (keys.j == keys.piece.from) {
-                // A new piece: its queries go into the buffer of its parity, free once the piece two
-                // rounds back has issued its last scores.
-                const int b = keys.round & 1;
-                if (keys.round >= 2 &&
-                    !sm100::mbar_wait_warp(bar.q_empty(b), ((keys.round >> 1) - 1) & 1, abort)) {
-                    ok = false;
-                    return;
+        int waiting = 0;     // K tiles whose V tile has not been asked for
+        while (ok) {
+            if (more) {
+                if (j == piece.from) {
+                    // A new piece. Its description's place was read long ago: the ring of tiles keeps this
+                    // warp within a few steps, and so within fewer than kPieces pieces, of the softmax warps.
+                    // Its queries go into the buffer of its parity, free once the piece two rounds
+                    // back has issued its last scores.
+                    const int b = round & 1;
+                    if (round >= 2 && !sm100::mbar_wait_warp(bar.q_empty(b), ((round >> 1) - 1) & 1, abort)) {
+                        break;
+                    }
+                    if (lane == 0) {
+                        pieces[round % kPieces] = PieceInfo{piece.from, piece.to, piece.tiles, piece.position(),
+                                                            piece.tokens, piece.sequence.first + piece.first_token,
+                                                            piece.head, piece.sequence.keys};
+                        sm100::mbar_arrive(bar.piece_full(round % kPieces));
+                        sm100::mbar_expect_tx(bar.q_full(b), kSubsets * static_cast<uint32_t>(p.group << p.log_tokens) *
+                                                                 (kHead * 2));
+#pragma unroll
+                        for (int copy = 0; copy < kSubsets; ++copy) {
+                            sm100::tma_load_3d(q_tiles + b * kTileBytes + copy * (kTileBytes / kSubsets), &p.map_q,
+                                               bar.q_full(b), 0, piece.head * p.group,
+                                               piece.sequence.first + piece.first_token);
+                        }
+                    }
+                    __syncwarp();
                 }
-                if (lane == 0) {
-                    sm100::mbar_expect_tx(bar.q_full(b), static_cast<uint32_t>(p.group << p.log_tokens) * (kHead * 2));
-                    sm100::tma_load_3d(q_tiles + b * kTileBytes, &p.map_q, bar.q_full(b), 0,
-                                       keys.piece.head * p.group, keys.piece.sequence.first + keys.piece.first_token);
+                find();
+                load(&p.map_k, at_now, head_now);
+                ++waiting;
+                if (++j == piece.to) {
+                    ++round;
+                    more = walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
+                    j = more ? piece.from : 0;
+                    if (!more && lane == 0) {
+                        pieces[round % kPieces].to = 0;
+                        sm100::mbar_arrive(bar.piece_full(round % kPieces));
+                    }
                 }
-            }
-            load(&p.map_k, keys);
-            keys.advance(p);
-        };
-        if (keys.valid) {
-            load_keys();
-        }
-        while (ok && values.valid) {
-            if (keys.valid) {
-                load_keys();
-            }
-            if (ok) {
-                load(&p.map_v, values);
-                values.advance(p);
+                if (waiting < 2) {
+                    continue;
+                }
+                if (ok) {
+                    load(&p.map_v, at_before, head_before);
+                    --waiting;
+                }
+            } else {
+                if (round == 0 && lane == 0) {
+                    pieces[0].to = 0;          // nothing to do at all
+                    sm100::mbar_arrive(bar.piece_full(0));
+                }
+                if (waiting > 0) {
+                    load(&p.map_v, at_now, head_now);
+                }
+                break;
             }
         }
     } else if (warp == 1) {
@@ -319,17 +390,34 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 phase ^= 1u;
             }
         };
-        Steps ahead, now;
-        ahead.begin(p, lo, end);
-        now.begin(p, lo, end);
-        uint32_t issued = 0;
-        auto issue_scores = [&]() {
-            if (!ok || !ahead.valid) {
+        // Where the next scores to issue stand, and how far the piece goes.
+        int round = 0, j = 0, to = 0, from = 0, keys = 0;
+        auto enter = [&]() {
+            if (!sm100::mbar_wait_warp(bar.piece_full(round % kPieces), (round / kPieces) & 1, abort)) {
+                ok = false;
+                to = 0;
                 return;
             }
-            const int b = ahead.round & 1;
-            if (ahead.j == ahead.piece.from &&
-                !sm100::mbar_wait_warp(bar.q_full(b), (ahead.round >> 1) & 1, abort)) {
+            const PieceInfo& info = pieces[round % kPieces];
+            from = j = info.from;
+            to = info.to;
+            keys = info.keys;
+        };
+        bool at_end = true;      // of a piece: the next one's description comes first
+        uint32_t issued = 0;
+        // Of the step whose scores were issued last: whether its piece begins with it, and the keys in its tile.
+        bool begins_ahead = false;
+        int present_ahead = 0;
+        auto issue_scores = [&]() {
+            if (ok && at_end) {
+                enter();
+                at_end = false;
+            }
+            if (!ok || to == 0) {
+                return;
+            }
+            const int b = round & 1;
+            if (j == from && !sm100::mbar_wait_warp(bar.q_full(b), (round >> 1) & 1, abort)) {
                 ok = false;
                 return;
             }
@@ -344,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             sm100::tc_fence_after_sync();
             const uint64_t q_desc = desc_kmajor(q_tiles + b * kTileBytes, 0);
             const uint64_t k_desc = desc_kmajor(k_tile, 0);
-            const bool last = ahead.j + 1 == ahead.piece.to;
+            const bool last = j + 1 == to;
             if (sm100::elect_one()) {
                 sm100::mma_f16_ss_at<0>(tmem_s, q_desc, 0, k_desc, 0, kIdescS);
                 sm100::mma_f16_ss_at<1>(tmem_s, q_desc, 2, k_desc, 2, kIdescS);
@@ -359,10 +447,18 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             __syncwarp();
             step_ring();
             ++issued;
-            ahead.advance(p);
+            begins_ahead = j == from;
+            present_ahead = keys - j * kKeyTile;
+            ++j;
+            if (last) {
+                ++round;
+                at_end = true;
+            }
         };
         issue_scores();
-        for (uint32_t n = 0; ok && now.valid; ++n) {
+        for (uint32_t n = 0; ok && n < issued; ++n) {
+            const bool begins = begins_ahead;
+            const int present = present_ahead;
             issue_scores();    // of the next step, as soon as this step's have been read
             if (!ok || !sm100::mbar_wait_warp(bar.p_ready(), n & 1, abort)) {
                 break;
@@ -371,11 +467,9 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             if (v_tile == 0) {
                 break;
             }
-            const int present = now.piece.sequence.keys - now.j * kKeyTile;
             if (present < kKeyTile) {
                 // Rows behind the sequence's last key hold anything, and 0 times that need not be 0.
-                const int from = max(present, 0) * (kHead * 2);
-                for (int at = from + lane * 16; at < kTileBytes; at += 512) {
+                for (int at = max(present, 0) * (kHead * 2) + lane * 16; at < kTileBytes; at += 512) {
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + at), "r"(0) : "memory");
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -383,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             }
             const uint64_t v_desc = desc_mnmajor(v_tile, 0, 16);
             if (sm100::elect_one()) {
-                sm100::mma_f16_ts_at<-1>(tmem_o, tmem_p, v_desc, 0, kIdescPV, now.j > now.piece.from);
+                sm100::mma_f16_ts_at<-1>(tmem_o, tmem_p, v_desc, 0, kIdescPV, begins ? 0u : 1u);
 #pragma unroll
                 for (int ks = 1; ks < 8; ++ks) {
                     sm100::mma_f16_ts_at<1>(tmem_o, tmem_p + ks * 8, v_desc, ks * 128, kIdescPV);
@@ -393,30 +487,57 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             }
             __syncwarp();
             step_ring();
-            now.advance(p);
         }
     } else {
+        constexpr int kColumns = kKeyTile / kSubsets;        // of a key tile, that this thread works on
+        constexpr int kChunks = kColumns / 32;
+        constexpr int kOut = kHead / kSubsets;               // columns of O that it writes
+        constexpr int kCopyRows = kRows / kSubsets;
         const int quadrant = warp % 4;
-        const int row = quadrant * 32 + lane;
+        const int subset = quadrant * kSubsets / 4;
+        const int row = (quadrant * 32 + lane) % kCopyRows;  // of the tile
         const uint32_t lane_base = static_cast<uint32_t>(quadrant * 32) << 16;
+        const uint32_t my_scores = tmem_s + lane_base + subset * kColumns;
+        const uint32_t my_weights = tmem_p + lane_base + subset * (kColumns / 2);
+        const uint32_t my_output = tmem_o + lane_base;
+        const uint32_t my_staging = staging + quadrant * 2048;
         const int token = row / p.group;
+        const int head_of_group = row - token * p.group;
         const float scale2 = p.a.scale * kLog2e;
         const F2 scale_pair = f2_pack(scale2, scale2);
-        if (row == 0) {
-            p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, lo, cuts[1]);
+        Meeting meeting{bar.meeting(), 0, abort, lane};
+        if (quadrant == 0 && lane == 0) {
+            p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, cuts[0], cuts[1]);
         }
-        Walk walk;
-        Piece piece;
-        walk.begin(SequenceOf{p.a}, lo, end);
+        if (kSubsets > 1) {
+            const uint32_t zeros[16] = {};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                sm100::tmem_st_32x16(tmem_p + lane_base + 16 * c, zeros);
+            }
+            sm100::tmem_st_wait();
+        }
         uint32_t n = 0;
         bool ok = true;
-        while (ok && walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece)) {
-            const bool valid = token < piece.tokens;
+        for (int round = 0; ok; ++round) {
+            if (!sm100::mbar_wait_warp(bar.piece_full(round % kPieces), (round / kPieces) & 1, abort)) {
+                break;
+            }
+            const PieceInfo& info = pieces[round % kPieces];
+            const int from = info.from, to = info.to;
+            if (to == 0) {
+                break;
+            }
+            const bool whole = from == 0 && to == info.tiles;
+            const int first_position = info.position;
+            const bool valid = token < info.tokens;
+            const int position = valid ? first_position + token : -1;
+            const long long out_row = info.first_row + token;
+            const int head = info.head * p.group + head_of_group;
             const bool active = __any_sync(kFullMask, valid);
-            const int position = valid ? piece.position() + token : -1;
             float m = kNoKey;     // reference exponent of the row (base 2)
             F2 l = 0;             // the row sum, in two partial sums
-            for (int j = piece.from; j < piece.to; ++j, ++n) {
+            for (int j = from; j < to; ++j, ++n) {
                 if (!sm100::mbar_wait_warp(bar.s_full(), n & 1, abort)) {
                     ok = false;
                     break;
@@ -425,17 +546,19 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 // The scores are read twice, 32 columns at a time and the next 32 on their way: a row's
                 // 128 at once left no registers (the kernel spilled 950 bytes and took three times as long).
                 uint32_t raw[2][32];
-                const int visible = position - j * kKeyTile;     // columns up to this one are seen
-                const bool masked = j * kKeyTile + kKeyTile - 1 > piece.position();
+                const int visible = position - j * kKeyTile - subset * kColumns;     // columns up to this one are seen
+                const bool masked = j * kKeyTile + kKeyTile - 1 > first_position;
                 float alpha = 1.0f;
                 bool moved = false;
                 if (active) {
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    sm100::tmem_ld_32x32(tmem_s + lane_base, raw[0]);
+                    sm100::tmem_ld_32x32(my_scores, raw[0]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < kChunks; ++c) {
                         sm100::tmem_ld_wait();
-                        sm100::tmem_ld_32x32(tmem_s + lane_base + 32 * ((c + 1) % 4), raw[(c + 1) & 1]);
+                        if (kChunks > 1) {
+                            sm100::tmem_ld_32x32(my_scores + 32 * ((c + 1) % kChunks), raw[(c + 1) & 1]);
+                        }
                         uint32_t (&now)[32] = raw[c & 1];
                         if (masked) {
 #pragma unroll
@@ -468,12 +591,12 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 }
                 sm100::tc_fence_after_sync();
                 if (active) {
-                    if (j > piece.from && __any_sync(kFullMask, moved)) {
+                    if (j > from && __any_sync(kFullMask, moved)) {
                         const F2 a2 = f2_pack(alpha, alpha);
 #pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
                             uint32_t acc[16];
-                            sm100::tmem_ld_32x16(tmem_o + lane_base + c * 16, acc);
+                            sm100::tmem_ld_32x16(my_output + c * 16, acc);
                             sm100::tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
@@ -482,15 +605,15 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                                 acc[i] = __float_as_uint(x);
                                 acc[i + 1] = __float_as_uint(y);
                             }
-                            sm100::tmem_st_32x16(tmem_o + lane_base + c * 16, acc);
+                            sm100::tmem_st_32x16(my_output + c * 16, acc);
                         }
                     }
                     const F2 shift = f2_pack(-m, -m);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < kChunks; ++c) {
                         sm100::tmem_ld_wait();
-                        if (c < 3) {
-                            sm100::tmem_ld_32x32(tmem_s + lane_base + 32 * (c + 1), raw[(c + 1) & 1]);
+                        if (c + 1 < kChunks) {
+                            sm100::tmem_ld_32x32(my_scores + 32 * (c + 1), raw[(c + 1) & 1]);
                         } else {
                             // All scores are read: the next step's may come.
                             sm100::tc_fence_before_sync();
@@ -500,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             }
                         }
                         uint32_t (&now)[32] = raw[c & 1];
-                        if (masked) {
+                        if (masked && kChunks > 1) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
                                 now[i] = 32 * c + i <= visible ? now[i] : 0xff800000u;
@@ -512,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             float x, y;
                             const F2 t = f2_fma(f2_pack(__uint_as_float(now[2 * i]), __uint_as_float(now[2 * i + 1])),
                                                 scale_pair, shift);
-                            if ((i & 3) == 0) {
+                            if (kSubsets == 1 && (i & 3) == 0) {
                                 exp2_pair_fma(t, x, y);
                             } else {
                                 f2_unpack(t, x, y);
@@ -522,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             l = f2_add(l, f2_pack(x, y));
                             packed[i] = pack2(x, y);
                         }
-                        sm100::tmem_st_32x16(tmem_p + lane_base + c * 16, packed);
+                        sm100::tmem_st_32x16(my_weights + c * 16, packed);
                     }
                     sm100::tmem_st_wait();
                 } else {
@@ -547,44 +670,145 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             if (m == kNoKey) {
                 total = 0.0f;    // (the polynomial's least power of two is not 0)
             }
-            const int head = piece.head * p.group + row - token * p.group;
-            const long long at_row = piece.sequence.first + piece.first_token + token;
-            const bool whole = piece.whole();
-            float* part = p.parts + (2 * size_t{blockIdx.x} + (piece.from == 0 ? 1 : 0)) * kPartFloats;
-            const float inv = position < 0 ? 0.0f : 1.0f / total;   // no key at all gives zeros
-            __half* out = p.a.o + at_row * p.a.o_stride + head * kHead;
-            uint32_t acc[64];
-            if (active) {
-                sm100::tmem_ld_32x32(tmem_o + lane_base, reinterpret_cast<uint32_t(&)[32]>(acc[0]));
-                sm100::tmem_ld_32x32(tmem_o + lane_base + 32, reinterpret_cast<uint32_t(&)[32]>(acc[32]));
-                sm100::tmem_ld_wait();
-            }
-            if (valid && whole) {
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[i] = position < 0 ? 0.0f : __uint_as_float(acc[b * 8 + i]) * inv;
-                    }
-                    *reinterpret_cast<uint4*>(out + 8 * b) = pack8(v);
+            float acc[kOut];
+            if constexpr (kSubsets == 1) {
+                if (active) {
+                    sm100::tmem_ld_32x32(my_output, reinterpret_cast<uint32_t(&)[32]>(acc[0]));
+                    sm100::tmem_ld_32x32(my_output + 32, reinterpret_cast<uint32_t(&)[32]>(acc[32]));
+                    sm100::tmem_ld_wait();
                 }
-            }
-            if (valid && !whole) {
+            } else {
+                // The copies of a row: one reference exponent, one sum, and O's columns 16 at a time.
+                merge_max[quadrant][lane] = m;
+                merge_sum[quadrant][lane] = total;
+                if (!meeting.meet()) {
+                    break;
+                }
+                constexpr int kApart = 4 / kSubsets;          // quadrants between a row's copies
+                float top = kNoKey;
 #pragma unroll
-                for (int b = 0; b < 16; ++b) {
-                    reinterpret_cast<uint4*>(part)[b * kRows + row] =
-                        make_uint4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
+                for (int s = 0; s < kSubsets; ++s) {
+                    top = max3_nan(top, merge_max[(quadrant % kApart) + s * kApart][lane], kNoKey);
+                }
+                const float mine = m == kNoKey ? 0.0f : fast_exp2(m - top);
+                total = 0.0f;
+#pragma unroll
+                for (int s = 0; s < kSubsets; ++s) {
+                    const float other = merge_max[(quadrant % kApart) + s * kApart][lane];
+                    total += other == kNoKey ? 0.0f
+                                             : merge_sum[(quadrant % kApart) + s * kApart][lane] * fast_exp2(other - top);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    uint32_t part[16];
+                    sm100::tmem_ld_32x16(my_output + 16 * r, part);
+                    sm100::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {     // (a copy that saw no key may hold 0 times anything)
+                            v[c] = m == kNoKey ? 0.0f : __uint_as_float(part[4 * i + c]) * mine;
+                        }
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(my_staging + i * 512 + lane * 16),
+                                     "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3])
+                                     : "memory");
+                    }
+                    ok = meeting.meet() && ok;
+                    if (subset == r * kSubsets / 4) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int s = 0; s < kSubsets; ++s) {
+                                float v[4];
+                                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                                             : "r"(staging + ((quadrant % kApart) + s * kApart) * 2048 + i * 512 + lane * 16)
+                                             : "memory");
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) {
+                                    sum[c] += v[c];
+                                }
+                            }
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                acc[(16 * r + 4 * i + c) % kOut] = sum[c];
+                            }
+                        }
+                    }
+                    ok = meeting.meet() && ok;     // (the staging is read)
+                }
+                m = top;
+                if (!ok) {
+                    break;
                 }
             }
             sm100::tc_fence_before_sync();
-            if (valid && whole && p.a.lse != nullptr) {
-                p.a.lse[static_cast<long long>(head) * p.a.rows + at_row] =
-                    position < 0 ? -INFINITY : (m + log2f(total)) * kLn2;
-            }
-            if (valid && !whole) {
-                part[kRows * kHead + row] = m;
-                part[kRows * kHead + kRows + row] = total;
+            if (whole) {
+                const float inv = position < 0 ? 0.0f : 1.0f / total;   // no key at all gives zeros
+                uint4 halves[kOut / 8];
+#pragma unroll
+                for (int b = 0; b < kOut / 8; ++b) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[i] = position < 0 ? 0.0f : acc[b * 8 + i] * inv;
+                    }
+                    halves[b] = pack8(v);
+                }
+                __half* out = p.a.o + out_row * p.a.o_stride + head * kHead + subset * kOut;
+                if constexpr (kSubsets == 1) {
+                    // Through shared memory, so that a row's 64 bytes leave by four lanes: rows are apart in memory,
+                    // and 32 of them at 16 bytes each took 3,000 clocks.
+                    const unsigned long long to_row = valid ? reinterpret_cast<unsigned long long>(out) : 0ull;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint4 q = halves[4 * half + b];
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                             my_staging + lane * 64 + ((b ^ ((lane >> 1) & 3)) << 4)),
+                                         "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
+                                         : "memory");
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const int r = 8 * b + lane / 4;
+                            uint4 q;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                                         : "r"(my_staging + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4))
+                                         : "memory");
+                            const unsigned long long there = __shfl_sync(kFullMask, to_row, r);
+                            if (there != 0) {
+                                reinterpret_cast<uint4*>(there)[4 * half + (lane & 3)] = q;
+                            }
+                        }
+                        __syncwarp();
+                    }
+                } else if (valid) {
+#pragma unroll
+                    for (int b = 0; b < kOut / 8; ++b) {
+                        reinterpret_cast<uint4*>(out)[b] = halves[b];
+                    }
+                }
+                if (valid && subset == 0 && p.a.lse != nullptr) {
+                    p.a.lse[static_cast<long long>(head) * p.a.rows + out_row] =
+                        position < 0 ? -INFINITY : (m + log2f(total)) * kLn2;
+                }
+            } else if (valid) {
+                float* part = p.parts + (2 * size_t{blockIdx.x} + (from == 0 ? 1 : 0)) * kPartFloats;
+#pragma unroll
+                for (int b = 0; b < kOut / 4; ++b) {
+                    reinterpret_cast<float4*>(part)[(subset * (kOut / 4) + b) * kRows + row] =
+                        make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
+                }
+                if (subset == 0) {
+                    part[kRows * kHead + row] = m;
+                    part[kRows * kHead + kRows + row] = total;
+                }
             }
         }
     }
@@ -616,63 +840,95 @@ struct JoinParams {
     int ctas, group;
 };
 
-// Block (k, y) joins rows 32 y .. of the tile that CTA k began and did not end, if there is one: eight threads
-// per row, eight columns each.
+constexpr int kJoinSplit = 4;     // blocks per tile
+
+// Blocks (k, 0 .. 3) join the tile that CTA k began and did not end, if there is one: a warp per row, 16 lanes by
+// four columns, the parts in two halves.
 __global__ void __launch_bounds__(256) fb_packed_join(const JoinParams p) {
+    __shared__ int ends;
     dependency_wait();
     dependency_release();
     const int k = static_cast<int>(blockIdx.x);
+    if (p.records[k].tail_part == 0) {
+        return;
+    }
     const Record mine = p.records[k];
-    if (mine.tail_part == 0) {
-        return;
+    if (threadIdx.x == 0) {
+        ends = p.ctas - 1;
     }
-    const int row = static_cast<int>(blockIdx.y) * 32 + threadIdx.x / 8;
-    const int piece = threadIdx.x % 8;
-    const int token = row / p.group;
-    if (token >= mine.tokens) {
-        return;
-    }
-    int last = k + 1;
-    while (last < p.ctas - 1 && p.records[last].head_part == 2) {
-        ++last;
-    }
-    auto part_of = [&](int cta) { return p.parts + (2 * static_cast<size_t>(cta) + (cta == k ? 1 : 0)) * kPartFloats; };
-    float top = kNoKey;
-    for (int cta = k; cta <= last; ++cta) {
-        top = max3_nan(top, part_of(cta)[kRows * kHead + row], kNoKey);
-    }
-    float total = 0.0f;
-    float acc[8] = {};
-#pragma unroll 4
-    for (int cta = k; cta <= last; ++cta) {
-        const float* part = part_of(cta);
-        const float m = part[kRows * kHead + row];
-        const float weight = m == kNoKey ? 0.0f : fast_exp2(m - top);
-        const float4 x = reinterpret_cast<const float4*>(part)[(2 * piece) * kRows + row];
-        const float4 y = reinterpret_cast<const float4*>(part)[(2 * piece + 1) * kRows + row];
-        const float sum = part[kRows * kHead + kRows + row];
-        if (m != kNoKey) {    // (a part of no key may hold 0 times anything)
-            total = fmaf(sum, weight, total);
-            acc[0] = fmaf(x.x, weight, acc[0]);
-            acc[1] = fmaf(x.y, weight, acc[1]);
-            acc[2] = fmaf(x.z, weight, acc[2]);
-            acc[3] = fmaf(x.w, weight, acc[3]);
-            acc[4] = fmaf(y.x, weight, acc[4]);
-            acc[5] = fmaf(y.y, weight, acc[5]);
-            acc[6] = fmaf(y.z, weight, acc[6]);
-            acc[7] = fmaf(y.w, weight, acc[7]);
+    __syncthreads();
+    // The first CTA behind k whose part of the tile is its last.
+    for (int cta = k + 1 + threadIdx.x; cta < p.ctas; cta += 256) {
+        if (p.records[cta].head_part != 2) {
+            atomicMin(&ends, cta);
+            break;
         }
     }
-    const bool none = mine.position + token < 0;
-    const int head = mine.kv_head * p.group + row - token * p.group;
-    const long long at_row = mine.first_row + token;
+    __syncthreads();
+    const int last = ends;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int column = lane % 16;     // by four
+    const float* first = p.parts + (2 * static_cast<size_t>(k) + 1) * kPartFloats;
+    const float* rest = p.parts + 2 * static_cast<size_t>(k) * kPartFloats;     // CTA k + i's head part: 2 i parts on
+    const int count = last - k + 1;
+    auto part_of = [&](int i) { return i == 0 ? first : rest + 2 * static_cast<size_t>(i) * kPartFloats; };
+    for (int row = warp * kJoinSplit + static_cast<int>(blockIdx.y); row < mine.tokens * p.group;
+         row += 8 * kJoinSplit) {
+        float top = kNoKey;
+        for (int i = lane; i < count; i += 32) {
+            top = max3_nan(top, part_of(i)[kRows * kHead + row], kNoKey);
+        }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        acc[i] = none ? 0.0f : acc[i] / total;
-    }
-    *reinterpret_cast<uint4*>(p.a.o + at_row * p.a.o_stride + head * kHead + 8 * piece) = pack8(acc);
-    if (piece == 0 && p.a.lse != nullptr) {
-        p.a.lse[static_cast<long long>(head) * p.a.rows + at_row] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+        for (int off = 16; off > 0; off >>= 1) {
+            top = max3_nan(top, __shfl_xor_sync(kFullMask, top, off), kNoKey);
+        }
+        float total = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int from = 0; from < count; from += 32) {
+            // A lane's part's weight (0 for a part of no key, which may hold 0 times anything), then all of them in turn.
+            float weight = 0.0f;
+            if (from + lane < count) {
+                const float* part = part_of(from + lane);
+                const float m = part[kRows * kHead + row];
+                weight = m == kNoKey ? 0.0f : fast_exp2(m - top);
+                total += m == kNoKey ? 0.0f : part[kRows * kHead + kRows + row] * weight;
+            }
+            const int here = min(32, count - from);
+#pragma unroll 4
+            for (int i = 0; i < here; i += 2) {
+                const int at = i + lane / 16;
+                const float w = __shfl_sync(kFullMask, weight, at % 32);
+                if (at < here) {
+                    const float4 x = reinterpret_cast<const float4*>(part_of(from + at))[column * kRows + row];
+                    if (w != 0.0f) {
+                        acc.x = fmaf(x.x, w, acc.x);
+                        acc.y = fmaf(x.y, w, acc.y);
+                        acc.z = fmaf(x.z, w, acc.z);
+                        acc.w = fmaf(x.w, w, acc.w);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            total += __shfl_xor_sync(kFullMask, total, off);
+        }
+        acc.x += __shfl_xor_sync(kFullMask, acc.x, 16);
+        acc.y += __shfl_xor_sync(kFullMask, acc.y, 16);
+        acc.z += __shfl_xor_sync(kFullMask, acc.z, 16);
+        acc.w += __shfl_xor_sync(kFullMask, acc.w, 16);
+        const int token = row / p.group;
+        const bool none = mine.position + token < 0;
+        const int head = mine.kv_head * p.group + row - token * p.group;
+        const long long at_row = mine.first_row + token;
+        if (lane < 16) {
+            const float inv = 1.0f / total;
+            const uint2 q = none ? make_uint2(0u, 0u) : make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+            *reinterpret_cast<uint2*>(p.a.o + at_row * p.a.o_stride + head * kHead + 4 * column) = q;
+        }
+        if (lane == 0 && p.a.lse != nullptr) {
+            p.a.lse[static_cast<long long>(head) * p.a.rows + at_row] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+        }
     }
 }
 
@@ -691,27 +947,30 @@ cudaError_t packed_forward_workspace(size_t* bytes) {
     return e;
 }
 
-cudaError_t packed_forward(const PackedArgs& args, void* workspace, cudaStream_t stream) {
+cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace, cudaStream_t stream) {
     TileParams p;
     std::memset(&p, 0, sizeof p);
     p.a = args;
     p.group = args.heads / args.kv_heads;
-    while ((2 << p.log_tokens) * p.group <= kRows) {
+    const bool paged = args.table != nullptr;
+    // Few rows per K/V head and sequence: in two or four copies.
+    const long long rows = static_cast<long long>(longest) * p.group;
+    const int subsets = !paged || rows > 64 ? 1 : rows > 32 ? 2 : 4;
+    while ((2 << p.log_tokens) * p.group <= kRows / subsets) {
         ++p.log_tokens;
     }
     int sms = 148;
     cudaError_t e = sm_count(&sms);
     const int ctas = 2 * sms;
-    const bool paged = args.table != nullptr;
     if (e == cudaSuccess) {
         e = encode_rows(&p.map_q, args.q, args.heads, args.rows, args.q_stride, p.group, 1 << p.log_tokens);
     }
     if (paged) {
         p.box_rows = std::min(args.page_size, kKeyTile);
         p.boxes = kKeyTile / p.box_rows;
-        const long long rows = args.pages * args.kv_heads * args.page_size;
-        if (e == cudaSuccess) e = encode_pages(&p.map_k, args.k, rows, p.box_rows);
-        if (e == cudaSuccess) e = encode_pages(&p.map_v, args.v, rows, p.box_rows);
+        const long long cache_rows = args.pages * args.kv_heads * args.page_size;
+        if (e == cudaSuccess) e = encode_pages(&p.map_k, args.k, cache_rows, p.box_rows);
+        if (e == cudaSuccess) e = encode_pages(&p.map_v, args.v, cache_rows, p.box_rows);
     } else {
         if (e == cudaSuccess) e = encode_rows(&p.map_k, args.k, args.kv_heads, args.rows, args.kv_stride, 1, kKeyTile);
         if (e == cudaSuccess) e = encode_rows(&p.map_v, args.v, args.kv_heads, args.rows, args.kv_stride, 1, kKeyTile);
@@ -721,9 +980,13 @@ cudaError_t packed_forward(const PackedArgs& args, void* workspace, cudaStream_t
     }
     p.records = static_cast<Record*>(workspace);
     p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + records_bytes(ctas));
-    const auto kernel = paged ? fb_packed_forward_tiles<true> : fb_packed_forward_tiles<false>;
-    static std::atomic<bool> configured[2][64] = {};
-    e = allow_shared_memory(kernel, kSmem, configured[paged]);
+    const int form = !paged ? 0 : subsets == 1 ? 1 : subsets == 2 ? 2 : 3;
+    const auto kernel = form == 0   ? fb_packed_forward_tiles<false, 1>
+                        : form == 1 ? fb_packed_forward_tiles<true, 1>
+                        : form == 2 ? fb_packed_forward_tiles<true, 2>
+                                    : fb_packed_forward_tiles<true, 4>;
+    static std::atomic<bool> configured[4][64] = {};
+    e = allow_shared_memory(kernel, kSmem, configured[form]);
     if (e != cudaSuccess) {
         return e;
     }
@@ -732,7 +995,7 @@ cudaError_t packed_forward(const PackedArgs& args, void* workspace, cudaStream_t
         return e;
     }
     JoinParams j = {args, p.records, p.parts, ctas, p.group};
-    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(ctas), kRows / 32), dim3(256), 0, stream, j);
+    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(ctas), kJoinSplit), dim3(256), 0, stream, j);
 }
 
 }  // namespace fb

@@ -19,6 +19,14 @@ namespace fb {
 
 constexpr int kKeyTile = 128;
 
+// a / b for b > 0, by the short division where it does (the long one takes hundreds of instructions).
+FB_SCHEDULE long long quotient(long long a, long long b) {
+    if (((a | b) >> 31) == 0) {
+        return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+    }
+    return a / b;
+}
+
 // Sum of w >> shift over w = 0 .. z.
 FB_SCHEDULE long long floor_sum(long long z, int shift) {
     const long long q = z >> shift;
@@ -32,7 +40,7 @@ FB_SCHEDULE long long floor_sum(long long z, int shift) {
 FB_SCHEDULE int key_tiles(int before, int tokens, int log_tokens, int i) {
     const long long end = (static_cast<long long>(i) + 1) << log_tokens;
     const long long visible = before + (end < tokens ? end : tokens);
-    return visible <= kKeyTile ? 1 : static_cast<int>((visible + kKeyTile - 1) / kKeyTile);
+    return visible <= kKeyTile ? 1 : static_cast<int>((visible + kKeyTile - 1) >> 7);
 }
 
 // Length on the line of the tiles 0 .. i - 1 of one head, all of them full: without a loop, since
@@ -75,7 +83,7 @@ FB_SCHEDULE Cut cut_at(long long at, long long into, int sequence, int before, i
                        long long length, long long tolerance) {
     Cut c;
     c.sequence = sequence;
-    c.head = static_cast<int>(into / length);
+    c.head = static_cast<int>(quotient(into, length));
     const long long x = into - c.head * length;
     int low = 0, high = tile_count(tokens, log_tokens) - 1;   // the last tile that begins at or before x
     while (low < high) {
@@ -102,14 +110,14 @@ FB_SCHEDULE Cut cut_at(long long at, long long into, int sequence, int before, i
 // Parts that the line is cut into (up to `most`, none shorter than `least`), the place of cut k, and how
 // far a cut may move.
 FB_SCHEDULE int part_count(long long total, int most, int least) {
-    const long long parts = (total + least - 1) / least;
+    const long long parts = quotient(total + least - 1, least);
     return parts < most ? static_cast<int>(parts) : most;
 }
 FB_SCHEDULE long long cut_place(long long total, int parts, int k) {
-    const long long each = total / parts, over = total - each * parts;
-    return each * k + over * k / parts;
+    const long long each = quotient(total, parts), over = total - each * parts;
+    return each * k + quotient(over * k, parts);
 }
-FB_SCHEDULE long long cut_tolerance(long long total, int parts) { return total / parts / 8; }
+FB_SCHEDULE long long cut_tolerance(long long total, int parts) { return quotient(total, parts) / 8; }
 
 // A sequence's place in the rows (its new tokens) and how many keys it has, those among them.
 struct Sequence {
