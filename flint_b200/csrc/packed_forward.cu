@@ -44,7 +44,8 @@ constexpr int kSlots = 4;       // ring of K and V tiles
 constexpr int kStagingBytes = 4 * 2048;
 constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
-constexpr int kLeastPart = 2;   // of the line of key tiles, per CTA
+constexpr int kLeastPart = 4;   // of the line of key tiles, per CTA
+constexpr int kWholeKeys = 256; // up to which a tile is never split
 
 constexpr size_t kPartFloats = size_t{kRows} * kHead + 2 * kRows;   // O [column / 4][row][4], maxima, sums
 
@@ -56,6 +57,7 @@ struct TileParams {
     int group, log_tokens;
     int boxes;          // loads per K or V tile
     int box_rows;
+    bool splits;        // tiles may be split between CTAs
 };
 
 struct Barriers {
@@ -87,87 +89,117 @@ struct SequenceOf {
     __device__ __forceinline__ Sequence operator()(int s) const { return sequence_at(a, s); }
 };
 
-// Which part of the line this CTA works on: every thread of the block takes part.
-__device__ void locate(const TileParams& p, Cut (&cuts)[2], long long (&scan)[kWarps + 1]) {
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
-    auto length_of = [&](int s, int& before, int& tokens) -> long long {
-        before = tokens = 0;
-        if (s >= p.a.sequences) {
-            return 0;
-        }
-        const Sequence q = sequence_at(p.a, s);
-        before = q.keys - q.count;
-        tokens = q.count;
-        return head_length(before, tokens, p.log_tokens);
-    };
-    int before = 0, tokens = 0;
-    long long length = length_of(tid, before, tokens);
-    long long sum = length;
-    for (int s = tid + kThreads; s < p.a.sequences; s += kThreads) {
-        int b, t;
-        sum += length_of(s, b, t);
-    }
+__device__ __forceinline__ long long warp_sum(long long v) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
-        sum += __shfl_xor_sync(kFullMask, sum, off);
+        v += __shfl_xor_sync(kFullMask, v, off);
     }
+    return v;
+}
+__device__ __forceinline__ long long warp_prefix(long long v, int lane) {     // inclusive
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long other = __shfl_up_sync(kFullMask, v, off);
+        v += lane >= off ? other : 0;
+    }
+    return v;
+}
+
+// The places of this CTA's two cuts among `parts`; none for a CTA without a part.
+struct Places {
+    int parts;
+    long long at[2], tolerance, total;
+    __device__ __forceinline__ Places(const TileParams& p, long long line) : total(line) {
+        parts = part_count(total, static_cast<int>(gridDim.x), kLeastPart);
+        const int cta = static_cast<int>(blockIdx.x);
+        if (cta < parts) {
+            at[0] = cut_place(total, parts, cta);
+            at[1] = cut_place(total, parts, cta + 1);
+            tolerance = p.splits ? cut_tolerance(total, parts) : total;
+        } else {
+            at[0] = at[1] = total;
+            tolerance = 0;
+        }
+    }
+};
+
+__device__ __forceinline__ long long length_of(const TileParams& p, int s, int& before, int& tokens) {
+    before = tokens = 0;
+    if (s >= p.a.sequences) {
+        return 0;
+    }
+    const Sequence q = sequence_at(p.a, s);
+    before = q.before();
+    tokens = q.count;
+    return head_length(before, tokens, p.log_tokens);
+}
+
+// Which part of the line this CTA works on, for up to 32 sequences: one warp.
+__device__ __forceinline__ void locate_in_warp(const TileParams& p, Cut (&cuts)[2], int lane) {
+    int before, tokens;
+    const long long length = length_of(p, lane, before, tokens);
+    const long long mine = length * p.a.kv_heads;
+    const long long upto = warp_prefix(mine, lane);
+    const Places place(p, __shfl_sync(kFullMask, upto, 31));
+    const long long begins = upto - mine;
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+        const long long at = place.at[c];
+        if (at == place.total) {
+            if (lane == 0) {
+                cuts[c] = Cut{at, p.a.sequences, 0, 0, 0};
+            }
+        } else if (at >= begins && at < upto) {
+            cuts[c] = cut_at(at, at - begins, lane, before, tokens, p.log_tokens, length, place.tolerance);
+        }
+    }
+}
+
+// The same for any number: every thread of the block takes part.
+__device__ __noinline__ void locate(const TileParams& p, Cut (&cuts)[2], long long (&scan)[kWarps + 1]) {
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
+    int before = 0, tokens = 0;
+    long long sum = 0;
+    for (int s = tid; s < p.a.sequences; s += kThreads) {
+        sum += length_of(p, s, before, tokens);
+    }
+    sum = warp_sum(sum);
     if (lane == 0) {
         scan[warp] = sum;
     }
     __syncthreads();
     long long total = 0;
-#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         total += scan[w];
     }
-    total *= p.a.kv_heads;
-    const int parts = part_count(total, static_cast<int>(gridDim.x), kLeastPart);
-    const int cta = static_cast<int>(blockIdx.x);
-    if (cta >= parts) {
-        if (tid < 2) {
-            cuts[tid] = Cut{0, 0, 0, 0, 0};
-        }
-        __syncthreads();
-        return;
-    }
-    const long long place[2] = {cut_place(total, parts, cta), cut_place(total, parts, cta + 1)};
-    const long long tolerance = cut_tolerance(total, parts);
-    if (tid < 2 && place[tid] == total) {
-        cuts[tid] = Cut{total, p.a.sequences, 0, 0, 0};
+    const Places place(p, total * p.a.kv_heads);
+    if (tid < 2 && place.at[tid] == place.total) {
+        cuts[tid] = Cut{place.total, p.a.sequences, 0, 0, 0};
     }
     long long running = 0;
     for (int first = 0; first < p.a.sequences; first += kThreads) {
-        if (first != 0) {
-            length = length_of(first + tid, before, tokens);
-        }
+        const long long length = length_of(p, first + tid, before, tokens);
         const long long mine = length * p.a.kv_heads;
-        long long upto = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const long long other = __shfl_up_sync(kFullMask, upto, off);
-            upto += lane >= off ? other : 0;
-        }
+        long long upto = warp_prefix(mine, lane);
         __syncthreads();
         if (lane == 31) {
             scan[warp] = upto;
         }
         __syncthreads();
         long long all = 0;
-#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             upto += w < warp ? scan[w] : 0;
             all += scan[w];
         }
         const long long begins = running + upto - mine;
         for (int c = 0; c < 2; ++c) {
-            if (place[c] >= begins && place[c] < begins + mine) {
-                cuts[c] = cut_at(place[c], place[c] - begins, first + tid, before, tokens, p.log_tokens, length,
-                                 tolerance);
+            if (place.at[c] >= begins && place.at[c] < begins + mine) {
+                cuts[c] = cut_at(place.at[c], place.at[c] - begins, first + tid, before, tokens, p.log_tokens, length,
+                                 place.tolerance);
             }
         }
         running += all;
     }
-    __syncthreads();
 }
 
 // A piece as the TMA warp hands it to the others; `to` of 0 ends the list.
@@ -243,7 +275,11 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         sm100::tmem_alloc(sm100::smem_u32(&tmem_slot), 256);
     }
     dependency_wait();
-    locate(p, cuts, scan);
+    if (p.a.sequences > 32) {
+        locate(p, cuts, scan);
+    } else if (warp == 2) {
+        locate_in_warp(p, cuts, lane);
+    }
     sm100::tc_fence_before_sync();
     __syncthreads();
     sm100::tc_fence_after_sync();
@@ -505,6 +541,15 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         const int head_of_group = row - token * p.group;
         const float scale2 = p.a.scale * kLog2e;
         const F2 scale_pair = f2_pack(scale2, scale2);
+        // The rows whose parts this lane stores for its warp: rows 8 b + lane / 4.
+        int store_token[4];
+        long long store_at[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int r = quadrant * 32 + 8 * b + lane / 4;
+            store_token[b] = r / p.group;
+            store_at[b] = store_token[b] * p.a.o_stride + (r - store_token[b] * p.group) * kHead;
+        }
         Meeting meeting{bar.meeting(), 0, abort, lane};
         if (quadrant == 0 && lane == 0) {
             p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, cuts[0], cuts[1]);
@@ -532,8 +577,10 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             const int first_position = info.position;
             const bool valid = token < info.tokens;
             const int position = valid ? first_position + token : -1;
-            const long long out_row = info.first_row + token;
-            const int head = info.head * p.group + head_of_group;
+            const long long info_row = info.first_row;
+            const int info_head = info.head * p.group, info_tokens = info.tokens;
+            const long long out_row = info_row + token;
+            const int head = info_head + head_of_group;
             const bool active = __any_sync(kFullMask, valid);
             float m = kNoKey;     // reference exponent of the row (base 2)
             F2 l = 0;             // the row sum, in two partial sums
@@ -753,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     float v[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        v[i] = position < 0 ? 0.0f : acc[b * 8 + i] * inv;
+                        v[i] = kPaged && position < 0 ? 0.0f : acc[b * 8 + i] * inv;
                     }
                     halves[b] = pack8(v);
                 }
@@ -761,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 if constexpr (kSubsets == 1) {
                     // Through shared memory, so that a row's 64 bytes leave by four lanes: rows are apart in memory,
                     // and 32 of them at 16 bytes each took 3,000 clocks.
-                    const unsigned long long to_row = valid ? reinterpret_cast<unsigned long long>(out) : 0ull;
+                    __half* tile_out = p.a.o + info_row * p.a.o_stride + info_head * kHead;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -781,9 +828,8 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                                          : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
                                          : "r"(my_staging + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4))
                                          : "memory");
-                            const unsigned long long there = __shfl_sync(kFullMask, to_row, r);
-                            if (there != 0) {
-                                reinterpret_cast<uint4*>(there)[4 * half + (lane & 3)] = q;
+                            if (store_token[b] < info_tokens) {
+                                reinterpret_cast<uint4*>(tile_out + store_at[b])[4 * half + (lane & 3)] = q;
                             }
                         }
                         __syncwarp();
@@ -840,95 +886,181 @@ struct JoinParams {
     int ctas, group;
 };
 
-constexpr int kJoinSplit = 4;     // blocks per tile
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kMostCtas = 1024;
+constexpr int kManyParts = 16;      // from which on a tile's parts are shared out among the warps
 
-// Blocks (k, 0 .. 3) join the tile that CTA k began and did not end, if there is one: a warp per row, 16 lanes by
-// four columns, the parts in two halves.
-__global__ void __launch_bounds__(256) fb_packed_join(const JoinParams p) {
-    __shared__ int ends;
+// Of a row's parts, weighted by 2^(m - top): what a lane adds up for its row and four columns.
+struct JoinSum {
+    float total;
+    float4 acc;
+    __device__ __forceinline__ void add(const float* part, int row, int column, float top) {
+        const float m = part[kRows * kHead + row];
+        const float sum = part[kRows * kHead + kRows + row];
+        const float4 x = reinterpret_cast<const float4*>(part)[column * kRows + row];
+        const float w = fast_exp2(m - top);
+        if (m != kNoKey) {     // (a part of no key may hold 0 times anything)
+            total = fmaf(sum, w, total);
+            acc.x = fmaf(x.x, w, acc.x);
+            acc.y = fmaf(x.y, w, acc.y);
+            acc.z = fmaf(x.z, w, acc.z);
+            acc.w = fmaf(x.w, w, acc.w);
+        }
+    }
+};
+
+// Every block lists the split tiles from the CTAs' records and takes its share of items: 32 rows of a tile and
+// 32 columns, four of them per warp and a row per lane; or, of a tile in many parts, four columns, the
+// parts among the warps. Parts are added in the order of the keys.
+__global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams p) {
+    __shared__ unsigned ends[kMostCtas / 32];        // bit k: CTA k's first piece is not the middle of a tile
+    __shared__ unsigned begins[kMostCtas / 32];      // bit k: CTA k's last tile goes on behind it
+    __shared__ int list[2][kMostCtas];               // CTAs that begin split tiles: of few, of many parts
+    __shared__ int counts[2];
+    __shared__ float tops[kJoinWarps][32];
+    __shared__ float sums[kJoinWarps][32][5];
+    __shared__ uint2 rows_out[32][9];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
     dependency_wait();
     dependency_release();
-    const int k = static_cast<int>(blockIdx.x);
-    if (p.records[k].tail_part == 0) {
+    if (tid < 2) {
+        counts[tid] = 0;
+    }
+    bool any = false;
+    for (int k = tid; k < (p.ctas + 31) / 32 * 32; k += kJoinThreads) {
+        const int head_part = k < p.ctas ? p.records[k].head_part : 0;
+        const int tail_part = k < p.ctas ? p.records[k].tail_part : 0;
+        const unsigned e = __ballot_sync(kFullMask, head_part != 2), b = __ballot_sync(kFullMask, tail_part != 0);
+        if (lane == 0) {
+            ends[k / 32] = e;
+            begins[k / 32] = b;
+        }
+        any = any || b != 0;
+    }
+    if (__syncthreads_or(any ? 1 : 0) == 0) {
         return;
     }
-    const Record mine = p.records[k];
-    if (threadIdx.x == 0) {
-        ends = p.ctas - 1;
+    auto last_of = [&](int k) {
+        // The first CTA behind k whose piece of the tile is its last.
+        int word = (k + 1) / 32;
+        unsigned bits = ends[word] & (kFullMask << ((k + 1) % 32));
+        while (bits == 0 && word + 1 < (p.ctas + 31) / 32) {
+            bits = ends[++word];
+        }
+        return bits != 0 ? min(word * 32 + __ffs(bits) - 1, p.ctas - 1) : p.ctas - 1;
+    };
+    // The list's order is the CTAs': warp 0 appends 32 at a time.
+    if (warp == 0) {
+        int few = 0, many = 0;
+        for (int from = 0; from < p.ctas; from += 32) {
+            const int k = from + lane;
+            const bool split = ((begins[from / 32] >> lane) & 1) != 0 && k + 1 < p.ctas;
+            const bool long_one = split && last_of(k) - k + 1 > kManyParts;
+            const unsigned f = __ballot_sync(kFullMask, split && !long_one), m = __ballot_sync(kFullMask, long_one);
+            const unsigned below = (1u << lane) - 1;
+            if (split) {
+                list[long_one][(long_one ? many : few) + __popc((long_one ? m : f) & below)] = k;
+            }
+            few += __popc(f);
+            many += __popc(m);
+        }
+        if (lane == 0) {
+            counts[0] = few;
+            counts[1] = many;
+        }
     }
     __syncthreads();
-    // The first CTA behind k whose part of the tile is its last.
-    for (int cta = k + 1 + threadIdx.x; cta < p.ctas; cta += 256) {
-        if (p.records[cta].head_part != 2) {
-            atomicMin(&ends, cta);
-            break;
+    const int few_items = counts[0] * (kRows / 32) * 2, many_items = counts[1] * (kRows / 32) * 16;
+    for (int item = static_cast<int>(blockIdx.x); item < few_items + many_items; item += static_cast<int>(gridDim.x)) {
+        const bool many = item >= few_items;
+        const int each = many ? (kRows / 32) * 16 : (kRows / 32) * 2;
+        const int at = many ? item - few_items : item;
+        const int k = list[many][at / each];
+        const int columns = at % each / (kRows / 32);
+        const int row = at % (kRows / 32) * 32 + lane;
+        const Record mine = p.records[k];
+        if (row - lane >= mine.tokens * p.group) {
+            continue;
         }
-    }
-    __syncthreads();
-    const int last = ends;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int column = lane % 16;     // by four
-    const float* first = p.parts + (2 * static_cast<size_t>(k) + 1) * kPartFloats;
-    const float* rest = p.parts + 2 * static_cast<size_t>(k) * kPartFloats;     // CTA k + i's head part: 2 i parts on
-    const int count = last - k + 1;
-    auto part_of = [&](int i) { return i == 0 ? first : rest + 2 * static_cast<size_t>(i) * kPartFloats; };
-    for (int row = warp * kJoinSplit + static_cast<int>(blockIdx.y); row < mine.tokens * p.group;
-         row += 8 * kJoinSplit) {
-        float top = kNoKey;
-        for (int i = lane; i < count; i += 32) {
-            top = max3_nan(top, part_of(i)[kRows * kHead + row], kNoKey);
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-            top = max3_nan(top, __shfl_xor_sync(kFullMask, top, off), kNoKey);
-        }
-        float total = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int from = 0; from < count; from += 32) {
-            // A lane's part's weight (0 for a part of no key, which may hold 0 times anything), then all of them in turn.
-            float weight = 0.0f;
-            if (from + lane < count) {
-                const float* part = part_of(from + lane);
-                const float m = part[kRows * kHead + row];
-                weight = m == kNoKey ? 0.0f : fast_exp2(m - top);
-                total += m == kNoKey ? 0.0f : part[kRows * kHead + kRows + row] * weight;
-            }
-            const int here = min(32, count - from);
-#pragma unroll 4
-            for (int i = 0; i < here; i += 2) {
-                const int at = i + lane / 16;
-                const float w = __shfl_sync(kFullMask, weight, at % 32);
-                if (at < here) {
-                    const float4 x = reinterpret_cast<const float4*>(part_of(from + at))[column * kRows + row];
-                    if (w != 0.0f) {
-                        acc.x = fmaf(x.x, w, acc.x);
-                        acc.y = fmaf(x.y, w, acc.y);
-                        acc.z = fmaf(x.z, w, acc.z);
-                        acc.w = fmaf(x.w, w, acc.w);
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-            total += __shfl_xor_sync(kFullMask, total, off);
-        }
-        acc.x += __shfl_xor_sync(kFullMask, acc.x, 16);
-        acc.y += __shfl_xor_sync(kFullMask, acc.y, 16);
-        acc.z += __shfl_xor_sync(kFullMask, acc.z, 16);
-        acc.w += __shfl_xor_sync(kFullMask, acc.w, 16);
+        const int last = last_of(k);
+        auto part_of = [&](int cta) {
+            return p.parts + (2 * static_cast<size_t>(cta) + (cta == k ? 1 : 0)) * kPartFloats;
+        };
         const int token = row / p.group;
+        const bool valid = token < mine.tokens;
         const bool none = mine.position + token < 0;
         const int head = mine.kv_head * p.group + row - token * p.group;
         const long long at_row = mine.first_row + token;
-        if (lane < 16) {
-            const float inv = 1.0f / total;
-            const uint2 q = none ? make_uint2(0u, 0u) : make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-            *reinterpret_cast<uint2*>(p.a.o + at_row * p.a.o_stride + head * kHead + 4 * column) = q;
+        float top = kNoKey;
+        JoinSum sum = {};
+        if (!many) {
+            const int column = columns * 8 + warp;
+#pragma unroll 4
+            for (int cta = k; cta <= last; ++cta) {
+                top = max3_nan(top, part_of(cta)[kRows * kHead + row], kNoKey);
+            }
+#pragma unroll 4
+            for (int cta = k; cta <= last; ++cta) {
+                sum.add(part_of(cta), row, column, top);
+            }
+        } else {
+            const int column = columns;
+#pragma unroll 4
+            for (int cta = k + warp; cta <= last; cta += kJoinWarps) {
+                top = max3_nan(top, part_of(cta)[kRows * kHead + row], kNoKey);
+            }
+            tops[warp][lane] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) {
+                top = max3_nan(top, tops[w][lane], kNoKey);
+            }
+#pragma unroll 4
+            for (int cta = k + warp; cta <= last; cta += kJoinWarps) {
+                sum.add(part_of(cta), row, column, top);
+            }
+            sums[warp][lane][0] = sum.total;
+            sums[warp][lane][1] = sum.acc.x;
+            sums[warp][lane][2] = sum.acc.y;
+            sums[warp][lane][3] = sum.acc.z;
+            sums[warp][lane][4] = sum.acc.w;
+            __syncthreads();
+            if (warp == 0) {
+                for (int w = 1; w < kJoinWarps; ++w) {
+                    sum.total += sums[w][lane][0];
+                    sum.acc.x += sums[w][lane][1];
+                    sum.acc.y += sums[w][lane][2];
+                    sum.acc.z += sums[w][lane][3];
+                    sum.acc.w += sums[w][lane][4];
+                }
+            }
         }
-        if (lane == 0 && p.a.lse != nullptr) {
-            p.a.lse[static_cast<long long>(head) * p.a.rows + at_row] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+        const float inv = 1.0f / sum.total;
+        const uint2 q = none ? make_uint2(0u, 0u) : make_uint2(pack2(sum.acc.x * inv, sum.acc.y * inv),
+                                                               pack2(sum.acc.z * inv, sum.acc.w * inv));
+        __half* out = p.a.o + at_row * p.a.o_stride + head * kHead;
+        if (many) {
+            if (warp == 0 && valid) {
+                reinterpret_cast<uint2*>(out)[columns] = q;
+            }
+        } else {
+            // A row's 64 bytes leave by four lanes.
+            rows_out[lane][warp] = q;
+            __syncthreads();
+            const int r = tid / 4, quarter = tid % 4;
+            const int row_there = row - lane + r, token_there = row_there / p.group;
+            if (tid < 128 && token_there < mine.tokens) {
+                const uint2 a = rows_out[r][2 * quarter], b = rows_out[r][2 * quarter + 1];
+                __half* to = p.a.o + (mine.first_row + static_cast<long long>(token_there)) * p.a.o_stride +
+                             (mine.kv_head * p.group + row_there - token_there * p.group) * kHead + columns * 32;
+                reinterpret_cast<uint4*>(to)[quarter] = make_uint4(a.x, a.y, b.x, b.y);
+            }
         }
+        if (columns == 0 && warp == 0 && valid && p.a.lse != nullptr) {
+            p.a.lse[static_cast<long long>(head) * p.a.rows + at_row] = none ? -INFINITY : (top + log2f(sum.total)) * kLn2;
+        }
+        __syncthreads();      // (the shared arrays are read)
     }
 }
 
@@ -943,7 +1075,8 @@ cudaError_t packed_forward_error_flag(int* value, bool reset) { return read_erro
 cudaError_t packed_forward_workspace(size_t* bytes) {
     int sms = 148;
     const cudaError_t e = sm_count(&sms);
-    *bytes = records_bytes(2 * sms) + 2 * static_cast<size_t>(2 * sms) * kPartFloats * sizeof(float);
+    const int ctas = std::min(2 * sms, kMostCtas);
+    *bytes = records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * kPartFloats * sizeof(float);
     return e;
 }
 
@@ -961,7 +1094,7 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     }
     int sms = 148;
     cudaError_t e = sm_count(&sms);
-    const int ctas = 2 * sms;
+    const int ctas = std::min(2 * sms, kMostCtas);
     if (e == cudaSuccess) {
         e = encode_rows(&p.map_q, args.q, args.heads, args.rows, args.q_stride, p.group, 1 << p.log_tokens);
     }
@@ -978,6 +1111,9 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     if (e != cudaSuccess) {
         return e;
     }
+    // Few rows have few key tiles each: whole tiles for every CTA, and no join.
+    const long long most_keys = paged ? static_cast<long long>(args.table_stride) * args.page_size : args.rows;
+    p.splits = most_keys > kWholeKeys;
     p.records = static_cast<Record*>(workspace);
     p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + records_bytes(ctas));
     const int form = !paged ? 0 : subsets == 1 ? 1 : subsets == 2 ? 2 : 3;
@@ -991,11 +1127,11 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
         return e;
     }
     e = launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmem, stream, p);
-    if (e != cudaSuccess) {
+    if (e != cudaSuccess || !p.splits) {
         return e;
     }
     JoinParams j = {args, p.records, p.parts, ctas, p.group};
-    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(ctas), kJoinSplit), dim3(256), 0, stream, j);
+    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(4 * sms)), dim3(kJoinThreads), 0, stream, j);
 }
 
 }  // namespace fb

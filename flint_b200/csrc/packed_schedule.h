@@ -4,7 +4,7 @@
 // A tile is 2^log_tokens tokens of one sequence with all query heads of one K/V head; it works on key
 // tiles of 128 positions from 0 up to its last token's own. The tiles of all sequences, in the order
 // (sequence, K/V head, tile), lie one behind the other on a line, each as long as its key tiles
-// and one more for what starting and ending it costs. The line is cut into as many equal parts as
+// and two more for what starting and ending it costs. The line is cut into as many equal parts as
 // there are CTAs, so that however long and short the sequences are, CTAs work equally long; a cut
 // that falls close to a tile's end moves there. A tile that a cut splits is put together from parts afterwards.
 #pragma once
@@ -18,6 +18,7 @@ namespace fb {
 #endif
 
 constexpr int kKeyTile = 128;
+constexpr int kTileEnds = 2;
 
 // a / b for b > 0, by the short division where it does (the long one takes hundreds of instructions).
 FB_SCHEDULE long long quotient(long long a, long long b) {
@@ -51,11 +52,11 @@ FB_SCHEDULE long long tiles_before(int before, int log_tokens, int i) {
     const long long from = before + (none << log_tokens);
     const long long rest = i - none;
     if (rest == 0) {
-        return 2 * none;
+        return (1 + kTileEnds) * none;
     }
     const long long u = (from + kKeyTile - 1) >> log_tokens;
     const int shift = 7 - log_tokens;
-    return 2 * none + rest + floor_sum(u + rest, shift) - floor_sum(u, shift);
+    return (1 + kTileEnds) * none + kTileEnds * rest + floor_sum(u + rest, shift) - floor_sum(u, shift);
 }
 
 FB_SCHEDULE int tile_count(int tokens, int log_tokens) {
@@ -68,7 +69,7 @@ FB_SCHEDULE long long head_length(int before, int tokens, int log_tokens) {
         return 0;
     }
     const int last = tile_count(tokens, log_tokens) - 1;
-    return tiles_before(before, log_tokens, last) + key_tiles(before, tokens, log_tokens, last) + 1;
+    return tiles_before(before, log_tokens, last) + key_tiles(before, tokens, log_tokens, last) + kTileEnds;
 }
 
 // A place on the line. `tile` may be one past a head's last, `offset` is then 0.
@@ -95,7 +96,7 @@ FB_SCHEDULE Cut cut_at(long long at, long long into, int sequence, int before, i
         }
     }
     const long long offset = x - tiles_before(before, log_tokens, low);
-    const long long rest = key_tiles(before, tokens, log_tokens, low) + 1 - offset;
+    const long long rest = key_tiles(before, tokens, log_tokens, low) + kTileEnds - offset;
     c.at = at;
     c.tile = low;
     c.offset = static_cast<int>(offset);
@@ -117,7 +118,13 @@ FB_SCHEDULE long long cut_place(long long total, int parts, int k) {
     const long long each = quotient(total, parts), over = total - each * parts;
     return each * k + quotient(over * k, parts);
 }
-FB_SCHEDULE long long cut_tolerance(long long total, int parts) { return quotient(total, parts) / 8; }
+// An eighth of a part, and at least what a split costs (a second start and end, and the join's share), but never so far
+// that two cuts could meet.
+FB_SCHEDULE long long cut_tolerance(long long total, int parts) {
+    const long long each = quotient(total, parts);
+    const long long wanted = each / 8 > 3 ? each / 8 : 3;
+    return wanted < (each - 1) / 2 ? wanted : (each - 1) / 2;
+}
 
 // A sequence's place in the rows (its new tokens) and how many keys it has, those among them.
 struct Sequence {
@@ -170,7 +177,7 @@ struct Walk {
                 continue;
             }
             const int tiles = key_tiles(sequence.before(), sequence.count, log_tokens, tile);
-            const long long rest = tiles + 1 - offset;
+            const long long rest = tiles + kTileEnds - offset;
             const long long taken = rest < end - at ? rest : end - at;
             const int stop = offset + static_cast<int>(taken);
             out.sequence = sequence;

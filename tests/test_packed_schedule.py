@@ -51,7 +51,7 @@ int main() {
                 const int last = std::min((i + 1) << log_tokens, q.count);
                 const int sees = std::max(0, q.before() + last);
                 NEED(key_tiles(q.before(), q.count, log_tokens, i) == std::max(1, (sees + 127) / 128));
-                sum += key_tiles(q.before(), q.count, log_tokens, i) + 1;
+                sum += key_tiles(q.before(), q.count, log_tokens, i) + kTileEnds;
             }
             NEED(head_length(q.before(), q.count, log_tokens) == sum);
             total += sum * kv_heads;
@@ -139,7 +139,7 @@ int main() {
     // The largest sizes: no 32-bit overflow.
     const int trial = -1;
     NEED(head_length(0, 1 << 24, 0) > (1LL << 40));
-    NEED(head_length((1 << 26) - 1, 1, 0) == (1 << 19) + 1);
+    NEED(head_length((1 << 26) - 1, 1, 0) == (1 << 19) + kTileEnds);
     NEED(key_tiles((1 << 26) - (1 << 24), 1 << 24, 7, (1 << 17) - 1) == 1 << 19);
     return 0;
 }
