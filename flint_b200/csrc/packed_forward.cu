@@ -38,10 +38,12 @@ constexpr int kTileBytes = 128 * kHead * 2;   // Q, K or V: 16 KB
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-constexpr int kThreads = 192;   // TMA warp, MMA warp, four softmax warps with a row per thread
+constexpr int kThreads = 320;   // TMA warp, MMA warp, eight softmax warps with two threads per row
 constexpr int kWarps = kThreads / 32;
 constexpr int kSlots = 4;       // ring of K and V tiles
-constexpr int kStagingBytes = 4 * 2048;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kStaging = 1024;     // bytes per softmax warp
+constexpr int kStagingBytes = kSoftmaxWarps * kStaging;
 constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
 constexpr int kLeastPart = 4;   // of the line of key tiles, per CTA
@@ -69,9 +71,10 @@ struct Barriers {
     __device__ uint32_t p_ready() const { return base + 48; }
     __device__ uint32_t pv_done() const { return base + 56; }
     __device__ uint32_t meeting() const { return base + 64; }
-    __device__ uint32_t piece_full(int i) const { return base + 72 + 8u * i; }
-    __device__ uint32_t slot_full(int s) const { return base + 72 + 8u * (kPieces + s); }
-    __device__ uint32_t slot_empty(int s) const { return base + 72 + 8u * (kPieces + kSlots + s); }
+    __device__ uint32_t pair(int quadrant) const { return base + 72 + 8u * quadrant; }
+    __device__ uint32_t piece_full(int i) const { return base + 104 + 8u * i; }
+    __device__ uint32_t slot_full(int s) const { return base + 104 + 8u * (kPieces + s); }
+    __device__ uint32_t slot_empty(int s) const { return base + 104 + 8u * (kPieces + kSlots + s); }
 };
 
 constexpr uint32_t kIdescS = sm100::instr_desc_f16(128, 128, false, false);
@@ -237,14 +240,15 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
     const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_tiles = base;
     const uint32_t ring = base + 2 * kTileBytes;
-    const uint32_t staging = ring + kSlots * kTileBytes;      // 2 KB per softmax warp
+    const uint32_t staging = ring + kSlots * kTileBytes;
     const Barriers bar{staging + kStagingBytes};
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ Cut cuts[2];
     __shared__ long long scan[kWarps + 1];
     __shared__ PieceInfo pieces[kPieces];
-    __shared__ float merge_max[4][32], merge_sum[4][32];
+    __shared__ float pair_max[2][2][kRows];           // [step parity][half of the columns][row]
+    __shared__ float merge_max[4][32], merge_sum[kSoftmaxWarps][32];
 
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x / 32), 0);
     const int lane = threadIdx.x % 32;
@@ -255,10 +259,13 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             sm100::mbar_init(bar.q_empty(b), 1);
         }
         sm100::mbar_init(bar.s_full(), 1);
-        sm100::mbar_init(bar.s_free(), 4);     // one arrival per softmax warp
-        sm100::mbar_init(bar.p_ready(), 4);
+        sm100::mbar_init(bar.s_free(), kSoftmaxWarps);     // one arrival per softmax warp
+        sm100::mbar_init(bar.p_ready(), kSoftmaxWarps);
         sm100::mbar_init(bar.pv_done(), 1);
-        sm100::mbar_init(bar.meeting(), 4);
+        sm100::mbar_init(bar.meeting(), kSoftmaxWarps);
+        for (int q = 0; q < 4; ++q) {
+            sm100::mbar_init(bar.pair(q), 2);
+        }
         for (int i = 0; i < kPieces; ++i) {
             sm100::mbar_init(bar.piece_full(i), 1);
         }
@@ -283,6 +290,9 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
     sm100::tc_fence_before_sync();
     __syncthreads();
     sm100::tc_fence_after_sync();
+    if (threadIdx.x == 0) {
+        dependency_release();    // (the join's blocks take the place of this kernel's as they end)
+    }
     const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + 128, tmem_p = tmem_slot + 192;
     volatile int* abort = &abort_flag;
 
@@ -496,10 +506,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             const bool begins = begins_ahead;
             const int present = present_ahead;
             issue_scores();    // of the next step, as soon as this step's have been read
-            if (!ok || !sm100::mbar_wait_warp(bar.p_ready(), n & 1, abort)) {
-                break;
-            }
-            const uint32_t v_tile = next_tile();
+            const uint32_t v_tile = ok ? next_tile() : 0u;
             if (v_tile == 0) {
                 break;
             }
@@ -511,6 +518,10 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
+            if (!sm100::mbar_wait_warp(bar.p_ready(), n & 1, abort)) {
+                break;
+            }
+            sm100::tc_fence_after_sync();
             const uint64_t v_desc = desc_mnmajor(v_tile, 0, 16);
             if (sm100::elect_one()) {
                 sm100::mma_f16_ts_at<-1>(tmem_o, tmem_p, v_desc, 0, kIdescPV, begins ? 0u : 1u);
@@ -525,40 +536,36 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             step_ring();
         }
     } else {
-        constexpr int kColumns = kKeyTile / kSubsets;        // of a key tile, that this thread works on
-        constexpr int kChunks = kColumns / 32;
-        constexpr int kOut = kHead / kSubsets;               // columns of O that it writes
+        constexpr int kColumns = kKeyTile / kSubsets / 2;    // of a key tile, that this thread works on
+        constexpr int kChunk = kColumns < 32 ? kColumns : 32;
+        constexpr int kChunks = kColumns / kChunk;
+        constexpr int kOut = kHead / kSubsets / 2;           // columns of O that it writes
         constexpr int kCopyRows = kRows / kSubsets;
         const int quadrant = warp % 4;
+        const int half = (warp - 2) / 4;
         const int subset = quadrant * kSubsets / 4;
         const int row = (quadrant * 32 + lane) % kCopyRows;  // of the tile
+        const int lane_row = quadrant * 32 + lane;           // of the 128 lanes
         const uint32_t lane_base = static_cast<uint32_t>(quadrant * 32) << 16;
-        const uint32_t my_scores = tmem_s + lane_base + subset * kColumns;
-        const uint32_t my_weights = tmem_p + lane_base + subset * (kColumns / 2);
+        const int first_column = (subset * 2 + half) * kColumns;
+        const uint32_t my_scores = tmem_s + lane_base + first_column;
+        const uint32_t my_weights = tmem_p + lane_base + first_column / 2;
         const uint32_t my_output = tmem_o + lane_base;
-        const uint32_t my_staging = staging + quadrant * 2048;
+        const uint32_t my_staging = staging + (half * 4 + quadrant) * kStaging;
         const int token = row / p.group;
         const int head_of_group = row - token * p.group;
         const float scale2 = p.a.scale * kLog2e;
         const F2 scale_pair = f2_pack(scale2, scale2);
-        // The rows whose parts this lane stores for its warp: rows 8 b + lane / 4.
-        int store_token[4];
-        long long store_at[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int r = quadrant * 32 + 8 * b + lane / 4;
-            store_token[b] = r / p.group;
-            store_at[b] = store_token[b] * p.a.o_stride + (r - store_token[b] * p.group) * kHead;
-        }
         Meeting meeting{bar.meeting(), 0, abort, lane};
-        if (quadrant == 0 && lane == 0) {
+        Meeting pair{bar.pair(quadrant), 0, abort, lane};
+        if (quadrant == 0 && half == 0 && lane == 0) {
             p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, cuts[0], cuts[1]);
         }
         if (kSubsets > 1) {
             const uint32_t zeros[16] = {};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                sm100::tmem_st_32x16(tmem_p + lane_base + 16 * c, zeros);
+            for (int c = 0; c < 2; ++c) {
+                sm100::tmem_st_32x16(tmem_p + lane_base + 32 * half + 16 * c, zeros);
             }
             sm100::tmem_st_wait();
         }
@@ -577,53 +584,71 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             const int first_position = info.position;
             const bool valid = token < info.tokens;
             const int position = valid ? first_position + token : -1;
-            const long long info_row = info.first_row;
-            const int info_head = info.head * p.group, info_tokens = info.tokens;
-            const long long out_row = info_row + token;
-            const int head = info_head + head_of_group;
-            const bool active = __any_sync(kFullMask, valid);
-            float m = kNoKey;     // reference exponent of the row (base 2)
-            F2 l = 0;             // the row sum, in two partial sums
+            const int info_row = info.first_row, info_head = info.head * p.group, info_tokens = info.tokens;
+            const bool active = __any_sync(kFullMask, valid);    // (the same for a quadrant's two warps)
+            float m = kNoKey;     // reference exponent of the row (base 2), shared by its two threads
+            F2 l = 0;             // this thread's share of the row sum, in two partial sums
             for (int j = from; j < to; ++j, ++n) {
                 if (!sm100::mbar_wait_warp(bar.s_full(), n & 1, abort)) {
                     ok = false;
                     break;
                 }
                 sm100::tc_fence_after_sync();
-                // The scores are read twice, 32 columns at a time and the next 32 on their way: a row's
-                // 128 at once left no registers (the kernel spilled 950 bytes and took three times as long).
-                uint32_t raw[2][32];
-                const int visible = position - j * kKeyTile - subset * kColumns;     // columns up to this one are seen
+                // One copy of 64 columns is read twice, 32 at a time (two threads' registers do not hold
+                // them beside everything else: 500 bytes spilled); up to 32 once.
+                uint32_t raw[kChunk];
+                auto read = [&](int c) {
+                    if constexpr (kChunk == 32) {
+                        sm100::tmem_ld_32x32(my_scores + 32 * c, raw);
+                    } else {
+                        sm100::tmem_ld_32x16(my_scores, raw);
+                    }
+                    sm100::tmem_ld_wait();
+                };
                 const bool masked = j * kKeyTile + kKeyTile - 1 > first_position;
+                const int visible = position - j * kKeyTile - first_column;
+                auto mask = [&](int c) {
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < kChunk; ++i) {
+                            raw[i] = kChunk * c + i <= visible ? raw[i] : 0xff800000u;
+                        }
+                    }
+                };
+                auto scores_are_read = [&]() {     // the next step's may come
+                    sm100::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        sm100::mbar_arrive(bar.s_free());
+                    }
+                };
                 float alpha = 1.0f;
                 bool moved = false;
                 if (active) {
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    sm100::tmem_ld_32x32(my_scores, raw[0]);
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        sm100::tmem_ld_wait();
-                        if (kChunks > 1) {
-                            sm100::tmem_ld_32x32(my_scores + 32 * ((c + 1) % kChunks), raw[(c + 1) & 1]);
-                        }
-                        uint32_t (&now)[32] = raw[c & 1];
-                        if (masked) {
+                        read(c);
+                        mask(c);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                now[i] = 32 * c + i <= visible ? now[i] : 0xff800000u;
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
+                        for (int i = 0; i < kChunk; i += 8) {
 #pragma unroll
                             for (int t = 0; t < 4; ++t) {
-                                top[t] = max3_nan(top[t], __uint_as_float(now[i + t]), __uint_as_float(now[i + 4 + t]));
+                                top[t] = max3_nan(top[t], __uint_as_float(raw[i + t]), __uint_as_float(raw[i + 4 + t]));
                             }
                         }
                     }
+                    if (kChunks == 1) {
+                        scores_are_read();
+                    }
                     // The scale is positive, so the maximum may be scaled after it is taken.
                     const float local = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale2;
-                    const float mx = max3_nan(m, local, local);
+                    pair_max[n & 1][half][lane_row] = local;
+                    if (!pair.meet()) {
+                        ok = false;
+                        break;
+                    }
+                    const float mx = max3_nan(m, local, pair_max[n & 1][half ^ 1][lane_row]);
                     moved = valid && !(mx - m <= kLazyShift);   // (a NaN moves it too)
                     if (moved) {
                         alpha = fast_exp2(m - mx);
@@ -641,9 +666,9 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     if (j > from && __any_sync(kFullMask, moved)) {
                         const F2 a2 = f2_pack(alpha, alpha);
 #pragma unroll 1
-                        for (int c = 0; c < 4; ++c) {
+                        for (int c = 0; c < 2; ++c) {
                             uint32_t acc[16];
-                            sm100::tmem_ld_32x16(my_output + c * 16, acc);
+                            sm100::tmem_ld_32x16(my_output + 32 * half + c * 16, acc);
                             sm100::tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
@@ -652,35 +677,24 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                                 acc[i] = __float_as_uint(x);
                                 acc[i + 1] = __float_as_uint(y);
                             }
-                            sm100::tmem_st_32x16(my_output + c * 16, acc);
+                            sm100::tmem_st_32x16(my_output + 32 * half + c * 16, acc);
                         }
                     }
                     const F2 shift = f2_pack(-m, -m);
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        sm100::tmem_ld_wait();
-                        if (c + 1 < kChunks) {
-                            sm100::tmem_ld_32x32(my_scores + 32 * (c + 1), raw[(c + 1) & 1]);
-                        } else {
-                            // All scores are read: the next step's may come.
-                            sm100::tc_fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0) {
-                                sm100::mbar_arrive(bar.s_free());
+                        if (kChunks > 1) {
+                            read(c);
+                            if (c + 1 == kChunks) {
+                                scores_are_read();
                             }
+                            mask(c);
                         }
-                        uint32_t (&now)[32] = raw[c & 1];
-                        if (masked && kChunks > 1) {
+                        uint32_t packed[kChunk / 2];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                now[i] = 32 * c + i <= visible ? now[i] : 0xff800000u;
-                            }
-                        }
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
+                        for (int i = 0; i < kChunk / 2; ++i) {
                             float x, y;
-                            const F2 t = f2_fma(f2_pack(__uint_as_float(now[2 * i]), __uint_as_float(now[2 * i + 1])),
+                            const F2 t = f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])),
                                                 scale_pair, shift);
                             if (kSubsets == 1 && (i & 3) == 0) {
                                 exp2_pair_fma(t, x, y);
@@ -692,14 +706,15 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             l = f2_add(l, f2_pack(x, y));
                             packed[i] = pack2(x, y);
                         }
-                        sm100::tmem_st_32x16(my_weights + c * 16, packed);
+                        if constexpr (kChunk == 32) {
+                            sm100::tmem_st_32x16(my_weights + c * 16, packed);
+                        } else {
+                            sm100::tmem_st_32x8(my_weights, packed);
+                        }
                     }
                     sm100::tmem_st_wait();
                 } else {
-                    __syncwarp();
-                    if (lane == 0) {
-                        sm100::mbar_arrive(bar.s_free());
-                    }
+                    scores_are_read();
                 }
                 sm100::tc_fence_before_sync();
                 __syncwarp();
@@ -713,21 +728,23 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             sm100::tc_fence_after_sync();
             float sum_x, sum_y;
             f2_unpack(l, sum_x, sum_y);
-            float total = sum_x + sum_y;
-            if (m == kNoKey) {
-                total = 0.0f;    // (the polynomial's least power of two is not 0)
+            float total = m == kNoKey ? 0.0f : sum_x + sum_y;    // (the polynomial's least power of two is not 0)
+            merge_sum[half * 4 + quadrant][lane] = total;
+            if (kSubsets > 1 && half == 0) {
+                merge_max[quadrant][lane] = m;
             }
             float acc[kOut];
             if constexpr (kSubsets == 1) {
                 if (active) {
-                    sm100::tmem_ld_32x32(my_output, reinterpret_cast<uint32_t(&)[32]>(acc[0]));
-                    sm100::tmem_ld_32x32(my_output + 32, reinterpret_cast<uint32_t(&)[32]>(acc[32]));
+                    sm100::tmem_ld_32x32(my_output + 32 * half, reinterpret_cast<uint32_t(&)[32]>(acc));
                     sm100::tmem_ld_wait();
                 }
+                if (!pair.meet()) {
+                    break;
+                }
+                total = merge_sum[quadrant][lane] + merge_sum[4 + quadrant][lane];
             } else {
                 // The copies of a row: one reference exponent, one sum, and O's columns 16 at a time.
-                merge_max[quadrant][lane] = m;
-                merge_sum[quadrant][lane] = total;
                 if (!meeting.meet()) {
                     break;
                 }
@@ -741,48 +758,43 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 total = 0.0f;
 #pragma unroll
                 for (int s = 0; s < kSubsets; ++s) {
-                    const float other = merge_max[(quadrant % kApart) + s * kApart][lane];
-                    total += other == kNoKey ? 0.0f
-                                             : merge_sum[(quadrant % kApart) + s * kApart][lane] * fast_exp2(other - top);
+                    const int other = (quadrant % kApart) + s * kApart;
+                    total += merge_max[other][lane] == kNoKey
+                                 ? 0.0f
+                                 : (merge_sum[other][lane] + merge_sum[4 + other][lane]) *
+                                       fast_exp2(merge_max[other][lane] - top);
                 }
+                // In four rounds a quadrant's two warps hand over 8 of their 32 columns of O each.
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    uint32_t part[16];
-                    sm100::tmem_ld_32x16(my_output + 16 * r, part);
+                    uint32_t part[8];
+                    sm100::tmem_ld_32x8(my_output + 32 * half + 8 * r, part);
                     sm100::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float v[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {     // (a copy that saw no key may hold 0 times anything)
-                            v[c] = m == kNoKey ? 0.0f : __uint_as_float(part[4 * i + c]) * mine;
-                        }
-                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(my_staging + i * 512 + lane * 16),
-                                     "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3])
+                    for (int i = 0; i < 4; ++i) {     // (a copy that saw no key may hold 0 times anything)
+                        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(my_staging + i * 256 + lane * 8),
+                                     "f"(m == kNoKey ? 0.0f : __uint_as_float(part[2 * i]) * mine),
+                                     "f"(m == kNoKey ? 0.0f : __uint_as_float(part[2 * i + 1]) * mine)
                                      : "memory");
                     }
                     ok = meeting.meet() && ok;
-                    if (subset == r * kSubsets / 4) {
+                    // Of these 8 columns, in pairs, this copy adds up its share: 8 / kSubsets.
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int i = 0; i < 4 / kSubsets; ++i) {
+                        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                            for (int s = 0; s < kSubsets; ++s) {
-                                float v[4];
-                                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                                             : "r"(staging + ((quadrant % kApart) + s * kApart) * 2048 + i * 512 + lane * 16)
-                                             : "memory");
-#pragma unroll
-                                for (int c = 0; c < 4; ++c) {
-                                    sum[c] += v[c];
-                                }
-                            }
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                acc[(16 * r + 4 * i + c) % kOut] = sum[c];
-                            }
+                        for (int s = 0; s < kSubsets; ++s) {
+                            float v[2];
+                            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                                         : "=f"(v[0]), "=f"(v[1])
+                                         : "r"(staging + (half * 4 + (quadrant % kApart) + s * kApart) * kStaging +
+                                               (subset * (4 / kSubsets) + i) * 256 + lane * 8)
+                                         : "memory");
+                            sum[0] += v[0];
+                            sum[1] += v[1];
                         }
+                        acc[r * (kOut / 4) + 2 * i] = sum[0];
+                        acc[r * (kOut / 4) + 2 * i + 1] = sum[1];
                     }
                     ok = meeting.meet() && ok;     // (the staging is read)
                 }
@@ -792,74 +804,80 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 }
             }
             sm100::tc_fence_before_sync();
+            // This thread's columns of O: runs of kRun from 32 half + 8 r + its copy's share.
+            constexpr int kRun = kSubsets == 1 ? 32 : 8 / kSubsets;
+            auto column_of = [&](int i) {
+                return kSubsets == 1 ? 32 * half + i : 32 * half + 8 * (i / kRun) + subset * kRun + i % kRun;
+            };
+            const long long out_row = static_cast<long long>(info_row) + token;
+            const int head = info_head + head_of_group;
             if (whole) {
                 const float inv = position < 0 ? 0.0f : 1.0f / total;   // no key at all gives zeros
-                uint4 halves[kOut / 8];
 #pragma unroll
-                for (int b = 0; b < kOut / 8; ++b) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[i] = kPaged && position < 0 ? 0.0f : acc[b * 8 + i] * inv;
-                    }
-                    halves[b] = pack8(v);
+                for (int i = 0; i < kOut; ++i) {
+                    acc[i] = kPaged && position < 0 ? 0.0f : acc[i] * inv;
                 }
-                __half* out = p.a.o + out_row * p.a.o_stride + head * kHead + subset * kOut;
                 if constexpr (kSubsets == 1) {
-                    // Through shared memory, so that a row's 64 bytes leave by four lanes: rows are apart in memory,
-                    // and 32 of them at 16 bytes each took 3,000 clocks.
-                    __half* tile_out = p.a.o + info_row * p.a.o_stride + info_head * kHead;
+                    // Through shared memory, 16 columns at a time, so that a row's 32 bytes leave by two lanes: rows are
+                    // apart in memory, and 32 of them at 16 bytes each took three times as long.
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
+                    for (int r = 0; r < 2; ++r) {
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            const uint4 q = halves[4 * half + b];
+                        for (int b = 0; b < 2; ++b) {
+                            float v[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                v[i] = acc[16 * r + 8 * b + i];
+                            }
+                            const uint4 q = pack8(v);
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                             my_staging + lane * 64 + ((b ^ ((lane >> 1) & 3)) << 4)),
+                                             my_staging + lane * 32 + ((b ^ ((lane >> 2) & 1)) << 4)),
                                          "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
                                          : "memory");
                         }
                         __syncwarp();
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            const int r = 8 * b + lane / 4;
+                        for (int b = 0; b < 2; ++b) {
+                            const int its = 16 * b + lane / 2;
                             uint4 q;
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
-                                         : "r"(my_staging + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4))
+                                         : "r"(my_staging + its * 32 + (((lane & 1) ^ ((its >> 2) & 1)) << 4))
                                          : "memory");
-                            if (store_token[b] < info_tokens) {
-                                reinterpret_cast<uint4*>(tile_out + store_at[b])[4 * half + (lane & 3)] = q;
+                            const int there = quadrant * 32 + its, token_there = there / p.group;
+                            if (token_there < info_tokens) {
+                                __half* to_row = p.a.o + (static_cast<long long>(info_row) + token_there) * p.a.o_stride +
+                                                 (info_head + there - token_there * p.group) * kHead + 32 * half + 16 * r;
+                                reinterpret_cast<uint4*>(to_row)[lane & 1] = q;
                             }
                         }
                         __syncwarp();
                     }
                 } else if (valid) {
+                    __half* out = p.a.o + out_row * p.a.o_stride + head * kHead;
 #pragma unroll
-                    for (int b = 0; b < kOut / 8; ++b) {
-                        reinterpret_cast<uint4*>(out)[b] = halves[b];
+                    for (int i = 0; i < kOut; i += 2) {
+                        *reinterpret_cast<unsigned*>(out + column_of(i)) = pack2(acc[i], acc[i + 1]);
                     }
                 }
-                if (valid && subset == 0 && p.a.lse != nullptr) {
+                if (valid && subset == 0 && half == 0 && p.a.lse != nullptr) {
                     p.a.lse[static_cast<long long>(head) * p.a.rows + out_row] =
                         position < 0 ? -INFINITY : (m + log2f(total)) * kLn2;
                 }
             } else if (valid) {
                 float* part = p.parts + (2 * size_t{blockIdx.x} + (from == 0 ? 1 : 0)) * kPartFloats;
 #pragma unroll
-                for (int b = 0; b < kOut / 4; ++b) {
-                    reinterpret_cast<float4*>(part)[(subset * (kOut / 4) + b) * kRows + row] =
-                        make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
+                for (int i = 0; i < kOut; i += 2) {
+                    const int column = column_of(i);
+                    *reinterpret_cast<float2*>(part + (column / 4 * kRows + row) * 4 + column % 4) =
+                        make_float2(acc[i], acc[i + 1]);
                 }
-                if (subset == 0) {
+                if (subset == 0 && half == 0) {
                     part[kRows * kHead + row] = m;
                     part[kRows * kHead + kRows + row] = total;
                 }
             }
         }
-    }
-    if (threadIdx.x == 0) {
-        dependency_release();
     }
     __syncthreads();
     if (abort_flag != 0) {
@@ -917,6 +935,7 @@ __global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams 
     __shared__ unsigned ends[kMostCtas / 32];        // bit k: CTA k's first piece is not the middle of a tile
     __shared__ unsigned begins[kMostCtas / 32];      // bit k: CTA k's last tile goes on behind it
     __shared__ int list[2][kMostCtas];               // CTAs that begin split tiles: of few, of many parts
+    __shared__ unsigned char groups[kMostCtas];      // of 32 rows, in the tile that CTA k began
     __shared__ int counts[2];
     __shared__ float tops[kJoinWarps][32];
     __shared__ float sums[kJoinWarps][32][5];
@@ -931,6 +950,7 @@ __global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams 
     for (int k = tid; k < (p.ctas + 31) / 32 * 32; k += kJoinThreads) {
         const int head_part = k < p.ctas ? p.records[k].head_part : 0;
         const int tail_part = k < p.ctas ? p.records[k].tail_part : 0;
+        groups[k] = static_cast<unsigned char>(tail_part != 0 ? (p.records[k].tokens * p.group + 31) / 32 : 0);
         const unsigned e = __ballot_sync(kFullMask, head_part != 2), b = __ballot_sync(kFullMask, tail_part != 0);
         if (lane == 0) {
             ends[k / 32] = e;
@@ -971,18 +991,20 @@ __global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams 
         }
     }
     __syncthreads();
+    // (The row groups outermost: most tiles of single tokens have one.)
     const int few_items = counts[0] * (kRows / 32) * 2, many_items = counts[1] * (kRows / 32) * 16;
     for (int item = static_cast<int>(blockIdx.x); item < few_items + many_items; item += static_cast<int>(gridDim.x)) {
         const bool many = item >= few_items;
-        const int each = many ? (kRows / 32) * 16 : (kRows / 32) * 2;
+        const int each = counts[many] * (many ? 16 : 2);
         const int at = many ? item - few_items : item;
-        const int k = list[many][at / each];
-        const int columns = at % each / (kRows / 32);
-        const int row = at % (kRows / 32) * 32 + lane;
-        const Record mine = p.records[k];
-        if (row - lane >= mine.tokens * p.group) {
+        const int group_row = at / each;
+        const int columns = (at - group_row * each) / counts[many];
+        const int k = list[many][(at - group_row * each) % counts[many]];
+        const int row = group_row * 32 + lane;
+        if (group_row >= groups[k]) {
             continue;
         }
+        const Record mine = p.records[k];
         const int last = last_of(k);
         auto part_of = [&](int cta) {
             return p.parts + (2 * static_cast<size_t>(cta) + (cta == k ? 1 : 0)) * kPartFloats;
@@ -1006,7 +1028,7 @@ __global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams 
             }
         } else {
             const int column = columns;
-#pragma unroll 4
+#pragma unroll 8
             for (int cta = k + warp; cta <= last; cta += kJoinWarps) {
                 top = max3_nan(top, part_of(cta)[kRows * kHead + row], kNoKey);
             }
@@ -1016,7 +1038,7 @@ __global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams 
             for (int w = 0; w < kJoinWarps; ++w) {
                 top = max3_nan(top, tops[w][lane], kNoKey);
             }
-#pragma unroll 4
+#pragma unroll 8
             for (int cta = k + warp; cta <= last; cta += kJoinWarps) {
                 sum.add(part_of(cta), row, column, top);
             }
