@@ -47,7 +47,7 @@ constexpr int kStagingBytes = kSoftmaxWarps * kStaging;
 constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
 constexpr int kLeastPart = 4;   // of the line of key tiles, per CTA
-constexpr int kWholeKeys = 256; // up to which a tile is never split
+constexpr int kWholeKeys = 1024;   // up to which a tile is never split
 
 constexpr size_t kPartFloats = size_t{kRows} * kHead + 2 * kRows;   // O [column / 4][row][4], maxima, sums
 

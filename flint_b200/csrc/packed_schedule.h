@@ -118,11 +118,10 @@ FB_SCHEDULE long long cut_place(long long total, int parts, int k) {
     const long long each = quotient(total, parts), over = total - each * parts;
     return each * k + quotient(over * k, parts);
 }
-// An eighth of a part, and at least what a split costs (a second start and end, and the join's share), but never so far
-// that two cuts could meet.
+// About what a split costs (a second start and end, and the join's share), but never so far that two cuts could meet.
 FB_SCHEDULE long long cut_tolerance(long long total, int parts) {
     const long long each = quotient(total, parts);
-    const long long wanted = each / 8 > 3 ? each / 8 : 3;
+    const long long wanted = each < 24 ? 2 : 3;
     return wanted < (each - 1) / 2 ? wanted : (each - 1) / 2;
 }
 
