@@ -46,6 +46,7 @@ constexpr double kKeyShare = 0.575;   // of the CTAs, for dK and dV (four produc
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kListThreads = 256;
 constexpr int kLevels = 1024;    // of work that the list tells apart
+constexpr int kItems = 8;        // ring of items that the TMA warp has taken
 
 // A block of 128 tokens of a sequence of `count`: `level` blocks from the sequence's end (for dK and dV), the
 // level-th from its beginning (for dQ), so that the work is proportional to it in either.
@@ -58,7 +59,7 @@ struct BackwardParams {
     PackedArgs a;
     PackedGradients g;
     const Entry* entries;
-    const int* entry_count;
+    int* counts;              // of the entries; of the items taken so far, for dK and dV and for dQ
     const float* lse2;        // [heads, stats_stride]: log2(e) times the log-sum-exps
     const float* delta;
     long long stats_stride;
@@ -74,6 +75,7 @@ struct Barriers {
     __device__ uint32_t operands_ready(int b) const { return base + 48 + 8u * b; }
     __device__ uint32_t stage_full(int s) const { return base + 64 + 8u * s; }
     __device__ uint32_t stage_empty(int s) const { return base + 96 + 8u * s; }
+    __device__ uint32_t item_full(int i) const { return base + 128 + 8u * i; }
 };
 
 constexpr uint32_t kIdescSub = sm100::instr_desc_f16(128, 64, false, false);
@@ -88,7 +90,7 @@ struct PrepareParams {
     PackedArgs a;
     const __half* d_o;
     Entry* entries;
-    int* entry_count;
+    int* counts;
     float* lse2;
     float* delta;
     long long stats_stride;
@@ -133,7 +135,8 @@ __device__ void list_blocks(const PrepareParams& p) {
         upto += sums[w];
     }
     if (tid == kListThreads - 1) {
-        *p.entry_count = min(upto, p.capacity);
+        p.counts[0] = min(upto, p.capacity);
+        p.counts[1] = p.counts[2] = 0;
     }
     int at = upto - sum;
 #pragma unroll
@@ -181,25 +184,45 @@ __global__ void __launch_bounds__(kListThreads) fb_packed_backward_prepare(const
         }
         const long long at = stats_at(q.first, low) + (row - q.first);
         const long long o_row = static_cast<long long>(row) * p.a.o_stride;
-        for (int head = lane / 8; head < (p.a.heads + 3) / 4 * 4; head += 4) {
-            float sum = 0.0f;
-            if (head < p.a.heads) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p.d_o + o_row + head * kHead + lane % 8 * 8);
-                const uint4 y = *reinterpret_cast<const uint4*>(p.a.o + o_row + head * kHead + lane % 8 * 8);
-                float a[8], b[8];
-                unpack8(a, x);
-                unpack8(b, y);
+        // Four heads at a time, and four times that on their way.
+        for (int first_head = 0; first_head < p.a.heads; first_head += 16) {
+            uint4 x[4], y[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum = fmaf(a[i], b[i], sum);
+            for (int i = 0; i < 4; ++i) {
+                const int head = first_head + 4 * i + lane / 8;
+                x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (head < p.a.heads) {
+                    x[i] = load_input(reinterpret_cast<const uint4*>(p.d_o + o_row + head * kHead) + lane % 8);
+                    y[i] = load_input(reinterpret_cast<const uint4*>(p.a.o + o_row + head * kHead) + lane % 8);
                 }
             }
-            sum += __shfl_xor_sync(kFullMask, sum, 4);
-            sum += __shfl_xor_sync(kFullMask, sum, 2);
-            sum += __shfl_xor_sync(kFullMask, sum, 1);
-            if (head < p.a.heads && lane % 8 == 0) {
-                p.delta[head * p.stats_stride + at] = sum;
-                p.lse2[head * p.stats_stride + at] = p.a.lse[static_cast<long long>(head) * p.a.rows + row] * kLog2e;
+            const int stat_head = first_head + lane;
+            const float lse = lane < 16 && stat_head < p.a.heads ? p.a.lse[static_cast<long long>(stat_head) * p.a.rows + row] : 0.0f;
+            float sums[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float a[8], b[8];
+                unpack8(a, x[i]);
+                unpack8(b, y[i]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    sum = fmaf(a[c], b[c], sum);
+                }
+                sum += __shfl_xor_sync(kFullMask, sum, 4);
+                sum += __shfl_xor_sync(kFullMask, sum, 2);
+                sums[i] = sum + __shfl_xor_sync(kFullMask, sum, 1);
+            }
+            // Lane h of the first 16 has head first_head + h: of quarter h / 4, from the eight lanes 8 (h % 4).
+            float delta = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float other = __shfl_sync(kFullMask, sums[i], 8 * (lane % 4));
+                delta = lane / 4 == i ? other : delta;
+            }
+            if (lane < 16 && stat_head < p.a.heads) {
+                p.delta[stat_head * p.stats_stride + at] = delta;
+                p.lse2[stat_head * p.stats_stride + at] = lse * kLog2e;
             }
         }
     }
@@ -270,12 +293,31 @@ struct Shared {
     int warp;
 };
 
-// Items in rounds of `stride`, alternately in ascending and descending CTA order (the list is sorted by
-// work, so this evens the CTAs' totals out); one past the last ends the list.
-__device__ __forceinline__ int item_of(int round, int first_item, int stride) {
-    const int slot = (round & 1) != 0 ? stride - 1 - first_item : first_item;
-    return round * stride + slot;
-}
+// The items of a kind, which CTAs take one after the other from the list, the longest first: whoever is done takes
+// the next one. (Dealt out in advance, the CTAs' sums differed by 30 % where a group of four shares keys.) The TMA warp
+// takes an item when the loads of the one before are issued (not earlier: an item taken ahead is one that another CTA
+// would have had time for) and leaves its number in a ring for the others.
+struct Items {
+    int* taken;
+    int count;
+    volatile int* ring;
+    Barriers bar;
+    volatile int* abort;
+    // TMA warp, one lane.
+    __device__ __forceinline__ int take(int round) const {
+        const int item = atomicAdd(taken, 1);
+        ring[round % kItems] = item < count ? item : -1;
+        sm100::mbar_arrive(bar.item_full(round % kItems));
+        return item < count ? item : -1;
+    }
+    // A whole warp: the item of this round, or -1 behind the last one.
+    __device__ __forceinline__ int of(int round) const {
+        if (!sm100::mbar_wait_warp(bar.item_full(round % kItems), (round / kItems) & 1, abort)) {
+            return -1;
+        }
+        return ring[round % kItems];
+    }
+};
 
 // An item for dK and dV: keys [key, key + 128) of an entry's sequence; per head of the group, sub-steps of 64
 // queries from the diagonal on.
@@ -314,8 +356,7 @@ struct QueryItem {
 // Tensor memory: S^T at 0/64, dP^T at 128/192 (P^T and dS^T overwrite 4 x 8 columns of each), dV 256,
 // dK 320, K 384, V 416.
 
-__device__ __forceinline__ void key_items(const BackwardParams& p, const Shared& shared, int first_item, int stride,
-                                          int items) {
+__device__ __forceinline__ void key_items(const BackwardParams& p, const Shared& shared, const Items& items) {
     const uint32_t k_tile = shared.base, v_tile = shared.base + kTileBytes;
     const uint32_t ring = shared.base + 2 * kTileBytes;           // stage: Q then dO
     const uint32_t stats = ring + kStages * 2 * kSubBytes;        // stage: lse2[64] then delta[64]
@@ -334,8 +375,7 @@ __device__ __forceinline__ void key_items(const BackwardParams& p, const Shared&
             uint32_t phase = 0;
             bool ok = true;
             int round = 0;
-            for (int item = item_of(0, first_item, stride); ok && item < items;
-                 item = item_of(++round, first_item, stride)) {
+            for (int item = items.take(0); ok && item >= 0; item = items.take(++round)) {
                 const KeyItem it(p, item);
                 // The K and V buffers are free once the item before was copied to tensor memory.
                 if (round > 0 && !sm100::mbar_wait(bar.a_ready(), (round - 1) & 1, abort)) {
@@ -377,8 +417,7 @@ __device__ __forceinline__ void key_items(const BackwardParams& p, const Shared&
         uint32_t before = 0;   // sub-steps of earlier items
         bool ok = true;
         int round = 0;
-        for (int item = item_of(0, first_item, stride); ok && item < items;
-             item = item_of(++round, first_item, stride)) {
+        for (int item = items.of(0); ok && item >= 0; item = items.of(++round)) {
             const KeyItem it(p, item);
             ok = sm100::mbar_wait_warp(bar.a_ready(), round & 1, abort);
             sm100::tc_fence_after_sync();
@@ -468,9 +507,9 @@ __device__ __forceinline__ void key_items(const BackwardParams& p, const Shared&
         };
         uint32_t before = 0;
         int round = 0;
-        int item = item_of(0, first_item, stride);
-        bool ok = item < items && install(0);
-        for (; ok && item < items; item = item_of(++round, first_item, stride)) {
+        int item = items.of(0);
+        bool ok = item >= 0 && install(0);
+        for (; ok && item >= 0; item = items.of(++round)) {
             const KeyItem it(p, item);
             const int key = it.key + row;
             int sub = 0;
@@ -535,7 +574,7 @@ __device__ __forceinline__ void key_items(const BackwardParams& p, const Shared&
             }
             // The next item's K and V go in now, so that its first products run while this item's
             // gradients are written out.
-            if (item_of(round + 1, first_item, stride) < items && !install(round + 1)) {
+            if (items.of(round + 1) >= 0 && !install(round + 1)) {
                 ok = false;
                 break;
             }
@@ -573,8 +612,7 @@ __device__ __forceinline__ void key_items(const BackwardParams& p, const Shared&
 // S = Q K^T and dP = dO V^T (A = Q, dO from tensor memory), dS written back over dP, dQ += dS K.
 // Tensor memory: S at 0/64, dP at 128/192, dQ 256, Q 320, dO 352.
 
-__device__ __forceinline__ void query_items(const BackwardParams& p, const Shared& shared, int first_item, int stride,
-                                            int items) {
+__device__ __forceinline__ void query_items(const BackwardParams& p, const Shared& shared, const Items& items) {
     const uint32_t q_tile = shared.base, do_tile = shared.base + kTileBytes;
     const uint32_t ring = shared.base + 2 * kTileBytes;           // stage: K then V
     const Barriers bar = shared.bar;
@@ -592,8 +630,7 @@ __device__ __forceinline__ void query_items(const BackwardParams& p, const Share
             uint32_t phase = 0;
             bool ok = true;
             int round = 0;
-            for (int item = item_of(0, first_item, stride); ok && item < items;
-                 item = item_of(++round, first_item, stride)) {
+            for (int item = items.take(0); ok && item >= 0; item = items.take(++round)) {
                 const QueryItem it(p, item);
                 if (round > 0 && !sm100::mbar_wait(bar.a_ready(), (round - 1) & 1, abort)) {
                     break;
@@ -627,8 +664,7 @@ __device__ __forceinline__ void query_items(const BackwardParams& p, const Share
         uint32_t before = 0;
         bool ok = true;
         int round = 0;
-        for (int item = item_of(0, first_item, stride); ok && item < items;
-             item = item_of(++round, first_item, stride)) {
+        for (int item = items.of(0); ok && item >= 0; item = items.of(++round)) {
             const QueryItem it(p, item);
             ok = sm100::mbar_wait_warp(bar.a_ready(), round & 1, abort);
             sm100::tc_fence_after_sync();
@@ -708,9 +744,9 @@ __device__ __forceinline__ void query_items(const BackwardParams& p, const Share
         };
         uint32_t before = 0;
         int round = 0;
-        int item = item_of(0, first_item, stride);
-        bool ok = item < items && install(0);
-        for (; ok && item < items; item = item_of(++round, first_item, stride)) {
+        int item = items.of(0);
+        bool ok = item >= 0 && install(0);
+        for (; ok && item >= 0; item = items.of(++round)) {
             const QueryItem it(p, item);
             const int query = it.query + row;
             const bool valid = query < it.e.count;
@@ -758,7 +794,7 @@ __device__ __forceinline__ void query_items(const BackwardParams& p, const Share
             if (!ok) {
                 break;
             }
-            if (item_of(round + 1, first_item, stride) < items && !install(round + 1)) {
+            if (items.of(round + 1) >= 0 && !install(round + 1)) {
                 ok = false;
                 break;
             }
@@ -794,9 +830,13 @@ __global__ void __launch_bounds__(kThreads, 1) fb_packed_backward(const __grid_c
     const Barriers bar{base + kUsed - 1024 - 256};
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ int ring[kItems];
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x / 32), 0);
     if (threadIdx.x == 0) {
         abort_flag = 0;
+        for (int i = 0; i < kItems; ++i) {
+            sm100::mbar_init(bar.item_full(i), 1);
+        }
         sm100::mbar_init(bar.resident(), 1);
         sm100::mbar_init(bar.done(), 1);
         sm100::mbar_init(bar.a_ready(), kComputeWarps);
@@ -820,14 +860,13 @@ __global__ void __launch_bounds__(kThreads, 1) fb_packed_backward(const __grid_c
     dependency_wait();
 
     // Both gradients have as many sub-steps; dK's and dV's take longer, which sets their share of the CTAs.
-    const int count = *p.entry_count;
-    const int key_count = count * p.a.kv_heads, query_count = count * p.a.heads;
+    const int count = *static_cast<volatile int*>(p.counts);
     const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
-    const int share = min(key_count, max(1, static_cast<int>(ctas * kKeyShare + 0.5)));
+    const int share = min(count * p.a.kv_heads, max(1, static_cast<int>(ctas * kKeyShare + 0.5)));
     if (cta < share) {
-        key_items(p, shared, cta, share, key_count);
+        key_items(p, shared, Items{p.counts + 1, count * p.a.kv_heads, ring, bar, &abort_flag});
     } else {
-        query_items(p, shared, cta - share, ctas - share, query_count);
+        query_items(p, shared, Items{p.counts + 2, count * p.a.heads, ring, bar, &abort_flag});
     }
     if (threadIdx.x == 0) {
         dependency_release();
@@ -904,7 +943,7 @@ cudaError_t packed_backward(const PackedArgs& args, const PackedGradients& gradi
     p.a = args;
     p.g = gradients;
     p.entries = prepare.entries;
-    p.entry_count = prepare.entry_count;
+    p.counts = prepare.counts;
     p.lse2 = prepare.lse2;
     p.delta = prepare.delta;
     p.stats_stride = l.stride;
