@@ -347,7 +347,7 @@ flint_status flint_b200_packed_attention_backward_workspace(const flint_b200_pac
     if (bytes == nullptr) {
         return fb::fail(kBad, "%s: bytes is null", name);
     }
-    *bytes = fb::packed_backward_workspace(shape->sequences, shape->rows, shape->heads);
+    FB_CUDA(fb::packed_backward_workspace(shape->sequences, shape->rows, shape->heads, shape->kv_heads, bytes));
     return FLINT_OK;
 }
 

@@ -42,7 +42,7 @@ cudaError_t packed_forward_error_flag(int* value, bool reset);
 // Backward, of packed keys: args.o and args.lse are the forward's results.
 cudaError_t packed_backward(const PackedArgs& args, const PackedGradients& gradients, void* workspace,
                             cudaStream_t stream);
-size_t packed_backward_workspace(size_t sequences, size_t rows, size_t heads);
+cudaError_t packed_backward_workspace(size_t sequences, size_t rows, size_t heads, size_t kv_heads, size_t* bytes);
 cudaError_t packed_backward_error_flag(int* value, bool reset);
 
 // Device error words of these kernels: a wait that gave up, or starts, lengths or page
