@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     constexpr int kWarps = kThreads / 32;
     constexpr int kLanes = kThreads / kBins;      // of a bin
     extern __shared__ __align__(128) uint4 staged[];
-    __shared__ float bins[2][kBins];
+    __shared__ alignas(16) float bins[2][kBins];
     __shared__ float maxima[2][kWarps];
     __shared__ float sums[2][2 * kWarps];
     __shared__ Key reduced[kWarps];
@@ -273,6 +273,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     const int last_count = p.vocab - (all_words - 1) * W::kValues;
     const int full = last_word == words - 1 && last_count < W::kValues ? words - 1 : words;   // words that count whole
     const int top = p.top;
+    // Threads of different warps have what one thread does per row: start copies, fetch the target and write results.
+    constexpr int kCopier = kThreads / 2, kScribe = kThreads - 32;
 
     if (tid < 2) {
         counts[tid] = 0;
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         return;     // (the whole cluster)
     }
     const int chunk = ((words + kChunks - 1) / kChunks + kThreads - 1) / kThreads * kThreads;
-    auto copy_row = [&](size_t from) {     // thread 0
+    auto copy_row = [&](size_t from) {     // one thread
         for (int c = 0; c < kChunks && c * chunk < words; ++c) {
             const uint32_t bytes = static_cast<uint32_t>(min(chunk, words - c * chunk)) * 16u;
             const uint32_t bar = sm100::smem_u32(&barriers[c]);
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     };
     uint4 held[kStaged ? 1 : kHeld];
     if constexpr (kStaged) {
-        if (tid == 0) {
+        if (tid == kCopier) {
             copy_row(row);
         }
     } else {
@@ -324,19 +326,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             }
         }
     }
+    // The scribe's: this row's target and its logit, fetched while the row before was worked on.
+    auto target_of = [&](size_t from) { return p.targets != nullptr ? static_cast<int>(fb::load_input(p.targets + from)) : 0; };
+    auto target_value_of = [&](size_t from, int column) {
+        return column < p.vocab ? W::value(static_cast<const T*>(p.logits) + from * p.cols, column) : 0.0f;
+    };
+    const bool scribe = tid == kScribe && rank == 0;
+    int target = scribe ? target_of(row) : 0;
+    float target_value = scribe ? target_value_of(row, target) : 0.0f;
     bool gave_up = false;
     uint32_t phase = 0;
     for (int parity = 0; row < p.rows; row += stride, parity ^= 1) {
         const T* values = static_cast<const T*>(p.logits) + row * p.cols;
         const size_t next = row + stride;
         const size_t soon = kStaged ? next : next + stride;
-        if (tid == 0 && soon < p.rows && words > 0) {
+        if (tid == kCopier && soon < p.rows && words > 0) {
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row_of(soon)),
                          "r"(static_cast<uint32_t>(words) * 16u)
                          : "memory");
         }
-        const int target = p.targets != nullptr && tid == 0 && rank == 0 ? p.targets[row] : 0;
-        const float target_value = tid == 0 && rank == 0 && target < p.vocab ? W::value(values, target) : 0.0f;
+        const int next_target = scribe && next < p.rows ? target_of(next) : 0;
 
         Max<T> running;
         bool there = true;
@@ -404,14 +413,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         float bound = INFINITY;
         if (top > 0) {
             const float mine = bins[parity][lane];
-            unsigned ordered = static_cast<unsigned>(order_key(mine, 0) >> 32);
-            for (int left = top; left > 0;) {
-                const unsigned largest = __reduce_max_sync(fb::kFullMask, ordered);
-                const unsigned those = __ballot_sync(fb::kFullMask, ordered == largest);
-                bound = __shfl_sync(fb::kFullMask, mine, __ffs(those) - 1);
-                left -= __popc(those);
-                ordered = ordered == largest ? 0u : ordered;
+            int larger = 0;
+#pragma unroll
+            for (int i = 0; i < kBins / 4; ++i) {
+                const float4 four = reinterpret_cast<const float4*>(bins[parity])[i];
+                const float other[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    larger += other[c] > mine || (other[c] == mine && 4 * i + c < lane) ? 1 : 0;
+                }
             }
+            const unsigned holds = __ballot_sync(fb::kFullMask, larger == top - 1);     // (none where bins are NaN)
+            bound = __shfl_sync(fb::kFullMask, mine, holds != 0 ? __ffs(holds) - 1 : 0);
         }
         const bool none = mx == -INFINITY;
         auto collect = [&](const uint4& q, int i) {
@@ -475,9 +488,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             sums[parity][2 * warp + 1] = mean;
         }
         __syncthreads();
-        if (kStaged && tid == 0 && next < p.rows && !gave_up) {
+        if (kStaged && tid == kCopier && next < p.rows && !gave_up) {
             copy_row(next);     // everybody has read this row's words
         }
+        const float next_value = scribe && next < p.rows ? target_value_of(next, next_target) : 0.0f;
         total = sums[parity][2 * (lane % kWarps)];
         mean = sums[parity][2 * (lane % kWarps) + 1];
 #pragma unroll
@@ -510,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                 for (int c = tid; c < found; c += kThreads) {
                     const Key key = candidates[parity][c];
                     int larger = 0;
+#pragma unroll 8
                     for (int other = 0; other < found; ++other) {
                         larger += candidates[parity][other] > key ? 1 : 0;
                     }
@@ -602,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                 }
             }
         }
-        if (tid == 0) {
+        if (scribe) {
             if (p.log_probs != nullptr) {
                 p.log_probs[row] = target < p.vocab ? log_prob(target_value) : 0.0f;
             }
@@ -612,6 +627,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             if (p.lse != nullptr) {
                 p.lse[row] = mx == -INFINITY ? -INFINITY : mx + log_total;
             }
+            target = next_target;
+            target_value = next_value;
         }
     }
     if (gave_up && tid == 0) {
