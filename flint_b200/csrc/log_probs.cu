@@ -413,18 +413,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         float bound = INFINITY;
         if (top > 0) {
             const float mine = bins[parity][lane];
-            int larger = 0;
-#pragma unroll
-            for (int i = 0; i < kBins / 4; ++i) {
-                const float4 four = reinterpret_cast<const float4*>(bins[parity])[i];
-                const float other[4] = {four.x, four.y, four.z, four.w};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    larger += other[c] > mine || (other[c] == mine && 4 * i + c < lane) ? 1 : 0;
-                }
+            unsigned ordered = static_cast<unsigned>(order_key(mine, 0) >> 32);
+            for (int left = top; left > 0;) {
+                const unsigned largest = __reduce_max_sync(fb::kFullMask, ordered);
+                const unsigned those = __ballot_sync(fb::kFullMask, ordered == largest);
+                bound = __shfl_sync(fb::kFullMask, mine, __ffs(those) - 1);
+                left -= __popc(those);
+                ordered = ordered == largest ? 0u : ordered;
             }
-            const unsigned holds = __ballot_sync(fb::kFullMask, larger == top - 1);     // (none where bins are NaN)
-            bound = __shfl_sync(fb::kFullMask, mine, holds != 0 ? __ffs(holds) - 1 : 0);
         }
         const bool none = mx == -INFINITY;
         auto collect = [&](const uint4& q, int i) {
@@ -452,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                     }
                 }
             }
-#pragma unroll 2
+#pragma unroll 4
             for (int i = tid; i < words; i += kThreads) {
                 sums_of.add(staged[i]);
             }
@@ -736,6 +732,7 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
 }
 
 constexpr int kStagedWords = 6400;     // 100 KB: two CTAs per SM
+constexpr int kStagedThreads = 512;    // 256 are 6 % faster without alternatives, 5 % slower with five of them
 
 template <typename T, int kThreads, int kHeld>
 cudaError_t launch_form(LogProbArgs p, int ranks, int sms, cudaStream_t stream) {
@@ -778,7 +775,7 @@ cudaError_t launch_forward(const LogProbArgs& p, int sms, cudaStream_t stream) {
         ranks *= 2;
     }
     return (words + ranks - 1) / ranks <= 4 * 512 ? launch_form<T, 512, 4>(p, ranks, sms, stream)
-                                                  : launch_form<T, 512, 0>(p, ranks, sms, stream);
+                                                  : launch_form<T, kStagedThreads, 0>(p, ranks, sms, stream);
 }
 
 template <typename T>
