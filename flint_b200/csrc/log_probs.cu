@@ -658,7 +658,56 @@ struct LogProbGradientArgs {
 constexpr int kGradientThreads = 512;
 constexpr int kGradientWords = 4;
 
-template <typename T>
+// What a row's gradient needs: e^d (slope d + constant), and `a` more at the target; zeros for a row without tokens.
+struct RowGradient {
+    fb::F2 minus_lse, slope, constant;
+    float a;
+    int target;
+    __device__ __forceinline__ RowGradient(const LogProbGradientArgs& p, size_t row) {
+        target = p.targets != nullptr ? p.targets[row] : p.vocab;
+        a = p.d_log_probs != nullptr && target < p.vocab ? p.d_log_probs[row] : 0.0f;
+        float b = p.d_entropy != nullptr ? p.d_entropy[row] : 0.0f;
+        float lse = p.lse[row], entropy = p.d_entropy != nullptr ? p.entropy[row] : 0.0f;
+        if (lse == -INFINITY) {
+            lse = a = b = entropy = 0.0f;
+            target = -1;
+        }
+        minus_lse = fb::f2_pack(-lse, -lse);
+        slope = fb::f2_pack(-b, -b);
+        const float rest = -fmaf(b, entropy, a);
+        constant = fb::f2_pack(rest, rest);
+    }
+    template <typename T>
+    __device__ __forceinline__ uint4 word(const uint4& q, int column, int vocab) const {
+        using W = Word<T>;
+        float v[W::kValues], out[W::kValues];
+        W::unpack_finite(v, q);
+#pragma unroll
+        for (int c = 0; c < W::kValues; c += 2) {
+            const fb::F2 d = W::clamp(fb::f2_add(fb::f2_pack(v[c], v[c + 1]), minus_lse));
+            float y0, y1, e0, e1;
+            fb::f2_unpack(fb::f2_mul(d, fb::f2_pack(kLog2e, kLog2e)), y0, y1);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
+            fb::f2_unpack(fb::f2_mul(fb::f2_pack(e0, e1), fb::f2_fma(slope, d, constant)), out[c], out[c + 1]);
+        }
+        // (Rare, and so kept out of the way as a branch.)
+        if (static_cast<unsigned>(target - column) < W::kValues || column + W::kValues > vocab) {
+#pragma unroll 1
+            for (int c = 0; c < W::kValues; ++c) {
+                const float at_target = column + c == target ? a : 0.0f;
+#pragma unroll
+                for (int k = 0; k < W::kValues; ++k) {
+                    out[k] = k == c ? (column + c < vocab ? out[k] + at_target : 0.0f) : out[k];
+                }
+            }
+        }
+        return W::pack(out);
+    }
+};
+
+// kLong: a block takes pieces of one row, whose numbers all its threads share; else whole rows.
+template <typename T, bool kLong>
 __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(const LogProbGradientArgs p) {
     using W = Word<T>;
     fb::dependency_wait();
@@ -667,66 +716,40 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
     const int read_words = (p.vocab + W::kValues - 1) / W::kValues;
     const size_t groups = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
     for (size_t item = blockIdx.x; item < groups * p.row_chunks; item += gridDim.x) {
-        const size_t first_row = item / p.row_chunks * p.chunk_rows;
-        const int first_word = static_cast<int>(item % p.row_chunks) * p.chunk;
-        const int here = p.row_chunks > 1 ? min(p.chunk, row_words - first_word)
-                                          : static_cast<int>(min(static_cast<size_t>(p.chunk_rows), p.rows - first_row)) *
-                                                row_words;
+        const size_t first_row = kLong ? item / p.row_chunks : item * p.chunk_rows;
+        const int first_word = kLong ? static_cast<int>(item - first_row * p.row_chunks) * p.chunk : 0;
+        const int here = kLong ? min(p.chunk, row_words - first_word)
+                               : static_cast<int>(min(static_cast<size_t>(p.chunk_rows), p.rows - first_row)) * row_words;
+        const uint4* in = static_cast<const uint4*>(p.logits) + first_row * row_words + first_word;
+        uint4* out = static_cast<uint4*>(p.dlogits) + first_row * row_words + first_word;
         uint4 held[kGradientWords];
-        size_t rows[kGradientWords];
-        int at[kGradientWords];
 #pragma unroll
         for (int j = 0; j < kGradientWords; ++j) {
             const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
-            const int r = p.row_chunks > 1 ? 0 : i / row_words;
-            rows[j] = first_row + r;
-            at[j] = first_word + i - r * row_words;
+            const int word = kLong ? first_word + i : i % row_words;
             held[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (i < here && at[j] < read_words) {
-                held[j] = fb::load_input(static_cast<const uint4*>(p.logits) + rows[j] * row_words + at[j]);
+            if (i < here && word < read_words) {
+                held[j] = fb::load_input(in + i);
             }
         }
+        if constexpr (kLong) {
+            const RowGradient row(p, first_row);
 #pragma unroll
-        for (int j = 0; j < kGradientWords; ++j) {
-            if (static_cast<int>(threadIdx.x) + j * kGradientThreads >= here) {
-                continue;
-            }
-            const size_t row = rows[j];
-            const int target = p.targets != nullptr ? p.targets[row] : p.vocab;
-            const float a = p.d_log_probs != nullptr && target < p.vocab ? p.d_log_probs[row] : 0.0f;
-            const float b = p.d_entropy != nullptr ? p.d_entropy[row] : 0.0f;
-            const float lse = p.lse[row], entropy = p.d_entropy != nullptr ? p.entropy[row] : 0.0f;
-            // -p (a + b (d + entropy)) = e^d (-b d - (a + b entropy)); a row without tokens gives zeros.
-            const bool none = lse == -INFINITY;
-            const fb::F2 minus_lse = fb::f2_pack(none ? 0.0f : -lse, none ? 0.0f : -lse);
-            const float constant = none ? 0.0f : -fmaf(b, entropy, a);
-            const fb::F2 constant2 = fb::f2_pack(constant, constant);
-            const fb::F2 slope2 = fb::f2_pack(none ? 0.0f : -b, none ? 0.0f : -b);
-            float v[W::kValues], out[W::kValues];
-            W::unpack_finite(v, held[j]);
-#pragma unroll
-            for (int c = 0; c < W::kValues; c += 2) {
-                const fb::F2 d = W::clamp(fb::f2_add(fb::f2_pack(v[c], v[c + 1]), minus_lse));
-                float y0, y1, e0, e1;
-                fb::f2_unpack(fb::f2_mul(d, fb::f2_pack(kLog2e, kLog2e)), y0, y1);
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
-                fb::f2_unpack(fb::f2_mul(fb::f2_pack(e0, e1), fb::f2_fma(slope2, d, constant2)), out[c], out[c + 1]);
-            }
-            const int column = at[j] * W::kValues;
-            if (static_cast<unsigned>(target - column) < W::kValues && !none) {
-#pragma unroll
-                for (int c = 0; c < W::kValues; ++c) {
-                    out[c] += column + c == target ? a : 0.0f;
+            for (int j = 0; j < kGradientWords; ++j) {
+                const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
+                if (i < here) {
+                    __stcs(out + i, row.word<T>(held[j], (first_word + i) * W::kValues, p.vocab));
                 }
             }
-            if (column + W::kValues > p.vocab) {
+        } else {
 #pragma unroll
-                for (int c = 0; c < W::kValues; ++c) {
-                    out[c] = column + c < p.vocab ? out[c] : 0.0f;
+            for (int j = 0; j < kGradientWords; ++j) {
+                const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
+                if (i < here) {
+                    const int r = i / row_words;
+                    __stcs(out + i, RowGradient(p, first_row + r).word<T>(held[j], (i - r * row_words) * W::kValues, p.vocab));
                 }
             }
-            __stcs(static_cast<uint4*>(p.dlogits) + row * row_words + at[j], W::pack(out));
         }
     }
 }
@@ -786,7 +809,8 @@ cudaError_t launch_backward(LogProbGradientArgs p, int sms, cudaStream_t stream)
     p.chunk_rows = p.row_chunks > 1 ? 1 : p.chunk / words;
     const size_t items = (p.rows + p.chunk_rows - 1) / p.chunk_rows * p.row_chunks;
     const unsigned blocks = static_cast<unsigned>(std::min<size_t>(items, 4 * static_cast<size_t>(sms)));
-    return fb::launch_dependent(fb_token_log_probs_backward<T>, dim3(blocks), dim3(kGradientThreads), 0, stream, p);
+    return fb::launch_dependent(p.row_chunks > 1 ? fb_token_log_probs_backward<T, true> : fb_token_log_probs_backward<T, false>,
+                                dim3(blocks), dim3(kGradientThreads), 0, stream, p);
 }
 
 constexpr flint_status kBad = FLINT_ERROR_INVALID_ARGUMENT;
