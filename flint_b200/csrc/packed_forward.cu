@@ -907,182 +907,233 @@ struct JoinParams {
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kMostCtas = 1024;
-constexpr int kManyParts = 16;      // from which on a tile's parts are shared out among the warps
+// Caches of more than kManyKeys keys per sequence can make tiles of many parts. Those of more than kFewParts are then
+// left to kHelpers other blocks (of shorter ones the block that has the tile joins them all, two at a time).
+constexpr int kFewParts = 8;
+constexpr int kManyKeys = 16384;
+constexpr int kHelpers = 148;
 
-// Of a row's parts, weighted by 2^(m - top): what a lane adds up for its row and four columns.
+// A row's sum over parts in the order of the keys, for kColumns of its columns: a running reference exponent, as in
+// the softmax itself. A part of no key (m = kNoKey) may hold 0 times anything and is passed over.
+template <int kColumns>
 struct JoinSum {
-    float total;
-    float4 acc;
-    __device__ __forceinline__ void add(const float* part, int row, int column, float top) {
-        const float m = part[kRows * kHead + row];
-        const float sum = part[kRows * kHead + kRows + row];
-        const float4 x = reinterpret_cast<const float4*>(part)[column * kRows + row];
-        const float w = fast_exp2(m - top);
-        if (m != kNoKey) {     // (a part of no key may hold 0 times anything)
-            total = fmaf(sum, w, total);
-            acc.x = fmaf(x.x, w, acc.x);
-            acc.y = fmaf(x.y, w, acc.y);
-            acc.z = fmaf(x.z, w, acc.z);
-            acc.w = fmaf(x.w, w, acc.w);
+    float m = kNoKey, total = 0.0f;
+    float acc[kColumns] = {};
+    __device__ __forceinline__ void add(float part_m, float part_total, const float4 (&x)[kColumns / 4]) {
+        if (part_m == kNoKey) {
+            return;
+        }
+        const float top = max3_nan(m, part_m, part_m);
+        const float mine = fast_exp2(m - top), other = fast_exp2(part_m - top);
+        m = top;
+        total = total * mine + part_total * other;
+#pragma unroll
+        for (int i = 0; i < kColumns / 4; ++i) {
+            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                acc[4 * i + c] = acc[4 * i + c] * mine + v[c] * other;
+            }
         }
     }
 };
 
-// Every block lists the split tiles from the CTAs' records and takes its share of items: 32 rows of a tile and
-// 32 columns, four of them per warp and a row per lane; or, of a tile in many parts, four columns, the
-// parts among the warps. Parts are added in the order of the keys.
+// Block k joins the tile that CTA k began and did not end, if there is one: a warp has 32 rows and 32 columns, a
+// row per lane, and two parts on their way at a time. The helpers, which come first, take the tiles in many
+// parts, 32 rows and four columns at a time, a warp's share of the parts each.
 __global__ void __launch_bounds__(kJoinThreads) fb_packed_join(const JoinParams p) {
-    __shared__ unsigned ends[kMostCtas / 32];        // bit k: CTA k's first piece is not the middle of a tile
-    __shared__ unsigned begins[kMostCtas / 32];      // bit k: CTA k's last tile goes on behind it
-    __shared__ int list[2][kMostCtas];               // CTAs that begin split tiles: of few, of many parts
-    __shared__ unsigned char groups[kMostCtas];      // of 32 rows, in the tile that CTA k began
-    __shared__ int counts[2];
-    __shared__ float tops[kJoinWarps][32];
-    __shared__ float sums[kJoinWarps][32][5];
-    __shared__ uint2 rows_out[32][9];
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
+    __shared__ uint4 staged[kJoinWarps][128];
+    __shared__ float sums[kJoinWarps][32][7];
+    __shared__ unsigned ends[kMostCtas / 32 + 1];      // bit k: CTA k's first piece is not the middle of a tile
+    __shared__ int many[kMostCtas / kFewParts + 1], many_last[kMostCtas / kFewParts + 1];
+    __shared__ int many_count;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     dependency_wait();
     dependency_release();
-    if (tid < 2) {
-        counts[tid] = 0;
-    }
-    bool any = false;
-    for (int k = tid; k < (p.ctas + 31) / 32 * 32; k += kJoinThreads) {
-        const int head_part = k < p.ctas ? p.records[k].head_part : 0;
-        const int tail_part = k < p.ctas ? p.records[k].tail_part : 0;
-        groups[k] = static_cast<unsigned char>(tail_part != 0 ? (p.records[k].tokens * p.group + 31) / 32 : 0);
-        const unsigned e = __ballot_sync(kFullMask, head_part != 2), b = __ballot_sync(kFullMask, tail_part != 0);
-        if (lane == 0) {
-            ends[k / 32] = e;
-            begins[k / 32] = b;
+    auto rows_of = [&](const Record& r) { return r.tokens * p.group; };
+    // Where a row of a tile goes.
+    auto out_of = [&](const Record& r, int row) {
+        const int token = row / p.group;
+        return p.a.o + (static_cast<long long>(r.first_row) + token) * p.a.o_stride +
+               (r.kv_head * p.group + row - token * p.group) * kHead;
+    };
+    auto none_of = [&](const Record& r, int row) { return r.position + row / p.group < 0; };
+    auto store_lse = [&](const Record& r, int row, float m, float total) {
+        const int token = row / p.group;
+        p.a.lse[static_cast<long long>(r.kv_head * p.group + row - token * p.group) * p.a.rows + r.first_row + token] =
+            none_of(r, row) ? -INFINITY : (m + log2f(total)) * kLn2;
+    };
+    // Part i of the tile that CTA k began.
+    auto part_of = [&](int k, int i) {
+        return p.parts + (2 * static_cast<size_t>(k + i) + (i == 0 ? 1 : 0)) * kPartFloats;
+    };
+    const int helpers = static_cast<int>(gridDim.x) - p.ctas;
+    if (static_cast<int>(blockIdx.x) >= helpers) {
+        const int k = static_cast<int>(blockIdx.x) - helpers;
+        // Own record, and whether the CTAs behind go on with the tile.
+        const Record mine = p.records[k];
+        int count = 0;      // of parts
+        for (int from = k + 1; count == 0; from += 32) {
+            const unsigned found =
+                __ballot_sync(kFullMask, from + lane >= p.ctas || p.records[from + lane].head_part != 2);
+            if (mine.tail_part == 0) {
+                return;
+            }
+            count = found != 0 ? min(from + __ffs(found) - 1, p.ctas - 1) - k + 1 : 0;
         }
-        any = any || b != 0;
-    }
-    if (__syncthreads_or(any ? 1 : 0) == 0) {
+        if (count > kFewParts && helpers > 0) {
+            return;
+        }
+        const int row = warp % 4 * 32 + lane, half = warp / 4;
+        if (warp % 4 * 32 >= rows_of(mine)) {
+            return;
+        }
+        JoinSum<32> sum;
+        for (int i = 0; i < count; i += 2) {
+            float4 x[2][8];
+            float m[2], total[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[c] = kNoKey;
+                total[c] = 0.0f;
+                if (i + c < count) {
+                    const float* part = part_of(k, i + c);
+                    m[c] = part[kRows * kHead + row];
+                    total[c] = part[kRows * kHead + kRows + row];
+#pragma unroll
+                    for (int b = 0; b < 8; ++b) {
+                        x[c][b] = reinterpret_cast<const float4*>(part)[(8 * half + b) * kRows + row];
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                sum.add(m[c], total[c], x[c]);
+            }
+        }
+        const bool none = none_of(mine, row);
+        const float inv = 1.0f / sum.total;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                v[c] = none ? 0.0f : sum.acc[8 * b + c] * inv;
+            }
+            staged[warp][lane * 4 + (b ^ ((lane >> 1) & 3))] = pack8(v);
+        }
+        __syncwarp();
+        // A row's 64 bytes leave by four lanes.
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int r = 8 * b + lane / 4, its = warp % 4 * 32 + r;
+            const uint4 q = staged[warp][r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
+            if (its < rows_of(mine)) {
+                reinterpret_cast<uint4*>(out_of(mine, its) + 32 * half)[lane & 3] = q;
+            }
+        }
+        if (half == 0 && row < rows_of(mine) && p.a.lse != nullptr) {
+            store_lse(mine, row, sum.m, sum.total);
+        }
         return;
     }
-    auto last_of = [&](int k) {
-        // The first CTA behind k whose piece of the tile is its last.
-        int word = (k + 1) / 32;
-        unsigned bits = ends[word] & (kFullMask << ((k + 1) % 32));
-        while (bits == 0 && word + 1 < (p.ctas + 31) / 32) {
-            bits = ends[++word];
+    // A helper: the tiles of many parts, in the order of their CTAs.
+    const int words = (p.ctas + 31) / 32;
+    for (int k = threadIdx.x; k < words * 32; k += kJoinThreads) {
+        const unsigned bits = __ballot_sync(kFullMask, k >= p.ctas || p.records[k].head_part != 2);
+        if (lane == 0) {
+            ends[k / 32] = bits;
         }
-        return bits != 0 ? min(word * 32 + __ffs(bits) - 1, p.ctas - 1) : p.ctas - 1;
-    };
-    // The list's order is the CTAs': warp 0 appends 32 at a time.
+    }
+    if (threadIdx.x == 0) {
+        many_count = 0;
+    }
+    __syncthreads();
     if (warp == 0) {
-        int few = 0, many = 0;
+        int listed = 0;
         for (int from = 0; from < p.ctas; from += 32) {
+            // The first CTA behind this one whose piece of the tile is its last.
             const int k = from + lane;
-            const bool split = ((begins[from / 32] >> lane) & 1) != 0 && k + 1 < p.ctas;
-            const bool long_one = split && last_of(k) - k + 1 > kManyParts;
-            const unsigned f = __ballot_sync(kFullMask, split && !long_one), m = __ballot_sync(kFullMask, long_one);
-            const unsigned below = (1u << lane) - 1;
-            if (split) {
-                list[long_one][(long_one ? many : few) + __popc((long_one ? m : f) & below)] = k;
+            int last = p.ctas;
+            if (k + 1 < p.ctas) {
+                int word = (k + 1) / 32;
+                unsigned bits = ends[word] & (kFullMask << ((k + 1) % 32));
+                while (bits == 0 && word + 1 < words) {
+                    bits = ends[++word];
+                }
+                last = bits != 0 ? word * 32 + __ffs(bits) - 1 : p.ctas;
             }
-            few += __popc(f);
-            many += __popc(m);
+            const bool is = k + 1 < p.ctas && last < p.ctas && last - k + 1 > kFewParts && p.records[k].tail_part != 0;
+            const unsigned those = __ballot_sync(kFullMask, is);
+            if (is) {
+                const int place = listed + __popc(those & ((1u << lane) - 1));
+                many[place] = k;
+                many_last[place] = last;
+            }
+            listed += __popc(those);
         }
         if (lane == 0) {
-            counts[0] = few;
-            counts[1] = many;
+            many_count = listed;
         }
     }
     __syncthreads();
-    // (The row groups outermost: most tiles of single tokens have one.)
-    const int few_items = counts[0] * (kRows / 32) * 2, many_items = counts[1] * (kRows / 32) * 16;
-    for (int item = static_cast<int>(blockIdx.x); item < few_items + many_items; item += static_cast<int>(gridDim.x)) {
-        const bool many = item >= few_items;
-        const int each = counts[many] * (many ? 16 : 2);
-        const int at = many ? item - few_items : item;
-        const int group_row = at / each;
-        const int columns = (at - group_row * each) / counts[many];
-        const int k = list[many][(at - group_row * each) % counts[many]];
-        const int row = group_row * 32 + lane;
-        if (group_row >= groups[k]) {
+    constexpr int kEach = (kRows / 32) * (kHead / 4);
+    for (int item = static_cast<int>(blockIdx.x); item < many_count * kEach; item += helpers) {
+        // (The row groups outermost: few rows have the first one only.)
+        const int at = item % (many_count * (kHead / 4));
+        const int first_row = item / (many_count * (kHead / 4)) * 32;
+        const int k = many[at / (kHead / 4)], column = at % (kHead / 4);     // by four
+        const Record mine = p.records[k];
+        if (first_row >= rows_of(mine)) {
             continue;
         }
-        const Record mine = p.records[k];
-        const int last = last_of(k);
-        auto part_of = [&](int cta) {
-            return p.parts + (2 * static_cast<size_t>(cta) + (cta == k ? 1 : 0)) * kPartFloats;
-        };
-        const int token = row / p.group;
-        const bool valid = token < mine.tokens;
-        const bool none = mine.position + token < 0;
-        const int head = mine.kv_head * p.group + row - token * p.group;
-        const long long at_row = mine.first_row + token;
-        float top = kNoKey;
-        JoinSum sum = {};
-        if (!many) {
-            const int column = columns * 8 + warp;
-#pragma unroll 4
-            for (int cta = k; cta <= last; ++cta) {
-                top = max3_nan(top, part_of(cta)[kRows * kHead + row], kNoKey);
-            }
-#pragma unroll 4
-            for (int cta = k; cta <= last; ++cta) {
-                sum.add(part_of(cta), row, column, top);
-            }
-        } else {
-            const int column = columns;
-#pragma unroll 8
-            for (int cta = k + warp; cta <= last; cta += kJoinWarps) {
-                top = max3_nan(top, part_of(cta)[kRows * kHead + row], kNoKey);
-            }
-            tops[warp][lane] = top;
-            __syncthreads();
+        const int count = many_last[at / (kHead / 4)] - k + 1;
+        const int row = first_row + lane;
+        JoinSum<4> sum;
+        for (int i = warp; i < count; i += 8 * kJoinWarps) {
+            float4 x[8][1];
+            float m[8], total[8];
 #pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) {
-                top = max3_nan(top, tops[w][lane], kNoKey);
+            for (int c = 0; c < 8; ++c) {
+                m[c] = kNoKey;
+                total[c] = 0.0f;
+                if (i + c * kJoinWarps < count) {
+                    const float* part = part_of(k, i + c * kJoinWarps);
+                    m[c] = part[kRows * kHead + row];
+                    total[c] = part[kRows * kHead + kRows + row];
+                    x[c][0] = reinterpret_cast<const float4*>(part)[column * kRows + row];
+                }
             }
-#pragma unroll 8
-            for (int cta = k + warp; cta <= last; cta += kJoinWarps) {
-                sum.add(part_of(cta), row, column, top);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                sum.add(m[c], total[c], x[c]);
             }
-            sums[warp][lane][0] = sum.total;
-            sums[warp][lane][1] = sum.acc.x;
-            sums[warp][lane][2] = sum.acc.y;
-            sums[warp][lane][3] = sum.acc.z;
-            sums[warp][lane][4] = sum.acc.w;
-            __syncthreads();
-            if (warp == 0) {
-                for (int w = 1; w < kJoinWarps; ++w) {
-                    sum.total += sums[w][lane][0];
-                    sum.acc.x += sums[w][lane][1];
-                    sum.acc.y += sums[w][lane][2];
-                    sum.acc.z += sums[w][lane][3];
-                    sum.acc.w += sums[w][lane][4];
+        }
+        sums[warp][lane][4] = sum.m;
+        sums[warp][lane][5] = sum.total;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            sums[warp][lane][c] = sum.acc[c];
+        }
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < kJoinWarps; ++w) {
+                const float* from = sums[w][lane];
+                const float4 x[1] = {make_float4(from[0], from[1], from[2], from[3])};
+                sum.add(from[4], from[5], x);
+            }
+            if (row < rows_of(mine)) {
+                const float inv = 1.0f / sum.total;
+                reinterpret_cast<uint2*>(out_of(mine, row))[column] =
+                    none_of(mine, row) ? make_uint2(0u, 0u)
+                                       : make_uint2(pack2(sum.acc[0] * inv, sum.acc[1] * inv),
+                                                    pack2(sum.acc[2] * inv, sum.acc[3] * inv));
+                if (column == 0 && p.a.lse != nullptr) {
+                    store_lse(mine, row, sum.m, sum.total);
                 }
             }
         }
-        const float inv = 1.0f / sum.total;
-        const uint2 q = none ? make_uint2(0u, 0u) : make_uint2(pack2(sum.acc.x * inv, sum.acc.y * inv),
-                                                               pack2(sum.acc.z * inv, sum.acc.w * inv));
-        __half* out = p.a.o + at_row * p.a.o_stride + head * kHead;
-        if (many) {
-            if (warp == 0 && valid) {
-                reinterpret_cast<uint2*>(out)[columns] = q;
-            }
-        } else {
-            // A row's 64 bytes leave by four lanes.
-            rows_out[lane][warp] = q;
-            __syncthreads();
-            const int r = tid / 4, quarter = tid % 4;
-            const int row_there = row - lane + r, token_there = row_there / p.group;
-            if (tid < 128 && token_there < mine.tokens) {
-                const uint2 a = rows_out[r][2 * quarter], b = rows_out[r][2 * quarter + 1];
-                __half* to = p.a.o + (mine.first_row + static_cast<long long>(token_there)) * p.a.o_stride +
-                             (mine.kv_head * p.group + row_there - token_there * p.group) * kHead + columns * 32;
-                reinterpret_cast<uint4*>(to)[quarter] = make_uint4(a.x, a.y, b.x, b.y);
-            }
-        }
-        if (columns == 0 && warp == 0 && valid && p.a.lse != nullptr) {
-            p.a.lse[static_cast<long long>(head) * p.a.rows + at_row] = none ? -INFINITY : (top + log2f(sum.total)) * kLn2;
-        }
-        __syncthreads();      // (the shared arrays are read)
+        __syncthreads();      // (the sums are read)
     }
 }
 
@@ -1153,7 +1204,8 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
         return e;
     }
     JoinParams j = {args, p.records, p.parts, ctas, p.group};
-    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(4 * sms)), dim3(kJoinThreads), 0, stream, j);
+    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(ctas + (most_keys > kManyKeys ? kHelpers : 0))),
+                            dim3(kJoinThreads), 0, stream, j);
 }
 
 }  // namespace fb

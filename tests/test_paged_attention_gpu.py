@@ -132,6 +132,18 @@ def test_many_sequences(flint, heads, kv_heads, page_size):
     cache.check(o, lse)
 
 
+@pytest.mark.parametrize("heads, kv_heads, new, total", [(4, 1, [1], [40000]), (8, 1, [1, 3], [20001, 300]),
+                                                         (16, 2, [9, 1], [33000, 17000]), (2, 2, [70], [25000])])
+def test_long_caches(flint, heads, kv_heads, new, total):
+    """Tiles in many parts, which are joined on their own."""
+    cache = Cache(new, total, heads, kv_heads, 128)
+    cache.store(flint)
+    o, lse = cache.attend(flint)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    cache.check(o, lse)
+
+
 @pytest.mark.parametrize("longest", [1, 64])
 def test_tokens_without_a_position(flint, longest):
     """A length below the number of new tokens: the first ones have no position, nothing to see."""
