@@ -108,21 +108,15 @@ __device__ __forceinline__ long long warp_prefix(long long v, int lane) {     //
     return v;
 }
 
-// The places of this CTA's two cuts among `parts`; none for a CTA without a part.
-struct Places {
-    int parts;
-    long long at[2], tolerance, total;
-    __device__ __forceinline__ Places(const TileParams& p, long long line) : total(line) {
-        parts = part_count(total, static_cast<int>(gridDim.x), kLeastPart);
+// The place of one of this CTA's two cuts (0 its part's beginning, 1 its end; both the line's end for a CTA without a
+// part), and how far it may move.
+struct Place {
+    long long at, tolerance;
+    __device__ __forceinline__ Place(const TileParams& p, long long total, int which) {
+        const int parts = part_count(total, static_cast<int>(gridDim.x), kLeastPart);
         const int cta = static_cast<int>(blockIdx.x);
-        if (cta < parts) {
-            at[0] = cut_place(total, parts, cta);
-            at[1] = cut_place(total, parts, cta + 1);
-            tolerance = p.splits ? cut_tolerance(total, parts) : total;
-        } else {
-            at[0] = at[1] = total;
-            tolerance = 0;
-        }
+        at = cta < parts ? cut_place(total, parts, cta + which) : total;
+        tolerance = cta >= parts ? 0 : p.splits ? cut_tolerance(total, parts) : total;
     }
 };
 
@@ -137,24 +131,27 @@ __device__ __forceinline__ long long length_of(const TileParams& p, int s, int& 
     return head_length(before, tokens, p.log_tokens);
 }
 
-// Which part of the line this CTA works on, for up to 32 sequences: one warp.
+// Which part of the line this CTA works on, for up to 32 sequences: one warp, its even lanes for one cut and the odd
+// ones for the other.
 __device__ __forceinline__ void locate_in_warp(const TileParams& p, Cut (&cuts)[2], int lane) {
     int before, tokens;
     const long long length = length_of(p, lane, before, tokens);
     const long long mine = length * p.a.kv_heads;
     const long long upto = warp_prefix(mine, lane);
-    const Places place(p, __shfl_sync(kFullMask, upto, 31));
+    const long long total = __shfl_sync(kFullMask, upto, 31);
+    const Place place(p, total, lane & 1);
     const long long begins = upto - mine;
-#pragma unroll 1
-    for (int c = 0; c < 2; ++c) {
-        const long long at = place.at[c];
-        if (at == place.total) {
-            if (lane == 0) {
-                cuts[c] = Cut{at, p.a.sequences, 0, 0, 0};
-            }
-        } else if (at >= begins && at < upto) {
-            cuts[c] = cut_at(at, at - begins, lane, before, tokens, p.log_tokens, length, place.tolerance);
-        }
+    const long long first = __shfl_sync(kFullMask, place.at, 0), second = __shfl_sync(kFullMask, place.at, 1);
+    const unsigned has_first = __ballot_sync(kFullMask, first >= begins && first < upto);
+    const unsigned has_second = __ballot_sync(kFullMask, second >= begins && second < upto);
+    const unsigned has = (lane & 1) == 0 ? has_first : has_second;
+    const int owner = has != 0 ? __ffs(has) - 1 : 0;
+    const int its_before = __shfl_sync(kFullMask, before, owner), its_tokens = __shfl_sync(kFullMask, tokens, owner);
+    const long long its_length = __shfl_sync(kFullMask, length, owner), its_begin = __shfl_sync(kFullMask, begins, owner);
+    if (lane < 2) {
+        cuts[lane] = has == 0 ? Cut{total, p.a.sequences, 0, 0, 0}
+                              : cut_at(place.at, place.at - its_begin, owner, its_before, its_tokens, p.log_tokens,
+                                       its_length, place.tolerance);
     }
 }
 
@@ -175,9 +172,10 @@ __device__ __noinline__ void locate(const TileParams& p, Cut (&cuts)[2], long lo
     for (int w = 0; w < kWarps; ++w) {
         total += scan[w];
     }
-    const Places place(p, total * p.a.kv_heads);
-    if (tid < 2 && place.at[tid] == place.total) {
-        cuts[tid] = Cut{place.total, p.a.sequences, 0, 0, 0};
+    total *= p.a.kv_heads;
+    const Place place[2] = {Place(p, total, 0), Place(p, total, 1)};
+    if (tid < 2 && place[tid].at == total) {
+        cuts[tid] = Cut{total, p.a.sequences, 0, 0, 0};
     }
     long long running = 0;
     for (int first = 0; first < p.a.sequences; first += kThreads) {
@@ -196,9 +194,9 @@ __device__ __noinline__ void locate(const TileParams& p, Cut (&cuts)[2], long lo
         }
         const long long begins = running + upto - mine;
         for (int c = 0; c < 2; ++c) {
-            if (place.at[c] >= begins && place.at[c] < begins + mine) {
-                cuts[c] = cut_at(place.at[c], place.at[c] - begins, first + tid, before, tokens, p.log_tokens, length,
-                                 place.tolerance);
+            if (place[c].at >= begins && place[c].at < begins + mine) {
+                cuts[c] = cut_at(place[c].at, place[c].at - begins, first + tid, before, tokens, p.log_tokens, length,
+                                 place[c].tolerance);
             }
         }
         running += all;
