@@ -240,7 +240,7 @@ __device__ __forceinline__ float key_value(Key key) {
 // them, the row is gone through once per alternative.
 constexpr int blocks_per_sm(int threads, int held) { return (threads == 128 ? 4 : 1) * (held > 4 ? 1 : 2); }
 
-constexpr int kChunks = 4;      // pieces in which a slice is copied into shared memory
+constexpr int kChunks = 2;      // pieces in which a slice is copied into shared memory
 
 // kHeld > 0: a thread holds that many words of the row in registers, and asks for the next row's while it takes
 // the exponentials. kHeld == 0: the slice is copied into shared memory, and the CTA beside it on the SM computes
@@ -488,18 +488,30 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             copy_row(next);     // everybody has read this row's words
         }
         const float next_value = scribe && next < p.rows ? target_value_of(next, next_target) : 0.0f;
-        total = sums[parity][2 * (lane % kWarps)];
-        mean = sums[parity][2 * (lane % kWarps) + 1];
+        // Only the warps that write results go on: the scribe's, those with candidates, and all where the
+        // alternatives take the long way. (A cluster's CTAs meet below.)
+        const int found = top > 0 ? counts[parity] : 0;
+        const bool collected = found <= kCandidates && mx == mx;
+        const bool goes_on = warp == kScribe / 32 || (p.ranks > 1 && warp == 0) ||
+                             (top > 0 && (!collected || warp * 32 < max(found, 1)));
+        if (!goes_on && p.ranks == 1) {
+            continue;
+        }
+        float log_total = 0.0f;
+        if (goes_on) {
+            total = sums[parity][2 * (lane % kWarps)];
+            mean = sums[parity][2 * (lane % kWarps) + 1];
 #pragma unroll
-        for (int off = 1; off < kWarps; off <<= 1) {
-            total += __shfl_xor_sync(fb::kFullMask, total, off);
-            mean += __shfl_xor_sync(fb::kFullMask, mean, off);
+            for (int off = 1; off < kWarps; off <<= 1) {
+                total += __shfl_xor_sync(fb::kFullMask, total, off);
+                mean += __shfl_xor_sync(fb::kFullMask, mean, off);
+            }
+            mean *= kLn2;
+            if (none) {
+                total = mean = 0.0f;
+            }
+            log_total = logf(total);
         }
-        mean *= kLn2;
-        if (none) {
-            total = mean = 0.0f;
-        }
-        float log_total = logf(total);
         auto log_prob = [&](float v) { return mx == -INFINITY ? -INFINITY : (v - mx) - log_total; };
         auto emit = [&](int place, Key key) {
             p.top_tokens[row * top + place] = static_cast<uint16_t>(key_column(key));
@@ -514,9 +526,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
             }
         };
-        if (top > 0) {
-            const int found = counts[parity];
-            if (found <= kCandidates && mx == mx) {
+        if (top > 0 && goes_on) {
+            if (collected) {
                 for (int c = tid; c < found; c += kThreads) {
                     const Key key = candidates[parity][c];
                     int larger = 0;
