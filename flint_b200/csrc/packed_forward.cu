@@ -3,7 +3,7 @@
 //
 // A tile is the 128 rows of (token, query head) that one K/V head's group makes of 128 / group
 // consecutive tokens (rounded down to a power of two): one load of keys and values serves the whole
-// group. S = Q K^T goes to tensor memory, a thread takes the softmax of a row in base 2, P goes
+// group. S = Q K^T goes to tensor memory, two threads take the softmax of a row in base 2, P goes
 // back as FP16 pairs and is the A operand of O += P V, which accumulates in tensor memory over the
 // row of key tiles; the exponent that probabilities are taken against moves only when a row's
 // maximum exceeds it by more than 2^8, so that O is rarely rescaled.
@@ -12,8 +12,11 @@
 // dependent launch joins them in the order of the keys.
 //
 // Two CTAs per SM with one tile each: one's matrix products, loads and ends run under the other's
-// exponentials, which bound the kernel (128 x 128 of them per key tile take the SM's special-function
-// unit 1,024 clocks and the products 512; a quarter of them runs on the FMA pipe instead).
+// exponentials. Those bound long sequences: 128 x 128 of them take the SM's special-function unit 1,024 clocks
+// and the products 512; a quarter of them runs on the FMA pipe instead (half of them: 10 % slower, none: 9 %). A key tile
+// takes 1,350 clocks of an SM; short sequences are bound by what a tile's beginning and end cost, about two key tiles.
+// Measured, with the join: 5 sequences of up to 4,096 tokens, 16 query heads on 4, 82 us (508 TFLOP/s); 24 of up to 700,
+// 12 heads, 32 us; 64 single tokens on caches of up to 8,192, 32 heads on 8, 77 us (5.1 TB/s).
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
