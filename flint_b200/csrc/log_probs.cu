@@ -17,7 +17,6 @@
 namespace {
 
 constexpr int kMostTop = 32;
-constexpr int kBins = 32;            // parts of a slice whose maxima bound the alternatives from below
 constexpr int kCandidates = 512;
 constexpr int kMostRanks = 8;        // CTAs of a cluster
 constexpr float kLog2e = 1.4426950408889634f;
@@ -234,7 +233,7 @@ __device__ __forceinline__ float key_value(Key key) {
 // the exponentials while it asks for the next row's words, so that memory never waits. Long
 // rows, and few of them, are divided over a cluster's CTAs: each takes sums against its own maximum, and the
 // first puts them together.
-// The alternatives: the slice falls into 32 bins of neighbouring lanes. The k-th largest of the bins' maxima
+// The alternatives: the slice falls into 64 (or 32) bins of neighbouring lanes. The k-th largest of the bins' maxima
 // is a lower bound of the k-th largest logit; what is not below it (about k values) is collected in the
 // second pass and put in order by counting. Where too many qualify (rows of equal logits), or a NaN is among
 // them, the row is gone through once per alternative.
@@ -254,9 +253,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     using W = Word<T>;
     constexpr bool kStaged = kHeld == 0;
     constexpr int kWarps = kThreads / 32;
+    constexpr int kBins = kThreads >= 512 ? 64 : 32;     // parts whose maxima bound the alternatives (up to 32) from below
     constexpr int kLanes = kThreads / kBins;      // of a bin
     extern __shared__ __align__(128) uint4 staged[];
-    __shared__ alignas(16) float bins[2][kBins];
+    __shared__ float bins[2][kBins];
+    __shared__ float least[2];
     __shared__ float maxima[2][kWarps];
     __shared__ float sums[2][2 * kWarps];
     __shared__ Key reduced[kWarps];
@@ -416,15 +417,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         // ones counted each.
         float bound = INFINITY;
         if (top > 0) {
-            const float mine = bins[parity][lane];
-            unsigned ordered = static_cast<unsigned>(order_key(mine, 0) >> 32);
-            for (int left = top; left > 0;) {
-                const unsigned largest = __reduce_max_sync(fb::kFullMask, ordered);
-                const unsigned those = __ballot_sync(fb::kFullMask, ordered == largest);
-                bound = __shfl_sync(fb::kFullMask, mine, __ffs(those) - 1);
-                left -= __popc(those);
-                ordered = ordered == largest ? 0u : ordered;
+            // A warp ranks its share of the bins, each against all of them, one or two per lane.
+            const float low = bins[parity][lane], high = kBins > 32 ? bins[parity][lane + kBins - 32] : 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < kBins / kWarps; ++i) {
+                const int bin = warp * (kBins / kWarps) + i;
+                const float value = bins[parity][bin];
+                int larger = __popc(__ballot_sync(fb::kFullMask, low > value || (low == value && lane < bin)));
+                if (kBins > 32) {
+                    larger += __popc(__ballot_sync(fb::kFullMask, high > value || (high == value && lane + 32 < bin)));
+                }
+                if (larger == top - 1 && lane == 0) {
+                    least[parity] = value;      // (none is where bins are NaN)
+                }
             }
+            __syncthreads();
+            bound = least[parity];
         }
         const bool none = mx == -INFINITY;
         auto collect = [&](const uint4& q, int i) {
