@@ -103,7 +103,8 @@ def test_forward_and_backward(flint, lengths, heads, kv_heads):
 
 
 @pytest.mark.parametrize("lengths, heads, kv_heads", [([700, 350, 1], 128, 1), ([90, 1, 400], 64, 2), ([33] * 40, 96, 3),
-                                                      ([1024] * 4, 12, 12), ([3000, 1500], 16, 4)])
+                                                      ([1024] * 4, 12, 12), ([3000, 1500], 16, 4), ([5, 3], 1024, 8),
+                                                      ([1200, 40, 700], 8, 1), ([130] * 3, 128, 2)])
 def test_wide_groups_and_many_items(flint, lengths, heads, kv_heads):
     batch = Batch(lengths, heads, kv_heads, extra=72)
     o, lse = batch.forward(flint)
@@ -286,6 +287,50 @@ def test_captured_and_replayed_on_another_stream(flint):
         assert not flint.kernel_fault()
         inside = slice(0, batch.first[-1])
         assert torch.equal(o, want_o) and torch.equal(lse, want_lse) and torch.equal(grads[inside], want[inside])
+
+
+def test_offsets_beyond_32_bits(flint):
+    """Rows so far apart that the last ones lie beyond 2^32 values, forward and backward."""
+    batch = Batch([150, 40], 4, 2, before=0, behind=0)
+    wide, before = 65536, 70000
+    rows = before + batch.rows
+    qkv = torch.empty(rows, wide, dtype=torch.half, device=DEV)
+    qkv[before:, :batch.width] = batch.qkv
+    grads = torch.empty_like(qkv)
+    d_o = torch.zeros(rows, 4 * 64, dtype=torch.half, device=DEV)
+    d_o[before:] = batch.d_o
+    starts = batch.starts + before
+    o, lse = torch.zeros_like(d_o), torch.zeros(4, rows, device=DEV)
+    shape = PackedShape(2, rows, 4, 2, 64, wide, wide, 4 * 64)
+    workspace = torch.empty(max(flint.packed_attention_workspace(shape),
+                                flint.packed_attention_backward_workspace(shape)), dtype=torch.uint8, device=DEV)
+    flint.packed_attention_forward(o, lse, *batch.parts(qkv), starts, shape, SCALE, workspace)
+    flint.packed_attention_backward(*batch.parts(grads), d_o, o, lse, *batch.parts(qkv), starts, shape, SCALE, workspace)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    batch.check(o[before:], lse[:, before:], grads[before:, :batch.width])
+
+
+def test_two_calls_at_once(flint):
+    """Two batches on two streams, each with its own workspace, again and again."""
+    batches = [Batch([700, 33, 1500], 8, 2, seed=1), Batch([2000, 1, 90, 400], 6, 6, seed=2)]
+    want, streams, outputs = [], [torch.cuda.Stream() for _ in batches], []
+    for batch in batches:
+        o, lse = batch.forward(flint)
+        want.append((o, lse, batch.backward(flint, o, lse)))
+    torch.cuda.synchronize()
+    for trial in range(6):
+        outputs = []
+        for batch, stream in zip(batches, streams):
+            with torch.cuda.stream(stream):
+                o, lse = batch.forward(flint)
+                outputs.append((o, lse, batch.backward(flint, o, lse)))
+        torch.cuda.synchronize()
+        assert not flint.kernel_fault()
+        for got, expected in zip(outputs, want):
+            assert torch.equal(got[0], expected[0]) and torch.equal(got[1], expected[1])
+            inside = expected[2] == expected[2]
+            assert torch.equal(got[2][inside], expected[2][inside])
 
 
 def test_one_shape_for_other_lengths(flint):

@@ -218,6 +218,71 @@ def test_results_repeat_and_replay(flint, heads, kv_heads, new, total):
         assert torch.equal(o, again) and torch.equal(lse, again_lse)
 
 
+@pytest.mark.parametrize("heads, kv_heads, new, total", [(128, 1, [1, 2], [300, 40]), (64, 1, [1], [129]),
+                                                         (33, 1, [1, 1], [500, 1]), (1024, 8, [1], [200])])
+def test_wide_groups(flint, heads, kv_heads, new, total):
+    cache = Cache(new, total, heads, kv_heads, 32)
+    cache.store(flint)
+    o, lse = cache.attend(flint)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    cache.check(o, lse)
+
+
+@pytest.mark.parametrize("longest", [1, 64])
+def test_offsets_beyond_32_bits(flint, longest):
+    """A cache of 5 * 10^9 values per tensor, of which the last pages are used."""
+    cache = Cache([2, 1], [700, 300], 8, 8, 256, longest=longest)
+    small, pages = cache.k_pages.shape[0], 40000
+    for name in ("k_pages", "v_pages"):
+        large = torch.empty(pages, 8, 256, 64, dtype=torch.half, device=DEV)
+        large[-small:] = getattr(cache, name)
+        setattr(cache, name, large)
+    counts = [3, 2]
+    for s, n in enumerate(counts):
+        cache.table[s, :n] += pages - small
+    cache.shape.pages = pages
+    cache.store(flint)
+    o, lse = cache.attend(flint)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    cache.check(o, lse)
+
+
+def test_a_captured_step_decodes_on(flint):
+    """One captured store and attention, replayed as the sequences grow by a token each time: lengths, tokens and
+    the page table change in place between replays."""
+    steps, totals = 20, [125, 3, 300]
+    final = Cache([steps] * 3, [t + steps for t in totals], 8, 2, 16, longest=1)
+    shape = final.shape
+    step_shape = PagedShape(3, 3, 8, 2, 64, final.width, final.width, 8 * 64, shape.pages, 16, shape.table_stride, 1)
+    qkv = torch.zeros(3, final.width, dtype=torch.half, device=DEV)
+    starts = torch.arange(4, dtype=torch.int32, device=DEV)
+    lengths = torch.ones(3, dtype=torch.int32, device=DEV)
+    table = torch.zeros_like(final.table)
+    o, lse = torch.zeros(3, 8 * 64, dtype=torch.half, device=DEV), torch.zeros(8, 3, device=DEV)
+    workspace = torch.empty(flint.paged_attention_workspace(step_shape), dtype=torch.uint8, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        flint.paged_store(final.k_pages, final.v_pages, qkv[:, 8 * 64:], qkv[:, 10 * 64:], starts, lengths, table, step_shape)
+        flint.paged_attention(o, lse, qkv, final.k_pages, final.v_pages, starts, lengths, table, step_shape, SCALE,
+                              workspace)
+    table.copy_(final.table)
+    for i in range(steps):
+        lengths.copy_(torch.tensor([t + i + 1 for t in totals], dtype=torch.int32))
+        for s in range(3):
+            qkv[s] = final.qkv[final.first[s] + i]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not flint.kernel_fault()
+        for s, t in enumerate(totals):
+            for h in range(8):
+                want = ragged.Head(qkv[s:s + 1, 64 * h:64 * h + 64], final.k[s][:t + i + 1, h // 4],
+                                   final.v[s][:t + i + 1, h // 4], t + i, SCALE)
+                assert ragged.within(o[s:s + 1, 64 * h:64 * h + 64], want.o, want.o_bound) <= 1
+                assert ragged.within(lse[h, s:s + 1], want.lse, ragged.LSE_BOUND) <= 1
+
+
 def test_a_prompt_in_chunks_and_token_by_token(flint):
     """The chain of a server: a prompt's attention at once, the same through the cache in chunks of
     odd sizes and then single tokens, and the words' probabilities at the end."""
