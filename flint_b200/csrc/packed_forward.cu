@@ -7,7 +7,8 @@
 // back as FP16 pairs and is the A operand of O += P V, which accumulates in tensor memory over the
 // row of key tiles; the exponent that probabilities are taken against moves only when a row's
 // maximum exceeds it by more than 2^8, so that O is rarely rescaled.
-// The batch is shared out evenly however ragged it is (packed_schedule.h); a tile split between CTAs
+// The batch is shared out evenly however ragged it is (packed_schedule.h): whole tiles, sorted by their length and dealt
+// out, or where a tile is too long for that a line of tiles cut into equal parts; a tile split between CTAs
 // leaves its parts (O before the division, row maxima and sums, FP32) in the workspace, and a second,
 // dependent launch joins them in the order of the keys.
 //
@@ -15,8 +16,8 @@
 // exponentials. Those bound long sequences: 128 x 128 of them take the SM's special-function unit 1,024 clocks
 // and the products 512; a quarter of them runs on the FMA pipe instead (half of them: 10 % slower, none: 9 %). A key tile
 // takes 1,350 clocks of an SM; short sequences are bound by what a tile's beginning and end cost, about two key tiles.
-// Measured, with the join: 5 sequences of up to 4,096 tokens, 16 query heads on 4, 82 us (508 TFLOP/s); 24 of up to 700,
-// 12 heads, 32 us; 64 single tokens on caches of up to 8,192, 32 heads on 8, 77 us (5.1 TB/s).
+// Measured, with the join: 5 sequences of up to 4,096 tokens, 16 query heads on 4, 73 us (570 TFLOP/s); 24 of up to 700,
+// 12 heads, 27 us; 64 single tokens on caches of up to 8,192, 32 heads on 8, 77 us (5.1 TB/s).
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -51,6 +52,8 @@ constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
 constexpr int kLeastPart = 4;   // of the line of key tiles, per CTA
 constexpr int kWholeKeys = 1024;   // up to which a tile is never split
+constexpr int kShortTile = 7;   // of the line: tiles up to it stay whole in any case, where tiles are dealt out
+constexpr int kMostDealt = 128;    // sequences whose tiles can be dealt out
 
 constexpr size_t kPartFloats = size_t{kRows} * kHead + 2 * kRows;   // O [column / 4][row][4], maxima, sums
 
@@ -134,14 +137,133 @@ __device__ __forceinline__ long long length_of(const TileParams& p, int s, int& 
     return head_length(before, tokens, p.log_tokens);
 }
 
+__device__ __forceinline__ int most_key_tiles(const TileParams& p, int before, int tokens) {
+    return tokens == 0 ? 0 : key_tiles(before, tokens, p.log_tokens, tile_count(tokens, p.log_tokens) - 1);
+}
+
+// Whether tiles stay whole and are dealt out: none has more key tiles than a part of the line is long, or all are
+// short. The longest CTA then works on 14 key tiles and ends instead of 17 (24 sequences of up to 700 tokens, 12 heads:
+// 32.4 -> 27.2 us with the join, which finds nothing to do; 16 of up to 1,024: 29.3 -> 21.6; 5 of up to 4,096: 82 -> 73).
+__device__ __forceinline__ bool deals_out(const TileParams& p, long long total, int longest) {
+    return p.a.sequences <= kMostDealt && total < 1LL << 30 &&
+           (!p.splits || longest <= max(kShortTile - kTileEnds, static_cast<int>(total) / static_cast<int>(gridDim.x)));
+}
+
+// Tiles dealt out whole. One warp, lane l with the sequences l, l + 32, ...
+struct Dealt {
+    static constexpr int kEach = kMostDealt / 32;
+    Sequence of[kEach];
+    int each = 1;
+    int count = 0;        // tiles
+    int longest = 0;      // key tiles of the next one at most
+    int round = 0;
+
+    __device__ __forceinline__ void load(const TileParams& p, int lane) {
+        each = (p.a.sequences + 31) / 32;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            of[i] = Sequence{0, 0, 0};
+            if (lane + 32 * i < p.a.sequences) {
+                of[i] = sequence_at(p.a, lane + 32 * i);
+            }
+        }
+    }
+    __device__ __forceinline__ int of_lane(const TileParams& p, int least) const {
+        int those = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (i < each) {
+                those += tiles_of_at_least(of[i].before(), of[i].count, p.log_tokens, least);
+            }
+        }
+        return those;
+    }
+    __device__ __forceinline__ int at_least(const TileParams& p, int least) const {
+        return __reduce_add_sync(kFullMask, of_lane(p, least)) * p.a.kv_heads;
+    }
+    __device__ __forceinline__ void begin(const TileParams& p, int most) {
+        longest = most;
+        count = at_least(p, 1);
+    }
+    // The next tile of this CTA, if there is one.
+    __device__ __forceinline__ bool next(const TileParams& p, int lane, Piece& out) {
+        const long long rank = dealt_rank(round, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+        ++round;
+        if (rank >= count) {
+            return false;
+        }
+        int low = 1;      // the most key tiles that more than `rank` tiles have
+        while (low < longest) {
+            const int middle = low + (longest - low + 1) / 2;
+            if (at_least(p, middle) > rank) {
+                low = middle;
+            } else {
+                longest = middle - 1;
+            }
+        }
+        // Among those of as many key tiles: by lane, the lane's sequences, heads, tiles.
+        const int more = of_lane(p, low + 1);
+        const int mine = (of_lane(p, low) - more) * p.a.kv_heads;
+        int upto = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int other = __shfl_up_sync(kFullMask, upto, off);
+            upto += lane >= off ? other : 0;
+        }
+        int at = static_cast<int>(rank) - __reduce_add_sync(kFullMask, more) * p.a.kv_heads - (upto - mine);
+        const int owner = __ffs(__ballot_sync(kFullMask, at >= 0 && at < mine)) - 1;
+        Sequence q = of[0];
+        int s = lane;
+#pragma unroll
+        for (int i = 0; i + 1 < kEach; ++i) {
+            if (s == lane + 32 * i && i + 1 < each) {
+                const int those = (tiles_of_at_least(q.before(), q.count, p.log_tokens, low) -
+                                   tiles_of_at_least(q.before(), q.count, p.log_tokens, low + 1)) * p.a.kv_heads;
+                if (at >= those) {
+                    at -= those;
+                    q = of[i + 1];
+                    s += 32;
+                }
+            }
+        }
+        at = __shfl_sync(kFullMask, at, owner);
+        out.index = __shfl_sync(kFullMask, s, owner);
+        out.sequence.first = __shfl_sync(kFullMask, q.first, owner);
+        out.sequence.count = __shfl_sync(kFullMask, q.count, owner);
+        out.sequence.keys = __shfl_sync(kFullMask, q.keys, owner);
+        const int of_low = tiles_of_at_least(out.sequence.before(), out.sequence.count, p.log_tokens, low);
+        const int these = of_low - tiles_of_at_least(out.sequence.before(), out.sequence.count, p.log_tokens, low + 1);
+        out.head = static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(these));
+        out.first_token = (tile_count(out.sequence.count, p.log_tokens) - of_low + at - out.head * these) << p.log_tokens;
+        out.tokens = min(out.sequence.count - out.first_token, 1 << p.log_tokens);
+        out.from = 0;
+        out.to = out.tiles = low;
+        return true;
+    }
+};
+
 // Which part of the line this CTA works on, for up to 32 sequences: one warp, its even lanes for one cut and the odd
 // ones for the other.
-__device__ __forceinline__ void locate_in_warp(const TileParams& p, Cut (&cuts)[2], int lane) {
+template <bool kDeals>
+__device__ __forceinline__ void locate_in_warp(const TileParams& p, Cut (&cuts)[2], int& whole, int lane) {
     int before, tokens;
     const long long length = length_of(p, lane, before, tokens);
     const long long mine = length * p.a.kv_heads;
     const long long upto = warp_prefix(mine, lane);
     const long long total = __shfl_sync(kFullMask, upto, 31);
+    if constexpr (kDeals) {
+        const int longest = __reduce_max_sync(kFullMask, most_key_tiles(p, before, tokens));
+        const bool deals = deals_out(p, total, longest);
+        if (lane == 0) {
+            whole = deals ? longest : 0;
+        }
+        if (deals) {
+            if (lane < 2) {
+                cuts[lane] = Cut{total, p.a.sequences, 0, 0, 0};
+            }
+            return;
+        }
+    }
     const Place place(p, total, lane & 1);
     const long long begins = upto - mine;
     const long long first = __shfl_sync(kFullMask, place.at, 0), second = __shfl_sync(kFullMask, place.at, 1);
@@ -159,23 +281,42 @@ __device__ __forceinline__ void locate_in_warp(const TileParams& p, Cut (&cuts)[
 }
 
 // The same for any number: every thread of the block takes part.
-__device__ __noinline__ void locate(const TileParams& p, Cut (&cuts)[2], long long (&scan)[kWarps + 1]) {
+template <bool kDeals>
+__device__ __noinline__ void locate(const TileParams& p, Cut (&cuts)[2], int& whole, long long (&scan)[kWarps + 1],
+                                    int (&scan_longest)[kWarps]) {
     const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
     int before = 0, tokens = 0;
     long long sum = 0;
+    int longest = 0;
     for (int s = tid; s < p.a.sequences; s += kThreads) {
         sum += length_of(p, s, before, tokens);
+        longest = kDeals ? max(longest, most_key_tiles(p, before, tokens)) : 0;
     }
     sum = warp_sum(sum);
+    longest = __reduce_max_sync(kFullMask, longest);
     if (lane == 0) {
         scan[warp] = sum;
+        scan_longest[warp] = longest;
     }
     __syncthreads();
     long long total = 0;
     for (int w = 0; w < kWarps; ++w) {
         total += scan[w];
+        longest = max(longest, scan_longest[w]);
     }
     total *= p.a.kv_heads;
+    if constexpr (kDeals) {
+        const bool deals = deals_out(p, total, longest);
+        if (tid == 0) {
+            whole = deals ? longest : 0;
+        }
+        if (deals) {
+            if (tid < 2) {
+                cuts[tid] = Cut{total, p.a.sequences, 0, 0, 0};
+            }
+            return;
+        }
+    }
     const Place place[2] = {Place(p, total, 0), Place(p, total, 1)};
     if (tid < 2 && place[tid].at == total) {
         cuts[tid] = Cut{total, p.a.sequences, 0, 0, 0};
@@ -237,6 +378,9 @@ struct Meeting {
 // work where one would; the copies are put together at the end of a piece.
 template <bool kPaged, int kSubsets>
 __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __grid_constant__ TileParams p) {
+    // Few rows' tiles are not dealt out: finding one takes longer than what it gains (8 single tokens on up to 1,000 keys
+    // 14.2 -> 15.2 us, 64 on up to 8,192 78 -> 82 us with the code alone).
+    constexpr bool kDeals = kSubsets == 1;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_tiles = base;
@@ -247,6 +391,8 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
     __shared__ int abort_flag;
     __shared__ Cut cuts[2];
     __shared__ long long scan[kWarps + 1];
+    __shared__ int scan_longest[kWarps];
+    __shared__ int whole_tiles;      // the longest tile's key tiles where tiles are dealt out, else 0
     __shared__ PieceInfo pieces[kPieces];
     __shared__ float pair_max[2][2][kRows];           // [step parity][half of the columns][row]
     __shared__ float merge_max[4][32], merge_sum[kSoftmaxWarps][32];
@@ -283,10 +429,14 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         sm100::tmem_alloc(sm100::smem_u32(&tmem_slot), 256);
     }
     dependency_wait();
+    Dealt dealt;
+    if (kDeals && warp == 0 && p.a.sequences <= kMostDealt) {
+        dealt.load(p, lane);
+    }
     if (p.a.sequences > 32) {
-        locate(p, cuts, scan);
+        locate<kDeals>(p, cuts, whole_tiles, scan, scan_longest);
     } else if (warp == 2) {
-        locate_in_warp(p, cuts, lane);
+        locate_in_warp<kDeals>(p, cuts, whole_tiles, lane);
     }
     sm100::tc_fence_before_sync();
     __syncthreads();
@@ -299,11 +449,15 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
 
     if (warp == 0) {
         Walk walk;
-        Piece piece;
+        Piece piece = {};
         walk.begin(SequenceOf{p.a}, cuts[0], cuts[1].at);
         int round = 0;
-        bool more = walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
-        int j = more ? piece.from : 0;
+        const bool whole = kDeals && whole_tiles > 0;
+        if (whole) {
+            dealt.begin(p, whole_tiles);
+        }
+        bool fetch = true, more = false;     // whether the next piece is to be found, and whether there was one
+        int j = 0;
         int slot = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -362,6 +516,16 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         };
         int waiting = 0;     // K tiles whose V tile has not been asked for
         while (ok) {
+            if (fetch) {
+                fetch = false;
+                more = whole ? dealt.next(p, lane, piece)
+                             : walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
+                j = piece.from;
+                if (!more && lane == 0) {
+                    pieces[round % kPieces].to = 0;
+                    sm100::mbar_arrive(bar.piece_full(round % kPieces));
+                }
+            }
             if (more) {
                 if (j == piece.from) {
                     // A new piece. Its description's place was read long ago: the ring of tiles keeps this
@@ -393,12 +557,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 ++waiting;
                 if (++j == piece.to) {
                     ++round;
-                    more = walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece);
-                    j = more ? piece.from : 0;
-                    if (!more && lane == 0) {
-                        pieces[round % kPieces].to = 0;
-                        sm100::mbar_arrive(bar.piece_full(round % kPieces));
-                    }
+                    fetch = true;
                 }
                 if (waiting < 2) {
                     continue;
@@ -408,10 +567,6 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     --waiting;
                 }
             } else {
-                if (round == 0 && lane == 0) {
-                    pieces[0].to = 0;          // nothing to do at all
-                    sm100::mbar_arrive(bar.piece_full(0));
-                }
                 if (waiting > 0) {
                     load(&p.map_v, at_now, head_now);
                 }

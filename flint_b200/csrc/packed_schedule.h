@@ -7,6 +7,8 @@
 // and two more for what starting and ending it costs. The line is cut into as many equal parts as
 // there are CTAs, so that however long and short the sequences are, CTAs work equally long; a cut
 // that falls close to a tile's end moves there. A tile that a cut splits is put together from parts afterwards.
+//
+// Batches of up to 128 sequences without a tile that is longer than a CTA's part keep their tiles whole (dealt_rank).
 #pragma once
 
 namespace fb {
@@ -61,6 +63,13 @@ FB_SCHEDULE long long tiles_before(int before, int log_tokens, int i) {
 
 FB_SCHEDULE int tile_count(int tokens, int log_tokens) {
     return static_cast<int>((static_cast<long long>(tokens) + (1LL << log_tokens) - 1) >> log_tokens);
+}
+
+// How many tiles of one head have `least` key tiles or more: they are its last ones.
+FB_SCHEDULE int tiles_of_at_least(int before, int tokens, int log_tokens, int least) {
+    const int count = tile_count(tokens, log_tokens);
+    const int beyond = (least - 1) * kKeyTile - before;      // so many tokens see less
+    return least <= 1 || beyond <= 0 ? count : tokens <= beyond ? 0 : count - (beyond >> log_tokens);
 }
 
 // Length on the line of one head of a sequence.
@@ -123,6 +132,12 @@ FB_SCHEDULE long long cut_tolerance(long long total, int parts) {
     const long long each = quotient(total, parts);
     const long long wanted = each < 24 ? 2 : 3;
     return wanted < (each - 1) / 2 ? wanted : (each - 1) / 2;
+}
+
+// Where no tile is much longer than a CTA's part, the tiles stay whole: sorted by their key tiles, longest first, and dealt
+// out to the CTAs forwards and backwards in turn. The rank of CTA k's tile in a round.
+FB_SCHEDULE long long dealt_rank(int round, int cta, int ctas) {
+    return static_cast<long long>(round) * ctas + (round % 2 == 0 ? cta : ctas - 1 - cta);
 }
 
 // A sequence's place in the rows (its new tokens) and how many keys it has, those among them.

@@ -114,6 +114,20 @@ def test_wide_groups_and_many_items(flint, lengths, heads, kv_heads):
     batch.check(o, lse, grads)
 
 
+@pytest.mark.parametrize("heads, kv_heads", [(12, 12), (8, 1), (6, 2)])
+@pytest.mark.parametrize("count, longest", [(3, 1000), (20, 60), (32, 500), (33, 500), (100, 260), (128, 130), (129, 130)])
+def test_batches_of_many_short_sequences(flint, count, longest, heads, kv_heads):
+    """Tiles of one to eight key tiles, several per CTA, in batches on both sides of what deals them out whole."""
+    g = torch.Generator().manual_seed(count + heads)
+    lengths = torch.randint(0, longest + 1, (count,), generator=g).tolist()
+    lengths[count // 2] = longest
+    batch = Batch(lengths, heads, kv_heads, before=9)
+    o, lse = batch.forward(flint)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    batch.check(o, lse)
+
+
 @pytest.mark.parametrize("size", [4.0, 0.01])
 def test_large_and_small_scores(flint, size):
     batch = Batch([300, 150, 700], 4, 2, size=size)

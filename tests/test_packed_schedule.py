@@ -155,3 +155,59 @@ def test_every_key_tile_is_worked_on_once(tmp_path):
                     str(tmp_path / "schedule.cpp"), "-o", str(tmp_path / "schedule")], check=True)
     result = subprocess.run([str(tmp_path / "schedule")], capture_output=True, text=True)
     assert result.returncode == 0, result.stdout + result.stderr
+
+
+DEALT = r"""
+#include <algorithm>
+#include <cstdio>
+#include <random>
+#include <vector>
+#include "packed_schedule.h"
+using namespace fb;
+#define NEED(x) do { if (!(x)) { std::printf("line %d: %s (trial %d)\n", __LINE__, #x, trial); return 1; } } while (0)
+
+int main() {
+    std::mt19937 rng(11);
+    auto pick = [&](int a, int b) { return static_cast<int>(a + rng() % (b - a + 1)); };
+    for (int trial = 0; trial < 2000; ++trial) {
+        const int log_tokens = pick(0, 7), tokens = trial % 6 == 0 ? 0 : pick(1, trial % 3 ? 400 : 5000);
+        const int before = trial % 5 == 0 ? -pick(0, tokens + 3) : trial % 2 ? 0 : pick(0, 3000);
+        std::vector<int> all;
+        for (int i = 0; i < tile_count(tokens, log_tokens); ++i) {
+            all.push_back(key_tiles(before, tokens, log_tokens, i));
+        }
+        NEED(std::is_sorted(all.begin(), all.end()));
+        for (int least = -1; least <= (all.empty() ? 1 : all.back()) + 2; ++least) {
+            const auto those = std::count_if(all.begin(), all.end(), [&](int t) { return t >= least; });
+            NEED(tiles_of_at_least(before, tokens, log_tokens, least) == those);
+        }
+        // Every rank is dealt to one CTA, in rounds.
+        const int ctas = pick(1, 50), tiles = pick(1, 300);
+        std::vector<int> dealt(tiles);
+        for (int cta = 0; cta < ctas; ++cta) {
+            long long before_it = -1;
+            for (int round = 0; dealt_rank(round, cta, ctas) < tiles; ++round) {
+                NEED(dealt_rank(round, cta, ctas) > before_it);
+                before_it = dealt_rank(round, cta, ctas);
+                ++dealt[before_it];
+            }
+        }
+        NEED(std::all_of(dealt.begin(), dealt.end(), [](int n) { return n == 1; }));
+    }
+    const int trial = -1;
+    NEED(tiles_of_at_least(0, 1 << 24, 0, 1 << 17) == 128);
+    NEED(tiles_of_at_least((1 << 26) - (1 << 24), 1 << 24, 7, 1 << 19) == 1);
+    return 0;
+}
+"""
+
+
+def test_every_rank_of_whole_tiles_is_dealt_once(tmp_path):
+    compiler = shutil.which("g++")
+    if compiler is None:
+        pytest.skip("no C++ compiler")
+    (tmp_path / "dealt.cpp").write_text(DEALT)
+    subprocess.run([compiler, "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}",
+                    str(tmp_path / "dealt.cpp"), "-o", str(tmp_path / "dealt")], check=True)
+    result = subprocess.run([str(tmp_path / "dealt")], capture_output=True, text=True)
+    assert result.returncode == 0, result.stdout + result.stderr

@@ -144,6 +144,21 @@ def test_long_caches(flint, heads, kv_heads, new, total):
     cache.check(o, lse)
 
 
+@pytest.mark.parametrize("heads, kv_heads", [(12, 12), (8, 1)])
+@pytest.mark.parametrize("count", [5, 40, 130])
+def test_many_chunks(flint, count, heads, kv_heads):
+    """Chunks of prompts behind what is there, some with tokens that have no position."""
+    g = torch.Generator().manual_seed(count)
+    new = torch.randint(0, 200, (count,), generator=g).tolist()
+    total = [max(n + int(d), 0) for n, d in zip(new, torch.randint(-20, 600, (count,), generator=g))]
+    cache = Cache(new, total, heads, kv_heads, 64)
+    cache.store(flint)
+    o, lse = cache.attend(flint)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    cache.check(o, lse)
+
+
 @pytest.mark.parametrize("longest", [1, 64])
 def test_tokens_without_a_position(flint, longest):
     """A length below the number of new tokens: the first ones have no position, nothing to see."""
