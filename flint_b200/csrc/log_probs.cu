@@ -242,10 +242,10 @@ __device__ __forceinline__ float key_value(Key key) {
 // is a lower bound of the k-th largest logit; what is not below it (about k values) is collected in the
 // second pass and put in order by counting. Where too many qualify (rows of equal logits), or a NaN is among
 // them, the row is gone through once per alternative.
-// Measured on rows of GPT-2's 50,257 words: 8,192 FP16 rows with five alternatives 207 us (4.0 TB/s), 4,096 without 93 us;
-// 1,000 FP32 rows, a pair of CTAs each, 57 us; one FP32 row on eight CTAs with twenty alternatives 8.8 us with its
-// launch. Bound by issue slots (42 instructions per eight logits for the sums) and what a row costs besides. (Rows held in
-// registers, one CTA per SM: 355 us where shared memory takes 207.)
+// Measured on rows of GPT-2's 50,257 words: 8,192 FP16 rows with five alternatives 208 us (4.0 TB/s), 4,096 without 92 us;
+// 1,000 FP32 rows, a pair of CTAs each, 56 us; one FP32 row on eight CTAs with twenty alternatives 7.9 us with its
+// launch. Bound by issue slots (40 instructions per eight logits for the sums) and what a row costs besides. (Rows held in
+// registers, one CTA per SM: 355 us where shared memory takes 208.)
 constexpr int blocks_per_sm(int threads, int held) { return (threads == 128 ? 4 : 1) * (held > 4 ? 1 : 2); }
 
 constexpr int kChunks = 2;      // pieces in which a slice is copied into shared memory
