@@ -52,7 +52,7 @@ constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
 constexpr int kLeastPart = 4;   // of the line of key tiles, per CTA
 constexpr int kWholeKeys = 1024;   // up to which a tile is never split
-constexpr int kShortTile = 7;   // of the line: tiles up to it stay whole in any case, where tiles are dealt out
+constexpr int kSplitCost = 6;      // about what splits and their join cost, in key tiles
 constexpr int kMostDealt = 128;    // sequences whose tiles can be dealt out
 
 constexpr size_t kPartFloats = size_t{kRows} * kHead + 2 * kRows;   // O [column / 4][row][4], maxima, sums
@@ -141,12 +141,14 @@ __device__ __forceinline__ int most_key_tiles(const TileParams& p, int before, i
     return tokens == 0 ? 0 : key_tiles(before, tokens, p.log_tokens, tile_count(tokens, p.log_tokens) - 1);
 }
 
-// Whether tiles stay whole and are dealt out: none has more key tiles than a part of the line is long, or all are
-// short. The longest CTA then works on 14 key tiles and ends instead of 17 (24 sequences of up to 700 tokens, 12 heads:
-// 32.4 -> 27.2 us with the join, which finds nothing to do; 16 of up to 1,024: 29.3 -> 21.6; 5 of up to 4,096: 82 -> 73).
+// Whether tiles stay whole and are dealt out: none has more key tiles than a part of the line is long and splits cost.
+// The longest CTA then works on 14 key tiles and ends instead of 17 (24 sequences of up to 700 tokens, 12 heads:
+// 32.4 -> 27.3 us with the join, which finds nothing to do; 16 of up to 1,024: 29.4 -> 21.8; 5 of up to 4,096: 82 -> 73).
+// Tiles longer than a part: 6 more key tiles 24.1 -> 20.6, 28.7 -> 24.9 and 21.7 -> 21.0 us (three batches), 9 more 20.2 ->
+// 21.0 and 22.8 -> 25.1, 11 more 24.0 -> 29.5.
 __device__ __forceinline__ bool deals_out(const TileParams& p, long long total, int longest) {
     return p.a.sequences <= kMostDealt && total < 1LL << 30 &&
-           (!p.splits || longest <= max(kShortTile - kTileEnds, static_cast<int>(total) / static_cast<int>(gridDim.x)));
+           (!p.splits || longest <= (static_cast<int>(total) - 1) / static_cast<int>(gridDim.x) + 1 + kSplitCost);
 }
 
 // Tiles dealt out whole. One warp, lane l with the sequences l, l + 32, ...

@@ -8,7 +8,7 @@
 // there are CTAs, so that however long and short the sequences are, CTAs work equally long; a cut
 // that falls close to a tile's end moves there. A tile that a cut splits is put together from parts afterwards.
 //
-// Batches of up to 128 sequences without a tile that is longer than a CTA's part keep their tiles whole (dealt_rank).
+// Batches of up to 128 sequences without a tile that is much longer than a CTA's part keep their tiles whole (dealt_rank).
 #pragma once
 
 namespace fb {
