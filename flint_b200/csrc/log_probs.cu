@@ -22,6 +22,9 @@ constexpr int kMostRanks = 8;        // CTAs of a cluster
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -200.0f;   // e^-200 is 0 in FP32, and 0 * -200 a number
+// FP16: minus infinity may stand as the lowest finite value, -65,504, where the row's largest logit (or log-sum-exp) is so
+// far above it that e^(the difference) is 0. Rows below this bound are low: their logits are raised first.
+constexpr float kLowRow = -65000.0f;
 
 using Key = unsigned long long;
 
@@ -190,7 +193,7 @@ struct SumsH : SumsBase {
         const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            // (The lowest finite value does for minus infinity.)
+            // (The lowest finite value does for minus infinity: low rows are raised.)
             const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&w[i]), __half2half2(__ushort_as_half(0xfbff)));
             pair(i, fb::f2_mul(fb::f2_pack(difference(__low2half(h)), difference(__high2half(h))), fb::f2_pack(kLog2e, kLog2e)));
         }
@@ -198,6 +201,19 @@ struct SumsH : SumsBase {
 };
 template <typename T>
 using Sums = typename std::conditional<sizeof(T) == 2, SumsH, SumsF>::type;
+
+// Low rows of FP16 (their values are multiples of 32 from -65,504 on, or minus infinity) are taken 32,768 higher: that is
+// exact, as it is for their FP32 log-sum-exps, and far above the lowest finite value.
+constexpr float kRaise = 32768.0f;
+__device__ __forceinline__ void raise_word(uint4&, float) {}
+__device__ __forceinline__ void raise_word(uint4& q, __half) {
+    unsigned* w = reinterpret_cast<unsigned*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __hadd2(*reinterpret_cast<const __half2*>(&w[i]), __float2half2_rn(kRaise));
+        w[i] = *reinterpret_cast<const unsigned*>(&h);
+    }
+}
 
 // A word's values from the `count`-th on become minus infinity, which counts for nothing.
 __device__ __forceinline__ void cut_word(uint4& q, int count, float) {
@@ -454,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             }
         };
         const bool collects = top > 0 && __any_sync(fb::kFullMask, my_max >= bound);
-        Sums<T> sums_of(mx);
+        const bool low = sizeof(T) == 2 && mx < kLowRow;
+        Sums<T> sums_of(low ? mx + kRaise : mx);
         if constexpr (kStaged) {
             if (collects) {
 #pragma unroll 4
@@ -464,6 +481,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                         collect(q, i);
                     }
                 }
+            }
+            if (low) {
+                for (int i = tid; i < words; i += kThreads) {     // (this thread's words, here and below)
+                    uint4 q = staged[i];
+                    raise_word(q, T());
+                    staged[i] = q;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // ahead of the next row's copy
             }
 #pragma unroll 4
             for (int i = tid; i < words; i += kThreads) {
@@ -477,6 +502,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                     if (i < words && Max<T>::word(held[j]) >= bound) {
                         collect(held[j], i);
                     }
+                }
+            }
+            if (low) {
+#pragma unroll
+                for (int j = 0; j < kHeld; ++j) {
+                    raise_word(held[j], T());
                 }
             }
             const uint4* next_in = row_of(next < p.rows ? next : row);
@@ -688,10 +719,12 @@ constexpr int kGradientThreads = 512;
 constexpr int kGradientWords = 4;
 
 // What a row's gradient needs: e^d (slope d + constant), and `a` more at the target; zeros for a row without tokens.
+template <typename T>
 struct RowGradient {
     fb::F2 minus_lse, slope, constant;
     float a;
     int target;
+    bool low;      // its logits are to be raised
     __device__ __forceinline__ RowGradient(const LogProbGradientArgs& p, size_t row) {
         target = p.targets != nullptr ? p.targets[row] : p.vocab;
         a = p.d_log_probs != nullptr && target < p.vocab ? p.d_log_probs[row] : 0.0f;
@@ -701,15 +734,19 @@ struct RowGradient {
             lse = a = b = entropy = 0.0f;
             target = -1;
         }
+        low = sizeof(T) == 2 && lse < kLowRow;
+        lse += low ? kRaise : 0.0f;
         minus_lse = fb::f2_pack(-lse, -lse);
         slope = fb::f2_pack(-b, -b);
         const float rest = -fmaf(b, entropy, a);
         constant = fb::f2_pack(rest, rest);
     }
-    template <typename T>
-    __device__ __forceinline__ uint4 word(const uint4& q, int column, int vocab) const {
+    __device__ __forceinline__ uint4 word(uint4 q, int column, int vocab) const {
         using W = Word<T>;
         float v[W::kValues], out[W::kValues];
+        if (low) {
+            raise_word(q, T());
+        }
         W::unpack_finite(v, q);
 #pragma unroll
         for (int c = 0; c < W::kValues; c += 2) {
@@ -762,12 +799,12 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
             }
         }
         if constexpr (kLong) {
-            const RowGradient row(p, first_row);
+            const RowGradient<T> row(p, first_row);
 #pragma unroll
             for (int j = 0; j < kGradientWords; ++j) {
                 const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
                 if (i < here) {
-                    __stcs(out + i, row.word<T>(held[j], (first_word + i) * W::kValues, p.vocab));
+                    __stcs(out + i, row.word(held[j], (first_word + i) * W::kValues, p.vocab));
                 }
             }
         } else {
@@ -776,7 +813,7 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
                 const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
                 if (i < here) {
                     const int r = i / row_words;
-                    __stcs(out + i, RowGradient(p, first_row + r).word<T>(held[j], (i - r * row_words) * W::kValues, p.vocab));
+                    __stcs(out + i, RowGradient<T>(p, first_row + r).word(held[j], (i - r * row_words) * W::kValues, p.vocab));
                 }
             }
         }

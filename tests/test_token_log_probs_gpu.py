@@ -218,3 +218,77 @@ def test_results_repeat_and_replay(flint, rows, vocab, fp32):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(want, again))
+
+
+LOWEST = [(1, 8), (3, 8), (31, 16), (100, 8), (1001, 8), (9001, 96), (20001, 8), (50257, 8), (50257, 200)]
+
+
+def near_the_lowest(rows, vocab):
+    """FP16 rows whose logits are minus infinity, the type's lowest value or a few steps of 32 above it."""
+    g = torch.Generator(device=DEV).manual_seed(rows * vocab)
+    logits = torch.full((rows, (vocab + 7) // 8 * 8), float("nan"), dtype=torch.half, device=DEV)
+    steps = torch.randint(0, 16, (rows, vocab), generator=g, device=DEV)
+    cannot = torch.rand(rows, vocab, generator=g, device=DEV) < 0.6
+    cannot[:, 0] = False
+    kind, column = torch.arange(rows, device=DEV)[:, None] % 8, torch.arange(vocab, device=DEV)[None, :]
+    middle = column == vocab // 2
+    steps = torch.where((kind == 3) | (kind == 4), steps, 0)
+    steps = torch.where((kind == 5) & middle, 3, steps)        # -65,408
+    steps = torch.where((kind == 6) & middle, 15, steps)       # -65,024
+    steps = torch.where((kind == 7) & middle, 17, steps)       # -64,960
+    x = (steps * 32 - 65504).double()
+    x = torch.where((kind == 1) & ~middle, float("-inf"), x)
+    x = torch.where((kind == 2) & (column % 2 == 1), float("-inf"), x)
+    x = torch.where(((kind == 4) | ((kind >= 6) & ~middle)) & cannot, float("-inf"), x)
+    logits[:, :vocab] = x.half()
+    assert torch.equal(logits[:, :vocab].double(), x)
+    targets = torch.where(kind[:, 0] % 2 == 0, vocab // 2, 0).to(torch.int32).to(torch.uint16)
+    return logits, targets
+
+
+@pytest.mark.parametrize("vocab, rows", LOWEST)
+def test_rows_near_the_types_lowest_value(flint, vocab, rows):
+    """Minus infinity stays apart from the lowest finite value, also where that is a row's largest logit. lse
+    is rounded to FP32 once more at 65,504, by 2^-9 at most."""
+    logits, targets = near_the_lowest(rows, vocab)
+    top = min(vocab, 5)
+    got = forward(flint, logits, targets, vocab, top)
+    torch.cuda.synchronize()
+    want = exact(logits, targets, vocab, top)
+    for mine, right, bound in ((got[0], want[0], SUM), (got[1], want[1], SUM * (1 + want[1])),
+                               (got[2], want[2], SUM + 2.0 ** -9), (got[3], want[3], SUM)):
+        assert torch.equal(mine.isinf(), right.isinf())
+        off = torch.where(right.isinf(), 0.0, (mine.double() - right).abs())
+        # (2^-22 of differences of up to 544, where these are not 0.)
+        assert (off <= bound + 2.0 ** -22 * torch.where(right.isinf(), 0.0, right.abs())).all()
+    assert torch.equal(got[4].to(torch.int64), want[4])
+    assert (got[1][1::8] == 0).all()          # one possible word
+
+
+@pytest.mark.parametrize("terms", ["both", "log_probs", "entropy"])
+@pytest.mark.parametrize("vocab, rows", LOWEST)
+def test_gradient_of_rows_near_the_types_lowest_value(flint, vocab, rows, terms):
+    """The gradient's p comes from the FP32 lse, which is off by 2^-9 at 65,504: log p by that, and p by that of itself
+    (twice as much is allowed below for the square of it)."""
+    logits, targets = near_the_lowest(rows, vocab)
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    a = torch.randn(rows, generator=g, device=DEV) * 8 if terms != "entropy" else None
+    b = torch.randn(rows, generator=g, device=DEV) if terms != "log_probs" else None
+    got = gradient(flint, logits, targets, vocab, a, b)
+    same = gradient(flint, logits, targets, vocab, a, b, in_place=True)
+    torch.cuda.synchronize()
+    log_p = torch.log_softmax(logits[:, :vocab].double(), 1)
+    p = log_p.exp()
+    none = log_p.isinf()
+    log_p = torch.where(none, 0.0, log_p)
+    entropy = -(p * log_p).sum(1, keepdim=True)
+    zero = torch.zeros(rows, 1, dtype=torch.float64, device=DEV)
+    da, db = (zero if d is None else d.double()[:, None] for d in (a, b))
+    at_target = torch.zeros_like(p).scatter_(1, targets.to(torch.int64)[:, None], 1.0)
+    want = da * (at_target - p) - db * p * (log_p + entropy)
+    moved = p * (da.abs() + db.abs() * (1 + log_p.abs() + entropy)) * 2 * (2.0 ** -9 + 4 * SUM)
+    bound = moved + want.abs() * 2.0 ** -11 + 2.0 ** -25
+    assert ((got[:, :vocab].double() - want).abs() <= bound).all()
+    away = none & (at_target == 0)
+    assert (got[:, :vocab][away] == 0).all() and (got[:, vocab:] == 0).all()
+    assert torch.equal(got, same)
