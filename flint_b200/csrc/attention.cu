@@ -98,7 +98,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 #endif
 __device__ __forceinline__ void exp2_two(int pair, float x0, float x1, float& e0, float& e1) {
     if ((pair & 3) < FB_ATTN_BWD_FMA_EXP_OF_4) {
-        exp2_pair_fma(fb::f2_pack(x0, x1), e0, e1);
+        exp2_pair_fma<true>(fb::f2_pack(x0, x1), e0, e1);
     } else {
         e0 = fast_exp2(x0);
         e1 = fast_exp2(x1);
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                                                    __uint_as_float(raw[32 * c + 2 * i + 1])),
                                        scale_pair, shift);
                         if ((i & 3) < FB_ATTN_FMA_EXP_OF_4) {
-                            exp2_pair_fma(x, lo, hi);
+                            exp2_pair_fma<false>(x, lo, hi);
                         } else {
                             fb::f2_unpack(x, lo, hi);
                             lo = fast_exp2(lo);

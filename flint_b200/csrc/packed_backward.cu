@@ -247,7 +247,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // Two exponentials; a quarter of the pairs takes the FMA pipe.
 __device__ __forceinline__ void exp2_two(int pair, float x0, float x1, float& e0, float& e1) {
     if ((pair & 3) == 0) {
-        exp2_pair_fma(f2_pack(x0, x1), e0, e1);
+        exp2_pair_fma<true>(f2_pack(x0, x1), e0, e1);
     } else {
         e0 = fast_exp2(x0);
         e1 = fast_exp2(x1);

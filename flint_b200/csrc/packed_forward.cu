@@ -855,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             const F2 t = f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])),
                                                 scale_pair, shift);
                             if (kSubsets == 1 && (i & 3) == 0) {
-                                exp2_pair_fma(t, x, y);
+                                exp2_pair_fma<false>(t, x, y);
                             } else {
                                 f2_unpack(t, x, y);
                                 x = fast_exp2(x);

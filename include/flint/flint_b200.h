@@ -264,7 +264,10 @@ FLINT_API flint_status flint_b200_packed_attention_backward_workspace(
     const flint_b200_packed_shape* shape, size_t* bytes);
 
 /* Gradients of the above from d_o and the forward call's o and lse. dk and dv are sums over the
- * query heads that share a head, taken in one fixed order: results repeat bit for bit. */
+ * query heads that share a head, taken in one fixed order: results repeat bit for bit. A row that is NaN makes its
+ * dq NaN, and dk and dv of the keys that it sees. Within a sequence a value that is not finite may also reach rows
+ * of its block of 128 that have no part in it: dq of up to 127 rows before one of k, and dk and dv of up
+ * to 127 rows behind one of q or d_o. */
 FLINT_API flint_status flint_b200_packed_attention_backward(
     void* dq, void* dk, void* dv, const void* d_o, const void* o, const void* lse, const void* q,
     const void* k, const void* v, const void* starts, const flint_b200_packed_shape* shape,

@@ -247,3 +247,20 @@ def test_attention_matches_the_golden_vectors(flint, golden, case):
     assert rel_error(dq, g[case + "_dq"]) <= 5e-3
     assert rel_error(dk, g[case + "_dk"]) <= 5e-3
     assert rel_error(dv, g[case + "_dv"]) <= 5e-3
+
+
+@pytest.mark.parametrize("query", [5, *range(192, 208), 255])
+def test_attention_gradients_of_a_query_that_is_nan(flint, query):
+    """Its row is NaN, and so are dk and dv of every key that it sees, whatever column of a step its scores are in."""
+    g = torch.Generator().manual_seed(query)
+    q, k, v, d_o = (torch.randn(2, 256, 64, generator=g).half().to(DEV) for _ in range(4))
+    q[0, query, 3] = float("nan")
+    o, dq, dk, dv = (torch.full_like(q, 7.0) for _ in range(4))
+    lse, delta = (torch.zeros(2, 256, device=DEV) for _ in range(2))
+    flint.attention_forward(o, lse, q, k, v, 2, 256, 64, 0.125)
+    flint.attention_backward(dq, dk, dv, d_o, o, lse, delta, q, k, v, 2, 256, 64, 0.125)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    assert o[0, query].isnan().all() and dq[0, query].isnan().all()
+    assert dk[0, :query + 1].isnan().all() and dv[0, :query + 1].isnan().all()
+    assert not any(t[1].isnan().any() for t in (o, dq, dk, dv))

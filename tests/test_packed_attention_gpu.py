@@ -376,3 +376,25 @@ def test_starts_out_of_range_are_reported(flint, starts):
     batch.backward(flint, o, lse)
     torch.cuda.synchronize()
     assert flint.kernel_fault()
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(2, 2), (4, 1)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_not_finite_reaches_the_gradients_of_all_its_keys(flint, heads, kv_heads, bad):
+    """Whatever column of a step's scores the query has: its row is NaN, and so are dq there and dk and dv of the keys
+    that it sees. Other sequences, and keys beyond its block, get nothing of it."""
+    for query in (5, 127, *range(192, 208), 299):
+        batch = Batch([300, 200], heads, kv_heads, behind=0)
+        batch.qkv[query, :64] = bad
+        batch.qkv[:300, heads * 64] = 1.0     # (so that an infinite query's scores are infinite or NaN)
+        o, lse = batch.forward(flint)
+        grads = batch.backward(flint, o, lse)
+        torch.cuda.synchronize()
+        assert not flint.kernel_fault()
+        dq, dk, dv = batch.parts(grads)
+        assert o[query, :64].isnan().all() and dq[query, :64].isnan().all()
+        assert dk[:query + 1, :64].isnan().all() and dv[:query + 1, :64].isnan().all()
+        assert not grads[300:].isnan().any() and not o[300:].isnan().any()
+        beyond = (query // 128 + 1) * 128
+        assert not dv[beyond:300].isnan().any() and not dk[beyond:300].isnan().any()
+        assert not dq[:, 64:].isnan().any() and not o[:, 64:].isnan().any()
