@@ -313,6 +313,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         sm100::mbar_fence_init();
     }
     fb::dependency_wait();
+    const T* logits = fb::after_wait(static_cast<const T*>(p.logits));
+    const uint16_t* targets = fb::after_wait(p.targets);
     if (p.ranks > 1) {
         sm100::cluster_sync_all();    // every CTA of the cluster runs before any writes to the first one's memory
     } else {
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     if (tid == 0) {
         fb::dependency_release();
     }
-    auto row_of = [&](size_t row) { return static_cast<const uint4*>(p.logits) + row * row_words + first_word; };
+    auto row_of = [&](size_t row) { return reinterpret_cast<const uint4*>(logits) + row * row_words + first_word; };
     size_t row = blockIdx.x / p.ranks;
     if (row >= p.rows) {
         return;     // (the whole cluster)
@@ -353,9 +355,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         }
     }
     // The scribe's: this row's target and its logit, fetched while the row before was worked on.
-    auto target_of = [&](size_t from) { return p.targets != nullptr ? static_cast<int>(fb::load_input(p.targets + from)) : 0; };
+    auto target_of = [&](size_t from) { return p.targets != nullptr ? static_cast<int>(fb::load_input(targets + from)) : 0; };
     auto target_value_of = [&](size_t from, int column) {
-        return column < p.vocab ? W::value(static_cast<const T*>(p.logits) + from * p.cols, column) : 0.0f;
+        return column < p.vocab ? W::value(logits + from * p.cols, column) : 0.0f;
     };
     const bool scribe = tid == kScribe && rank == 0;
     int target = scribe ? target_of(row) : 0;
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     bool gave_up = false;
     uint32_t phase = 0;
     for (int parity = 0; row < p.rows; row += stride, parity ^= 1) {
-        const T* values = static_cast<const T*>(p.logits) + row * p.cols;
+        const T* values = logits + row * p.cols;
         const size_t next = row + stride;
         const size_t soon = kStaged ? next : next + stride;
         if (tid == kCopier && soon < p.rows && words > 0) {
@@ -778,6 +780,7 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
     using W = Word<T>;
     fb::dependency_wait();
     fb::dependency_release();
+    const uint4* logits = fb::after_wait(static_cast<const uint4*>(p.logits));
     const int row_words = p.cols / W::kValues;
     const int read_words = (p.vocab + W::kValues - 1) / W::kValues;
     const size_t groups = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
         const int first_word = kLong ? static_cast<int>(item - first_row * p.row_chunks) * p.chunk : 0;
         const int here = kLong ? min(p.chunk, row_words - first_word)
                                : static_cast<int>(min(static_cast<size_t>(p.chunk_rows), p.rows - first_row)) * row_words;
-        const uint4* in = static_cast<const uint4*>(p.logits) + first_row * row_words + first_word;
+        const uint4* in = logits + first_row * row_words + first_word;
         uint4* out = static_cast<uint4*>(p.dlogits) + first_row * row_words + first_word;
         uint4 held[kGradientWords];
 #pragma unroll
@@ -795,7 +798,7 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
             const int word = kLong ? first_word + i : i % row_words;
             held[j] = make_uint4(0u, 0u, 0u, 0u);
             if (i < here && word < read_words) {
-                held[j] = fb::load_input(in + i);
+                held[j] = in[i];       // (not load_input: dlogits may be logits)
             }
         }
         if constexpr (kLong) {

@@ -173,6 +173,8 @@ __global__ void __launch_bounds__(kListThreads) fb_packed_backward_prepare(const
         list_blocks(p);
         return;
     }
+    const uint4* d_o = reinterpret_cast<const uint4*>(after_wait(p.d_o));
+    const uint4* o = reinterpret_cast<const uint4*>(after_wait(static_cast<const __half*>(p.a.o)));
     const int lane = threadIdx.x % 32;
     const int warps = (gridDim.x - 1) * (kListThreads / 32);
     for (int row = (blockIdx.x - 1) * (kListThreads / 32) + threadIdx.x / 32; row < p.a.rows; row += warps) {
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kListThreads) fb_packed_backward_prepare(const
             continue;
         }
         const long long at = stats_at(q.first, low) + (row - q.first);
-        const long long o_row = static_cast<long long>(row) * p.a.o_stride;
+        const long long o_row = static_cast<long long>(row) * p.a.o_stride / 8;      // in words of eight values
         // Four heads at a time, and four times that on their way.
         for (int first_head = 0; first_head < p.a.heads; first_head += 16) {
             uint4 x[4], y[4];
@@ -199,8 +201,8 @@ __global__ void __launch_bounds__(kListThreads) fb_packed_backward_prepare(const
                 const int head = first_head + 4 * i + lane / 8;
                 x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (head < p.a.heads) {
-                    x[i] = load_input(reinterpret_cast<const uint4*>(p.d_o + o_row + head * kHead) + lane % 8);
-                    y[i] = load_input(reinterpret_cast<const uint4*>(p.a.o + o_row + head * kHead) + lane % 8);
+                    x[i] = load_input(d_o + o_row + head * (kHead / 8) + lane % 8);
+                    y[i] = load_input(o + o_row + head * (kHead / 8) + lane % 8);
                 }
             }
             const int stat_head = first_head + lane;
@@ -915,14 +917,15 @@ __global__ void __launch_bounds__(kThreads, 1) fb_packed_backward(const __grid_c
 __global__ void __launch_bounds__(256) fb_packed_backward_join(const BackwardParams p) {
     dependency_wait();
     dependency_release();
+    const float4* partial = reinterpret_cast<const float4*>(after_wait(static_cast<const float*>(p.partial)));
     const int first = max(p.a.starts[0], 0), end = min(p.a.starts[p.a.sequences], p.a.rows);
     const long long per_row = static_cast<long long>(p.a.kv_heads) * 16;     // 16-byte pieces of dK and dV
-    const long long slice = static_cast<long long>(p.a.rows) * p.a.kv_heads * 2 * kHead;
+    const long long slice = static_cast<long long>(p.a.rows) * p.a.kv_heads * 2 * kHead / 4;   // in words of four values
     for (long long i = first * per_row + blockIdx.x * 256ll + threadIdx.x; i < end * per_row; i += gridDim.x * 256ll) {
         float sum[8] = {};
         for (int s = 0; s < p.slices; ++s) {
             float v[8];
-            load8_input(v, reinterpret_cast<const float4*>(p.partial + s * slice + i * 8));
+            load8_input(v, partial + s * slice + i * 2);
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 sum[c] += v[c];

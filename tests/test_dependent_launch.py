@@ -131,3 +131,77 @@ def test_the_check_notices_an_expansion_right_before_its_gemm():
     norm = re.search(r"\n *FB_TRY\(layernorm\(g, l\.ln1_w[^\n]*", text).group(0)
     assert expansion + norm in text
     assert not steady_weights_have_a_kernel_between(text.replace(expansion + norm, norm + expansion))
+
+
+def pointer_members():
+    """Names of pointers in the structures that kernels get."""
+    names = set()
+    for path in (*SOURCES, *SOURCES[0].parent.glob("*.h"), *SOURCES[0].parent.glob("*.cuh")):
+        text = re.sub(r"//[^\n]*", "", path.read_text())
+        for body in re.findall(r"\bstruct \w+ \{(.*?)\n\};", text, re.S):
+            names |= set(re.findall(r"\*\s*(\w+);", body))
+    return names
+
+
+def arguments(body, function):
+    """What `function` is called with, in full."""
+    for call in re.finditer(rf"\b{function}\(", body):
+        depth, end = 1, call.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(body[end], 0)
+            end += 1
+        yield body[call.end():end - 1]
+
+
+def roots(body, expression, known=()):
+    """The expression and, again and again, what the names in it stand for in the kernel's body."""
+    found = [expression]
+    for name in set(re.findall(r"(?<![.\w])[a-z]\w*", expression)) - set(known):
+        known = (*known, name)
+        # (A lambda's value is what it returns; each of those here is one statement.)
+        for value in re.findall(rf"(?:\*|\bauto)\s*{name} = ([^;]*);", body):
+            found += roots(body, value, known)
+    return found
+
+
+def unwaited_inputs(body):
+    """Pointers that load_input reads as they came in the kernel's parameters."""
+    pointers = pointer_members()
+    bad = []
+    for function in ("load_input", "load8_input"):
+        for argument in arguments(body, function):
+            for text in roots(body, argument.split(", ")[-1]):
+                text = re.sub(r"after_wait\((?:[^()]|\([^()]*\))*\)", "", text)
+                bad += [m for m in re.findall(r"\bp\.(?:\w+\.)*(\w+)", text) if m in pointers]
+    return bad
+
+
+def test_what_load_input_reads_comes_from_behind_the_wait():
+    """To the compiler load_input is a function of its address alone: only an after_wait() pointer holds it behind the
+    wait. (Parameters that are pointers themselves: above.)"""
+    checked = set()
+    for parameter in waiting_kernels():
+        body = parameter.values[1]
+        assert not unwaited_inputs(body), parameter.id
+        if "load_input(" in body or "load8_input(" in body:
+            checked.add(parameter.id.split(":")[1])
+    assert {"fb_token_log_probs", "fb_packed_backward_prepare", "fb_packed_backward_join", "fb_embedding_forward"} <= checked
+
+
+def test_that_check_notices_a_pointer_of_the_parameters():
+    text = (SOURCES[0].parent / "packed_backward.cu").read_text()
+    assert "load_input(d_o + " in text
+    for plain in ("load_input(p.d_o + ", "load_input(reinterpret_cast<const uint4*>(p.d_o) + "):
+        bodies = {name: body for name, _, body in kernels(text.replace("load_input(d_o + ", plain))}
+        assert unwaited_inputs(bodies["fb_packed_backward_prepare"]) == ["d_o"]
+    text = (SOURCES[0].parent / "log_probs.cu").read_text()
+    lambda_of = "reinterpret_cast<const uint4*>(logits) + row * row_words"
+    assert lambda_of in text
+    bodies = {name: body for name, _, body in kernels(text.replace(lambda_of, lambda_of.replace("(logits)", "(p.logits)")))}
+    assert "logits" in unwaited_inputs(bodies["fb_token_log_probs"])
+
+
+def test_the_gradient_that_may_take_its_logits_place_does_not_use_load_input():
+    """load_input may pass the kernel's own stores."""
+    bodies = {name: body for name, _, body in kernels((SOURCES[0].parent / "log_probs.cu").read_text())}
+    assert "load_input" not in bodies["fb_token_log_probs_backward"]
