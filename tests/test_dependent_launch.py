@@ -185,7 +185,7 @@ def test_what_load_input_reads_comes_from_behind_the_wait():
         assert not unwaited_inputs(body), parameter.id
         if "load_input(" in body or "load8_input(" in body:
             checked.add(parameter.id.split(":")[1])
-    assert {"fb_token_log_probs", "fb_packed_backward_prepare", "fb_packed_backward_join", "fb_embedding_forward"} <= checked
+    assert {"fb_packed_backward_prepare", "fb_packed_backward_join", "fb_embedding_forward"} <= checked
 
 
 def test_that_check_notices_a_pointer_of_the_parameters():
@@ -194,11 +194,13 @@ def test_that_check_notices_a_pointer_of_the_parameters():
     for plain in ("load_input(p.d_o + ", "load_input(reinterpret_cast<const uint4*>(p.d_o) + "):
         bodies = {name: body for name, _, body in kernels(text.replace("load_input(d_o + ", plain))}
         assert unwaited_inputs(bodies["fb_packed_backward_prepare"]) == ["d_o"]
-    text = (SOURCES[0].parent / "log_probs.cu").read_text()
-    lambda_of = "reinterpret_cast<const uint4*>(logits) + row * row_words"
+    # Through a lambda and a pointer as well.
+    lambda_of = "auto words_of = [&](int head) { return reinterpret_cast<const uint4*>(p.d_o) + o_row + head * (kHead / 8); };"
+    text = text.replace("load_input(d_o + o_row + head * (kHead / 8) + lane % 8);",
+                        lambda_of + " const uint4* at = words_of(head); load_input(at + lane % 8);")
     assert lambda_of in text
-    bodies = {name: body for name, _, body in kernels(text.replace(lambda_of, lambda_of.replace("(logits)", "(p.logits)")))}
-    assert "logits" in unwaited_inputs(bodies["fb_token_log_probs"])
+    bodies = {name: body for name, _, body in kernels(text)}
+    assert unwaited_inputs(bodies["fb_packed_backward_prepare"]) == ["d_o"]
 
 
 def test_the_gradient_that_may_take_its_logits_place_does_not_use_load_input():
