@@ -266,6 +266,32 @@ constexpr int blocks_per_sm(int threads, int held) { return (threads == 128 ? 4 
 
 constexpr int kChunks = 2;      // pieces in which a slice is copied into shared memory
 
+// What a block keeps of two rows in turn, besides staged words.
+template <int kWarps, int kBins>
+struct RowMemory {
+    union Lists {
+        float bins[kBins];               // read before the first candidate of the row is written, and
+        Key candidates[kCandidates];     // written when all are done with those of two rows before
+    } lists[2];
+    Key best[2][kMostRanks * kMostTop];
+    Key reduced[kWarps];
+    unsigned long long barriers[kChunks];
+    float maxima[2][kWarps];
+    float sums[2][2 * kWarps];
+    float parts[2][kMostRanks][3];     // the first CTA's: every CTA's m, S, D
+    float least[2];
+    int counts[2];
+    int abort_flag;
+};
+
+constexpr int kStagedThreads = 512;    // 256 are 6 % faster without alternatives, 5 % slower with five of them
+constexpr int kStagedBins = 64;
+// Words of a slice in shared memory: two CTAs per SM. An SM has 228 KB, of which a CTA costs 1 KB more than it asks for.
+// (One CTA where 6,400 words did not fit twice: 8,192 rows of 51,200 FP16 logits with five alternatives 267 us, 197 with two.)
+constexpr int kStagedWords = 6400;
+static_assert(2 * (kStagedWords * 16 + (sizeof(RowMemory<kStagedThreads / 32, kStagedBins>) + 127) / 128 * 128 + 1024) <= 228 * 1024,
+              "two CTAs fit on an SM");
+
 // kHeld > 0: a thread holds that many words of the row in registers, and asks for the next row's while it takes
 // the exponentials. kHeld == 0: the slice is copied into shared memory, and the CTA beside it on the SM computes
 // meanwhile.
@@ -274,20 +300,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
     using W = Word<T>;
     constexpr bool kStaged = kHeld == 0;
     constexpr int kWarps = kThreads / 32;
-    constexpr int kBins = kThreads >= 512 ? 64 : 32;     // parts whose maxima bound the alternatives (up to 32) from below
+    constexpr int kBins = kThreads >= 512 ? kStagedBins : 32;     // parts whose maxima bound the alternatives (up to 32) from below
     constexpr int kLanes = kThreads / kBins;      // of a bin
     extern __shared__ __align__(128) uint4 staged[];
-    __shared__ float bins[2][kBins];
-    __shared__ float least[2];
-    __shared__ float maxima[2][kWarps];
-    __shared__ float sums[2][2 * kWarps];
-    __shared__ Key reduced[kWarps];
-    __shared__ int counts[2];
-    __shared__ Key candidates[2][kCandidates];
-    __shared__ float parts[2][kMostRanks][3];     // the first CTA's: every CTA's m, S, D
-    __shared__ Key best[2][kMostRanks * kMostTop];
-    __shared__ alignas(8) unsigned long long barriers[kChunks];
-    __shared__ int abort_flag;
+    __shared__ RowMemory<kWarps, kBins> shared;
+    auto& least = shared.least;
+    auto& maxima = shared.maxima;
+    auto& sums = shared.sums;
+    auto& reduced = shared.reduced;
+    auto& counts = shared.counts;
+    auto& parts = shared.parts;
+    auto& best = shared.best;
+    auto& barriers = shared.barriers;
+    int& abort_flag = shared.abort_flag;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
     const int rank = p.ranks > 1 ? static_cast<int>(sm100::cluster_cta_rank()) : 0;
     const size_t stride = gridDim.x / p.ranks;
@@ -413,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
             mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
         }
         if (tid % kLanes == 0) {
-            bins[parity][tid / kLanes] = mx;
+            shared.lists[parity].bins[tid / kLanes] = mx;
         }
 #pragma unroll
         for (int off = kLanes; off < 32; off <<= 1) {
@@ -440,11 +465,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         float bound = INFINITY;
         if (top > 0) {
             // A warp ranks its share of the bins, each against all of them, one or two per lane.
-            const float low = bins[parity][lane], high = kBins > 32 ? bins[parity][lane + kBins - 32] : 0.0f;
+            const float low = shared.lists[parity].bins[lane], high = kBins > 32 ? shared.lists[parity].bins[lane + kBins - 32] : 0.0f;
 #pragma unroll 4
             for (int i = 0; i < kBins / kWarps; ++i) {
                 const int bin = warp * (kBins / kWarps) + i;
-                const float value = bins[parity][bin];
+                const float value = shared.lists[parity].bins[bin];
                 int larger = __popc(__ballot_sync(fb::kFullMask, low > value || (low == value && lane < bin)));
                 if (kBins > 32) {
                     larger += __popc(__ballot_sync(fb::kFullMask, high > value || (high == value && lane + 32 < bin)));
@@ -465,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
                 if (v[c] >= bound && v[c] > -INFINITY) {
                     const int at = atomicAdd(&counts[parity], 1);
                     if (at < kCandidates) {
-                        candidates[parity][at] = order_key(v[c], (first_word + i) * W::kValues + c);
+                        shared.lists[parity].candidates[at] = order_key(v[c], (first_word + i) * W::kValues + c);
                     }
                 }
             }
@@ -578,11 +603,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kThreads, kHeld)) fb_t
         if (top > 0 && goes_on) {
             if (collected) {
                 for (int c = tid; c < found; c += kThreads) {
-                    const Key key = candidates[parity][c];
+                    const Key key = shared.lists[parity].candidates[c];
                     int larger = 0;
 #pragma unroll 8
                     for (int other = 0; other < found; ++other) {
-                        larger += candidates[parity][other] > key ? 1 : 0;
+                        larger += shared.lists[parity].candidates[other] > key ? 1 : 0;
                     }
                     if (larger < top) {
                         place_key(larger, key);
@@ -821,9 +846,6 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
         }
     }
 }
-
-constexpr int kStagedWords = 6400;     // 100 KB: two CTAs per SM
-constexpr int kStagedThreads = 512;    // 256 are 6 % faster without alternatives, 5 % slower with five of them
 
 template <typename T, int kThreads, int kHeld>
 cudaError_t launch_form(LogProbArgs p, int ranks, int sms, cudaStream_t stream) {

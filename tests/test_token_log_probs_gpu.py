@@ -292,3 +292,14 @@ def test_gradient_of_rows_near_the_types_lowest_value(flint, vocab, rows, terms)
     away = none & (at_target == 0)
     assert (got[:, :vocab][away] == 0).all() and (got[:, vocab:] == 0).all()
     assert torch.equal(got, same)
+
+
+@pytest.mark.parametrize("rows, vocab, fp32, top", [(400, 51200, False, 5), (310, 51073, False, 0), (300, 51200, True, 32),
+                                                    (320, 25600, True, 5), (3, 51200, False, 20)])
+def test_rows_at_the_limit_of_two_blocks_on_an_sm(flint, rows, vocab, fp32, top):
+    """Slices of 6,385 to 6,400 words of shared memory, several rows to a block."""
+    cols = (vocab + 7) // 8 * 8
+    logits, targets = make(rows, vocab, cols, fp32)
+    got = forward(flint, logits, targets, vocab, top)
+    torch.cuda.synchronize()
+    check(got, exact(logits, targets, vocab, top), 30)
