@@ -767,12 +767,9 @@ struct RowGradient {
         const float rest = -fmaf(b, entropy, a);
         constant = fb::f2_pack(rest, rest);
     }
-    __device__ __forceinline__ uint4 word(uint4 q, int column, int vocab) const {
+    __device__ __forceinline__ uint4 word(const uint4& q, int column, int vocab) const {
         using W = Word<T>;
         float v[W::kValues], out[W::kValues];
-        if (low) {
-            raise_word(q, T());
-        }
         W::unpack_finite(v, q);
 #pragma unroll
         for (int c = 0; c < W::kValues; c += 2) {
@@ -827,6 +824,12 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
         }
         if constexpr (kLong) {
             const RowGradient<T> row(p, first_row);
+            if (row.low) {
+#pragma unroll
+                for (int j = 0; j < kGradientWords; ++j) {
+                    raise_word(held[j], T());
+                }
+            }
 #pragma unroll
             for (int j = 0; j < kGradientWords; ++j) {
                 const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
@@ -840,7 +843,11 @@ __global__ void __launch_bounds__(kGradientThreads) fb_token_log_probs_backward(
                 const int i = static_cast<int>(threadIdx.x) + j * kGradientThreads;
                 if (i < here) {
                     const int r = i / row_words;
-                    __stcs(out + i, RowGradient<T>(p, first_row + r).word(held[j], (i - r * row_words) * W::kValues, p.vocab));
+                    const RowGradient<T> row(p, first_row + r);
+                    if (row.low) {
+                        raise_word(held[j], T());
+                    }
+                    __stcs(out + i, row.word(held[j], (i - r * row_words) * W::kValues, p.vocab));
                 }
             }
         }
