@@ -398,3 +398,69 @@ def test_a_query_that_is_not_finite_reaches_the_gradients_of_all_its_keys(flint,
         beyond = (query // 128 + 1) * 128
         assert not dv[beyond:300].isnan().any() and not dk[beyond:300].isnan().any()
         assert not dq[:, 64:].isnan().any() and not o[:, 64:].isnan().any()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** 11])
+def test_small_and_large_output_gradients(flint, size):
+    batch = Batch([300, 1, 40, 700], 8, 2)
+    batch.d_o = (batch.d_o.float() * size).half()
+    o, lse = batch.forward(flint)
+    grads = batch.backward(flint, o, lse)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    batch.check(o, lse, grads)
+
+
+def test_two_training_calls_at_once_against_64_bits(flint):
+    batches = [Batch([700, 33, 1500], 8, 2, seed=1), Batch([2000, 1, 90, 400], 6, 6, seed=2)]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    for _ in range(2):
+        outputs = []
+        for batch, stream in zip(batches, streams):
+            with torch.cuda.stream(stream):
+                o, lse = batch.forward(flint)
+                outputs.append((o, lse, batch.backward(flint, o, lse)))
+        torch.cuda.synchronize()
+        assert not flint.kernel_fault()
+        for batch, results in zip(batches, outputs):
+            batch.check(*results)
+
+
+def test_as_many_sequences_as_there_can_be(flint):
+    """65,535 sequences of one token or none, a few of them longer."""
+    lengths = [i % 2 for i in range(65535)]
+    lengths[7], lengths[30000], lengths[65534] = 300, 129, 5
+    heads, kv_heads = 4, 2
+    batch = Batch([1], heads, kv_heads)
+    rows = sum(lengths)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    batch.qkv = torch.randn(rows, batch.width, generator=g, device=DEV).half()
+    batch.d_o = torch.randn(rows, heads * 64, generator=g, device=DEV).half()
+    ends = torch.tensor(lengths).cumsum(0)
+    batch.starts = torch.cat([torch.zeros(1, dtype=torch.int64), ends]).to(torch.int32).to(DEV)
+    batch.rows = rows
+    batch.shape = PackedShape(65535, rows, heads, kv_heads, 64, batch.width, batch.width, heads * 64)
+    o, lse = batch.forward(flint)
+    grads = batch.backward(flint, o, lse)
+    torch.cuda.synchronize()
+    assert not flint.kernel_fault()
+    q, k, v = batch.parts(batch.qkv)
+    # One token: p is 1, so o is v and dv the group's sum of d_o; its score has no gradient.
+    single = torch.tensor([n == 1 for n in lengths])
+    at = (ends - 1)[single].to(DEV)
+    spread = lambda t: t.view(rows, kv_heads, 1, 64).expand(-1, -1, 2, -1).reshape(rows, -1)
+    assert torch.equal(o[at], spread(v)[at])
+    scores = (q.double() * spread(k).double()).view(rows, heads, 64).sum(2).T * SCALE
+    assert ((lse.double() - scores)[:, at]).abs().max() <= ragged.LSE_BOUND
+    dq, dk, dv = batch.parts(grads)
+    summed = batch.d_o.double().view(rows, kv_heads, 2, 64).sum(2).reshape(rows, -1)
+    assert ((dv.double() - summed)[at].abs() <= ragged.HALF * summed[at].abs() + 2 * (ragged.HALF + ragged.SCORE) *
+            batch.d_o.double().view(rows, kv_heads, 2, 64).abs().sum(2).reshape(rows, -1)[at] + ragged.TINY).all()
+    # The longer ones in full.
+    for s in (7, 30000, 65534):
+        batch.first = [int(ends[s]) - lengths[s], int(ends[s])]
+        whole = slice(*batch.first)
+        small = Batch([lengths[s]], heads, kv_heads, behind=0)
+        small.qkv, small.d_o = batch.qkv[whole], batch.d_o[whole]
+        small.check(o[whole], lse[:, whole], grads[whole])

@@ -303,3 +303,23 @@ def test_rows_at_the_limit_of_two_blocks_on_an_sm(flint, rows, vocab, fp32, top)
     got = forward(flint, logits, targets, vocab, top)
     torch.cuda.synchronize()
     check(got, exact(logits, targets, vocab, top), 30)
+
+
+@pytest.mark.parametrize("vocab, rows", [(1, 4), (3, 4), (100, 8), (9001, 4), (50257, 4), (50257, 200)])
+def test_fp32_rows_of_the_types_lowest_value(flint, vocab, rows):
+    """All of a row masked with the lowest finite value, some of it with minus infinity, and all but one word."""
+    lowest = torch.finfo(torch.float32).min
+    logits, targets = make(rows, vocab, (vocab + 7) // 8 * 8, True)
+    logits[:, :vocab] = lowest
+    logits[1::4, 1:vocab:2] = -float("inf")
+    logits[2::4, vocab // 2] = 0.0
+    logits[3::4, :vocab // 2] = -float("inf")
+    got = forward(flint, logits, targets, vocab, min(vocab, 5))
+    torch.cuda.synchronize()
+    want = exact(logits, targets, vocab, min(vocab, 5))
+    for mine, right in zip(got[:4], want[:4]):
+        assert torch.equal(mine.isneginf(), right.float().isneginf()) and not mine.isnan().any()
+        off = torch.where(right.float().isneginf(), 0.0, (mine.double() - right).abs())
+        # (One rounding of values up to 2^128, or SUM of logarithms.)
+        assert (off <= SUM + torch.where(right.isinf(), 0.0, right.abs()) * 2.0 ** -24).all()
+    assert torch.equal(got[4].to(torch.int64), want[4])
