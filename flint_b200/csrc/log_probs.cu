@@ -256,12 +256,12 @@ __device__ __forceinline__ float key_value(Key key) {
 // first puts them together.
 // The alternatives: the slice falls into 64 (or 32) bins of neighbouring lanes. The k-th largest of the bins' maxima
 // is a lower bound of the k-th largest logit; what is not below it (about k values) is collected in the
-// second pass and put in order by counting. Where too many qualify (rows of equal logits), or a NaN is among
-// them, the row is gone through once per alternative.
-// Measured on rows of GPT-2's 50,257 words: 8,192 FP16 rows with five alternatives 208 us (4.0 TB/s), 4,096 without 92 us;
-// 1,000 FP32 rows, a pair of CTAs each, 56 us; one FP32 row on eight CTAs with twenty alternatives 7.9 us with its
+// second pass and put in order by counting. Where too many qualify (rows of equal logits, or fewer bins with words in them
+// than there are alternatives), or a NaN is among them, the row is gone through once per alternative.
+// Measured on rows of GPT-2's 50,257 words: 8,192 FP16 rows with five alternatives 206 us (4.0 TB/s), 4,096 without 88 us;
+// 1,000 FP32 rows, a pair of CTAs each, 56 us; one FP32 row on eight CTAs with twenty alternatives 7.6 us with its
 // launch. Bound by issue slots (40 instructions per eight logits for the sums) and what a row costs besides. (Rows held in
-// registers, one CTA per SM: 355 us where shared memory takes 208.)
+// registers, one CTA per SM: 355 us where shared memory takes 206.)
 constexpr int blocks_per_sm(int threads, int held) { return (threads == 128 ? 4 : 1) * (held > 4 ? 1 : 2); }
 
 constexpr int kChunks = 2;      // pieces in which a slice is copied into shared memory

@@ -17,7 +17,7 @@
 // and the products 512; a quarter of them runs on the FMA pipe instead (half of them: 10 % slower, none: 9 %). A key tile
 // takes 1,350 clocks of an SM; short sequences are bound by what a tile's beginning and end cost, about two key tiles.
 // Measured, with the join: 5 sequences of up to 4,096 tokens, 16 query heads on 4, 73 us (570 TFLOP/s); 24 of up to 700,
-// 12 heads, 27 us; 64 single tokens on caches of up to 8,192, 32 heads on 8, 77 us (5.1 TB/s).
+// 12 heads, 28.7 us; 64 single tokens on caches of up to 8,192, 32 heads on 8, 77 us (5.1 TB/s).
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -752,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     break;
                 }
                 sm100::tc_fence_after_sync();
-                // One copy of 64 columns is read twice, 32 at a time (two threads' registers do not hold
-                // them beside everything else: 500 bytes spilled); up to 32 once.
+                // One copy of 64 columns is read twice, 32 at a time (64 bytes spilled; all at once, 500: two threads'
+                // registers do not hold them beside everything else); up to 32 once.
                 uint32_t raw[kChunk];
                 auto read = [&](int c) {
                     if constexpr (kChunk == 32) {

@@ -155,7 +155,6 @@ struct Piece {
     int tokens;         // in the tile
     int from, to, tiles;
     FB_SCHEDULE int position() const { return sequence.before() + first_token; }   // of the first token
-    FB_SCHEDULE bool whole() const { return from == 0 && to == tiles; }
 };
 
 // The pieces between two cuts, in order; get(s) is sequence s. Every role of a CTA walks on its own.

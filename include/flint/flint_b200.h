@@ -15,7 +15,7 @@
 extern "C" {
 #endif
 
-/* 1 if a kernel (GEMM, attention, column sums, cross-entropy) gave up on a
+/* 1 if a kernel (GEMM, attention, column sums, cross-entropy, log-probabilities) gave up on a
  * bounded barrier wait since the last call, or one that reads starts, lengths or page numbers
  * met one out of range (the flag is cleared), 0 otherwise.
  * Synchronises the device; meant for tests. */
@@ -267,7 +267,10 @@ FLINT_API flint_status flint_b200_packed_attention_backward_workspace(
  * query heads that share a head, taken in one fixed order: results repeat bit for bit. A row that is NaN makes its
  * dq NaN, and dk and dv of the keys that it sees. Within a sequence a value that is not finite may also reach rows
  * of its block of 128 that have no part in it: dq of up to 127 rows before one of k, and dk and dv of up
- * to 127 rows behind one of q or d_o. */
+ * to 127 rows behind one of q or d_o.
+ * The scores' gradients p (d_o . v - d_o . o) are rounded to FP16 before they meet scale: beyond 65,504 they are
+ * infinite, and so are dq and dk, and below 2^-25 they are lost. d_o of up to some thousands for inputs of size
+ * one stays clear of the first. */
 FLINT_API flint_status flint_b200_packed_attention_backward(
     void* dq, void* dk, void* dv, const void* d_o, const void* o, const void* lse, const void* q,
     const void* k, const void* v, const void* starts, const flint_b200_packed_shape* shape,
@@ -340,8 +343,10 @@ FLINT_API flint_status flint_b200_token_log_probs(void* log_probs, void* entropy
  * the above's outputs, from its lse and entropy:
  *   dlogits_c = d_log_probs ([c == target] - p_c) - d_entropy p_c (log p_c + entropy)
  * in the logits' type, +0 in columns from vocab on; targets not below vocab count as
- * d_log_probs = 0. A column of minus infinity gets 0, and so does a row of nothing else. dlogits may be
- * logits itself. */
+ * d_log_probs = 0. A column of minus infinity gets 0 (but for its own d_log_probs as a target), and so does a row of
+ * nothing else. dlogits may be logits itself. lse has no gradient. p is exp(x - lse) with lse in FP32, off by up to
+ * |lse| 2^-24 of itself: 2^-9 for FP16 rows near -65,504; FP32 rows that lie farther from 0 as a whole are better shifted
+ * first, which changes no output but lse. */
 FLINT_API flint_status flint_b200_token_log_probs_backward(
     void* dlogits, const void* logits, const void* targets, const void* lse, const void* entropy,
     const void* d_log_probs, const void* d_entropy, int fp32_logits, size_t rows, size_t vocab,
