@@ -241,3 +241,80 @@ def test_lanes_of_a_warp_do_not_decide_for_themselves(source, least):
         alone = any(re.search(r"\blane == 0\b", header) for header in headers)
         agreed = re.search(r"\b(there|ok) = .*(&& (there|ok))?$", statement) and "if (" not in statement
         assert alone or agreed, statement
+
+
+class Copies:
+    """The end of a piece in the few-rows forms: eight warps put their rows' copies together through shared memory, with
+    a barrier of eight that they meet at nine times. Nothing else is taken to hold them together between pieces."""
+
+    def __init__(self, subsets, pieces, seed, missing=None):
+        self.apart, self.subsets, self.pieces, self.missing = 4 // subsets, subsets, pieces, missing
+        self.rng = random.Random(seed)
+        self.bar = Barrier("meeting", WARPS)
+        self.merge, self.staging = [None] * WARPS, [None] * WARPS
+
+    def warp(self, half, quadrant):
+        met = 0
+
+        def meet(which):
+            nonlocal met
+            if which == self.missing:
+                return
+            self.bar.arrive()
+            while not self.bar.passed(met & 1):
+                yield
+            need(self.bar.completed > met, "aliased wait")
+            met += 1
+
+        others = [quadrant % self.apart + s * self.apart for s in range(self.subsets)]
+        for r in range(self.pieces):
+            self.merge[half * 4 + quadrant] = r
+            yield
+            yield from meet("maxima and sums")
+            for other in others:
+                need(self.merge[other] == r and self.merge[4 + other] == r, "maxima and sums of another piece")
+                yield
+            for part in range(4):
+                self.staging[half * 4 + quadrant] = (r, part)
+                yield
+                yield from meet("columns written")
+                for other in others:
+                    need(self.staging[half * 4 + other] == (r, part), "columns of another copy or round")
+                    yield
+                yield from meet("columns read")
+
+    def run(self):
+        roles = [self.warp(h, q) for h in range(2) for q in range(4)]
+        steps = 0
+        while roles:
+            role = self.rng.choice(roles)
+            try:
+                next(role)
+            except StopIteration:
+                roles.remove(role)
+            steps += 1
+            need(steps < 200000, "deadlock")
+
+
+@pytest.mark.parametrize("subsets", [2, 4])
+def test_copies_of_few_rows_are_put_together(subsets):
+    for seed in range(40):
+        Copies(subsets, 4, seed).run()
+    for missing in ("maxima and sums", "columns written", "columns read"):
+        found = 0
+        for seed in range(40):
+            try:
+                Copies(subsets, 4, seed, missing).run()
+            except Violation:
+                found += 1
+        assert found > 0, missing
+
+
+def test_the_copies_meet_where_the_model_does():
+    text = (test_warp_waits.CSRC / "packed_forward.cu").read_text()
+    merge = text[text.index("// The copies of a row:"):text.index("// This thread's columns of O:")]
+    ahead = text[:text.index("// The copies of a row:")]
+    assert ahead.rindex("meeting.meet()") > ahead.rindex("merge_max[quadrant][lane] = m;")
+    assert merge.count("meeting.meet()") == 2
+    assert merge.index("st.shared.v2.f32") < merge.index("meeting.meet()") < merge.index("ld.shared.v2.f32") < \
+        merge.rindex("meeting.meet()")
