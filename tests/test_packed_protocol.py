@@ -312,9 +312,7 @@ def test_copies_of_few_rows_are_put_together(subsets):
 
 def test_the_copies_meet_where_the_model_does():
     text = (test_warp_waits.CSRC / "packed_forward.cu").read_text()
-    merge = text[text.index("// The copies of a row:"):text.index("// This thread's columns of O:")]
-    ahead = text[:text.index("// The copies of a row:")]
-    assert ahead.rindex("meeting.meet()") > ahead.rindex("merge_max[quadrant][lane] = m;")
-    assert merge.count("meeting.meet()") == 2
-    assert merge.index("st.shared.v2.f32") < merge.index("meeting.meet()") < merge.index("ld.shared.v2.f32") < \
-        merge.rindex("meeting.meet()")
+    merge = text[text.index("merge_max[quadrant][lane] = m;"):text.index("// This thread's columns of O:")]
+    steps = re.findall(r"meeting\.meet\(\)|top = max3_nan\(top, merge_max|merge_sum\[other\]|r < 4|st\.shared\.v2|ld\.shared\.v2", merge)
+    assert steps == ["meeting.meet()", "top = max3_nan(top, merge_max", "merge_sum[other]", "r < 4", "st.shared.v2",
+                     "meeting.meet()", "ld.shared.v2", "meeting.meet()"]
