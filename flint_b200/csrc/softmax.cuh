@@ -43,7 +43,8 @@ constexpr float kNoKey = -3.402823466e38f;
 // 127 - 1; anything below -120 counts as -120 (2^-120 is zero in FP16).
 // kKeepNan: a NaN stays one, where else it counts as -120 too. 2 2^f is then multiplied by 2^(n - 1), whose exponent field,
 // n + 126, is what the low bits of x + 1.5 * 2^23 + 126 hold: the same bits otherwise. (The forward kernels have no
-// need of it, as the maximum of a row with a NaN is NaN and so are the row's other exponentials: 43.5 us without, 44.1 with it.)
+// need of it, as the maximum of a row with a NaN is NaN and so are the row's other exponentials: 150 heads of 1,024 tokens take
+// 43.5 us without, 44.1 with it. Backward, 24 heads: 26.05 and 26.1.)
 template <bool kKeepNan>
 __device__ __forceinline__ void exp2_pair_fma(F2 x, float& lo, float& hi) {
     auto both = [](float c) { return f2_pack(c, c); };
