@@ -468,7 +468,7 @@ def _own_fork(s):
                      s["references"], s["parents"], pool)
     flint.pages_reserve(s["next_table"], s["next_lengths"], s["next_references"], s["moves"], s["counts"], s["added"],
                         pool, workspace)
-    flint.pages_copy(arrays, s["moves"], s["moves"].shape[0])
+    flint.pages_copy(arrays, s["moves"], s["counts"], s["moves"].shape[0])
     return (s["next_table"], s["next_lengths"], s["next_references"], s["moves"], s["counts"], *s["caches"])
 
 
@@ -481,7 +481,7 @@ def _own_compact(s):
     workspace = _workspace(s, lambda: flint.pages_workspace(pool))
     flint.pages_compact(s["next_table"], s["next_references"], s["moves"], s["counts"], s["table"], s["lengths"],
                         s["references"], pool, workspace)
-    flint.pages_copy(arrays, s["moves"], s["moves"].shape[0])
+    flint.pages_copy(arrays, s["moves"], s["counts"], s["moves"].shape[0])
     return (s["next_table"], s["next_references"], s["moves"], s["counts"], *s["caches"])
 
 
