@@ -15,6 +15,8 @@ from .binding import (  # noqa: F401
     Gpt2Config,
     Gpt2ParameterInfo,
     PackedShape,
+    PageArrays,
     PagedShape,
+    PagePool,
     library_path,
 )

@@ -85,6 +85,29 @@ class PagedShape(ctypes.Structure):
                 *((name, ctypes.c_size_t) for name in ("pages", "page_size", "table_stride", "longest"))]
 
 
+class PagePool(ctypes.Structure):
+    """flint_b200_page_pool."""
+
+    _fields_ = [(name, ctypes.c_size_t) for name in ("sequences", "table_stride", "pages", "page_size")]
+
+
+class PageArrays:
+    """The arrays [pages, ...] of a cache (keys, values and scales of every layer) as pages_copy takes them; made
+    once and kept."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.count = len(self.tensors)
+        self.pages = self.tensors[0].shape[0] if self.tensors else 0
+        for tensor in self.tensors:
+            if tensor.shape[0] != self.pages or not tensor.is_contiguous():
+                raise ValueError(f"an array of pages of shape {tuple(tensor.shape)}: expected {self.pages} pages, "
+                                 "one behind the other")
+        self.addresses = (ctypes.c_void_p * self.count)(*[tensor.data_ptr() for tensor in self.tensors])
+        self.page_bytes = (ctypes.c_size_t * self.count)(*[_nbytes(tensor) // max(1, self.pages)
+                                                           for tensor in self.tensors])
+
+
 class TrainerConfigC(ctypes.Structure):
     """flint_trainer_config."""
 
@@ -169,6 +192,9 @@ _C_TYPES = {
     "flint_trainer**": ctypes.POINTER(ctypes.c_void_p),
     "const flint_b200_packed_shape*": ctypes.POINTER(PackedShape),
     "const flint_b200_paged_shape*": ctypes.POINTER(PagedShape),
+    "const flint_b200_page_pool*": ctypes.POINTER(PagePool),
+    "void* const*": ctypes.POINTER(ctypes.c_void_p),
+    "const size_t*": ctypes.POINTER(ctypes.c_size_t),
     "const flint_trainer_config*": ctypes.POINTER(TrainerConfigC),
     "flint_trainer_status*": ctypes.POINTER(TrainerStatus),
     "const flint_trainer_status*": ctypes.POINTER(TrainerStatus),
@@ -543,6 +569,69 @@ class Flint:
             workspace_bytes = _nbytes(workspace)
         self.call("flint_b200_paged_attention", o, lse, q, k_pages, v_pages, starts, lengths, page_table, shape,
                   scale, workspace, workspace_bytes, stream=stream)
+
+    def paged8_store(self, k_pages, v_pages, k_scales, v_scales, k, v, starts, lengths, page_table, shape,
+                     stream=None) -> None:
+        """paged_store into pages of 8 bits with a scale for 16 positions of a head."""
+        self.call("flint_b200_paged8_store", k_pages, v_pages, k_scales, v_scales, k, v, starts, lengths, page_table,
+                  shape, stream=stream)
+
+    def paged8_attention_workspace(self, shape) -> int:
+        return self._size_query("flint_b200_paged8_attention_workspace", shape)
+
+    def paged8_attention(self, o, lse, q, k_pages, v_pages, k_scales, v_scales, starts, lengths, page_table, shape,
+                         scale, workspace=None, workspace_bytes=None, stream=None) -> None:
+        """paged_attention over pages of 8 bits."""
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_paged8_attention", o, lse, q, k_pages, v_pages, k_scales, v_scales, starts, lengths,
+                  page_table, shape, scale, workspace, workspace_bytes, stream=stream)
+
+    def pages_workspace(self, pool) -> int:
+        return self._size_query("flint_b200_pages_workspace", pool)
+
+    def pages_fork(self, next_table, next_lengths, next_references, page_table, lengths, references, parents, pool,
+                   stream=None) -> None:
+        """Every sequence goes on as its parent stands, sharing its pages; pool is a PagePool."""
+        self.call("flint_b200_pages_fork", next_table, next_lengths, next_references, page_table, lengths, references,
+                  parents, pool, stream=stream)
+
+    def pages_reserve(self, page_table, lengths, references, moves, counts, added, pool, workspace=None,
+                      workspace_bytes=None, stream=None) -> None:
+        """Pages for `added` more tokens of every sequence; copies of shared pages are listed in moves."""
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_pages_reserve", page_table, lengths, references, moves, counts, added, pool, workspace,
+                  workspace_bytes, stream=stream)
+
+    def pages_truncate(self, page_table, lengths, references, keep, pool, stream=None) -> None:
+        self.call("flint_b200_pages_truncate", page_table, lengths, references, keep, pool, stream=stream)
+
+    def pages_compact(self, next_table, next_references, moves, counts, page_table, lengths, references, pool,
+                      workspace=None, workspace_bytes=None, stream=None) -> None:
+        """Pages in use become the first ones; what is to be moved is listed in moves."""
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_pages_compact", next_table, next_references, moves, counts, page_table, lengths,
+                  references, pool, workspace, workspace_bytes, stream=stream)
+
+    def pages_copy(self, arrays, moves, counts, most_moves, stream=None) -> None:
+        """The copies that pages_reserve or pages_compact listed, in every array of a PageArrays."""
+        self.call("flint_b200_pages_copy", arrays.addresses, arrays.page_bytes, arrays.count, arrays.pages, moves,
+                  counts, most_moves, stream=stream)
+
+    def beam_select_workspace(self, groups, beams) -> int:
+        return self._size_query("flint_b200_beam_select_workspace", groups, beams)
+
+    def beam_select(self, next_scores, parents, tokens, next_finished, next_lengths, next_histories, logits, scores,
+                    finished, lengths, histories, fp32_logits, groups, beams, vocab, cols, history_stride=0,
+                    end_token=-1, length_power=0.0, workspace=None, workspace_bytes=None, stream=None) -> None:
+        """The best continuations of each group of beams, with their histories."""
+        if workspace_bytes is None:
+            workspace_bytes = _nbytes(workspace)
+        self.call("flint_b200_beam_select", next_scores, parents, tokens, next_finished, next_lengths,
+                  next_histories, logits, scores, finished, lengths, histories, bool(fp32_logits), groups, beams,
+                  vocab, cols, history_stride, end_token, length_power, workspace, workspace_bytes, stream=stream)
 
     def token_log_probs(self, log_probs, entropy, lse, top_log_probs, top_tokens, logits, targets, fp32_logits,
                         rows, vocab, cols, top=0, stream=None) -> None:

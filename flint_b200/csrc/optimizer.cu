@@ -19,6 +19,7 @@
 #include "flint/flint_b200.h"
 #include "attention.h"
 #include "packed.h"
+#include "pages.h"
 #include "gemm.h"
 
 namespace {
@@ -446,7 +447,11 @@ flint_status flint_b200_kernel_fault(int* raised) {
     FB_CUDA(fb::packed_error_flag(&packed, true));
     int log_probs = 0;
     FB_CUDA(fb::log_probs_error_flag(&log_probs, true));
-    const int all[] = {gemm, attention, reductions, rowwise, packed, log_probs};
+    int pages = 0;
+    FB_CUDA(fb::pages_error_flag(&pages, true));
+    int beams = 0;
+    FB_CUDA(fb::beams_error_flag(&beams, true));
+    const int all[] = {gemm, attention, reductions, rowwise, packed, log_probs, pages, beams};
     *raised = std::any_of(std::begin(all), std::end(all), [](int flag) { return flag != 0; }) ? 1 : 0;
     return FLINT_OK;
 }

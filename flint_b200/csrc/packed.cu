@@ -117,11 +117,12 @@ cudaError_t encode_pages(CUtensorMap* map, const __half* base, long long rows, i
 }
 
 cudaError_t packed_error_flag(int* value, bool reset) {
-    int here = 0, forward = 0, backward = 0;
+    int here = 0, forward = 0, backward = 0, eight = 0;
     cudaError_t e = read_error_word(&here, reset);
     if (e == cudaSuccess) e = packed_forward_error_flag(&forward, reset);
     if (e == cudaSuccess) e = packed_backward_error_flag(&backward, reset);
-    *value = here != 0 || forward != 0 || backward != 0 ? 1 : 0;
+    if (e == cudaSuccess) e = paged8_error_flag(&eight, reset);
+    *value = here != 0 || forward != 0 || backward != 0 || eight != 0 ? 1 : 0;
     return e;
 }
 
@@ -291,6 +292,15 @@ bool nothing(const Shape& s) {
 }
 
 size_t cache_bytes(const flint_b200_paged_shape& s) { return s.pages * s.kv_heads * s.page_size * 128; }
+
+// Of 8-bit pages.
+size_t scale_bytes(const flint_b200_paged_shape& s) { return s.pages * s.kv_heads * (s.page_size / 16) * 4; }
+
+fb::Cache8 cache8(const void* k, const void* v, const void* k_scales, const void* v_scales) {
+    return fb::Cache8{static_cast<int8_t*>(const_cast<void*>(k)), static_cast<int8_t*>(const_cast<void*>(v)),
+                      static_cast<float*>(const_cast<void*>(k_scales)),
+                      static_cast<float*>(const_cast<void*>(v_scales))};
+}
 
 }  // namespace
 
@@ -471,6 +481,86 @@ flint_status flint_b200_paged_attention(void* o, void* lse, const void* q, const
     p.lengths = static_cast<const int*>(lengths);
     p.table = static_cast<const int*>(page_table);
     FB_CUDA(fb::packed_forward(p, static_cast<int>(shape->longest), workspace, stream));
+    return FLINT_OK;
+}
+
+flint_status flint_b200_paged8_store(void* k_pages, void* v_pages, void* k_scales, void* v_scales, const void* k,
+                                     const void* v, const void* starts, const void* lengths, const void* page_table,
+                                     const flint_b200_paged_shape* shape, flint_stream stream) {
+    constexpr const char* name = "flint_b200_paged8_store";
+    FB_TRY(check_shape(name, shape));
+    if (nothing(*shape)) {
+        return FLINT_OK;
+    }
+    const Rows list[] = {
+        flat("k_pages", k_pages, cache_bytes(*shape) / 2),
+        flat("v_pages", v_pages, cache_bytes(*shape) / 2),
+        flat("k_scales", k_scales, scale_bytes(*shape)),
+        flat("v_scales", v_scales, scale_bytes(*shape)),
+        token_rows("k", k, shape->rows, shape->kv_heads, shape->kv_stride),
+        token_rows("v", v, shape->rows, shape->kv_heads, shape->kv_stride),
+        flat("starts", starts, (shape->sequences + 1) * 4),
+        flat("lengths", lengths, shape->sequences * 4),
+        flat("page_table", page_table, shape->sequences * shape->table_stride * 4),
+    };
+    FB_TRY(check_all(name, list, 4));
+    fb::PackedArgs p = paged_args(*shape, 1.0f);
+    p.k = static_cast<const __half*>(k);
+    p.v = static_cast<const __half*>(v);
+    p.starts = static_cast<const int*>(starts);
+    p.lengths = static_cast<const int*>(lengths);
+    p.table = static_cast<const int*>(page_table);
+    FB_CUDA(fb::paged8_store(p, cache8(k_pages, v_pages, k_scales, v_scales), stream));
+    return FLINT_OK;
+}
+
+flint_status flint_b200_paged8_attention_workspace(const flint_b200_paged_shape* shape, size_t* bytes) {
+    constexpr const char* name = "flint_b200_paged8_attention_workspace";
+    FB_TRY(check_shape(name, shape));
+    if (bytes == nullptr) {
+        return fb::fail(kBad, "%s: bytes is null", name);
+    }
+    FB_CUDA(fb::packed_forward_workspace(bytes));
+    return FLINT_OK;
+}
+
+flint_status flint_b200_paged8_attention(void* o, void* lse, const void* q, const void* k_pages, const void* v_pages,
+                                         const void* k_scales, const void* v_scales, const void* starts,
+                                         const void* lengths, const void* page_table,
+                                         const flint_b200_paged_shape* shape, float scale, void* workspace,
+                                         size_t workspace_bytes, flint_stream stream) {
+    constexpr const char* name = "flint_b200_paged8_attention";
+    FB_TRY(check_shape(name, shape));
+    FB_TRY(check_scale(name, scale));
+    if (nothing(*shape)) {
+        return FLINT_OK;
+    }
+    size_t needed = 0;
+    FB_TRY(flint_b200_paged8_attention_workspace(shape, &needed));
+    FB_TRY(check_workspace(name, needed, workspace_bytes));
+    const Rows list[] = {
+        token_rows("o", o, shape->rows, shape->heads, shape->o_stride),
+        optional("lse", lse, shape->heads * shape->rows * 4, o),
+        flat("workspace", workspace, needed),
+        token_rows("q", q, shape->rows, shape->heads, shape->q_stride),
+        flat("k_pages", k_pages, cache_bytes(*shape) / 2),
+        flat("v_pages", v_pages, cache_bytes(*shape) / 2),
+        flat("k_scales", k_scales, scale_bytes(*shape)),
+        flat("v_scales", v_scales, scale_bytes(*shape)),
+        flat("starts", starts, (shape->sequences + 1) * 4),
+        flat("lengths", lengths, shape->sequences * 4),
+        flat("page_table", page_table, shape->sequences * shape->table_stride * 4),
+    };
+    FB_TRY(check_all(name, list, 3));
+    fb::PackedArgs p = paged_args(*shape, scale);
+    p.q = static_cast<const __half*>(q);
+    p.o = static_cast<__half*>(o);
+    p.lse = static_cast<float*>(lse);
+    p.starts = static_cast<const int*>(starts);
+    p.lengths = static_cast<const int*>(lengths);
+    p.table = static_cast<const int*>(page_table);
+    FB_CUDA(fb::paged8_attention(p, cache8(k_pages, v_pages, k_scales, v_scales), static_cast<int>(shape->longest),
+                                 workspace, stream));
     return FLINT_OK;
 }
 

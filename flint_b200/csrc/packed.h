@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cstddef>
+#include <cstdint>
 
 #include <cuda_fp16.h>
 #include <cuda_runtime_api.h>
@@ -44,6 +45,32 @@ cudaError_t packed_backward(const PackedArgs& args, const PackedGradients& gradi
                             cudaStream_t stream);
 cudaError_t packed_backward_workspace(size_t sequences, size_t rows, size_t heads, size_t kv_heads, size_t* bytes);
 cudaError_t packed_backward_error_flag(int* value, bool reset);
+
+// What the few-rows kernel over 8-bit pages shares with the above: CTAs of the grid, the workspace's records and parts of split
+// tiles (O [column / 4][row of 128][4], maxima, sums, two per CTA), and the launch that joins them.
+struct Record;
+constexpr size_t kPartFloats = size_t{128} * 64 + 2 * 128;
+int packed_ctas(int sms);
+Record* packed_records(void* workspace);
+float* packed_parts(void* workspace, int ctas);
+cudaError_t packed_join(const PackedArgs& args, const Record* records, const float* parts, int ctas,
+                        long long most_keys, cudaStream_t stream);
+
+// Pages of 8 bits in the place of args.k and args.v: codes [pages, kv_heads, page_size, 64] and a scale for 16
+// positions of a head.
+struct Cache8 {
+    int8_t* k;
+    int8_t* v;
+    float* k_scales;
+    float* v_scales;
+};
+
+// args.k and args.v: the new tokens' rows.
+cudaError_t paged8_store(const PackedArgs& args, const Cache8& cache, cudaStream_t stream);
+// args.k and args.v are not read; the workspace is packed_forward's.
+cudaError_t paged8_attention(const PackedArgs& args, const Cache8& cache, int longest, void* workspace,
+                             cudaStream_t stream);
+cudaError_t paged8_error_flag(int* value, bool reset);
 
 // Device error words of these kernels: a wait that gave up, or starts, lengths or page
 // numbers outside their ranges (which are clamped, so that nothing outside is touched).

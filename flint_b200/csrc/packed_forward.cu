@@ -29,6 +29,7 @@
 #include "common.h"
 #include "device_utils.cuh"
 #include "packed.cuh"
+#include "packed_locate.cuh"
 #include "packed_maps.h"
 #include "sm100.cuh"
 #include "softmax.cuh"
@@ -50,12 +51,9 @@ constexpr int kStaging = 1024;     // bytes per softmax warp
 constexpr int kStagingBytes = kSoftmaxWarps * kStaging;
 constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
-constexpr int kLeastPart = 4;   // of the line of key tiles, per CTA
 constexpr int kWholeKeys = 1024;   // up to which a tile is never split
-constexpr int kSplitCost = 6;      // about what splits and their join cost, in key tiles
-constexpr int kMostDealt = 128;    // sequences whose tiles can be dealt out
 
-constexpr size_t kPartFloats = size_t{kRows} * kHead + 2 * kRows;   // O [column / 4][row][4], maxima, sums
+static_assert(kPartFloats == size_t{kRows} * kHead + 2 * kRows, "a part is as packed.h has it");
 
 struct TileParams {
     CUtensorMap map_q, map_k, map_v;
@@ -91,262 +89,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-
-struct SequenceOf {
-    const PackedArgs& a;
-    __device__ __forceinline__ Sequence operator()(int s) const { return sequence_at(a, s); }
-};
-
-__device__ __forceinline__ long long warp_sum(long long v) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        v += __shfl_xor_sync(kFullMask, v, off);
-    }
-    return v;
-}
-__device__ __forceinline__ long long warp_prefix(long long v, int lane) {     // inclusive
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const long long other = __shfl_up_sync(kFullMask, v, off);
-        v += lane >= off ? other : 0;
-    }
-    return v;
-}
-
-// The place of one of this CTA's two cuts (0 its part's beginning, 1 its end; both the line's end for a CTA without a
-// part), and how far it may move.
-struct Place {
-    long long at, tolerance;
-    __device__ __forceinline__ Place(const TileParams& p, long long total, int which) {
-        const int parts = part_count(total, static_cast<int>(gridDim.x), kLeastPart);
-        const int cta = static_cast<int>(blockIdx.x);
-        at = cta < parts ? cut_place(total, parts, cta + which) : total;
-        tolerance = cta >= parts ? 0 : p.splits ? cut_tolerance(total, parts) : total;
-    }
-};
-
-__device__ __forceinline__ long long length_of(const TileParams& p, int s, int& before, int& tokens) {
-    before = tokens = 0;
-    if (s >= p.a.sequences) {
-        return 0;
-    }
-    const Sequence q = sequence_at(p.a, s);
-    before = q.before();
-    tokens = q.count;
-    return head_length(before, tokens, p.log_tokens);
-}
-
-__device__ __forceinline__ int most_key_tiles(const TileParams& p, int before, int tokens) {
-    return tokens == 0 ? 0 : key_tiles(before, tokens, p.log_tokens, tile_count(tokens, p.log_tokens) - 1);
-}
-
-// Whether tiles stay whole and are dealt out: none has more key tiles than a part of the line is long and splits cost.
-// The longest CTA then works on 14 key tiles and ends instead of 17 (24 sequences of up to 700 tokens, 12 heads:
-// 32.4 -> 27.3 us with the join, which finds nothing to do; 16 of up to 1,024: 29.4 -> 21.8; 5 of up to 4,096: 82 -> 73).
-// Tiles longer than a part: 6 more key tiles 24.1 -> 20.6, 28.7 -> 24.9 and 21.7 -> 21.0 us (three batches), 9 more 20.2 ->
-// 21.0 and 22.8 -> 25.1, 11 more 24.0 -> 29.5.
-__device__ __forceinline__ bool deals_out(const TileParams& p, long long total, int longest) {
-    return p.a.sequences <= kMostDealt && total < 1LL << 30 &&
-           (!p.splits || longest <= (static_cast<int>(total) - 1) / static_cast<int>(gridDim.x) + 1 + kSplitCost);
-}
-
-// Tiles dealt out whole. One warp, lane l with the sequences l, l + 32, ...
-struct Dealt {
-    static constexpr int kEach = kMostDealt / 32;
-    Sequence of[kEach];
-    int each = 1;
-    int count = 0;        // tiles
-    int longest = 0;      // key tiles of the next one at most
-    int round = 0;
-
-    __device__ __forceinline__ void load(const TileParams& p, int lane) {
-        each = (p.a.sequences + 31) / 32;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            of[i] = Sequence{0, 0, 0};
-            if (lane + 32 * i < p.a.sequences) {
-                of[i] = sequence_at(p.a, lane + 32 * i);
-            }
-        }
-    }
-    __device__ __forceinline__ int of_lane(const TileParams& p, int least) const {
-        int those = 0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (i < each) {
-                those += tiles_of_at_least(of[i].before(), of[i].count, p.log_tokens, least);
-            }
-        }
-        return those;
-    }
-    __device__ __forceinline__ int at_least(const TileParams& p, int least) const {
-        return __reduce_add_sync(kFullMask, of_lane(p, least)) * p.a.kv_heads;
-    }
-    __device__ __forceinline__ void begin(const TileParams& p, int most) {
-        longest = most;
-        count = at_least(p, 1);
-    }
-    // The next tile of this CTA, if there is one.
-    __device__ __forceinline__ bool next(const TileParams& p, int lane, Piece& out) {
-        const long long rank = dealt_rank(round, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-        ++round;
-        if (rank >= count) {
-            return false;
-        }
-        int low = 1;      // the most key tiles that more than `rank` tiles have
-        while (low < longest) {
-            const int middle = low + (longest - low + 1) / 2;
-            if (at_least(p, middle) > rank) {
-                low = middle;
-            } else {
-                longest = middle - 1;
-            }
-        }
-        // Among those of as many key tiles: by lane, the lane's sequences, heads, tiles.
-        const int more = of_lane(p, low + 1);
-        const int mine = (of_lane(p, low) - more) * p.a.kv_heads;
-        int upto = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int other = __shfl_up_sync(kFullMask, upto, off);
-            upto += lane >= off ? other : 0;
-        }
-        int at = static_cast<int>(rank) - __reduce_add_sync(kFullMask, more) * p.a.kv_heads - (upto - mine);
-        const int owner = __ffs(__ballot_sync(kFullMask, at >= 0 && at < mine)) - 1;
-        Sequence q = of[0];
-        int s = lane;
-#pragma unroll
-        for (int i = 0; i + 1 < kEach; ++i) {
-            if (s == lane + 32 * i && i + 1 < each) {
-                const int those = (tiles_of_at_least(q.before(), q.count, p.log_tokens, low) -
-                                   tiles_of_at_least(q.before(), q.count, p.log_tokens, low + 1)) * p.a.kv_heads;
-                if (at >= those) {
-                    at -= those;
-                    q = of[i + 1];
-                    s += 32;
-                }
-            }
-        }
-        at = __shfl_sync(kFullMask, at, owner);
-        out.index = __shfl_sync(kFullMask, s, owner);
-        out.sequence.first = __shfl_sync(kFullMask, q.first, owner);
-        out.sequence.count = __shfl_sync(kFullMask, q.count, owner);
-        out.sequence.keys = __shfl_sync(kFullMask, q.keys, owner);
-        const int of_low = tiles_of_at_least(out.sequence.before(), out.sequence.count, p.log_tokens, low);
-        const int these = of_low - tiles_of_at_least(out.sequence.before(), out.sequence.count, p.log_tokens, low + 1);
-        out.head = static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(these));
-        out.first_token = (tile_count(out.sequence.count, p.log_tokens) - of_low + at - out.head * these) << p.log_tokens;
-        out.tokens = min(out.sequence.count - out.first_token, 1 << p.log_tokens);
-        out.from = 0;
-        out.to = out.tiles = low;
-        return true;
-    }
-};
-
-// Which part of the line this CTA works on, for up to 32 sequences: one warp, its even lanes for one cut and the odd
-// ones for the other.
-template <bool kDeals>
-__device__ __forceinline__ void locate_in_warp(const TileParams& p, Cut (&cuts)[2], int& whole, int lane) {
-    int before, tokens;
-    const long long length = length_of(p, lane, before, tokens);
-    const long long mine = length * p.a.kv_heads;
-    const long long upto = warp_prefix(mine, lane);
-    const long long total = __shfl_sync(kFullMask, upto, 31);
-    if constexpr (kDeals) {
-        const int longest = __reduce_max_sync(kFullMask, most_key_tiles(p, before, tokens));
-        const bool deals = deals_out(p, total, longest);
-        if (lane == 0) {
-            whole = deals ? longest : 0;
-        }
-        if (deals) {
-            if (lane < 2) {
-                cuts[lane] = Cut{total, p.a.sequences, 0, 0, 0};
-            }
-            return;
-        }
-    }
-    const Place place(p, total, lane & 1);
-    const long long begins = upto - mine;
-    const long long first = __shfl_sync(kFullMask, place.at, 0), second = __shfl_sync(kFullMask, place.at, 1);
-    const unsigned has_first = __ballot_sync(kFullMask, first >= begins && first < upto);
-    const unsigned has_second = __ballot_sync(kFullMask, second >= begins && second < upto);
-    const unsigned has = (lane & 1) == 0 ? has_first : has_second;
-    const int owner = has != 0 ? __ffs(has) - 1 : 0;
-    const int its_before = __shfl_sync(kFullMask, before, owner), its_tokens = __shfl_sync(kFullMask, tokens, owner);
-    const long long its_length = __shfl_sync(kFullMask, length, owner), its_begin = __shfl_sync(kFullMask, begins, owner);
-    if (lane < 2) {
-        cuts[lane] = has == 0 ? Cut{total, p.a.sequences, 0, 0, 0}
-                              : cut_at(place.at, place.at - its_begin, owner, its_before, its_tokens, p.log_tokens,
-                                       its_length, place.tolerance);
-    }
-}
-
-// The same for any number: every thread of the block takes part.
-template <bool kDeals>
-__device__ __noinline__ void locate(const TileParams& p, Cut (&cuts)[2], int& whole, long long (&scan)[kWarps + 1],
-                                    int (&scan_longest)[kWarps]) {
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
-    int before = 0, tokens = 0;
-    long long sum = 0;
-    int longest = 0;
-    for (int s = tid; s < p.a.sequences; s += kThreads) {
-        sum += length_of(p, s, before, tokens);
-        longest = kDeals ? max(longest, most_key_tiles(p, before, tokens)) : 0;
-    }
-    sum = warp_sum(sum);
-    longest = __reduce_max_sync(kFullMask, longest);
-    if (lane == 0) {
-        scan[warp] = sum;
-        scan_longest[warp] = longest;
-    }
-    __syncthreads();
-    long long total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-        total += scan[w];
-        longest = max(longest, scan_longest[w]);
-    }
-    total *= p.a.kv_heads;
-    if constexpr (kDeals) {
-        const bool deals = deals_out(p, total, longest);
-        if (tid == 0) {
-            whole = deals ? longest : 0;
-        }
-        if (deals) {
-            if (tid < 2) {
-                cuts[tid] = Cut{total, p.a.sequences, 0, 0, 0};
-            }
-            return;
-        }
-    }
-    const Place place[2] = {Place(p, total, 0), Place(p, total, 1)};
-    if (tid < 2 && place[tid].at == total) {
-        cuts[tid] = Cut{total, p.a.sequences, 0, 0, 0};
-    }
-    long long running = 0;
-    for (int first = 0; first < p.a.sequences; first += kThreads) {
-        const long long length = length_of(p, first + tid, before, tokens);
-        const long long mine = length * p.a.kv_heads;
-        long long upto = warp_prefix(mine, lane);
-        __syncthreads();
-        if (lane == 31) {
-            scan[warp] = upto;
-        }
-        __syncthreads();
-        long long all = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            upto += w < warp ? scan[w] : 0;
-            all += scan[w];
-        }
-        const long long begins = running + upto - mine;
-        for (int c = 0; c < 2; ++c) {
-            if (place[c].at >= begins && place[c].at < begins + mine) {
-                cuts[c] = cut_at(place[c].at, place[c].at - begins, first + tid, before, tokens, p.log_tokens, length,
-                                 place[c].tolerance);
-            }
-        }
-        running += all;
-    }
 }
 
 // A piece as the TMA warp hands it to the others; `to` of 0 ends the list.
@@ -436,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         dealt.load(p, lane);
     }
     if (p.a.sequences > 32) {
-        locate<kDeals>(p, cuts, whole_tiles, scan, scan_longest);
+        locate<kDeals, kThreads>(p, cuts, whole_tiles, scan, scan_longest);
     } else if (warp == 2) {
         locate_in_warp<kDeals>(p, cuts, whole_tiles, lane);
     }
@@ -1306,9 +1048,24 @@ cudaError_t packed_forward_error_flag(int* value, bool reset) { return read_erro
 cudaError_t packed_forward_workspace(size_t* bytes) {
     int sms = 148;
     const cudaError_t e = sm_count(&sms);
-    const int ctas = std::min(2 * sms, kMostCtas);
+    const int ctas = packed_ctas(sms);
     *bytes = records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * kPartFloats * sizeof(float);
     return e;
+}
+
+int packed_ctas(int sms) { return std::min(2 * sms, kMostCtas); }
+
+Record* packed_records(void* workspace) { return static_cast<Record*>(workspace); }
+
+float* packed_parts(void* workspace, int ctas) {
+    return reinterpret_cast<float*>(static_cast<char*>(workspace) + records_bytes(ctas));
+}
+
+cudaError_t packed_join(const PackedArgs& args, const Record* records, const float* parts, int ctas,
+                        long long most_keys, cudaStream_t stream) {
+    JoinParams j = {args, records, parts, ctas, args.heads / args.kv_heads};
+    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(ctas + (most_keys > kManyKeys ? kHelpers : 0))),
+                            dim3(kJoinThreads), 0, stream, j);
 }
 
 cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace, cudaStream_t stream) {
@@ -1325,7 +1082,7 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     }
     int sms = 148;
     cudaError_t e = sm_count(&sms);
-    const int ctas = std::min(2 * sms, kMostCtas);
+    const int ctas = packed_ctas(sms);
     if (e == cudaSuccess) {
         e = encode_rows(&p.map_q, args.q, args.heads, args.rows, args.q_stride, p.group, 1 << p.log_tokens);
     }
@@ -1345,8 +1102,8 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     // Few rows have few key tiles each: whole tiles for every CTA, and no join.
     const long long most_keys = paged ? static_cast<long long>(args.table_stride) * args.page_size : args.rows;
     p.splits = most_keys > kWholeKeys;
-    p.records = static_cast<Record*>(workspace);
-    p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + records_bytes(ctas));
+    p.records = packed_records(workspace);
+    p.parts = packed_parts(workspace, ctas);
     const int form = !paged ? 0 : subsets == 1 ? 1 : subsets == 2 ? 2 : 3;
     const auto kernel = form == 0   ? fb_packed_forward_tiles<false, 1>
                         : form == 1 ? fb_packed_forward_tiles<true, 1>
@@ -1361,9 +1118,7 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     if (e != cudaSuccess || !p.splits) {
         return e;
     }
-    JoinParams j = {args, p.records, p.parts, ctas, p.group};
-    return launch_dependent(fb_packed_join, dim3(static_cast<unsigned>(ctas + (most_keys > kManyKeys ? kHelpers : 0))),
-                            dim3(kJoinThreads), 0, stream, j);
+    return packed_join(args, p.records, p.parts, ctas, most_keys, stream);
 }
 
 }  // namespace fb

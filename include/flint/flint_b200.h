@@ -322,6 +322,96 @@ FLINT_API flint_status flint_b200_paged_attention(void* o, void* lse, const void
                                                   void* workspace, size_t workspace_bytes,
                                                   flint_stream stream);
 
+/* ---- a cache of 8 bits ---------------------------------------------------------------------------
+ *
+ * Pages as above whose values are int8 codes: k_pages and v_pages are int8 [pages, kv_heads, page_size, 64], and
+ * k_scales and v_scales FP32 [pages, kv_heads, page_size / 16], one for each block of 16 positions of a head; a code q
+ * stands for q * scale. Half the memory of FP16 pages, and half of what attention reads.
+ *
+ * flint_b200_paged8_store writes the new tokens' keys and values, block by block. With a the largest |x| of the new
+ * values in a block of a head, its scale becomes s = a / 127 if the call writes the block's first position, and the larger of
+ * that and the scale it had otherwise; the codes of earlier positions become rint((q * s_before) / s), and the new ones
+ * rint(x / s), ties to even, every step rounded to FP32 (0 where s is 0). A block that grows token by token is thus rounded anew
+ * whenever a token exceeds what was there: up to half a step of the scale of that time, each time. A new value that is
+ * not finite makes its block's scale NaN, until the block's first position is written again. */
+FLINT_API flint_status flint_b200_paged8_store(void* k_pages, void* v_pages, void* k_scales, void* v_scales,
+                                               const void* k, const void* v, const void* starts,
+                                               const void* lengths, const void* page_table,
+                                               const flint_b200_paged_shape* shape, flint_stream stream);
+
+FLINT_API flint_status flint_b200_paged8_attention_workspace(const flint_b200_paged_shape* shape,
+                                                             size_t* bytes);
+
+/* flint_b200_paged_attention over these pages. Slots behind a sequence's last position, and the scales of blocks behind it,
+ * may hold anything. A block whose scale is NaN makes the rows NaN that see one of its positions, and no others. */
+FLINT_API flint_status flint_b200_paged8_attention(void* o, void* lse, const void* q, const void* k_pages,
+                                                   const void* v_pages, const void* k_scales,
+                                                   const void* v_scales, const void* starts,
+                                                   const void* lengths, const void* page_table,
+                                                   const flint_b200_paged_shape* shape, float scale,
+                                                   void* workspace, size_t workspace_bytes,
+                                                   flint_stream stream);
+
+/* ---- pages of a cache -----------------------------------------------------------------------------
+ *
+ * Which sequence holds which pages, kept on the device: page_table int32 [sequences, table_stride] (of row s the first
+ * ceil(lengths[s] / page_size) entries, anything behind them), lengths int32 [sequences] and references int32 [pages],
+ * how often each page stands in tables (0: it is free). Sequences may share pages; a page that several hold is only read. The calls
+ * change numbers alone; they name pages to be copied in `moves` (int32 [.., 2], from and to, -1 behind the last), which
+ * flint_b200_pages_copy carries out for every layer's arrays. Results do not depend on timing: free pages are taken in
+ * ascending order by sequences in ascending order.
+ * Limits: sequences up to 65,535, pages up to 2^24, page_size a power of two from 16 to 1,024, table_stride * page_size up
+ * to 2^26. Numbers in device memory that are out of range are passed over and reported by flint_b200_kernel_fault. */
+typedef struct {
+    size_t sequences;
+    size_t table_stride;
+    size_t pages;
+    size_t page_size;
+} flint_b200_page_pool;
+
+/* For reserve and compact. */
+FLINT_API flint_status flint_b200_pages_workspace(const flint_b200_page_pool* pool, size_t* bytes);
+
+/* Sequence t goes on as parents[t] (int32 [sequences]) stands, sharing all of its pages; -1 leaves it empty, so that keeping,
+ * repeating, dropping and freeing sequences are one call. next_table's entries behind a sequence's pages become -1. */
+FLINT_API flint_status flint_b200_pages_fork(void* next_table, void* next_lengths, void* next_references,
+                                             const void* page_table, const void* lengths,
+                                             const void* references, const void* parents,
+                                             const flint_b200_page_pool* pool, flint_stream stream);
+
+/* Room for added[s] (int32 [sequences]) more tokens of every sequence, whose lengths grow by them: free pages for what lies
+ * behind the last one, and a free page as a copy of the last one where that is partly filled and shared. Of r sequences
+ * that share such a page and all grow the first keeps it; where others hold it too, all take copies. moves
+ * [sequences, 2] receives the copies, counts (int32 [2]) their number and how many free pages were missing: if
+ * any were, nothing else is changed. */
+FLINT_API flint_status flint_b200_pages_reserve(void* page_table, void* lengths, void* references, void* moves,
+                                                void* counts, const void* added,
+                                                const flint_b200_page_pool* pool, void* workspace,
+                                                size_t workspace_bytes, flint_stream stream);
+
+/* Cuts every sequence to its first keep[s] (int32 [sequences]) positions, 0 to free it, its length or more to leave it as it
+ * is; gives back the pages behind them, whose entries become -1. */
+FLINT_API flint_status flint_b200_pages_truncate(void* page_table, void* lengths, void* references,
+                                                 const void* keep, const flint_b200_page_pool* pool,
+                                                 flint_stream stream);
+
+/* Renumbers pages so that the n in use are pages 0 .. n - 1: the i-th used page from n on takes the place of the i-th free one
+ * below. moves [pages / 2, 2] receives those, counts (int32 [2]) their number and n. The table is the only one
+ * that is rewritten; its entries behind a sequence's pages become -1. */
+FLINT_API flint_status flint_b200_pages_compact(void* next_table, void* next_references, void* moves,
+                                                void* counts, const void* page_table, const void* lengths,
+                                                const void* references, const flint_b200_page_pool* pool,
+                                                void* workspace, size_t workspace_bytes,
+                                                flint_stream stream);
+
+/* Copies pages within each of `count` (up to 128) arrays: arrays[i] is [pages, page_bytes[i]] bytes on the device (the two
+ * lists are on the host and are read during the call), page_bytes multiples of 4. moves and counts are as reserve and
+ * compact leave them: the first counts[0] of up to most_moves rows; rows with a number that is not a page are passed over. No page may be
+ * both copied from and to, or copied to twice. */
+FLINT_API flint_status flint_b200_pages_copy(void* const* arrays, const size_t* page_bytes, size_t count,
+                                             size_t pages, const void* moves, const void* counts,
+                                             size_t most_moves, flint_stream stream);
+
 /* ---- probabilities of tokens ----------------------------------------------------------------
  *
  * Over the first vocab columns of each row x of logits [rows, cols], FP16 or (fp32_logits not 0)
@@ -351,6 +441,36 @@ FLINT_API flint_status flint_b200_token_log_probs_backward(
     void* dlogits, const void* logits, const void* targets, const void* lse, const void* entropy,
     const void* d_log_probs, const void* d_entropy, int fp32_logits, size_t rows, size_t vocab,
     size_t cols, flint_stream stream);
+
+/* ---- beam search ---------------------------------------------------------------------------------
+ *
+ * groups of `beams` (up to 32) beams, beam b of group g being row g * beams + b of everything here. From the first vocab
+ * columns of logits [rows, cols] (FP16, or FP32 where fp32_logits is not 0) and scores (FP32 [rows], a beam's
+ * log-probability so far; minus infinity for one that is not in use) every beam's continuations by a token get the
+ * total score + log p(token); a beam that is finished (int32 [rows], not 0) goes on in one way, by end_token at
+ * its score. The `beams` best of each group by total / length^length_power, length being the continuation's, become the next beams
+ * in descending order, equal ones by beam and token: next_scores (FP32, the totals), parents (int32, rows), tokens (uint16),
+ * next_finished (parent finished, or token end_token), next_lengths (the parent's, one more unless it was finished) and
+ * next_histories (uint16 [rows, history_stride]: the parent's first tokens, and the new one unless it was finished;
+ * what lies behind is left as it is; a history that is full takes no more and is reported by flint_b200_kernel_fault).
+ * A total of minus infinity or NaN is no continuation, nor is anything of a row of logits with a NaN or plus infinity; where
+ * a group has fewer than `beams`, places left are filled by the beams of the same places, with token 0 (end_token
+ * where that beam is finished) at a score of minus infinity.
+ * Totals are compared in FP64, with log-sum-exps to FP32's accuracy.
+ * end_token is -1 for none (beams that are finished all the same go on by token 0): finished and next_finished may then be null. lengths and next_lengths may be null
+ * where histories (with next_histories) are and length_power is 0. cols is a multiple of 8 from 8 to 65,536,
+ * groups * beams up to 2^20, length_power finite and not negative, history_stride up to 2^24. */
+FLINT_API flint_status flint_b200_beam_select_workspace(size_t groups, size_t beams, size_t* bytes);
+
+FLINT_API flint_status flint_b200_beam_select(void* next_scores, void* parents, void* tokens,
+                                              void* next_finished, void* next_lengths,
+                                              void* next_histories, const void* logits, const void* scores,
+                                              const void* finished, const void* lengths,
+                                              const void* histories, int fp32_logits, size_t groups,
+                                              size_t beams, size_t vocab, size_t cols,
+                                              size_t history_stride, int end_token, float length_power,
+                                              void* workspace, size_t workspace_bytes,
+                                              flint_stream stream);
 
 /* Sets *found_nonfinite (device int) to 1 if any of the count FP32 values is
  * inf or NaN; leaves it unchanged otherwise, so several calls can share it.
