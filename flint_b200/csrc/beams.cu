@@ -2,12 +2,12 @@
 // reference has no decoding).
 //
 // A beam's continuation by token c has the total  score + x_c - lse.  Within a beam the order is that of the logits, so a row
-// needs its log-sum-exp and its `beams` largest logits alone. The first launch reads the logits once: a row falls into parts, a
-// part into 64 bins of neighbouring lanes, and what is not below the beams-th largest of the bins' maxima (a lower
-// bound of the beams-th largest logit; about `beams` values) is collected and put in order by counting. The second launch
-// has a block per group: the beams-th largest of its lists' heads bounds the totals in the same way, and few are left to be
-// ordered. Totals are FP64 there, because two beams' continuations can be closer than FP32 tells apart; a tie goes to the
-// lower beam, then the lower token.
+// needs its log-sum-exp and its `beams` largest logits alone. The first launch reads the logits once: a warp has a
+// part of a row to itself, so that nothing waits for anything but memory. It takes sums against each lane's own running maximum and
+// notes the maxima of groups of a few words. The beams-th largest of the lanes' two largest groups bounds the beams-th largest logit
+// from below; the groups that reach it (about `beams`) are read again, from L2, and what reaches it is put in order by counting. The
+// second launch has a block per group of beams and does the same with totals, in FP64, because two beams'
+// continuations can be closer than FP32 tells apart; a tie goes to the lower beam, then the lower token.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -27,11 +27,13 @@ namespace {
 constexpr int kMostBeams = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 64;
-constexpr int kLanes = kThreads / kBins;
-constexpr int kCandidates = 512;
+constexpr int kHeld = 4;             // 16-byte words that a lane has on their way
+constexpr int kBlocks = 4;           // per SM
+constexpr int kChunk = 32 * kHeld;   // words that a warp works on at a time
+constexpr int kCandidates = 128;     // of a warp
+constexpr int kMany = 96;            // from which on the bound rises
+constexpr int kGroups = 32;          // of a lane's words, whose maxima are noted
 constexpr int kMostLists = 256;      // of a group
-constexpr int kHeldWords = 8;        // 16-byte words of a part per thread
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int g_beams_error = 0;
@@ -41,7 +43,7 @@ struct RowArgs {
     const int* finished;      // may be null
     float2* stats;            // [row][part] the part's maximum m and its sum of e^(x - m)
     Key* best;                // [row][part][beams] its largest logits in order; 0 where it has no more above minus infinity
-    long long items;          // rows * parts
+    unsigned items;           // rows * parts
     int vocab, cols, beams;
     int parts, slice;         // words of a part
 };
@@ -68,13 +70,21 @@ struct Row<__half> {
     __device__ static __forceinline__ void unpack(float (&v)[8], const uint4& q) { fb::unpack8(v, q); }
 };
 
-// Sums of e^(x - m): the difference first, which is exact near m.
-struct Exponentials {
-    float minus_m, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    __device__ __forceinline__ explicit Exponentials(float m) : minus_m(-m) {}
+// A lane's sum of e^(x - m) against its running maximum m.
+struct LaneSum {
+    float m = -INFINITY, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void raise(float next) {
+        const float factor = m == -INFINITY ? 0.0f : exp2f((m - next) * kLog2e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i] *= factor;
+        }
+        m = next;
+    }
+    // (m is above minus infinity. The difference first, which is exact near m.)
     template <int kValues>
     __device__ __forceinline__ void add(const float (&v)[kValues]) {
-        const fb::F2 minus = fb::f2_pack(minus_m, minus_m), log2e = fb::f2_pack(kLog2e, kLog2e);
+        const fb::F2 minus = fb::f2_pack(-m, -m), log2e = fb::f2_pack(kLog2e, kLog2e);
 #pragma unroll
         for (int c = 0; c < kValues; c += 2) {
             float y0, y1, e0, e1;
@@ -88,192 +98,219 @@ struct Exponentials {
     __device__ __forceinline__ float total() const { return (sum[0] + sum[1]) + (sum[2] + sum[3]); }
 };
 
-template <typename T, int kHeld>
-__global__ void __launch_bounds__(kThreads, kHeld > 2 ? 3 : 4) fb_beam_rows(const RowArgs p) {
+__device__ __forceinline__ unsigned upper(Key key) { return static_cast<unsigned>(key >> 32); }
+
+// The largest number of kBits upper bits that k of the warp's values (kEach per lane, order_key's upper halves) reach.
+template <int kBits, int kEach>
+__device__ __forceinline__ unsigned reached_by(const unsigned (&mine)[kEach], int k) {
+    unsigned least = 0;
+#pragma unroll 4
+    for (int bit = 31; bit >= 32 - kBits; --bit) {
+        const unsigned trial = least | (1u << bit);
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            reach += mine[i] >= trial ? 1 : 0;
+        }
+        if (__reduce_add_sync(fb::kFullMask, reach) >= k) {
+            least = trial;
+        }
+    }
+    return least;
+}
+
+// What is not below the k-th largest value of a warp's `count` candidates (up to kCandidates) stays, in order; how many that are,
+// and the value.
+__device__ __noinline__ int keep_largest(Key* list, int count, int k, float& bound, int lane) {
+    Key mine[kCandidates / 32];
+#pragma unroll
+    for (int i = 0; i < kCandidates / 32; ++i) {
+        mine[i] = lane + 32 * i < count ? list[lane + 32 * i] : 0;
+    }
+    unsigned values[kCandidates / 32];
+#pragma unroll
+    for (int i = 0; i < kCandidates / 32; ++i) {
+        values[i] = upper(mine[i]);
+    }
+    const unsigned least = reached_by<32>(values, k);
+    __syncwarp();
+    int kept = 0;
+#pragma unroll
+    for (int i = 0; i < kCandidates / 32; ++i) {
+        const bool stays = upper(mine[i]) >= least && mine[i] != 0;
+        const unsigned those = __ballot_sync(fb::kFullMask, stays);
+        if (stays) {
+            list[kept + __popc(those & ((1u << lane) - 1))] = mine[i];
+        }
+        kept += __popc(those);
+    }
+    __syncwarp();
+    bound = fmaxf(bound, key_value(static_cast<Key>(least) << 32));
+    return kept;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs p) {
     using R = Row<T>;
-    // Two of each, for parts in turn: one barrier less at a part's end.
-    __shared__ float bins[2][kBins];
-    __shared__ Key candidates[2][kCandidates];
-    __shared__ float maxima[2][kWarps], sums[2][kWarps], least[2];
-    __shared__ int counts[2];
-    __shared__ Key reduced[kWarps];
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, warp = tid / 32;
+    __shared__ Key lists[kWarps][kCandidates];
+    __shared__ float group_max[kWarps][kGroups][32];
+    const int lane = static_cast<int>(threadIdx.x) % 32, warp = __shfl_sync(fb::kFullMask, static_cast<int>(threadIdx.x) / 32, 0);
     const int row_words = p.cols / R::kValues;
     const int all_words = (p.vocab + R::kValues - 1) / R::kValues;
     const int last_count = p.vocab - (all_words - 1) * R::kValues;
-    if (tid < 2) {
-        counts[tid] = 0;
-    }
+    Key* list = lists[warp];
+    // Chunks whose words make up a group, and the chunks in a part.
+    const int chunks = (p.slice + kChunk - 1) / kChunk, of_group = (chunks + kGroups - 1) / kGroups;
     fb::dependency_wait();
     fb::dependency_release();
-    __syncthreads();
-    struct Part {
-        long long row;
-        int first, words;      // 0 words: the beam is finished, or there is no part
-    };
-    auto part_at = [&](long long item) {
-        Part part = {0, 0, 0};
-        if (item < p.items) {
-            part.row = item / p.parts;
-            part.first = static_cast<int>(item - part.row * p.parts) * p.slice;
-            part.words = p.finished != nullptr && p.finished[part.row] != 0 ? 0 : max(0, min(p.slice, all_words - part.first));
-        }
-        return part;
-    };
-    auto words_of = [&](const Part& part) { return static_cast<const uint4*>(p.logits) + part.row * row_words + part.first; };
-    const long long stride = gridDim.x;
-    Part part = part_at(blockIdx.x), next = part_at(blockIdx.x + stride);
-    uint4 held[kHeld];
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-        if (tid + j * kThreads < part.words) {
-            held[j] = words_of(part)[tid + j * kThreads];
-        }
-    }
-    int parity = 0;
-    for (long long item = blockIdx.x; item < p.items; item += stride) {
-        const Part after = part_at(item + 2 * stride);
-        const uint4* next_words = words_of(next);
-        if (part.words == 0) {
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                if (tid + j * kThreads < next.words) {
-                    held[j] = next_words[tid + j * kThreads];
-                }
-            }
-            part = next;
-            next = after;
+    const unsigned warps = gridDim.x * kWarps;
+    // (Neighbouring parts go to different SMs, so that a short list does not fill a few of them.)
+    for (unsigned item = warp * gridDim.x + blockIdx.x; item < p.items; item += warps) {
+        const unsigned row = item / static_cast<unsigned>(p.parts);
+        if (p.finished != nullptr && p.finished[row] != 0) {
             continue;
         }
-        Max<T> running;
+        const int first = static_cast<int>(item - row * p.parts) * p.slice;
+        const int words = max(0, min(p.slice, all_words - first));
+        const uint4* from = static_cast<const uint4*>(p.logits) + static_cast<size_t>(row) * row_words + first;
+        // Word i of the part; minus infinity, which counts for nothing, behind its end.
+        auto word_at = [&](int i) {
+            uint4 q = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+            if (sizeof(T) == 4) {
+                q = make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+            }
+            if (i < words) {
+                q = from[i];
+            }
+            return q;
+        };
+        auto cut = [&](uint4& q, int i) {
+            if (first + i == all_words - 1) {
+                cut_word(q, last_count, T());
+            }
+        };
+        uint4 held[kHeld];
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < part.words) {
-                if (part.first + i == all_words - 1) {
-                    cut_word(held[j], last_count, T());
+            held[j] = word_at(lane + 32 * j);
+        }
+        LaneSum sum;
+        float best_group = -INFINITY, second_group = -INFINITY;
+        int group = 0;
+        for (int c = 0; c * kChunk < words;) {
+            Max<T> running;
+            for (int end = c + of_group; c < end && c * kChunk < words; ++c) {
+                const int at = c * kChunk + lane;
+                if (first + (c + 1) * kChunk >= all_words) {
+#pragma unroll
+                    for (int j = 0; j < kHeld; ++j) {
+                        cut(held[j], at + 32 * j);
+                    }
                 }
-                running.add(held[j]);
-            }
-        }
-        const float my_max = running.value();
-        float mx = my_max;
+                Max<T> here;
 #pragma unroll
-        for (int off = 1; off < kLanes; off <<= 1) {
-            mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
-        }
-        if (tid % kLanes == 0) {
-            bins[parity][tid / kLanes] = mx;
-        }
+                for (int j = 0; j < kHeld; ++j) {
+                    here.add(held[j]);
+                }
+                running.add(here);
+                const float mx = here.value();
+                if (!(mx <= sum.m)) {       // (a NaN stays)
+                    sum.raise(mx);
+                }
+                const bool adds = sum.m != -INFINITY;
 #pragma unroll
-        for (int off = kLanes; off < 32; off <<= 1) {
-            mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
-        }
-        if (lane == 0) {
-            maxima[parity][warp] = mx;
-        }
-        __syncthreads();
-        if (tid == 0) {
-            counts[parity ^ 1] = 0;      // (of the part before, which everybody is done with)
-        }
-        mx = maxima[parity][lane % kWarps];
-#pragma unroll
-        for (int off = 1; off < kWarps; off <<= 1) {
-            mx = max_nan(mx, __shfl_xor_sync(fb::kFullMask, mx, off));
-        }
-        // The beams-th largest of the bins' maxima, equal ones counted each: a warp ranks its share of the bins.
-        const float low = bins[parity][lane], high = bins[parity][lane + 32];
-#pragma unroll
-        for (int i = 0; i < kBins / kWarps; ++i) {
-            const int bin = warp * (kBins / kWarps) + i;
-            const float value = bins[parity][bin];
-            const int larger = __popc(__ballot_sync(fb::kFullMask, low > value || (low == value && lane < bin))) +
-                               __popc(__ballot_sync(fb::kFullMask, high > value || (high == value && lane + 32 < bin)));
-            if (larger == p.beams - 1 && lane == 0) {
-                least[parity] = value;      // (none is where bins are NaN)
-            }
-        }
-        __syncthreads();
-        const float bound = least[parity];
-        const bool counts_for_nothing = !(mx > -INFINITY && mx < INFINITY);      // NaN, plus infinity, or nothing there
-        if (!counts_for_nothing && __any_sync(fb::kFullMask, my_max >= bound)) {
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int i = tid + j * kThreads;
-                if (i < part.words && Max<T>::word(held[j]) >= bound) {
+                for (int j = 0; j < kHeld; ++j) {
                     float v[R::kValues];
                     R::unpack(v, held[j]);
-#pragma unroll
-                    for (int c = 0; c < R::kValues; ++c) {
-                        if (v[c] >= bound && v[c] > -INFINITY) {
-                            const int at = atomicAdd(&counts[parity], 1);
-                            if (at < kCandidates) {
-                                candidates[parity][at] = order_key(v[c], (part.first + i) * R::kValues + c);
-                            }
-                        }
+                    held[j] = word_at(at + kChunk + 32 * j);
+                    if (adds) {
+                        sum.add(v);
                     }
                 }
             }
+            const float mx = running.value();
+            group_max[warp][group++][lane] = mx;
+            second_group = fmaxf(second_group, fminf(best_group, mx));
+            best_group = fmaxf(best_group, mx);
         }
-        Exponentials exponentials(mx);
+        float m = sum.m;
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < part.words) {
-                float v[R::kValues];
-                R::unpack(v, held[j]);
-                exponentials.add(v);
-            }
-            if (i < next.words) {
-                held[j] = next_words[i];
-            }
+        for (int off = 16; off > 0; off >>= 1) {
+            m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, off));
         }
-        float total = exponentials.total();
+        float total = sum.m == -INFINITY ? 0.0f : sum.total() * exp2f((sum.m - m) * kLog2e);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
             total += __shfl_xor_sync(fb::kFullMask, total, off);
         }
         if (lane == 0) {
-            sums[parity][warp] = total;
+            // (A part of nothing but minus infinity adds nothing, one with a NaN or plus infinity makes the row NaN.)
+            p.stats[item] = make_float2(m, total);
         }
-        __syncthreads();
-        Key* best = p.best + item * p.beams;
-        const int found = counts[parity];
-        if (warp == kWarps - 1) {
-            total = sums[parity][lane % kWarps];
+        // 20 bits are sign, exponent and 11 bits of the fraction: all of an FP16 number, and enough of others for a bound.
+        const unsigned tops[2] = {upper(order_key(best_group, 0)), upper(order_key(second_group, 0))};
+        float bound = key_value(static_cast<Key>(reached_by<20>(tops, p.beams)) << 32);
+        bound = bound == bound ? bound : -INFINITY;      // (fewer groups than beams)
+        unsigned mask = 0;
+        for (int g = 0; g < group; ++g) {
+            const float mx = group_max[warp][g][lane];
+            mask |= mx >= bound && mx > -INFINITY ? 1u << g : 0u;
+        }
+        int count = 0;
+        bool overflow = false;
+        while (__any_sync(fb::kFullMask, mask != 0)) {
+            const int g = __ffs(mask) - 1;
+            mask &= mask - 1;
+            for (int i = g * of_group * kChunk + lane, end = i + of_group * kChunk; i < end; i += 32) {
+                uint4 q = word_at(g >= 0 ? i : words);
+                cut(q, i);
+                float v[R::kValues];
+                R::unpack(v, q);
 #pragma unroll
-            for (int off = 1; off < kWarps; off <<= 1) {
-                total += __shfl_xor_sync(fb::kFullMask, total, off);
-            }
-            if (lane == 0) {
-                // (A part of nothing but minus infinity adds nothing, one with a NaN or plus infinity makes the row NaN.)
-                p.stats[item] = make_float2(mx, mx == -INFINITY ? 0.0f : total);
+                for (int c = 0; c < R::kValues; ++c) {
+                    const bool reaches = v[c] >= bound && v[c] > -INFINITY;
+                    const unsigned those = __ballot_sync(fb::kFullMask, reaches);
+                    if (those != 0 && !overflow) {
+                        if (reaches) {
+                            list[count + __popc(those & ((1u << lane) - 1))] = order_key(v[c], (first + i) * R::kValues + c);
+                        }
+                        count += __popc(those);
+                        if (count > kMany) {
+                            __syncwarp();
+                            count = keep_largest(list, count, p.beams, bound, lane);
+                            overflow = count > kMany;
+                        }
+                    }
+                }
             }
         }
-        if (found <= kCandidates) {
-            for (int c = tid; c < found; c += kThreads) {
-                const Key key = candidates[parity][c];
+        __syncwarp();
+        Key* best = p.best + static_cast<size_t>(item) * p.beams;
+        if (!overflow) {
+            for (int c = lane; c < count; c += 32) {
+                const Key key = list[c];
                 int larger = 0;
-#pragma unroll 8
-                for (int other = 0; other < found; ++other) {
-                    larger += candidates[parity][other] > key ? 1 : 0;
+#pragma unroll 4
+                for (int other = 0; other < count; ++other) {
+                    larger += list[other] > key ? 1 : 0;
                 }
                 if (larger < p.beams) {
                     best[larger] = key;
                 }
             }
-            for (int c = found + tid; c < p.beams; c += kThreads) {
+            for (int c = count + lane; c < p.beams; c += 32) {
                 best[c] = 0;
             }
         } else {
             // Many equal ones: the part is gone through once for every place.
-            const char* row = static_cast<const char*>(p.logits) + part.row * p.cols * sizeof(T);
-            const int begin = part.first * R::kValues, end = min((part.first + part.words) * R::kValues, p.vocab);
+            const char* values = static_cast<const char*>(p.logits) + static_cast<size_t>(row) * p.cols * sizeof(T);
+            const int begin = first * R::kValues, end = min((first + words) * R::kValues, p.vocab);
             Key before = ~Key{0};
             for (int k = 0; k < p.beams; ++k) {
                 Key mine = 0;
-                for (int c = begin + tid; c < end; c += kThreads) {
-                    const float v = R::value(row, c);
+#pragma unroll 4
+                for (int c = begin + lane; c < end; c += 32) {
+                    const float v = R::value(values, c);
                     const Key key = v > -INFINITY ? order_key(v, c) : 0;
                     mine = key < before && key > mine ? key : mine;
                 }
@@ -282,23 +319,13 @@ __global__ void __launch_bounds__(kThreads, kHeld > 2 ? 3 : 4) fb_beam_rows(cons
                     const Key other = __shfl_xor_sync(fb::kFullMask, mine, off);
                     mine = other > mine ? other : mine;
                 }
-                __syncthreads();
-                if (lane == 0) {
-                    reduced[warp] = mine;
-                }
-                __syncthreads();
-                for (int w = 0; w < kWarps; ++w) {
-                    mine = reduced[w] > mine ? reduced[w] : mine;
-                }
                 before = mine;
-                if (tid == 0) {
+                if (lane == 0) {
                     best[k] = mine;
                 }
             }
         }
-        parity ^= 1;
-        part = next;
-        next = after;
+        __syncwarp();      // (the list is read)
     }
 }
 
@@ -329,6 +356,11 @@ __device__ __forceinline__ Key order_total(double v) {
     return (bits >> 63) != 0 ? ~bits : bits | (Key{1} << 63);
 }
 
+constexpr int kBins = 64;
+constexpr int kHeldEntries = 4;      // of a group's lists, that a thread holds
+constexpr int kMostEntries = 4096;   // of them all: 64 in each bin, and the bound leaves entries of kMostBeams bins
+constexpr int kLeft = kMostBeams * (kMostEntries / kBins);
+
 struct Candidate {
     Key rank;
     unsigned place;      // beam, token
@@ -337,14 +369,20 @@ struct Candidate {
     }
 };
 
+// What is known of a group's beams.
+struct Beams {
+    double score[kMostBeams], lse[kMostBeams], weight[kMostBeams];     // weight: length^-power
+    int over[kMostBeams], length[kMostBeams];
+};
+
 __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
-    __shared__ double score_of[kMostBeams], lse_of[kMostBeams], norm_of[kMostBeams];
-    __shared__ int over_of[kMostBeams], length_of[kMostBeams];
+    __shared__ Beams of;
     __shared__ float2 stats[kMostLists];
-    __shared__ Candidate heads[kMostLists];
+    __shared__ Candidate bins[kBins];
     __shared__ Candidate bound;
-    __shared__ Candidate left[kMostBeams * kMostBeams];
-    __shared__ double left_total[kMostBeams * kMostBeams];
+    __shared__ Key left_rank[kLeft];
+    __shared__ unsigned left_place[kLeft];
+    __shared__ double left_total[kLeft];
     __shared__ int left_count;
     __shared__ unsigned chosen[kMostBeams];
     __shared__ double chosen_total[kMostBeams];
@@ -352,94 +390,143 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
     fb::dependency_wait();
     fb::dependency_release();
     const long long first = static_cast<long long>(blockIdx.x) * p.beams;
-    const int lists = p.beams * p.parts;
+    const int lists = p.beams * p.parts, entries = lists * p.beams;
+    const Key* keys = p.best + first * p.parts * p.beams;
+    Key held[kHeldEntries];       // this thread's first entries
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+        held[i] = tid + i * kThreads < entries ? keys[tid + i * kThreads] : 0;
+    }
     if (tid < lists) {
         stats[tid] = p.stats[first * p.parts + tid];
+    }
+    // A warp takes the beams' lengths while others wait for statistics.
+    if (warp == kWarps - 1 && lane < p.beams) {
+        const int over = p.finished != nullptr && p.finished[first + lane] != 0 ? 1 : 0;
+        int length = p.lengths != nullptr ? p.lengths[first + lane] : 0;
+        if (length < 0 || (p.histories != nullptr && length > p.history_stride)) {
+            atomicExch(&g_beams_error, 1);
+            length = length < 0 ? 0 : static_cast<int>(p.history_stride);
+        }
+        const float score = p.scores[first + lane];
+        of.over[lane] = over;
+        of.length[lane] = length;
+        of.score[lane] = fabsf(score) < INFINITY ? static_cast<double>(score) : -INFINITY;
+        chosen[lane] = ~0u;
     }
     if (tid == 0) {
         left_count = 0;
         bound = Candidate{1, ~0u};      // anything that is a continuation
     }
-    if (tid < p.beams) {
-        chosen[tid] = ~0u;
-        const float score = p.scores[first + tid];
-        over_of[tid] = p.finished != nullptr && p.finished[first + tid] != 0 ? 1 : 0;
-        int length = p.lengths != nullptr ? p.lengths[first + tid] : 0;
-        if (length < 0 || (p.histories != nullptr && length > p.history_stride)) {
-            atomicExch(&g_beams_error, 1);
-            length = length < 0 ? 0 : static_cast<int>(p.history_stride);
-        }
-        length_of[tid] = length;
-        score_of[tid] = fabsf(score) < INFINITY ? static_cast<double>(score) : -INFINITY;
-        const double grown = over_of[tid] != 0 ? max(length, 1) : static_cast<double>(length) + 1.0;
-        norm_of[tid] = p.power == 0.0f ? 1.0 : pow(grown, static_cast<double>(p.power));
-    }
     __syncthreads();
-    if (tid < p.beams) {
-        // (A finished beam's row was not read.)
-        double lse = 0.0;
-        if (over_of[tid] == 0) {
+    if (warp == kWarps - 1) {
+        if (lane < p.beams) {
+            const double grown = of.over[lane] != 0 ? max(of.length[lane], 1) : static_cast<double>(of.length[lane]) + 1.0;
+            of.weight[lane] = p.power == 0.0f ? 1.0 : 1.0 / pow(grown, static_cast<double>(p.power));
+        }
+    } else {
+        for (int beam = warp; beam < p.beams; beam += kWarps - 1) {
             float m = -INFINITY, sum = 0.0f;
-            for (int i = 0; i < p.parts; ++i) {
-                m = max_nan(m, stats[tid * p.parts + i].x);
+            for (int i = lane; i < p.parts; i += 32) {
+                m = max_nan(m, stats[beam * p.parts + i].x);
             }
-            for (int i = 0; i < p.parts; ++i) {
-                const float2 part = stats[tid * p.parts + i];
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) {
+                m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, off));
+            }
+            for (int i = lane; i < p.parts; i += 32) {
+                const float2 part = stats[beam * p.parts + i];
                 sum += part.x == -INFINITY ? 0.0f : part.y * expf(part.x - m);
             }
-            lse = static_cast<double>(m) + log(static_cast<double>(sum));
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) {
+                sum += __shfl_xor_sync(fb::kFullMask, sum, off);
+            }
+            if (lane == 0) {
+                of.lse[beam] = static_cast<double>(m) + log(static_cast<double>(sum));
+            }
         }
-        lse_of[tid] = lse;
     }
     __syncthreads();
-    auto candidate_at = [&](int list, int i, double& total) {
-        const int beam = list / p.parts;
-        if (over_of[beam] != 0) {
-            total = list % p.parts == 0 && i == 0 ? score_of[beam] : -INFINITY;
-            return Candidate{order_total(total / norm_of[beam]), static_cast<unsigned>(beam) << 16 | static_cast<unsigned>(max(p.end_token, 0))};
+    // Entry i, of list i / beams.
+    auto candidate_of = [&](int i, Key key, double& total) {
+        const int list = i / p.beams, beam = list / p.parts;
+        if (of.over[beam] != 0) {
+            // (A finished beam's row was not read; it has one continuation.)
+            total = i == beam * p.parts * p.beams ? of.score[beam] : -INFINITY;
+            return Candidate{order_total(total * of.weight[beam]), static_cast<unsigned>(beam) << 16 | static_cast<unsigned>(max(p.end_token, 0))};
         }
-        const Key key = p.best[(first * p.parts + list) * p.beams + i];
         // (An lse that is not a number, or minus infinity, gives none.)
-        total = key != 0 ? score_of[beam] + (static_cast<double>(key_value(key)) - lse_of[beam]) : -INFINITY;
+        total = key != 0 ? of.score[beam] + (static_cast<double>(key_value(key)) - of.lse[beam]) : -INFINITY;
         total = total < INFINITY ? total : -INFINITY;
-        return Candidate{order_total(total / norm_of[beam]), static_cast<unsigned>(beam) << 16 | static_cast<unsigned>(key_column(key) & 0xffff)};
+        return Candidate{order_total(total * of.weight[beam]), static_cast<unsigned>(beam) << 16 | static_cast<unsigned>(key_column(key) & 0xffff)};
     };
-    double total;
-    if (tid < lists) {
-        heads[tid] = candidate_at(tid, 0, total);
-    }
-    __syncthreads();
-    if (tid < lists && heads[tid].rank != 0) {
-        int larger = 0;
-        for (int other = 0; other < lists; ++other) {
-            larger += heads[other].above(heads[tid]) ? 1 : 0;
-        }
-        if (larger == p.beams - 1) {
-            bound = heads[tid];
+    Candidate mine[kHeldEntries], top = {0, ~0u};
+    double total[kHeldEntries];
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+        mine[i] = Candidate{0, ~0u};
+        if (tid + i * kThreads < entries) {
+            mine[i] = candidate_of(tid + i * kThreads, held[i], total[i]);
+            top = mine[i].above(top) ? mine[i] : top;
         }
     }
+    for (int i = tid + kHeldEntries * kThreads; i < entries; i += kThreads) {
+        double its;
+        const Candidate other = candidate_of(i, keys[i], its);
+        top = other.above(top) ? other : top;
+    }
+    const Candidate own_top = top;
+#pragma unroll
+    for (int off = 1; off < kThreads / kBins; off <<= 1) {
+        const Candidate other = {__shfl_xor_sync(fb::kFullMask, top.rank, off), __shfl_xor_sync(fb::kFullMask, top.place, off)};
+        top = other.above(top) ? other : top;
+    }
+    if (tid % (kThreads / kBins) == 0) {
+        bins[tid / (kThreads / kBins)] = top;
+    }
     __syncthreads();
-    for (int i = tid; i < lists * p.beams; i += kThreads) {
-        const int list = i / p.beams;
-        if (heads[list].rank == 0 || bound.above(heads[list])) {
-            continue;
+    // The beams-th largest of the bins' tops: a warp ranks its share of the bins.
+    const Candidate low = bins[lane], high = bins[lane + 32];
+#pragma unroll
+    for (int i = 0; i < kBins / kWarps; ++i) {
+        const Candidate bin = bins[warp * (kBins / kWarps) + i];
+        const int larger = __popc(__ballot_sync(fb::kFullMask, low.above(bin))) + __popc(__ballot_sync(fb::kFullMask, high.above(bin)));
+        if (larger == p.beams - 1 && bin.rank != 0 && lane == 0) {
+            bound = bin;
         }
-        const Candidate mine = candidate_at(list, i - list * p.beams, total);
-        if (mine.rank != 0 && !bound.above(mine)) {
-            const int at = atomicAdd(&left_count, 1);
-            left[at] = mine;
-            left_total[at] = total;
+    }
+    __syncthreads();
+    if (own_top.rank != 0 && !bound.above(own_top)) {
+        auto collect = [&](const Candidate& c, double its) {
+            if (c.rank != 0 && !bound.above(c)) {
+                const int at = atomicAdd(&left_count, 1);
+                left_rank[at] = c.rank;
+                left_place[at] = c.place;
+                left_total[at] = its;
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kHeldEntries; ++i) {
+            collect(mine[i], total[i]);
+        }
+        for (int i = tid + kHeldEntries * kThreads; i < entries; i += kThreads) {
+            double its;
+            const Candidate other = candidate_of(i, keys[i], its);
+            collect(other, its);
         }
     }
     __syncthreads();
     const int count = left_count;
     for (int i = tid; i < count; i += kThreads) {
+        const Candidate its = {left_rank[i], left_place[i]};
         int larger = 0;
+#pragma unroll 4
         for (int other = 0; other < count; ++other) {
-            larger += left[other].above(left[i]) ? 1 : 0;
+            larger += Candidate{left_rank[other], left_place[other]}.above(its) ? 1 : 0;
         }
         if (larger < p.beams) {
-            chosen[larger] = left[i].place;
+            chosen[larger] = its.place;
             chosen_total[larger] = left_total[i];
         }
     }
@@ -448,13 +535,14 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
     for (int t = warp; t < p.beams; t += kWarps) {
         const bool none = chosen[t] == ~0u;
         const int parent = none ? t : static_cast<int>(chosen[t] >> 16);
-        const bool over = over_of[parent] != 0;
+        const bool over = of.over[parent] != 0;
         const int token = none ? (over ? max(p.end_token, 0) : 0) : static_cast<int>(chosen[t] & 0xffffu);
-        int length = length_of[parent];
+        int length = of.length[parent];
         const long long row = first + t;
         if (p.next_histories != nullptr) {
             const uint16_t* from = p.histories + (first + parent) * p.history_stride;
             uint16_t* to = p.next_histories + row * p.history_stride;
+#pragma unroll 8
             for (int c = lane; c < length; c += 32) {
                 to[c] = from[c];
             }
@@ -479,29 +567,37 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
     }
 }
 
-// Parts of a row: as many as have room in a block's registers, and where rows are few as many as give two blocks to every
-// SM something to do, but each at least a word per thread.
-int parts_of(int words, size_t rows, int beams, int sms) {
-    const int least = (words + kThreads * kHeldWords - 1) / (kThreads * kHeldWords);
-    const size_t wanted = std::min<size_t>(2 * static_cast<size_t>(sms) / std::max<size_t>(rows, 1),
-                                           static_cast<size_t>((words + kThreads - 1) / kThreads));
-    return std::max(least, static_cast<int>(std::min<size_t>(wanted, static_cast<size_t>(kMostLists / beams))));
-}
+// Parts of a row: those with which the warps are done soonest, each part costing two chunks more than it has; never so many that
+// a group has more than kMostLists or kMostEntries, or the GPU more than kMostRounds parts per warp on their account.
+constexpr int kMostRounds = 8;
+unsigned warps_of(int sms) { return static_cast<unsigned>(sms * kBlocks * kWarps); }
 
-// Rows' parts are at most eight, or two per SM together.
-size_t most_lists(size_t rows, int sms) { return 8 * rows + 2 * static_cast<size_t>(sms); }
+int parts_of(int words, size_t rows, int beams, int sms) {
+    const unsigned warps = warps_of(sms);
+    const size_t most = std::min<size_t>(std::min(kMostLists / beams, kMostEntries / (beams * beams)),
+                                         kMostRounds * static_cast<size_t>(warps) / std::max<size_t>(rows, 1));
+    unsigned best = 1, least = ~0u;
+    for (unsigned parts = 1; parts == 1 || (parts <= most && words / parts >= 32); ++parts) {
+        const unsigned rounds = (static_cast<unsigned>(rows) * parts + warps - 1) / warps;
+        const unsigned chunks = ((words + parts - 1) / parts + kChunk - 1) / kChunk;
+        if (rounds * (chunks + 2) < least) {
+            best = parts;
+            least = rounds * (chunks + 2);
+        }
+    }
+    return static_cast<int>(best);
+}
+size_t most_lists(size_t rows, int sms) { return rows + kMostRounds * static_cast<size_t>(warps_of(sms)); }
+
 size_t stats_bytes(size_t lists) { return (lists * sizeof(float2) + 255) / 256 * 256; }
 
 template <typename T>
 cudaError_t launch_rows(RowArgs p, size_t rows, int sms, cudaStream_t stream) {
     const int words = (p.vocab + Row<T>::kValues - 1) / Row<T>::kValues;
-    p.parts = parts_of(words, rows, p.beams, sms);
     p.slice = (words + p.parts - 1) / p.parts;
-    p.items = static_cast<long long>(rows) * p.parts;
-    const bool few = p.slice <= 2 * kThreads;
-    const unsigned blocks = static_cast<unsigned>(std::min<long long>(p.items, (few ? 4LL : 3LL) * sms));
-    return fb::launch_dependent(few ? fb_beam_rows<T, 2> : fb_beam_rows<T, kHeldWords>, dim3(blocks), dim3(kThreads), 0,
-                                stream, p);
+    p.items = static_cast<unsigned>(rows * p.parts);
+    const size_t blocks = std::min<size_t>(p.items, static_cast<size_t>(kBlocks) * sms);
+    return fb::launch_dependent(fb_beam_rows<T>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
 }
 
 constexpr flint_status kBad = FLINT_ERROR_INVALID_ARGUMENT;
@@ -645,7 +741,7 @@ flint_status flint_b200_beam_select(void* next_scores, void* parents, void* toke
     g.history_stride = static_cast<long long>(history_stride);
     g.beams = p.beams;
     const int values = fp32_logits != 0 ? Row<float>::kValues : Row<__half>::kValues;
-    g.parts = parts_of((p.vocab + values - 1) / values, rows, p.beams, sms);
+    g.parts = p.parts = parts_of((p.vocab + values - 1) / values, rows, p.beams, sms);
     g.end_token = end_token;
     g.power = length_power;
     FB_CUDA(fp32_logits != 0 ? launch_rows<float>(p, rows, sms, stream) : launch_rows<__half>(p, rows, sms, stream));

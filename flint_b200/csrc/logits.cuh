@@ -25,6 +25,7 @@ struct MaxF {
         m = max_nan(m, max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)),
                                max_nan(__uint_as_float(q.z), __uint_as_float(q.w))));
     }
+    __device__ __forceinline__ void add(const MaxF& other) { m = max_nan(m, other.m); }
     __device__ __forceinline__ float value() const { return m; }
     __device__ static __forceinline__ float word(const uint4& q) {
         return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
@@ -36,6 +37,7 @@ struct MaxH {
         const __half2* h = reinterpret_cast<const __half2*>(&q);
         m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
     }
+    __device__ __forceinline__ void add(const MaxH& other) { m = __hmax2_nan(m, other.m); }
     __device__ __forceinline__ float value() const { return max_nan(__low2float(m), __high2float(m)); }
     __device__ static __forceinline__ float word(const uint4& q) {
         const __half2* h = reinterpret_cast<const __half2*>(&q);
