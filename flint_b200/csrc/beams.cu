@@ -81,19 +81,32 @@ struct LaneSum {
         }
         m = next;
     }
-    // (m is above minus infinity. The difference first, which is exact near m.)
-    template <int kValues>
-    __device__ __forceinline__ void add(const float (&v)[kValues]) {
-        const fb::F2 minus = fb::f2_pack(-m, -m), log2e = fb::f2_pack(kLog2e, kLog2e);
+    // (m is above minus infinity. The difference first, which is exact near m; from FP16 it is one instruction.)
+    __device__ __forceinline__ void add(const uint4& q, float) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int c = 0; c < kValues; c += 2) {
-            float y0, y1, e0, e1;
-            fb::f2_unpack(fb::f2_mul(fb::f2_add(fb::f2_pack(v[c], v[c + 1]), minus), log2e), y0, y1);
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
-            sum[c & 2] += e0;
-            sum[(c & 2) + 1] += e1;
+        for (int i = 0; i < 4; i += 2) {
+            pair(i, __uint_as_float(w[i]) - m, __uint_as_float(w[i + 1]) - m);
         }
+    }
+    __device__ __forceinline__ void add(const uint4& q, __half) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float d0, d1;
+            asm("{\n.reg .f16 lo, hi;\nmov.b32 {lo, hi}, %2;\nadd.rn.f32.f16 %0, lo, %3;\nadd.rn.f32.f16 %1, hi, %3;\n}"
+                : "=f"(d0), "=f"(d1)
+                : "r"(w[i]), "f"(-m));
+            pair(2 * i, d0, d1);
+        }
+    }
+    __device__ __forceinline__ void pair(int i, float d0, float d1) {
+        float y0, y1, e0, e1;
+        fb::f2_unpack(fb::f2_mul(fb::f2_pack(d0, d1), fb::f2_pack(kLog2e, kLog2e)), y0, y1);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
+        sum[i & 2] += e0;
+        sum[(i & 2) + 1] += e1;
     }
     __device__ __forceinline__ float total() const { return (sum[0] + sum[1]) + (sum[2] + sum[3]); }
 };
@@ -155,7 +168,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
     __shared__ Key lists[kWarps][kCandidates];
     __shared__ float group_max[kWarps][kGroups][32];
     const int lane = static_cast<int>(threadIdx.x) % 32, warp = __shfl_sync(fb::kFullMask, static_cast<int>(threadIdx.x) / 32, 0);
-    const int row_words = p.cols / R::kValues;
     const int all_words = (p.vocab + R::kValues - 1) / R::kValues;
     const int last_count = p.vocab - (all_words - 1) * R::kValues;
     Key* list = lists[warp];
@@ -172,7 +184,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
         }
         const int first = static_cast<int>(item - row * p.parts) * p.slice;
         const int words = max(0, min(p.slice, all_words - first));
-        const uint4* from = static_cast<const uint4*>(p.logits) + static_cast<size_t>(row) * row_words + first;
+        const char* values = static_cast<const char*>(p.logits) + static_cast<size_t>(row) * p.cols * sizeof(T);
+        const uint4* from = reinterpret_cast<const uint4*>(values) + first;
         // Word i of the part; minus infinity, which counts for nothing, behind its end.
         auto word_at = [&](int i) {
             uint4 q = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
@@ -217,15 +230,27 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
                 if (!(mx <= sum.m)) {       // (a NaN stays)
                     sum.raise(mx);
                 }
-                const bool adds = sum.m != -INFINITY;
+                uint4 next[kHeld];
+                if ((c + 2) * kChunk <= words) {
+#pragma unroll
+                    for (int j = 0; j < kHeld; ++j) {
+                        next[j] = from[at + kChunk + 32 * j];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kHeld; ++j) {
+                        next[j] = word_at(at + kChunk + 32 * j);
+                    }
+                }
+                if (sum.m != -INFINITY) {
+#pragma unroll
+                    for (int j = 0; j < kHeld; ++j) {
+                        sum.add(held[j], T());
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < kHeld; ++j) {
-                    float v[R::kValues];
-                    R::unpack(v, held[j]);
-                    held[j] = word_at(at + kChunk + 32 * j);
-                    if (adds) {
-                        sum.add(v);
-                    }
+                    held[j] = next[j];
                 }
             }
             const float mx = running.value();
@@ -261,25 +286,35 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
         while (__any_sync(fb::kFullMask, mask != 0)) {
             const int g = __ffs(mask) - 1;
             mask &= mask - 1;
-            for (int i = g * of_group * kChunk + lane, end = i + of_group * kChunk; i < end; i += 32) {
-                uint4 q = word_at(g >= 0 ? i : words);
-                cut(q, i);
-                float v[R::kValues];
-                R::unpack(v, q);
+            for (int of = 0; of < of_group; ++of) {
+                const int at = (g * of_group + of) * kChunk + lane;
+                unsigned those = 0;      // of this lane's values, that reach the bound
 #pragma unroll
-                for (int c = 0; c < R::kValues; ++c) {
-                    const bool reaches = v[c] >= bound && v[c] > -INFINITY;
-                    const unsigned those = __ballot_sync(fb::kFullMask, reaches);
-                    if (those != 0 && !overflow) {
-                        if (reaches) {
-                            list[count + __popc(those & ((1u << lane) - 1))] = order_key(v[c], (first + i) * R::kValues + c);
-                        }
-                        count += __popc(those);
-                        if (count > kMany) {
-                            __syncwarp();
-                            count = keep_largest(list, count, p.beams, bound, lane);
-                            overflow = count > kMany;
-                        }
+                for (int j = 0; j < kHeld; ++j) {
+                    uint4 q = word_at(g >= 0 ? at + 32 * j : words);
+                    cut(q, at + 32 * j);
+                    float v[R::kValues];
+                    R::unpack(v, q);
+#pragma unroll
+                    for (int c = 0; c < R::kValues; ++c) {
+                        those |= v[c] >= bound && v[c] > -INFINITY ? 1u << (j * R::kValues + c) : 0u;
+                    }
+                }
+                while (!overflow && __any_sync(fb::kFullMask, those != 0)) {
+                    const int k = __ffs(those) - 1;
+                    const int column = (first + at + 32 * (k / R::kValues)) * R::kValues + k % R::kValues;
+                    const float v = k >= 0 ? R::value(values, column) : -INFINITY;
+                    const bool reaches = k >= 0 && v >= bound;      // (which may have risen)
+                    const unsigned lanes = __ballot_sync(fb::kFullMask, reaches);
+                    those &= those - 1;
+                    if (reaches) {
+                        list[count + __popc(lanes & ((1u << lane) - 1))] = order_key(v, column);
+                    }
+                    count += __popc(lanes);
+                    if (count > kMany) {
+                        __syncwarp();
+                        count = keep_largest(list, count, p.beams, bound, lane);
+                        overflow = count > kMany;
                     }
                 }
             }
@@ -303,7 +338,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
             }
         } else {
             // Many equal ones: the part is gone through once for every place.
-            const char* values = static_cast<const char*>(p.logits) + static_cast<size_t>(row) * p.cols * sizeof(T);
             const int begin = first * R::kValues, end = min((first + words) * R::kValues, p.vocab);
             Key before = ~Key{0};
             for (int k = 0; k < p.beams; ++k) {
@@ -419,32 +453,30 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
         bound = Candidate{1, ~0u};      // anything that is a continuation
     }
     __syncthreads();
+    // Four lanes take a beam's log-sum-exp, and a warp the weights of lengths meanwhile.
+    constexpr int kLanes = 4;
+    const int beam = tid / kLanes;
     if (warp == kWarps - 1) {
         if (lane < p.beams) {
             const double grown = of.over[lane] != 0 ? max(of.length[lane], 1) : static_cast<double>(of.length[lane]) + 1.0;
             of.weight[lane] = p.power == 0.0f ? 1.0 : 1.0 / pow(grown, static_cast<double>(p.power));
         }
-    } else {
-        for (int beam = warp; beam < p.beams; beam += kWarps - 1) {
-            float m = -INFINITY, sum = 0.0f;
-            for (int i = lane; i < p.parts; i += 32) {
-                m = max_nan(m, stats[beam * p.parts + i].x);
-            }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) {
-                m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, off));
-            }
-            for (int i = lane; i < p.parts; i += 32) {
-                const float2 part = stats[beam * p.parts + i];
-                sum += part.x == -INFINITY ? 0.0f : part.y * expf(part.x - m);
-            }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) {
-                sum += __shfl_xor_sync(fb::kFullMask, sum, off);
-            }
-            if (lane == 0) {
-                of.lse[beam] = static_cast<double>(m) + log(static_cast<double>(sum));
-            }
+    } else if (warp < kMostBeams * kLanes / 32) {
+        float m = -INFINITY, sum = 0.0f;
+        const int its = min(beam, p.beams - 1) * p.parts;
+        for (int i = tid % kLanes; i < p.parts; i += kLanes) {
+            m = max_nan(m, stats[its + i].x);
+        }
+        m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, 1));
+        m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, 2));
+        for (int i = tid % kLanes; i < p.parts; i += kLanes) {
+            const float2 part = stats[its + i];
+            sum += part.x == -INFINITY ? 0.0f : part.y * expf(part.x - m);
+        }
+        sum += __shfl_xor_sync(fb::kFullMask, sum, 1);
+        sum += __shfl_xor_sync(fb::kFullMask, sum, 2);
+        if (tid % kLanes == 0 && beam < p.beams) {
+            of.lse[beam] = static_cast<double>(m) + log(static_cast<double>(sum));
         }
     }
     __syncthreads();
