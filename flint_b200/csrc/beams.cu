@@ -167,17 +167,31 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
     using R = Row<T>;
     __shared__ Key lists[kWarps][kCandidates];
     __shared__ float group_max[kWarps][kGroups][32];
+    __shared__ int claimed;
     const int lane = static_cast<int>(threadIdx.x) % 32, warp = __shfl_sync(fb::kFullMask, static_cast<int>(threadIdx.x) / 32, 0);
     const int all_words = (p.vocab + R::kValues - 1) / R::kValues;
     const int last_count = p.vocab - (all_words - 1) * R::kValues;
     Key* list = lists[warp];
     // Chunks whose words make up a group, and the chunks in a part.
     const int chunks = (p.slice + kChunk - 1) / kChunk, of_group = (chunks + kGroups - 1) / kGroups;
+    if (threadIdx.x == 0) {
+        claimed = 0;
+    }
     fb::dependency_wait();
     fb::dependency_release();
-    const unsigned warps = gridDim.x * kWarps;
-    // (Neighbouring parts go to different SMs, so that a short list does not fill a few of them.)
-    for (unsigned item = warp * gridDim.x + blockIdx.x; item < p.items; item += warps) {
+    __syncthreads();
+    // A block's warps take its parts as they come to them (finished beams have nothing to read); neighbouring parts go to
+    // different SMs.
+    for (;;) {
+        int turn = 0;
+        if (lane == 0) {
+            turn = atomicAdd(&claimed, 1);
+        }
+        turn = __shfl_sync(fb::kFullMask, turn, 0);
+        const unsigned item = static_cast<unsigned>(turn) * gridDim.x + blockIdx.x;
+        if (item >= p.items) {
+            break;
+        }
         const unsigned row = item / static_cast<unsigned>(p.parts);
         if (p.finished != nullptr && p.finished[row] != 0) {
             continue;
@@ -391,9 +405,13 @@ __device__ __forceinline__ Key order_total(double v) {
 }
 
 constexpr int kBins = 64;
-constexpr int kHeldEntries = 4;      // of a group's lists, that a thread holds
-constexpr int kMostEntries = 4096;   // of them all: 64 in each bin, and the bound leaves entries of kMostBeams bins
-constexpr int kLeft = kMostBeams * (kMostEntries / kBins);
+constexpr int kMostEntries = 4096;   // of a group's lists
+constexpr int kFewEntries = 512;
+
+// The bound leaves entries of at most `beams` bins, each with those of its threads.
+__host__ __device__ constexpr int most_left(int entries, int beams) {
+    return beams * (kThreads / kBins) * ((entries + kThreads - 1) / kThreads);
+}
 
 struct Candidate {
     Key rank;
@@ -409,14 +427,14 @@ struct Beams {
     int over[kMostBeams], length[kMostBeams];
 };
 
-__global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
+// kHeldEntries: of a group's lists, per thread.
+template <int kHeldEntries>
+__global__ void __launch_bounds__(kThreads, kHeldEntries > 2 ? 2 : 5) fb_beam_groups(const GroupArgs p) {
+    extern __shared__ __align__(16) unsigned char left_memory[];
     __shared__ Beams of;
     __shared__ float2 stats[kMostLists];
     __shared__ Candidate bins[kBins];
     __shared__ Candidate bound;
-    __shared__ Key left_rank[kLeft];
-    __shared__ unsigned left_place[kLeft];
-    __shared__ double left_total[kLeft];
     __shared__ int left_count;
     __shared__ unsigned chosen[kMostBeams];
     __shared__ double chosen_total[kMostBeams];
@@ -424,7 +442,11 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
     fb::dependency_wait();
     fb::dependency_release();
     const long long first = static_cast<long long>(blockIdx.x) * p.beams;
-    const int lists = p.beams * p.parts, entries = lists * p.beams;
+    const int lists = p.beams * p.parts, entries = lists * p.beams, of_beam = p.parts * p.beams;
+    const int most = most_left(entries, p.beams);
+    Key* left_rank = reinterpret_cast<Key*>(left_memory);
+    double* left_total = reinterpret_cast<double*>(left_rank + most);
+    unsigned* left_place = reinterpret_cast<unsigned*>(left_total + most);
     const Key* keys = p.best + first * p.parts * p.beams;
     Key held[kHeldEntries];       // this thread's first entries
 #pragma unroll
@@ -480,33 +502,31 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
         }
     }
     __syncthreads();
-    // Entry i, of list i / beams.
+    // Entry i, of beam i / of_beam.
     auto candidate_of = [&](int i, Key key, double& total) {
-        const int list = i / p.beams, beam = list / p.parts;
-        if (of.over[beam] != 0) {
+        const int its = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(of_beam));
+        const unsigned high = static_cast<unsigned>(its) << 16;
+        if (of.over[its] != 0) {
             // (A finished beam's row was not read; it has one continuation.)
-            total = i == beam * p.parts * p.beams ? of.score[beam] : -INFINITY;
-            return Candidate{order_total(total * of.weight[beam]), static_cast<unsigned>(beam) << 16 | static_cast<unsigned>(max(p.end_token, 0))};
+            total = i == its * of_beam ? of.score[its] : -INFINITY;
+            return Candidate{order_total(total * of.weight[its]), high | static_cast<unsigned>(max(p.end_token, 0))};
         }
         // (An lse that is not a number, or minus infinity, gives none.)
-        total = key != 0 ? of.score[beam] + (static_cast<double>(key_value(key)) - of.lse[beam]) : -INFINITY;
+        total = key != 0 ? of.score[its] + (static_cast<double>(key_value(key)) - of.lse[its]) : -INFINITY;
         total = total < INFINITY ? total : -INFINITY;
-        return Candidate{order_total(total * of.weight[beam]), static_cast<unsigned>(beam) << 16 | static_cast<unsigned>(key_column(key) & 0xffff)};
+        return Candidate{order_total(total * of.weight[its]), high | static_cast<unsigned>(key_column(key) & 0xffff)};
     };
-    Candidate mine[kHeldEntries], top = {0, ~0u};
-    double total[kHeldEntries];
+    Candidate top = {0, ~0u};
+    Key ranks[kHeldEntries];
 #pragma unroll
     for (int i = 0; i < kHeldEntries; ++i) {
-        mine[i] = Candidate{0, ~0u};
+        ranks[i] = 0;
         if (tid + i * kThreads < entries) {
-            mine[i] = candidate_of(tid + i * kThreads, held[i], total[i]);
-            top = mine[i].above(top) ? mine[i] : top;
+            double total;
+            const Candidate mine = candidate_of(tid + i * kThreads, held[i], total);
+            ranks[i] = mine.rank;
+            top = mine.above(top) ? mine : top;
         }
-    }
-    for (int i = tid + kHeldEntries * kThreads; i < entries; i += kThreads) {
-        double its;
-        const Candidate other = candidate_of(i, keys[i], its);
-        top = other.above(top) ? other : top;
     }
     const Candidate own_top = top;
 #pragma unroll
@@ -530,22 +550,18 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
     }
     __syncthreads();
     if (own_top.rank != 0 && !bound.above(own_top)) {
-        auto collect = [&](const Candidate& c, double its) {
-            if (c.rank != 0 && !bound.above(c)) {
-                const int at = atomicAdd(&left_count, 1);
-                left_rank[at] = c.rank;
-                left_place[at] = c.place;
-                left_total[at] = its;
-            }
-        };
 #pragma unroll
         for (int i = 0; i < kHeldEntries; ++i) {
-            collect(mine[i], total[i]);
-        }
-        for (int i = tid + kHeldEntries * kThreads; i < entries; i += kThreads) {
-            double its;
-            const Candidate other = candidate_of(i, keys[i], its);
-            collect(other, its);
+            if (ranks[i] != 0 && ranks[i] >= bound.rank) {
+                double total;
+                const Candidate mine = candidate_of(tid + i * kThreads, held[i], total);
+                if (!bound.above(mine)) {
+                    const int at = atomicAdd(&left_count, 1);
+                    left_rank[at] = mine.rank;
+                    left_place[at] = mine.place;
+                    left_total[at] = total;
+                }
+            }
         }
     }
     __syncthreads();
@@ -599,7 +615,7 @@ __global__ void __launch_bounds__(kThreads) fb_beam_groups(const GroupArgs p) {
     }
 }
 
-// Parts of a row: those with which the warps are done soonest, each part costing two chunks more than it has; never so many that
+// Parts of a row: those with which the warps are done soonest, each part costing four chunks more than it has; never so many that
 // a group has more than kMostLists or kMostEntries, or the GPU more than kMostRounds parts per warp on their account.
 constexpr int kMostRounds = 8;
 unsigned warps_of(int sms) { return static_cast<unsigned>(sms * kBlocks * kWarps); }
@@ -608,13 +624,16 @@ int parts_of(int words, size_t rows, int beams, int sms) {
     const unsigned warps = warps_of(sms);
     const size_t most = std::min<size_t>(std::min(kMostLists / beams, kMostEntries / (beams * beams)),
                                          kMostRounds * static_cast<size_t>(warps) / std::max<size_t>(rows, 1));
-    unsigned best = 1, least = ~0u;
+    unsigned best = 1;
+    float least = 0.0f;
     for (unsigned parts = 1; parts == 1 || (parts <= most && words / parts >= 32); ++parts) {
-        const unsigned rounds = (static_cast<unsigned>(rows) * parts + warps - 1) / warps;
+        // (A block's warps are done at about the same time, half a part apart.)
+        const float items = static_cast<float>(rows) * parts / static_cast<float>(warps);
         const unsigned chunks = ((words + parts - 1) / parts + kChunk - 1) / kChunk;
-        if (rounds * (chunks + 2) < least) {
+        const float cost = (items <= 1.0f ? 1.0f : items + 0.5f) * static_cast<float>(chunks + 4);
+        if (parts == 1 || cost < least) {
             best = parts;
-            least = rounds * (chunks + 2);
+            least = cost;
         }
     }
     return static_cast<int>(best);
@@ -777,7 +796,14 @@ flint_status flint_b200_beam_select(void* next_scores, void* parents, void* toke
     g.end_token = end_token;
     g.power = length_power;
     FB_CUDA(fp32_logits != 0 ? launch_rows<float>(p, rows, sms, stream) : launch_rows<__half>(p, rows, sms, stream));
-    FB_CUDA(fb::launch_dependent(fb_beam_groups, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream, g));
+    const int entries = p.parts * p.beams * p.beams;
+    const size_t smem = static_cast<size_t>(most_left(entries, p.beams)) * (sizeof(Key) + sizeof(double) + sizeof(unsigned));
+    const bool few = entries <= kFewEntries;
+    static std::atomic<bool> configured[2][64] = {};
+    const auto kernel = few ? fb_beam_groups<kFewEntries / kThreads> : fb_beam_groups<kMostEntries / kThreads>;
+    constexpr int kMostSmem = most_left(kMostEntries, kMostBeams) * (sizeof(Key) + sizeof(double) + sizeof(unsigned));
+    FB_CUDA(fb::allow_shared_memory(kernel, kMostSmem, configured[few ? 1 : 0]));
+    FB_CUDA(fb::launch_dependent(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), smem, stream, g));
     return FLINT_OK;
 }
 
