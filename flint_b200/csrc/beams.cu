@@ -27,8 +27,12 @@ namespace {
 constexpr int kMostBeams = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kHeld = 4;             // 16-byte words that a lane has on their way
-constexpr int kBlocks = 4;           // per SM
+#ifndef VHELD
+#define VHELD 4
+#define VBLOCKS 4
+#endif
+constexpr int kHeld = VHELD;             // 16-byte words that a lane has on their way
+constexpr int kBlocks = VBLOCKS;           // per SM
 constexpr int kChunk = 32 * kHeld;   // words that a warp works on at a time
 constexpr int kCandidates = 128;     // of a warp
 constexpr int kMany = 96;            // from which on the bound rises
@@ -70,18 +74,19 @@ struct Row<__half> {
     __device__ static __forceinline__ void unpack(float (&v)[8], const uint4& q) { fb::unpack8(v, q); }
 };
 
-// A lane's sum of e^(x - m) against its running maximum m.
+// A lane's sum of e^(x - m) against its running maximum m. It begins at the lowest number, so that minus infinity adds nothing.
+// The difference comes first, which is exact near m; from FP16 it is one instruction.
+constexpr float kLowest = -3.402823466e38f;
 struct LaneSum {
-    float m = -INFINITY, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kLowest, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     __device__ __forceinline__ void raise(float next) {
-        const float factor = m == -INFINITY ? 0.0f : exp2f((m - next) * kLog2e);
+        const float factor = exp2f((m - next) * kLog2e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             sum[i] *= factor;
         }
         m = next;
     }
-    // (m is above minus infinity. The difference first, which is exact near m; from FP16 it is one instruction.)
     __device__ __forceinline__ void add(const uint4& q, float) {
         const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -244,27 +249,18 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
                 if (!(mx <= sum.m)) {       // (a NaN stays)
                     sum.raise(mx);
                 }
-                uint4 next[kHeld];
                 if ((c + 2) * kChunk <= words) {
 #pragma unroll
                     for (int j = 0; j < kHeld; ++j) {
-                        next[j] = from[at + kChunk + 32 * j];
+                        sum.add(held[j], T());
+                        held[j] = from[at + kChunk + 32 * j];
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < kHeld; ++j) {
-                        next[j] = word_at(at + kChunk + 32 * j);
-                    }
-                }
-                if (sum.m != -INFINITY) {
-#pragma unroll
-                    for (int j = 0; j < kHeld; ++j) {
                         sum.add(held[j], T());
+                        held[j] = word_at(at + kChunk + 32 * j);
                     }
-                }
-#pragma unroll
-                for (int j = 0; j < kHeld; ++j) {
-                    held[j] = next[j];
                 }
             }
             const float mx = running.value();
@@ -277,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
         for (int off = 16; off > 0; off >>= 1) {
             m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, off));
         }
-        float total = sum.m == -INFINITY ? 0.0f : sum.total() * exp2f((sum.m - m) * kLog2e);
+        float total = sum.total() * exp2f((sum.m - m) * kLog2e);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
             total += __shfl_xor_sync(fb::kFullMask, total, off);
@@ -406,7 +402,7 @@ __device__ __forceinline__ Key order_total(double v) {
 
 constexpr int kBins = 64;
 constexpr int kMostEntries = 4096;   // of a group's lists
-constexpr int kFewEntries = 512;
+constexpr int kFewEntries = 512, kSomeEntries = 1024;
 
 // The bound leaves entries of at most `beams` bins, each with those of its threads.
 __host__ __device__ constexpr int most_left(int entries, int beams) {
@@ -421,6 +417,38 @@ struct Candidate {
     }
 };
 
+// log x to about 2^-25 absolute, the accuracy of a sum of FP32 exponentials: x = 2^e f with f from 3/4 to 3/2, whose logarithm
+// is at most 0.41. (FP64's own takes microseconds for what is one number per beam.)
+__device__ __forceinline__ double log_of(float x) {
+    if (!(x > 0.0f && x < INFINITY)) {
+        return logf(x);
+    }
+    const int e = ((__float_as_int(x) - 0x3f400000) >> 23);
+    const float f = __int_as_float(__float_as_int(x) - (e << 23));
+    return e * 0.69314718055994531 + static_cast<double>(log1pf(f - 1.0f));
+}
+
+// n^-power to about 2^-40, from log n = e log 2 + 2 artanh((f - 1) / (f + 1)) with f from 3/4 to 3/2, and the exponential's series.
+// (Weights that were off by FP32's roundings would move totals past each other; FP64's own power takes 5 us.)
+__device__ __forceinline__ double weight_of(double n, double power) {
+    const long long bits = __double_as_longlong(n);
+    const int e = static_cast<int>((bits - 0x3fe8000000000000LL) >> 52);
+    const double f = __longlong_as_double(bits - (static_cast<long long>(e) << 52));
+    double r = 1.0f / (static_cast<float>(f) + 1.0f);
+    r = r * (2.0 - (f + 1.0) * r);
+    const double s = (f - 1.0) * r, z = s * s, z2 = z * z;
+    const double tail = (1.0 / 3 + z * (1.0 / 5)) + z2 * ((1.0 / 7 + z * (1.0 / 9)) + z2 * (1.0 / 11 + z * (1.0 / 13)));
+    const double y = -power * (e * 0.69314718055994531 + 2.0 * s * (1.0 + z * tail));
+    if (!(y > -600.0)) {
+        return pow(n, -power);
+    }
+    const int k = __double2int_rn(y * 1.4426950408889634);
+    const double x = y - k * 0.69314718055994531, x2 = x * x, x4 = x2 * x2;
+    const double series = (1.0 + x) + x2 * (1.0 / 2 + x * (1.0 / 6)) +
+                          x4 * ((1.0 / 24 + x * (1.0 / 120)) + x2 * (1.0 / 720 + x * (1.0 / 5040)) + x4 * (1.0 / 40320 + x * (1.0 / 362880)));
+    return series * __longlong_as_double(static_cast<long long>(1023 + k) << 52);
+}
+
 // What is known of a group's beams.
 struct Beams {
     double score[kMostBeams], lse[kMostBeams], weight[kMostBeams];     // weight: length^-power
@@ -429,7 +457,7 @@ struct Beams {
 
 // kHeldEntries: of a group's lists, per thread.
 template <int kHeldEntries>
-__global__ void __launch_bounds__(kThreads, kHeldEntries > 2 ? 2 : 5) fb_beam_groups(const GroupArgs p) {
+__global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_groups(const GroupArgs p) {
     extern __shared__ __align__(16) unsigned char left_memory[];
     __shared__ Beams of;
     __shared__ float2 stats[kMostLists];
@@ -481,10 +509,10 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 2 ? 2 : 5) fb_beam_gr
     if (warp == kWarps - 1) {
         if (lane < p.beams) {
             const double grown = of.over[lane] != 0 ? max(of.length[lane], 1) : static_cast<double>(of.length[lane]) + 1.0;
-            of.weight[lane] = p.power == 0.0f ? 1.0 : 1.0 / pow(grown, static_cast<double>(p.power));
+            of.weight[lane] = p.power == 0.0f ? 1.0 : weight_of(grown, static_cast<double>(p.power));
         }
     } else if (warp < kMostBeams * kLanes / 32) {
-        float m = -INFINITY, sum = 0.0f;
+        float m = kLowest, sum = 0.0f;
         const int its = min(beam, p.beams - 1) * p.parts;
         for (int i = tid % kLanes; i < p.parts; i += kLanes) {
             m = max_nan(m, stats[its + i].x);
@@ -493,12 +521,12 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 2 ? 2 : 5) fb_beam_gr
         m = max_nan(m, __shfl_xor_sync(fb::kFullMask, m, 2));
         for (int i = tid % kLanes; i < p.parts; i += kLanes) {
             const float2 part = stats[its + i];
-            sum += part.x == -INFINITY ? 0.0f : part.y * expf(part.x - m);
+            sum += part.y * expf(part.x - m);
         }
         sum += __shfl_xor_sync(fb::kFullMask, sum, 1);
         sum += __shfl_xor_sync(fb::kFullMask, sum, 2);
         if (tid % kLanes == 0 && beam < p.beams) {
-            of.lse[beam] = static_cast<double>(m) + log(static_cast<double>(sum));
+            of.lse[beam] = static_cast<double>(m) + log_of(sum);
         }
     }
     __syncthreads();
@@ -566,14 +594,17 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 2 ? 2 : 5) fb_beam_gr
     }
     __syncthreads();
     const int count = left_count;
-    for (int i = tid; i < count; i += kThreads) {
+    for (int i = tid / kLanes; i < count; i += kThreads / kLanes) {
         const Candidate its = {left_rank[i], left_place[i]};
         int larger = 0;
 #pragma unroll 4
-        for (int other = 0; other < count; ++other) {
+        for (int other = tid % kLanes; other < count; other += kLanes) {
             larger += Candidate{left_rank[other], left_place[other]}.above(its) ? 1 : 0;
         }
-        if (larger < p.beams) {
+        const unsigned four = 0xfu << (lane / kLanes * kLanes);
+        larger += __shfl_xor_sync(four, larger, 1);
+        larger += __shfl_xor_sync(four, larger, 2);
+        if (larger < p.beams && tid % kLanes == 0) {
             chosen[larger] = its.place;
             chosen_total[larger] = left_total[i];
         }
@@ -798,11 +829,13 @@ flint_status flint_b200_beam_select(void* next_scores, void* parents, void* toke
     FB_CUDA(fp32_logits != 0 ? launch_rows<float>(p, rows, sms, stream) : launch_rows<__half>(p, rows, sms, stream));
     const int entries = p.parts * p.beams * p.beams;
     const size_t smem = static_cast<size_t>(most_left(entries, p.beams)) * (sizeof(Key) + sizeof(double) + sizeof(unsigned));
-    const bool few = entries <= kFewEntries;
-    static std::atomic<bool> configured[2][64] = {};
-    const auto kernel = few ? fb_beam_groups<kFewEntries / kThreads> : fb_beam_groups<kMostEntries / kThreads>;
+    const int form = entries <= kFewEntries ? 0 : entries <= kSomeEntries ? 1 : 2;
+    static std::atomic<bool> configured[3][64] = {};
+    const auto kernel = form == 0   ? fb_beam_groups<kFewEntries / kThreads>
+                        : form == 1 ? fb_beam_groups<kSomeEntries / kThreads>
+                                    : fb_beam_groups<kMostEntries / kThreads>;
     constexpr int kMostSmem = most_left(kMostEntries, kMostBeams) * (sizeof(Key) + sizeof(double) + sizeof(unsigned));
-    FB_CUDA(fb::allow_shared_memory(kernel, kMostSmem, configured[few ? 1 : 0]));
+    FB_CUDA(fb::allow_shared_memory(kernel, kMostSmem, configured[form]));
     FB_CUDA(fb::launch_dependent(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), smem, stream, g));
     return FLINT_OK;
 }
