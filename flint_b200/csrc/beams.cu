@@ -27,12 +27,8 @@ namespace {
 constexpr int kMostBeams = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-#ifndef VHELD
-#define VHELD 4
-#define VBLOCKS 4
-#endif
-constexpr int kHeld = VHELD;             // 16-byte words that a lane has on their way
-constexpr int kBlocks = VBLOCKS;           // per SM
+constexpr int kHeld = 4;             // 16-byte words that a lane has on their way
+constexpr int kBlocks = 4;           // per SM
 constexpr int kChunk = 32 * kHeld;   // words that a warp works on at a time
 constexpr int kCandidates = 128;     // of a warp
 constexpr int kMany = 96;            // from which on the bound rises
@@ -57,34 +53,50 @@ struct Row;
 template <>
 struct Row<float> {
     static constexpr int kValues = 4;
+    static constexpr float kLowestValue = -3.402823466e38f;
     __device__ static __forceinline__ float value(const void* row, int c) { return static_cast<const float*>(row)[c]; }
-    __device__ static __forceinline__ void unpack(float (&v)[4], const uint4& q) {
-        v[0] = __uint_as_float(q.x);
-        v[1] = __uint_as_float(q.y);
-        v[2] = __uint_as_float(q.z);
-        v[3] = __uint_as_float(q.w);
+    // A bit for each of a word's values that is not below the bound.
+    __device__ static __forceinline__ unsigned reaching(const uint4& q, float bound) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+        unsigned those = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            those |= __uint_as_float(w[c]) >= bound ? 1u << c : 0u;
+        }
+        return those;
     }
 };
 template <>
 struct Row<__half> {
     static constexpr int kValues = 8;
+    static constexpr float kLowestValue = -65504.0f;
     __device__ static __forceinline__ float value(const void* row, int c) {
         return __half2float(static_cast<const __half*>(row)[c]);
     }
-    __device__ static __forceinline__ void unpack(float (&v)[8], const uint4& q) { fb::unpack8(v, q); }
+    // (The bound has no more bits than an FP16 number.)
+    __device__ static __forceinline__ unsigned reaching(const uint4& q, float bound) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+        const __half2 both = __float2half2_rn(bound);
+        unsigned those = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            those |= __hge2_mask(*reinterpret_cast<const __half2*>(&w[c]), both) & (0x20001u << (2 * c));
+        }
+        // Bits 2 c and 2 c + 17: the upper halves' go beside the lower ones'.
+        return (those & 0xffffu) | (those >> 16);
+    }
 };
 
 // A lane's sum of e^(x - m) against its running maximum m. It begins at the lowest number, so that minus infinity adds nothing.
 // The difference comes first, which is exact near m; from FP16 it is one instruction.
 constexpr float kLowest = -3.402823466e38f;
 struct LaneSum {
-    float m = kLowest, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kLowest;
+    fb::F2 sum[2] = {0, 0};
     __device__ __forceinline__ void raise(float next) {
         const float factor = exp2f((m - next) * kLog2e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sum[i] *= factor;
-        }
+        sum[0] = fb::f2_mul(sum[0], fb::f2_pack(factor, factor));
+        sum[1] = fb::f2_mul(sum[1], fb::f2_pack(factor, factor));
         m = next;
     }
     __device__ __forceinline__ void add(const uint4& q, float) {
@@ -110,10 +122,13 @@ struct LaneSum {
         fb::f2_unpack(fb::f2_mul(fb::f2_pack(d0, d1), fb::f2_pack(kLog2e, kLog2e)), y0, y1);
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(y0));
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(y1));
-        sum[i & 2] += e0;
-        sum[(i & 2) + 1] += e1;
+        sum[i / 2 & 1] = fb::f2_add(sum[i / 2 & 1], fb::f2_pack(e0, e1));
     }
-    __device__ __forceinline__ float total() const { return (sum[0] + sum[1]) + (sum[2] + sum[3]); }
+    __device__ __forceinline__ float total() const {
+        float a, b;
+        fb::f2_unpack(fb::f2_add(sum[0], sum[1]), a, b);
+        return a + b;
+    }
 };
 
 __device__ __forceinline__ unsigned upper(Key key) { return static_cast<unsigned>(key >> 32); }
@@ -187,45 +202,55 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
     __syncthreads();
     // A block's warps take its parts as they come to them (finished beams have nothing to read); neighbouring parts go to
     // different SMs.
-    for (;;) {
-        int turn = 0;
-        if (lane == 0) {
-            turn = atomicAdd(&claimed, 1);
-        }
-        turn = __shfl_sync(fb::kFullMask, turn, 0);
-        const unsigned item = static_cast<unsigned>(turn) * gridDim.x + blockIdx.x;
-        if (item >= p.items) {
-            break;
-        }
-        const unsigned row = item / static_cast<unsigned>(p.parts);
-        if (p.finished != nullptr && p.finished[row] != 0) {
-            continue;
-        }
-        const int first = static_cast<int>(item - row * p.parts) * p.slice;
-        const int words = max(0, min(p.slice, all_words - first));
-        const char* values = static_cast<const char*>(p.logits) + static_cast<size_t>(row) * p.cols * sizeof(T);
-        const uint4* from = reinterpret_cast<const uint4*>(values) + first;
-        // Word i of the part; minus infinity, which counts for nothing, behind its end.
-        auto word_at = [&](int i) {
-            uint4 q = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
-            if (sizeof(T) == 4) {
-                q = make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+    struct Part {
+        unsigned item;           // p.items: there is none
+        int first, words;        // its first word's place in the row, and how many
+        const char* values;      // of the row
+    };
+    auto claim = [&]() {
+        for (;;) {
+            int turn = 0;
+            if (lane == 0) {
+                turn = atomicAdd(&claimed, 1);
             }
-            if (i < words) {
-                q = from[i];
+            turn = __shfl_sync(fb::kFullMask, turn, 0);
+            const unsigned item = static_cast<unsigned>(turn) * gridDim.x + blockIdx.x;
+            if (item >= p.items) {
+                return Part{p.items, 0, 0, nullptr};
             }
-            return q;
-        };
+            const unsigned row = item / static_cast<unsigned>(p.parts);
+            if (p.finished == nullptr || p.finished[row] == 0) {
+                const int first = static_cast<int>(item - row * p.parts) * p.slice;
+                return Part{item, first, max(0, min(p.slice, all_words - first)),
+                            static_cast<const char*>(p.logits) + static_cast<size_t>(row) * p.cols * sizeof(T)};
+            }
+        }
+    };
+    // Word i of a part; minus infinity, which counts for nothing, behind its end.
+    auto word_at = [&](const Part& part, int i) {
+        uint4 q = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+        if (sizeof(T) == 4) {
+            q = make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+        }
+        if (i < part.words) {
+            q = reinterpret_cast<const uint4*>(part.values)[part.first + i];
+        }
+        return q;
+    };
+    uint4 held[kHeld];
+    Part part = claim();
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        held[j] = word_at(part, lane + 32 * j);
+    }
+    while (part.item < p.items) {
+        const int first = part.first, words = part.words;
+        const uint4* from = reinterpret_cast<const uint4*>(part.values) + first;
         auto cut = [&](uint4& q, int i) {
             if (first + i == all_words - 1) {
                 cut_word(q, last_count, T());
             }
         };
-        uint4 held[kHeld];
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            held[j] = word_at(lane + 32 * j);
-        }
         LaneSum sum;
         float best_group = -INFINITY, second_group = -INFINITY;
         int group = 0;
@@ -259,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
 #pragma unroll
                     for (int j = 0; j < kHeld; ++j) {
                         sum.add(held[j], T());
-                        held[j] = word_at(at + kChunk + 32 * j);
+                        held[j] = word_at(part, at + kChunk + 32 * j);
                     }
                 }
             }
@@ -267,6 +292,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
             group_max[warp][group++][lane] = mx;
             second_group = fmaxf(second_group, fminf(best_group, mx));
             best_group = fmaxf(best_group, mx);
+        }
+        // The next part's first words come while this one's largest are sought.
+        const Part next = claim();
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            held[j] = word_at(next, lane + 32 * j);
         }
         float m = sum.m;
 #pragma unroll
@@ -280,16 +311,16 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
         }
         if (lane == 0) {
             // (A part of nothing but minus infinity adds nothing, one with a NaN or plus infinity makes the row NaN.)
-            p.stats[item] = make_float2(m, total);
+            p.stats[part.item] = make_float2(m, total);
         }
-        // 20 bits are sign, exponent and 11 bits of the fraction: all of an FP16 number, and enough of others for a bound.
+        // 16 bits are sign, exponent and 7 bits of the fraction: enough for a bound. Minus infinity does not reach it.
         const unsigned tops[2] = {upper(order_key(best_group, 0)), upper(order_key(second_group, 0))};
-        float bound = key_value(static_cast<Key>(reached_by<20>(tops, p.beams)) << 32);
-        bound = bound == bound ? bound : -INFINITY;      // (fewer groups than beams)
+        float bound = key_value(static_cast<Key>(reached_by<16>(tops, p.beams)) << 32);
+        bound = bound >= R::kLowestValue ? bound : R::kLowestValue;      // (a NaN: fewer groups than beams)
         unsigned mask = 0;
+#pragma unroll 4
         for (int g = 0; g < group; ++g) {
-            const float mx = group_max[warp][g][lane];
-            mask |= mx >= bound && mx > -INFINITY ? 1u << g : 0u;
+            mask |= group_max[warp][g][lane] >= bound ? 1u << g : 0u;
         }
         int count = 0;
         bool overflow = false;
@@ -298,22 +329,26 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
             mask &= mask - 1;
             for (int of = 0; of < of_group; ++of) {
                 const int at = (g * of_group + of) * kChunk + lane;
+                uint4 q[kHeld];
+#pragma unroll
+                for (int j = 0; j < kHeld; ++j) {
+                    q[j] = word_at(part, g >= 0 ? at + 32 * j : words);
+                }
+                if (__any_sync(fb::kFullMask, first + at + 32 * (kHeld - 1) >= all_words - 1)) {
+#pragma unroll
+                    for (int j = 0; j < kHeld; ++j) {
+                        cut(q[j], at + 32 * j);
+                    }
+                }
                 unsigned those = 0;      // of this lane's values, that reach the bound
 #pragma unroll
                 for (int j = 0; j < kHeld; ++j) {
-                    uint4 q = word_at(g >= 0 ? at + 32 * j : words);
-                    cut(q, at + 32 * j);
-                    float v[R::kValues];
-                    R::unpack(v, q);
-#pragma unroll
-                    for (int c = 0; c < R::kValues; ++c) {
-                        those |= v[c] >= bound && v[c] > -INFINITY ? 1u << (j * R::kValues + c) : 0u;
-                    }
+                    those |= R::reaching(q[j], bound) << (j * R::kValues);
                 }
                 while (!overflow && __any_sync(fb::kFullMask, those != 0)) {
                     const int k = __ffs(those) - 1;
                     const int column = (first + at + 32 * (k / R::kValues)) * R::kValues + k % R::kValues;
-                    const float v = k >= 0 ? R::value(values, column) : -INFINITY;
+                    const float v = k >= 0 ? R::value(part.values, column) : -INFINITY;
                     const bool reaches = k >= 0 && v >= bound;      // (which may have risen)
                     const unsigned lanes = __ballot_sync(fb::kFullMask, reaches);
                     those &= those - 1;
@@ -330,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
             }
         }
         __syncwarp();
-        Key* best = p.best + static_cast<size_t>(item) * p.beams;
+        Key* best = p.best + static_cast<size_t>(part.item) * p.beams;
         if (!overflow) {
             for (int c = lane; c < count; c += 32) {
                 const Key key = list[c];
@@ -354,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
                 Key mine = 0;
 #pragma unroll 4
                 for (int c = begin + lane; c < end; c += 32) {
-                    const float v = R::value(values, c);
+                    const float v = R::value(part.values, c);
                     const Key key = v > -INFINITY ? order_key(v, c) : 0;
                     mine = key < before && key > mine ? key : mine;
                 }
@@ -370,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
             }
         }
         __syncwarp();      // (the list is read)
+        part = next;
     }
 }
 
