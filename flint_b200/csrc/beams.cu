@@ -657,9 +657,20 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_gr
         if (p.next_histories != nullptr) {
             const uint16_t* from = p.histories + (first + parent) * p.history_stride;
             uint16_t* to = p.next_histories + row * p.history_stride;
-#pragma unroll 8
-            for (int c = lane; c < length; c += 32) {
-                to[c] = from[c];
+            // (Loads first: to the compiler a store may change what is loaded next, and each would wait for the one before.)
+            constexpr int kAtOnce = 16;
+            for (int c = lane; c < length; c += 32 * kAtOnce) {
+                uint16_t some[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    some[i] = c + 32 * i < length ? from[c + 32 * i] : 0;
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (c + 32 * i < length) {
+                        to[c + 32 * i] = some[i];
+                    }
+                }
             }
             if (!over && length == p.history_stride) {
                 atomicExch(&g_beams_error, 1);
