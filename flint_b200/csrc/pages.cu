@@ -20,6 +20,9 @@ namespace {
 
 constexpr int kMostArrays = 128;
 constexpr int kChunkBytes = 8192;      // that a block copies at a time
+// Up to which pools and tables are small (their kernels' comments).
+constexpr int kSmallPages = 32768;
+constexpr int kSmallEntries = 8 * 8192;
 
 __device__ int g_pages_error = 0;
 
@@ -47,102 +50,6 @@ __device__ __forceinline__ bool is_page(const Pool& pool, int page) {
         report();
     }
     return is;
-}
-
-// ---- fork ---------------------------------------------------------------------------------------------
-
-struct ForkArgs {
-    Pool pool;
-    int* next_table;
-    int* next_lengths;
-    int* next_references;
-    const int* table;
-    const int* lengths;
-    const int* references;
-    const int* parents;
-};
-
-// Tables, lengths, and the references to start from; a warp has a row, 32 entries at a time.
-__global__ void __launch_bounds__(256) fb_pages_fork_tables(const ForkArgs p) {
-    fb::dependency_wait();
-    fb::dependency_release();
-    const int lane = threadIdx.x % 32;
-    const int warps = gridDim.x * 8, first = blockIdx.x * 8 + threadIdx.x / 32;
-    for (int page = blockIdx.x * 256 + threadIdx.x; page < p.pool.pages; page += gridDim.x * 256) {
-        p.next_references[page] = p.references[page];
-    }
-    for (int t = first; t < p.pool.sequences; t += warps) {
-        const int parent = p.parents[t];
-        const bool has = parent >= 0 && parent < p.pool.sequences;
-        if (!has && parent != -1) {
-            report();
-        }
-        const int length = has ? length_of(p.pool, p.lengths, parent) : 0;
-        const int entries = entries_of(p.pool, length);
-        for (int e = lane; e < p.pool.stride; e += 32) {
-            p.next_table[static_cast<long long>(t) * p.pool.stride + e] =
-                e < entries ? p.table[static_cast<long long>(parent) * p.pool.stride + e] : -1;
-        }
-        if (lane == 0) {
-            p.next_lengths[t] = length;
-        }
-    }
-}
-
-// One reference less for what stood in the old tables, one more for what stands in the new ones.
-__global__ void __launch_bounds__(256) fb_pages_fork_references(const ForkArgs p) {
-    fb::dependency_wait();
-    fb::dependency_release();
-    const int lane = threadIdx.x % 32;
-    const int warps = gridDim.x * 8, first = blockIdx.x * 8 + threadIdx.x / 32;
-    for (int item = first; item < 2 * p.pool.sequences; item += warps) {
-        const bool is_new = item >= p.pool.sequences;
-        const int s = is_new ? item - p.pool.sequences : item;
-        const int entries = entries_of(p.pool, length_of(p.pool, is_new ? p.next_lengths : p.lengths, s));
-        const int* row = (is_new ? p.next_table : p.table) + static_cast<long long>(s) * p.pool.stride;
-        for (int e = lane; e < entries; e += 32) {
-            const int page = row[e];
-            if (is_page(p.pool, page)) {
-                atomicAdd(p.next_references + page, is_new ? 1 : -1);
-            }
-        }
-    }
-}
-
-// ---- truncate -------------------------------------------------------------------------------------------
-
-struct TruncateArgs {
-    Pool pool;
-    int* table;
-    int* lengths;
-    int* references;
-    const int* keep;
-};
-
-__global__ void __launch_bounds__(256) fb_pages_truncate(const TruncateArgs p) {
-    fb::dependency_wait();
-    fb::dependency_release();
-    const int lane = threadIdx.x % 32;
-    const int warps = gridDim.x * 8, first = blockIdx.x * 8 + threadIdx.x / 32;
-    for (int s = first; s < p.pool.sequences; s += warps) {
-        const int length = length_of(p.pool, p.lengths, s), keep = p.keep[s];
-        if (keep < 0) {
-            report();
-        }
-        const int kept = min(length, max(keep, 0));
-        int* row = p.table + static_cast<long long>(s) * p.pool.stride;
-        for (int e = entries_of(p.pool, kept) + lane; e < entries_of(p.pool, length); e += 32) {
-            const int page = row[e];
-            if (is_page(p.pool, page)) {
-                atomicSub(p.references + page, 1);
-            }
-            row[e] = -1;
-        }
-        __syncwarp();      // (everybody has the length)
-        if (lane == 0) {
-            p.lengths[s] = kept;
-        }
-    }
 }
 
 // ---- one cluster's prefix sums ----------------------------------------------------------------------------
@@ -209,6 +116,155 @@ __device__ __forceinline__ long long sum_of(const long long* slots, int ranks) {
     return sum;
 }
 
+// ---- fork ---------------------------------------------------------------------------------------------
+
+struct ForkArgs {
+    Pool pool;
+    int* next_table;
+    int* next_lengths;
+    int* next_references;
+    const int* table;
+    const int* lengths;
+    const int* references;
+    const int* parents;
+};
+
+// Tables, lengths, and the references to start from; a warp has a row, 32 entries at a time.
+__global__ void __launch_bounds__(256) fb_pages_fork_tables(const ForkArgs p) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int lane = threadIdx.x % 32;
+    const int warps = gridDim.x * 8, first = blockIdx.x * 8 + threadIdx.x / 32;
+    for (int page = blockIdx.x * 256 + threadIdx.x; page < p.pool.pages; page += gridDim.x * 256) {
+        p.next_references[page] = p.references[page];
+    }
+    for (int t = first; t < p.pool.sequences; t += warps) {
+        const int parent = p.parents[t];
+        const bool has = parent >= 0 && parent < p.pool.sequences;
+        if (!has && parent != -1) {
+            report();
+        }
+        const int length = has ? length_of(p.pool, p.lengths, parent) : 0;
+        const int entries = entries_of(p.pool, length);
+        for (int e = lane; e < p.pool.stride; e += 32) {
+            p.next_table[static_cast<long long>(t) * p.pool.stride + e] =
+                e < entries ? p.table[static_cast<long long>(parent) * p.pool.stride + e] : -1;
+        }
+        if (lane == 0) {
+            p.next_lengths[t] = length;
+        }
+    }
+}
+
+// One reference less for what stood in the old tables, one more for what stands in the new ones.
+__global__ void __launch_bounds__(256) fb_pages_fork_references(const ForkArgs p) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int lane = threadIdx.x % 32;
+    const int warps = gridDim.x * 8, first = blockIdx.x * 8 + threadIdx.x / 32;
+    for (int item = first; item < 2 * p.pool.sequences; item += warps) {
+        const bool is_new = item >= p.pool.sequences;
+        const int s = is_new ? item - p.pool.sequences : item;
+        const int entries = entries_of(p.pool, length_of(p.pool, is_new ? p.next_lengths : p.lengths, s));
+        const int* row = (is_new ? p.next_table : p.table) + static_cast<long long>(s) * p.pool.stride;
+        for (int e = lane; e < entries; e += 32) {
+            const int page = row[e];
+            if (is_page(p.pool, page)) {
+                atomicAdd(p.next_references + page, is_new ? 1 : -1);
+            }
+        }
+    }
+}
+
+// The same in one launch, for pools that a cluster's threads take a few entries each of: 512 sequences of 66 entries on 3,500
+// pages XX us against YY in two.
+__global__ void __launch_bounds__(kThreads) fb_pages_fork_small(const ForkArgs p) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int first = static_cast<int>(sm100::cluster_cta_rank()) * kThreads + static_cast<int>(threadIdx.x);
+    const int entries = p.pool.sequences * p.pool.stride;
+    for (int page = first; page < p.pool.pages; page += kRanks * kThreads) {
+        p.next_references[page] = p.references[page];
+    }
+    constexpr int kEach = kSmallEntries / (kRanks * kThreads);
+    int had[kEach], gets[kEach];      // the page that an entry had, and the one that it gets; -1 for none
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int i = first + k * kRanks * kThreads;
+        had[k] = gets[k] = -1;
+        if (i < entries) {
+            const int t = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride));
+            const int e = i - t * p.pool.stride, parent = p.parents[t];
+            const bool has = parent >= 0 && parent < p.pool.sequences;
+            if (!has && parent != -1) {
+                report();
+            }
+            const int length = has ? length_of(p.pool, p.lengths, parent) : 0;
+            int page = -1;
+            if (e < entries_of(p.pool, length)) {
+                page = p.table[parent * p.pool.stride + e];
+                gets[k] = is_page(p.pool, page) ? page : -1;
+            }
+            p.next_table[i] = page;
+            if (e == 0) {
+                p.next_lengths[t] = length;
+            }
+            if (e < entries_of(p.pool, length_of(p.pool, p.lengths, t))) {
+                page = p.table[i];
+                had[k] = is_page(p.pool, page) ? page : -1;
+            }
+        }
+    }
+    meet();
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (had[k] != gets[k]) {
+            if (gets[k] >= 0) {
+                atomicAdd(p.next_references + gets[k], 1);
+            }
+            if (had[k] >= 0) {
+                atomicAdd(p.next_references + had[k], -1);
+            }
+        }
+    }
+}
+
+// ---- truncate -------------------------------------------------------------------------------------------
+
+struct TruncateArgs {
+    Pool pool;
+    int* table;
+    int* lengths;
+    int* references;
+    const int* keep;
+};
+
+__global__ void __launch_bounds__(256) fb_pages_truncate(const TruncateArgs p) {
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int lane = threadIdx.x % 32;
+    const int warps = gridDim.x * 8, first = blockIdx.x * 8 + threadIdx.x / 32;
+    for (int s = first; s < p.pool.sequences; s += warps) {
+        const int length = length_of(p.pool, p.lengths, s), keep = p.keep[s];
+        if (keep < 0) {
+            report();
+        }
+        const int kept = min(length, max(keep, 0));
+        int* row = p.table + static_cast<long long>(s) * p.pool.stride;
+        for (int e = entries_of(p.pool, kept) + lane; e < entries_of(p.pool, length); e += 32) {
+            const int page = row[e];
+            if (is_page(p.pool, page)) {
+                atomicSub(p.references + page, 1);
+            }
+            row[e] = -1;
+        }
+        __syncwarp();      // (everybody has the length)
+        if (lane == 0) {
+            p.lengths[s] = kept;
+        }
+    }
+}
+
 // ---- reserve --------------------------------------------------------------------------------------------
 
 struct ReserveArgs {
@@ -225,6 +281,7 @@ struct ReserveArgs {
     int* needs;        // [sequences][2]: where a sequence's pages stand in that list, its move's place or -1
 };
 
+// (ReserveArgs' lists are used where shared memory has no room.)
 struct Growth {
     int length, entries, fresh, last;     // last: the partly filled page that it writes into, or -1
 };
@@ -362,6 +419,132 @@ __global__ void __launch_bounds__(kThreads) fb_pages_reserve(const ReserveArgs p
         __syncwarp();      // (everybody has the length)
         if (lane == 0) {
             p.lengths[s] = g.length;
+        }
+    }
+}
+
+// The same for up to a thread per sequence and pools that are read soon: one block, whose barriers take a tenth of a cluster's.
+// Sequences that write into the same page meet in a table of pages in shared memory.
+constexpr int kSlots = 2048;
+constexpr int kListed = 4096;      // free pages that shared memory holds
+
+__global__ void __launch_bounds__(kThreads) fb_pages_reserve_small(const ReserveArgs p) {
+    __shared__ long long scan[kWarps];
+    __shared__ int page_of_slot[kSlots], growers[kSlots], lowest[kSlots];
+    __shared__ int listed[kListed];
+    fb::dependency_wait();
+    fb::dependency_release();
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % 32, s = tid;
+    const bool is = s < p.pool.sequences;
+    Growth g = {0, 0, 0, -1};
+    if (is) {
+        g = growth_of(p, s);
+    }
+    const int references = g.last >= 0 ? p.references[g.last] : 0;
+    // Free pages among the first 4,096, four per thread.
+    auto free_of = [&](int at) {      // a bit for each of four pages
+        unsigned free = 0;
+        if (at + 4 <= p.pool.pages) {
+            const int4 four = *reinterpret_cast<const int4*>(p.references + at);
+            free = (four.x == 0 ? 1u : 0u) | (four.y == 0 ? 2u : 0u) | (four.z == 0 ? 4u : 0u) | (four.w == 0 ? 8u : 0u);
+        } else {
+            for (int i = 0; at + i < p.pool.pages; ++i) {
+                free |= p.references[at + i] == 0 ? 1u << i : 0u;
+            }
+        }
+        return free;
+    };
+    unsigned free = free_of(4 * tid);
+    for (int i = tid; i < kSlots; i += kThreads) {
+        page_of_slot[i] = -1;
+        growers[i] = 0;
+        lowest[i] = INT_MAX;
+    }
+    __syncthreads();
+    int slot = 0;
+    if (g.last >= 0) {
+        slot = static_cast<int>((static_cast<unsigned>(g.last) * 2654435761u) >> 21);
+        static_assert(kSlots == 1 << (32 - 21) && kSlots > kThreads, "the table is never full");
+        for (;;) {
+            const int before = atomicCAS(&page_of_slot[slot], -1, g.last);
+            if (before == -1 || before == g.last) {
+                break;
+            }
+            slot = (slot + 1) % kSlots;
+        }
+        atomicAdd(&growers[slot], 1);
+        atomicMin(&lowest[slot], s);
+    }
+    __syncthreads();
+    const bool copies = g.last >= 0 && !(growers[slot] >= references && lowest[slot] == s);
+    // Pages that are needed, and in the upper bits copies.
+    constexpr int kShift = 44;
+    const long long mine = static_cast<long long>(g.fresh) + (copies ? 1 + (1LL << kShift) : 0);
+    long long all = 0;
+    const long long before = block_prefix(mine, all, scan);
+    const long long all_need = all & ((1LL << kShift) - 1);
+    int place = 0;
+    long long found = 0;
+    for (int from = 0; from < p.pool.pages && found < all_need; from += 4 * kThreads) {
+        if (from > 0) {
+            free = free_of(from + 4 * tid);
+        }
+        int here = 0;
+        long long at = found + block_prefix(__popc(free), here, scan);
+        for (; free != 0 && at < all_need; free &= free - 1, ++at) {
+            const int page = from + 4 * tid + __ffs(free) - 1;
+            if (at < kListed) {
+                listed[at] = page;
+            } else {
+                p.fresh[at] = page;
+            }
+        }
+        found += here;
+    }
+    const bool enough = found >= all_need;
+    const int all_moves = enough ? static_cast<int>(all >> kShift) : 0;
+    if (tid == 0) {
+        p.counts[0] = all_moves;
+        p.counts[1] = static_cast<int>(min(max(all_need - found, 0LL), static_cast<long long>(INT_MAX)));
+    }
+    if (s >= all_moves && is) {
+        p.moves[2 * s] = p.moves[2 * s + 1] = -1;
+    }
+    __syncthreads();      // the list is written, and references are read
+    if (!enough) {
+        return;
+    }
+    auto page_at = [&](int i) { return i < kListed ? listed[i] : p.fresh[i]; };
+    place = static_cast<int>(before & ((1LL << kShift) - 1));
+    int* row = p.table + static_cast<long long>(s) * p.pool.stride;
+    if (copies) {
+        const int page = page_at(place++), move = static_cast<int>(before >> kShift);
+        p.moves[2 * move] = g.last;
+        p.moves[2 * move + 1] = page;
+        atomicSub(p.references + g.last, 1);
+        p.references[page] = 1;
+        row[g.entries - 1] = page;
+    }
+    if (is) {
+        p.lengths[s] = g.length;
+    }
+    // A warp's sequences one by one where one has many pages, else all at once.
+    if (__any_sync(fb::kFullMask, g.fresh > 4)) {
+        for (int l = 0; l < 32; ++l) {
+            const int count = __shfl_sync(fb::kFullMask, g.fresh, l), at = __shfl_sync(fb::kFullMask, place, l);
+            const int entries = __shfl_sync(fb::kFullMask, g.entries, l);
+            int* its = p.table + static_cast<long long>(s - lane + l) * p.pool.stride + entries;
+            for (int e = lane; e < count; e += 32) {
+                const int page = page_at(at + e);
+                p.references[page] = 1;
+                its[e] = page;
+            }
+        }
+    } else {
+        for (int e = 0; e < g.fresh; ++e) {
+            const int page = page_at(place + e);
+            p.references[page] = 1;
+            row[g.entries + e] = page;
         }
     }
 }
@@ -649,6 +832,10 @@ flint_status flint_b200_pages_fork(void* next_table, void* next_lengths, void* n
                         static_cast<const int*>(lengths),
                         static_cast<const int*>(references),
                         static_cast<const int*>(parents)};
+    if (static_cast<long long>(pool.sequences) * pool.stride <= kSmallEntries && pool.pages <= kSmallPages) {
+        FB_CUDA(fb::launch_dependent_cluster(fb_pages_fork_small, dim3(kRanks), dim3(kThreads), kRanks, 0, stream, p));
+        return FLINT_OK;
+    }
     dim3 grid;
     FB_CUDA(row_grid(pool.sequences, pool.pages, &grid));
     FB_CUDA(fb::launch_dependent(fb_pages_fork_tables, grid, dim3(256), 0, stream, p));
@@ -690,6 +877,10 @@ flint_status flint_b200_pages_reserve(void* page_table, void* lengths, void* ref
                            space + pages,
                            space + 2 * pages,
                            space + 3 * pages};
+    if (pool.sequences <= kThreads && pool.pages <= kSmallPages) {
+        FB_CUDA(fb::launch_dependent(fb_pages_reserve_small, dim3(1), dim3(kThreads), 0, stream, p));
+        return FLINT_OK;
+    }
     FB_CUDA(fb::launch_dependent_cluster(fb_pages_reserve, dim3(kRanks), dim3(kThreads), kRanks, 0, stream, p));
     return FLINT_OK;
 }
