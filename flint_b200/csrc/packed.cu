@@ -520,7 +520,7 @@ flint_status flint_b200_paged8_attention_workspace(const flint_b200_paged_shape*
     if (bytes == nullptr) {
         return fb::fail(kBad, "%s: bytes is null", name);
     }
-    FB_CUDA(fb::packed_forward_workspace(bytes));
+    FB_CUDA(fb::paged8_workspace(bytes));
     return FLINT_OK;
 }
 

@@ -50,7 +50,8 @@ cudaError_t packed_backward_error_flag(int* value, bool reset);
 // tiles (O [column / 4][row of 128][4], maxima, sums, two per CTA), and the launch that joins them.
 struct Record;
 constexpr size_t kPartFloats = size_t{128} * 64 + 2 * 128;
-int packed_ctas(int sms);
+constexpr int kMostPackedCtas = 1024;
+size_t packed_workspace(int ctas);
 Record* packed_records(void* workspace);
 float* packed_parts(void* workspace, int ctas);
 cudaError_t packed_join(const PackedArgs& args, const Record* records, const float* parts, int ctas,
@@ -67,9 +68,10 @@ struct Cache8 {
 
 // args.k and args.v: the new tokens' rows.
 cudaError_t paged8_store(const PackedArgs& args, const Cache8& cache, cudaStream_t stream);
-// args.k and args.v are not read; the workspace is packed_forward's.
+// args.k and args.v are not read.
 cudaError_t paged8_attention(const PackedArgs& args, const Cache8& cache, int longest, void* workspace,
                              cudaStream_t stream);
+cudaError_t paged8_workspace(size_t* bytes);
 cudaError_t paged8_error_flag(int* value, bool reset);
 
 // Device error words of these kernels: a wait that gave up, or starts, lengths or page

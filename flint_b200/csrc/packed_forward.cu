@@ -806,7 +806,7 @@ struct JoinParams {
 
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kMostCtas = 1024;
+constexpr int kMostCtas = kMostPackedCtas;
 // Caches of more than kManyKeys keys per sequence can make tiles of many parts. Those of more than kFewParts are then
 // left to kHelpers other blocks (of shorter ones the block that has the tile joins them all, two at a time).
 constexpr int kFewParts = 8;
@@ -1045,15 +1045,16 @@ size_t records_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(Reco
 
 cudaError_t packed_forward_error_flag(int* value, bool reset) { return read_error_word(value, reset); }
 
+size_t packed_workspace(int ctas) {
+    return records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * kPartFloats * sizeof(float);
+}
+
 cudaError_t packed_forward_workspace(size_t* bytes) {
     int sms = 148;
     const cudaError_t e = sm_count(&sms);
-    const int ctas = packed_ctas(sms);
-    *bytes = records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * kPartFloats * sizeof(float);
+    *bytes = packed_workspace(std::min(2 * sms, kMostCtas));
     return e;
 }
-
-int packed_ctas(int sms) { return std::min(2 * sms, kMostCtas); }
 
 Record* packed_records(void* workspace) { return static_cast<Record*>(workspace); }
 
@@ -1082,7 +1083,7 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     }
     int sms = 148;
     cudaError_t e = sm_count(&sms);
-    const int ctas = packed_ctas(sms);
+    const int ctas = std::min(2 * sms, kMostCtas);
     if (e == cudaSuccess) {
         e = encode_rows(&p.map_q, args.q, args.heads, args.rows, args.q_stride, p.group, 1 << p.log_tokens);
     }

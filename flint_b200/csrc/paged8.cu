@@ -22,6 +22,9 @@
 namespace fb {
 namespace {
 
+#ifndef VPS
+#define VPS 3
+#endif
 constexpr int kHead = 64;
 constexpr int kBlock = 16;      // positions that share a scale
 constexpr float kLog2e = 1.4426950408889634f;
@@ -119,17 +122,18 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
 
 // ---- attention of few rows ------------------------------------------------------------------------------
 
-// Bound by what it reads, so the warp-wide product is the right one: mma.sync takes codes that a lane has just turned into FP16
-// in its registers, where the tensor cores' larger instruction would want them written to shared memory first. A tile
-// (packed_schedule.h) has up to 16 kTiles rows; a warp takes 16 of them and every (8 / kTiles)-th block of 16 keys, whose codes
-// come to it alone through four stages of asynchronous copies, and the warps' sums meet at the end of a piece.
+// Bound by what it reads and by what turning codes into FP16 takes, so a warp's own product is the right one: mma.sync takes codes
+// that a lane has just turned into FP16 in its registers, where the tensor cores' larger instruction would want
+// them written to shared memory first. Keys are the products' rows and queries their columns, eight of them to a
+// product: S^T = K Q^T, O^T = V^T P^T. With 16 rows of queries instead, a group of four heads would leave three quarters of the
+// exponentials to nobody. A tile (packed_schedule.h) has up to 8 kTiles kSplit rows, of which a warp takes every kSplit-th eight, and
+// every (8 / kSplit)-th block of 16 keys, whose codes come to it alone through stages of asynchronous copies; the
+// warps' sums meet at the end of a piece.
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kStages = 4;
 constexpr int kStageBytes = 2 * kBlock * kHead;       // K and V of a block
-constexpr int kRingBytes = kWarps * kStages * kStageBytes;
 constexpr int kMergeStride = kHead + 4;               // floats between rows that meet
-static_assert(kWarps * 16 * kMergeStride * 4 <= kRingBytes, "the rows that meet take the ring's place");
 
 struct FewParams {
     PackedArgs a;
@@ -140,11 +144,17 @@ struct FewParams {
     bool splits;
 };
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                          unsigned b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The transpose of 8 x 8 values of 16 bits, a row to four lanes.
+__device__ __forceinline__ unsigned transposed(unsigned x) {
+    unsigned r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 
 // Bytes kLow and kLow + 1 of x, which are codes + 128, as FP16: 1,024 + byte has the byte as its low bits.
@@ -155,61 +165,64 @@ __device__ __forceinline__ unsigned two_codes(unsigned x) {
     return *reinterpret_cast<const unsigned*>(&h);
 }
 
-template <int kTiles>
-__global__ void __launch_bounds__(kThreads, 2) fb_paged8_few(const FewParams p) {
-    constexpr int kApart = kWarps / kTiles;      // warps that share rows
-    extern __shared__ __align__(128) unsigned char ring[];
-    __shared__ Cut cuts[2];
-    __shared__ long long scan[kWarps + 1];
-    __shared__ int scan_longest[kWarps];
-    __shared__ int whole_tiles;
-    __shared__ float merge_max[kWarps][16], merge_sum[kWarps][16];
+// CTAs that fit on an SM (registers).
+constexpr int few_per_sm(int tiles) { return tiles > 2 ? 1 : tiles == 2 ? 2 : VPS; }
+constexpr int kMostPerSm = VPS;
+
+template <int kTiles, int kSplit>
+struct FewMemory {
+    static constexpr int kRows = 8 * kTiles * kSplit;
+    static constexpr int kOf = 8 * kTiles;            // rows of a warp
+    union {
+        unsigned char ring[kWarps][kStages][kStageBytes];
+        float merge[kWarps][kOf][kMergeStride];       // (in the ring's place at the end of a piece)
+    };
+    uint4 queries[kTiles * kSplit][2][32];
+    int position[kRows];
+    float merge_max[kWarps][kOf], merge_sum[kWarps][kOf];
+    Cut cuts[2];
+    long long scan[kWarps + 1];
+    int scan_longest[kWarps];
+    int whole_tiles;
+};
+
+template <int kTiles, int kSplit>
+__global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(const FewParams p) {
+    using Memory = FewMemory<kTiles, kSplit>;
+    constexpr int kApart = kWarps / kSplit;      // warps that share rows
+    extern __shared__ __align__(128) unsigned char memory[];
+    Memory& shared = *reinterpret_cast<Memory*>(memory);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x / 32), 0), lane = threadIdx.x % 32;
     const int g = lane / 4, t = lane % 4;        // row and column of the products' fragments
     dependency_wait();
     if (p.a.sequences > 32) {
-        locate<false, kThreads>(p, cuts, whole_tiles, scan, scan_longest);
+        locate<false, kThreads>(p, shared.cuts, shared.whole_tiles, shared.scan, shared.scan_longest);
     } else if (warp == 0) {
-        locate_in_warp<false>(p, cuts, whole_tiles, lane);
+        locate_in_warp<false>(p, shared.cuts, shared.whole_tiles, lane);
     }
     __syncthreads();
     dependency_release();
     if (threadIdx.x == 0) {
-        p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, cuts[0], cuts[1]);
+        p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, shared.cuts[0], shared.cuts[1]);
     }
-    const int tile = warp % kTiles, share = warp / kTiles;
-    unsigned char* stages = ring + warp * (kStages * kStageBytes);
+    const int split = warp % kSplit, share = warp / kSplit;
+    const unsigned char* stages = &shared.ring[warp][0][0];
     const uint32_t stages_at = sm100::smem_u32(stages);
     const float scale2 = p.a.scale * kLog2e;
     Walk walk;
     Piece piece;
-    walk.begin(SequenceOf{p.a}, cuts[0], cuts[1].at);
+    walk.begin(SequenceOf{p.a}, shared.cuts[0], shared.cuts[1].at);
     while (walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece)) {
         const int first_position = piece.position();
         const int first_block = piece.from * (kKeyTile / kBlock);
         const int end_block = min(piece.to * (kKeyTile / kBlock), (piece.sequence.keys + kBlock - 1) / kBlock);
         const int rows = piece.tokens * p.group;
+        const int tiles = (rows + 7) / 8;                          // of eight rows
+        const int mine = (tiles - split + kSplit - 1) / kSplit;    // of them this warp's, from `split` on
         // This warp's blocks: first_block + share + i kApart.
-        const int count = tile * 16 >= rows ? 0 : max(0, (end_block - first_block - share + kApart - 1) / kApart);
-        // Its rows g and g + 8: queries as they are multiplied, and positions.
-        uint4 query[2][2];
-        int position[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = tile * 16 + g + 8 * h, token = row / p.group;
-            position[h] = -1;
-            query[h][0] = query[h][1] = make_uint4(0u, 0u, 0u, 0u);
-            if (row < rows) {
-                position[h] = first_position + token;
-                const __half* from = p.a.q + (static_cast<long long>(piece.sequence.first) + piece.first_token + token) * p.a.q_stride +
-                                     (piece.head * p.group + row - token * p.group) * kHead + 16 * t;
-                query[h][0] = reinterpret_cast<const uint4*>(from)[0];
-                query[h][1] = reinterpret_cast<const uint4*>(from)[1];
-            }
-        }
-        float m[2] = {kNoKey, kNoKey}, l[2] = {0.0f, 0.0f};
-        float out[8][4] = {};
-        // Lane i has the place of block 32 batch + i (the row of its first key in the cache, -1 for none) and its scales.
+        const int count = mine <= 0 ? 0 : max(0, (end_block - first_block - share + kApart - 1) / kApart);
+        // Lane i has the place of block 32 batch + i (the row of its first key in the cache, -1 for none) and what its scales
+        // come to.
         auto place_of = [&](int i) {
             if (i >= count) {
                 return -1;
@@ -220,15 +233,15 @@ __global__ void __launch_bounds__(kThreads, 2) fb_paged8_few(const FewParams p) 
                             : static_cast<int>((page * p.a.kv_heads + piece.head) << p.log_page) + (key & (p.a.page_size - 1));
         };
         int place_next = place_of(lane), place = -1;
-        float k_scale_next = 0.0f, v_scale_next = 0.0f, k_scale = 0.0f, v_scale = 0.0f;
+        float k_next = 0.0f, v_next = 0.0f, slope_of = 0.0f, offset_of = 0.0f, inverse_of = 0.0f;
         auto fetch = [&](int i) {
             if (i < count) {
                 if (i % 32 == 0) {
                     place = place_next;
-                    k_scale_next = v_scale_next = 0.0f;
+                    k_next = v_next = 0.0f;
                     if (place >= 0) {
-                        k_scale_next = p.cache.k_scales[place / kBlock];
-                        v_scale_next = p.cache.v_scales[place / kBlock];
+                        k_next = p.cache.k_scales[place / kBlock];
+                        v_next = p.cache.v_scales[place / kBlock];
                     }
                     place_next = place_of(i + 32 + lane);
                 }
@@ -249,148 +262,196 @@ __global__ void __launch_bounds__(kThreads, 2) fb_paged8_few(const FewParams p) 
         for (int i = 0; i < kStages - 1; ++i) {
             fetch(i);
         }
+        // Queries as they are multiplied: of eight rows, lane (g, t) has the 16 values from 16 t on of row g, four of
+        // which are a product's term with the four codes that lie beside each other in a key.
+        for (int i = threadIdx.x; i < tiles * 64; i += kThreads) {
+            const int row = i / 64 * 8 + i % 32 / 4, token = row / p.group;
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (row < rows) {
+                const __half* from = p.a.q + (static_cast<long long>(piece.sequence.first) + piece.first_token + token) * p.a.q_stride +
+                                     (piece.head * p.group + row - token * p.group) * kHead + 16 * (i % 4);
+                q = reinterpret_cast<const uint4*>(from)[i / 32 % 2];
+            }
+            shared.queries[i / 64][i / 32 % 2][i % 32] = q;
+        }
+        for (int row = threadIdx.x; row < tiles * 8; row += kThreads) {
+            shared.position[row] = row < rows ? first_position + row / p.group : -1;
+        }
+        __syncthreads();
+        float m[kTiles][2], l[kTiles][2];
+        float out[kTiles][4][4];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            m[n][0] = m[n][1] = kNoKey;
+            l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                out[n][j][0] = out[n][j][1] = out[n][j][2] = out[n][j][3] = 0.0f;
+            }
+        }
         for (int i = 0; i < count; ++i) {
             if (i % 32 == 0) {
-                k_scale = k_scale_next;
-                v_scale = v_scale_next;
+                const float v = v_next == 0.0f ? 1.0f : v_next;      // (codes are 0 then)
+                slope_of = k_next * scale2;
+                offset_of = __log2f(v);
+                inverse_of = 1.0f / v;
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             __syncwarp();       // everybody's copies have landed, and the stage before is read
             fetch(i + kStages - 1);
             const unsigned char* stage = stages + (i % kStages) * kStageBytes;
             const int key = (first_block + share + i * kApart) * kBlock;
-            // Scores: of the products' eight columns the even ones are keys 0 to 3 and the odd ones 4 to 7, which is the order that
-            // V's rows below are read in, four in a row at a time; a lane's four terms of a product are
-            // neighbours, as they lie in its 16 bytes of a key.
-            float scores[2][4] = {};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint4 codes = *reinterpret_cast<const uint4*>(stage + (8 * u + (g & 1) * 4 + (g >> 1)) * kHead + 16 * t);
-                const unsigned w[4] = {codes.x ^ 0x80808080u, codes.y ^ 0x80808080u, codes.z ^ 0x80808080u, codes.w ^ 0x80808080u};
-                const unsigned low[8] = {query[0][0].x, query[0][0].y, query[0][0].z, query[0][0].w,
-                                         query[0][1].x, query[0][1].y, query[0][1].z, query[0][1].w};
-                const unsigned high[8] = {query[1][0].x, query[1][0].y, query[1][0].z, query[1][0].w,
-                                          query[1][1].x, query[1][1].y, query[1][1].z, query[1][1].w};
+            const bool masked = key + kBlock - 1 > first_position;
+            const float slope = __shfl_sync(kFullMask, slope_of, i % 32), offset = __shfl_sync(kFullMask, offset_of, i % 32);
+            const float inverse = __shfl_sync(kFullMask, inverse_of, i % 32);
+            // Of the products' rows the even ones are keys 0 to 3 and the odd ones 4 to 7, and so on: V's are then read four in
+            // a row at a time below.
+            const int low = (g & 1) * 4 + (g >> 1);      // key of the product's row g; 8 more for row g + 8
+            float scores[kTiles][4];
+            {
+                const uint4 first = *reinterpret_cast<const uint4*>(stage + low * kHead + 16 * t);
+                const uint4 second = *reinterpret_cast<const uint4*>(stage + (8 + low) * kHead + 16 * t);
+                const unsigned x[4] = {first.x ^ 0x80808080u, first.y ^ 0x80808080u, first.z ^ 0x80808080u, first.w ^ 0x80808080u};
+                const unsigned y[4] = {second.x ^ 0x80808080u, second.y ^ 0x80808080u, second.z ^ 0x80808080u,
+                                       second.w ^ 0x80808080u};
+                unsigned keys[4][4];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    mma_16816(scores[u], low[2 * s], high[2 * s], low[2 * s + 1], high[2 * s + 1], two_codes<0>(w[s]),
-                              two_codes<2>(w[s]));
+                    keys[s][0] = two_codes<0>(x[s]);
+                    keys[s][1] = two_codes<0>(y[s]);
+                    keys[s][2] = two_codes<2>(x[s]);
+                    keys[s][3] = two_codes<2>(y[s]);
+                }
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    scores[n][0] = scores[n][1] = scores[n][2] = scores[n][3] = 0.0f;
+                    if (kTiles == 1 || n < mine) {
+                        const uint4 q0 = shared.queries[n * kSplit + split][0][lane], q1 = shared.queries[n * kSplit + split][1][lane];
+                        mma_16816(scores[n], keys[0], q0.x, q0.y);
+                        mma_16816(scores[n], keys[1], q0.z, q0.w);
+                        mma_16816(scores[n], keys[2], q1.x, q1.y);
+                        mma_16816(scores[n], keys[3], q1.z, q1.w);
+                    }
                 }
             }
-            const float weight = __shfl_sync(kFullMask, v_scale, i % 32);
-            const float v_here = weight == 0.0f ? 1.0f : weight;      // (codes are 0 then)
-            const float slope = __shfl_sync(kFullMask, k_scale, i % 32) * scale2, offset = __log2f(v_here);
-            const float inverse = 1.0f / v_here;
-            bool moves = false;
-            float top[2];
+            unsigned values[4][4];       // of the products with V: rows g and g + 8 are columns 8 g + 2 j and 8 g + 2 j + 1
+            {
+                uint2 read[4];           // keys t, t + 4, t + 8 and t + 12
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                top[h] = -INFINITY;
+                for (int k = 0; k < 4; ++k) {
+                    read[k] = *reinterpret_cast<const uint2*>(stage + kBlock * kHead + (4 * k + t) * kHead + 8 * g);
+                    read[k].x ^= 0x80808080u;
+                    read[k].y ^= 0x80808080u;
+                }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int j = 0; j < 4; ++j) {
+                    // Two columns of two keys side by side.
+                    const unsigned first = j < 2 ? __byte_perm(read[0].x, read[1].x, j % 2 == 0 ? 0x5140 : 0x7362)
+                                                 : __byte_perm(read[0].y, read[1].y, j % 2 == 0 ? 0x5140 : 0x7362);
+                    const unsigned second = j < 2 ? __byte_perm(read[2].x, read[3].x, j % 2 == 0 ? 0x5140 : 0x7362)
+                                                  : __byte_perm(read[2].y, read[3].y, j % 2 == 0 ? 0x5140 : 0x7362);
+                    values[j][0] = two_codes<0>(first);
+                    values[j][1] = two_codes<2>(first);
+                    values[j][2] = two_codes<0>(second);
+                    values[j][3] = two_codes<2>(second);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+                if (kTiles > 1 && n >= mine) {
+                    break;
+                }
+                // Lane (g, t) has keys `low` and low + 8 of rows 2 t and 2 t + 1.
+                float (&x)[4] = scores[n];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    x[c] = fmaf(x[c], slope, offset);
+                }
+                if (masked) {
+                    const int2 position = *reinterpret_cast<const int2*>(&shared.position[(n * kSplit + split) * 8 + 2 * t]);
+                    x[0] = key + low <= position.x ? x[0] : -INFINITY;
+                    x[1] = key + low <= position.y ? x[1] : -INFINITY;
+                    x[2] = key + low + 8 <= position.x ? x[2] : -INFINITY;
+                    x[3] = key + low + 8 <= position.y ? x[3] : -INFINITY;
+                }
+                float top[2] = {max_nan(x[0], x[2]), max_nan(x[1], x[3])};
+                if (__any_sync(kFullMask, !(top[0] - m[n][0] <= kLazyShift) || !(top[1] - m[n][1] <= kLazyShift))) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        float& x = scores[u][2 * h + c];
-                        x = fmaf(x, slope, offset);
-                        if (key + kBlock - 1 > first_position) {
-                            x = key + 8 * u + 4 * c + t <= position[h] ? x : -INFINITY;
+                        top[c] = max_nan(top[c], __shfl_xor_sync(kFullMask, top[c], 4));
+                        top[c] = max_nan(top[c], __shfl_xor_sync(kFullMask, top[c], 8));
+                        top[c] = max_nan(top[c], __shfl_xor_sync(kFullMask, top[c], 16));
+                        const float next = max_nan(m[n][c], top[c]);
+                        const float alpha = fast_exp2(m[n][c] - next);
+                        m[n][c] = next;
+                        l[n][c] *= alpha;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            out[n][j][c] *= alpha;
+                            out[n][j][2 + c] *= alpha;
                         }
-                        top[h] = max_nan(top[h], x);
                     }
                 }
-                moves = moves || !(top[h] - m[h] <= kLazyShift);
-            }
-            if (__any_sync(kFullMask, moves)) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    top[h] = max_nan(top[h], __shfl_xor_sync(kFullMask, top[h], 1));
-                    top[h] = max_nan(top[h], __shfl_xor_sync(kFullMask, top[h], 2));
-                    const float next = max_nan(m[h], top[h]);
-                    const float alpha = fast_exp2(m[h] - next);
-                    m[h] = next;
-                    l[h] *= alpha;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        out[j][2 * h] *= alpha;
-                        out[j][2 * h + 1] *= alpha;
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    x[c] = fast_exp2(x[c] - m[n][c % 2]);
                 }
-            }
-            unsigned weights[2][2];        // [half of the keys][row]
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float x = fast_exp2(scores[u][2 * h] - m[h]), y = fast_exp2(scores[u][2 * h + 1] - m[h]);
-                    sum += x + y;
-                    weights[u][h] = pack2(x, y);
+                if (masked) {
+                    // (A row that sees nothing of the block has nothing to do with its scale, whatever that is.)
+                    l[n][0] = fmaf(x[0] + x[2], x[0] + x[2] == 0.0f ? 0.0f : inverse, l[n][0]);
+                    l[n][1] = fmaf(x[1] + x[3], x[1] + x[3] == 0.0f ? 0.0f : inverse, l[n][1]);
+                } else {
+                    l[n][0] = fmaf(x[0] + x[2], inverse, l[n][0]);
+                    l[n][1] = fmaf(x[1] + x[3], inverse, l[n][1]);
                 }
-                // (A row that sees nothing of the block has nothing to do with its scale, whatever that is.)
-                l[h] = fmaf(sum, sum == 0.0f ? 0.0f : inverse, l[h]);
-            }
-            uint2 values[4];       // of keys t, t + 4, t + 8 and t + 12, columns 8 g to 8 g + 7
+                const unsigned b0 = transposed(pack2(x[0], x[1])), b1 = transposed(pack2(x[2], x[3]));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                values[k] = *reinterpret_cast<const uint2*>(stage + kBlock * kHead + (4 * k + t) * kHead + 8 * g);
-                values[k].x ^= 0x80808080u;
-                values[k].y ^= 0x80808080u;
-            }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const unsigned w[4] = {half == 0 ? values[0].x : values[0].y, half == 0 ? values[1].x : values[1].y,
-                                       half == 0 ? values[2].x : values[2].y, half == 0 ? values[3].x : values[3].y};
-#pragma unroll
-                for (int pair = 0; pair < 2; ++pair) {
-                    // Two columns of two keys side by side.
-                    const unsigned first = __byte_perm(w[0], w[1], pair == 0 ? 0x5140 : 0x7362);
-                    const unsigned second = __byte_perm(w[2], w[3], pair == 0 ? 0x5140 : 0x7362);
-                    const int j = 4 * half + 2 * pair;
-                    mma_16816(out[j], weights[0][0], weights[0][1], weights[1][0], weights[1][1], two_codes<0>(first),
-                              two_codes<0>(second));
-                    mma_16816(out[j + 1], weights[0][0], weights[0][1], weights[1][0], weights[1][1], two_codes<2>(first),
-                              two_codes<2>(second));
+                for (int j = 0; j < 4; ++j) {
+                    mma_16816(out[n][j], values[j], b0, b1);
                 }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();       // the ring is everybody's from here on
-        float* mine = reinterpret_cast<float*>(ring) + warp * 16 * kMergeStride;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(kFullMask, l[h], 1);
-            l[h] += __shfl_xor_sync(kFullMask, l[h], 2);
-            if (t == 0) {
-                merge_max[warp][g + 8 * h] = m[h];
-                merge_sum[warp][g + 8 * h] = l[h];
-            }
-            // Column 16 t + j of the row is out[j][2 h], column 16 t + 8 + j out[j][2 h + 1].
-            float4* to = reinterpret_cast<float4*>(mine + (g + 8 * h) * kMergeStride + 16 * t);
+        for (int n = 0; n < kTiles; ++n) {
+            if (n < mine) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                to[2 * c] = make_float4(out[0][2 * h + c], out[1][2 * h + c], out[2][2 * h + c], out[3][2 * h + c]);
-                to[2 * c + 1] = make_float4(out[4][2 * h + c], out[5][2 * h + c], out[6][2 * h + c], out[7][2 * h + c]);
+                for (int c = 0; c < 2; ++c) {
+                    const int row = 8 * n + 2 * t + c;      // of this warp's
+                    l[n][c] += __shfl_xor_sync(kFullMask, l[n][c], 4);
+                    l[n][c] += __shfl_xor_sync(kFullMask, l[n][c], 8);
+                    l[n][c] += __shfl_xor_sync(kFullMask, l[n][c], 16);
+                    if (g == 0) {
+                        shared.merge_max[warp][row] = m[n][c];
+                        shared.merge_sum[warp][row] = l[n][c];
+                    }
+                    // Column 8 g + 2 j of the row is out[j][c], column 8 g + 2 j + 1 out[j][2 + c].
+                    float4* to = reinterpret_cast<float4*>(&shared.merge[warp][row][8 * g]);
+                    to[0] = make_float4(out[n][0][c], out[n][0][2 + c], out[n][1][c], out[n][1][2 + c]);
+                    to[1] = make_float4(out[n][2][c], out[n][2][2 + c], out[n][3][c], out[n][3][2 + c]);
+                }
             }
         }
         __syncthreads();
         const bool whole = piece.from == 0 && piece.to == piece.tiles;
         for (int row = threadIdx.x / 16; row < rows; row += kThreads / 16) {
             const int column = threadIdx.x % 16 * 4;
+            const int its_split = row / 8 % kSplit, its_row = row / (8 * kSplit) * 8 + row % 8;
             float all = kNoKey;
 #pragma unroll
             for (int w = 0; w < kApart; ++w) {
-                all = max_nan(all, merge_max[w * kTiles + row / 16][row % 16]);
+                all = max_nan(all, shared.merge_max[w * kSplit + its_split][its_row]);
             }
             float total = 0.0f;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < kApart; ++w) {
-                const int its = w * kTiles + row / 16;
-                const float factor = fast_exp2(merge_max[its][row % 16] - all);
-                const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(ring) +
-                                                                  (its * 16 + row % 16) * kMergeStride + column);
-                if (merge_max[its][row % 16] != kNoKey) {
-                    total = fmaf(merge_sum[its][row % 16], factor, total);
+                const int its = w * kSplit + its_split;
+                const float top = shared.merge_max[its][its_row], factor = fast_exp2(top - all);
+                const float4 x = *reinterpret_cast<const float4*>(&shared.merge[its][its_row][column]);
+                if (top != kNoKey) {
+                    total = fmaf(shared.merge_sum[its][its_row], factor, total);
                     sum.x = fmaf(x.x, factor, sum.x);
                     sum.y = fmaf(x.y, factor, sum.y);
                     sum.z = fmaf(x.z, factor, sum.z);
@@ -421,6 +482,27 @@ __global__ void __launch_bounds__(kThreads, 2) fb_paged8_few(const FewParams p) 
     }
 }
 
+template <int kTiles, int kSplit>
+cudaError_t launch_few(FewParams p, int sms, void* workspace, long long most_keys, cudaStream_t stream) {
+    const int ctas = std::min(few_per_sm(kTiles) * sms, kMostPackedCtas);
+    p.records = packed_records(workspace);
+    p.parts = packed_parts(workspace, ctas);
+    p.splits = most_keys > 1024;
+    constexpr int kBytes = sizeof(FewMemory<kTiles, kSplit>);
+    while ((2 << p.log_tokens) * p.group <= FewMemory<kTiles, kSplit>::kRows) {
+        ++p.log_tokens;
+    }
+    static std::atomic<bool> configured[64] = {};
+    cudaError_t e = allow_shared_memory(fb_paged8_few<kTiles, kSplit>, kBytes, configured);
+    if (e == cudaSuccess) {
+        e = launch_dependent(fb_paged8_few<kTiles, kSplit>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kBytes, stream, p);
+    }
+    if (e != cudaSuccess || !p.splits) {
+        return e;
+    }
+    return packed_join(p.a, p.records, p.parts, ctas, most_keys, stream);
+}
+
 }  // namespace
 
 cudaError_t paged8_error_flag(int* value, bool reset) { return read_error_word(value, reset); }
@@ -447,36 +529,27 @@ cudaError_t paged8_attention(const PackedArgs& args, const Cache8& cache, int lo
     p.cache = cache;
     p.group = args.heads / args.kv_heads;
     const long long rows = static_cast<long long>(longest) * p.group;
-    const int form = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
-    while ((2 << p.log_tokens) * p.group <= 16 << form) {
-        ++p.log_tokens;
-    }
     while ((1 << p.log_page) < args.page_size) {
         ++p.log_page;
     }
     int sms = 148;
-    cudaError_t e = sm_count(&sms);
+    const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) {
         return e;
     }
-    const int ctas = packed_ctas(sms);
     const long long most_keys = static_cast<long long>(args.table_stride) * args.page_size;
-    p.splits = most_keys > 1024;
-    p.records = packed_records(workspace);
-    p.parts = packed_parts(workspace, ctas);
-    const auto kernel = form == 0   ? fb_paged8_few<1>
-                        : form == 1 ? fb_paged8_few<2>
-                        : form == 2 ? fb_paged8_few<4>
-                                    : fb_paged8_few<8>;
-    static std::atomic<bool> configured[4][64] = {};
-    e = allow_shared_memory(kernel, kRingBytes, configured[form]);
-    if (e == cudaSuccess) {
-        e = launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kRingBytes, stream, p);
-    }
-    if (e != cudaSuccess || !p.splits) {
-        return e;
-    }
-    return packed_join(args, p.records, p.parts, ctas, most_keys, stream);
+    return rows <= 8    ? launch_few<1, 1>(p, sms, workspace, most_keys, stream)
+           : rows <= 16 ? launch_few<2, 1>(p, sms, workspace, most_keys, stream)
+           : rows <= 32 ? launch_few<4, 1>(p, sms, workspace, most_keys, stream)
+           : rows <= 64 ? launch_few<4, 2>(p, sms, workspace, most_keys, stream)
+                        : launch_few<4, 4>(p, sms, workspace, most_keys, stream);
+}
+
+cudaError_t paged8_workspace(size_t* bytes) {
+    int sms = 148;
+    const cudaError_t e = sm_count(&sms);
+    *bytes = packed_workspace(std::min(kMostPerSm * sms, kMostPackedCtas));
+    return e;
 }
 
 }  // namespace fb
