@@ -86,15 +86,16 @@ cudaError_t encode_fn(EncodeTiled* out) {
 }
 
 cudaError_t encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
-                   const cuuint32_t* box) {
+                   const cuuint32_t* box, bool halves = true) {
     EncodeTiled fn = nullptr;
     const cudaError_t e = encode_fn(&fn);
     if (e != cudaSuccess) {
         return e;
     }
     const cuuint32_t step[3] = {1, 1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
-                          dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUresult r = fn(map, halves ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                          static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, halves ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
@@ -114,6 +115,13 @@ cudaError_t encode_pages(CUtensorMap* map, const __half* base, long long rows, i
     const cuuint64_t strides[1] = {kHeadWidth * 2};
     const cuuint32_t box[2] = {kHeadWidth, static_cast<cuuint32_t>(box_rows)};
     return encode(map, base, 2, dims, strides, box);
+}
+
+cudaError_t encode_pages8(CUtensorMap* map, const int8_t* base, long long rows, int box_rows) {
+    const cuuint64_t dims[2] = {kHeadWidth, static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {kHeadWidth};
+    const cuuint32_t box[2] = {kHeadWidth, static_cast<cuuint32_t>(box_rows)};
+    return encode(map, base, 2, dims, strides, box, false);
 }
 
 cudaError_t packed_error_flag(int* value, bool reset) {

@@ -34,9 +34,21 @@ struct PackedGradients {
     const __half* d_o;      // rows as o's
 };
 
+// Pages of 8 bits in the place of args.k and args.v: codes [pages, kv_heads, page_size, 64] and a scale for 16
+// positions of a head.
+struct Cache8 {
+    int8_t* k;
+    int8_t* v;
+    float* k_scales;
+    float* v_scales;
+};
+
 // Forward, over packed or paged keys; the workspace's size depends on the GPU only. `longest` is about how many new
 // tokens a sequence has at most (paged keys; it chooses the kernel's form).
 cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace, cudaStream_t stream);
+// Over pages of 8 bits where `eight` is given.
+cudaError_t packed_forward(const PackedArgs& args, const Cache8* eight, int longest, void* workspace,
+                           cudaStream_t stream);
 cudaError_t packed_forward_workspace(size_t* bytes);
 cudaError_t packed_forward_error_flag(int* value, bool reset);
 
@@ -56,15 +68,6 @@ Record* packed_records(void* workspace);
 float* packed_parts(void* workspace, int ctas);
 cudaError_t packed_join(const PackedArgs& args, const Record* records, const float* parts, int ctas,
                         long long most_keys, cudaStream_t stream);
-
-// Pages of 8 bits in the place of args.k and args.v: codes [pages, kv_heads, page_size, 64] and a scale for 16
-// positions of a head.
-struct Cache8 {
-    int8_t* k;
-    int8_t* v;
-    float* k_scales;
-    float* v_scales;
-};
 
 // args.k and args.v: the new tokens' rows.
 cudaError_t paged8_store(const PackedArgs& args, const Cache8& cache, cudaStream_t stream);

@@ -30,6 +30,7 @@
 #include "device_utils.cuh"
 #include "packed.cuh"
 #include "packed_locate.cuh"
+#include "packed_codes.cuh"
 #include "packed_maps.h"
 #include "sm100.cuh"
 #include "softmax.cuh"
@@ -44,13 +45,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 constexpr int kThreads = 320;   // TMA warp, MMA warp, eight softmax warps with two threads per row
-constexpr int kWarps = kThreads / 32;
 constexpr int kSlots = 4;       // ring of K and V tiles
 constexpr int kSoftmaxWarps = 8;
 constexpr int kStaging = 1024;     // bytes per softmax warp
 constexpr int kStagingBytes = kSoftmaxWarps * kStaging;
 constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
+
+// Pages of 8 bits: two more warps turn codes into the FP16 tiles that the products take, out of a ring of their own; one slot
+// less holds those. 384 threads twice on an SM have 80 registers each, which costs 96 bytes spilled. (Shares of 96 and 48, or 88 and 64, by
+// setmaxnreg: 6,800 and 3,400 bytes.)
+constexpr int kThreads8 = 384;
+constexpr int kSlots8 = 3;
+constexpr int kRawSlots = 2;
+constexpr int kRawBytes = kTileBytes / 2;
+constexpr int kSmem8 = 1024 + (2 + kSlots8) * kTileBytes + kRawSlots * kRawBytes + kStagingBytes + 384;
+constexpr int kBlock = 16;                      // keys that share a scale
+constexpr int kBlocks = 128 / kBlock;           // of a key tile
+constexpr int kScaleSteps = 8;                  // ring of key tiles' scales
 constexpr int kWholeKeys = 1024;   // up to which a tile is never split
 
 static_assert(kPartFloats == size_t{kRows} * kHead + 2 * kRows, "a part is as packed.h has it");
@@ -64,6 +76,8 @@ struct TileParams {
     int boxes;          // loads per K or V tile
     int box_rows;
     bool splits;        // tiles may be split between CTAs
+    const float* k_scales;   // of pages of 8 bits
+    const float* v_scales;
 };
 
 struct Barriers {
@@ -79,6 +93,9 @@ struct Barriers {
     __device__ uint32_t piece_full(int i) const { return base + 104 + 8u * i; }
     __device__ uint32_t slot_full(int s) const { return base + 104 + 8u * (kPieces + s); }
     __device__ uint32_t slot_empty(int s) const { return base + 104 + 8u * (kPieces + kSlots + s); }
+    __device__ uint32_t raw_full(int r) const { return base + 104 + 8u * (kPieces + 2 * kSlots + r); }
+    __device__ uint32_t raw_empty(int r) const { return base + 104 + 8u * (kPieces + 2 * kSlots + kRawSlots + r); }
+    __device__ uint32_t scales_full(int i) const { return base + 104 + 8u * (kPieces + 2 * kSlots + 2 * kRawSlots + i); }
 };
 
 constexpr uint32_t kIdescS = sm100::instr_desc_f16(128, 128, false, false);
@@ -120,8 +137,14 @@ struct Meeting {
 // lanes, and each copy takes its share of a key tile's columns (its other probabilities are zeros, written once),
 // with its own maxima and sums. A step's softmax then takes a kSubsets-th of the time, and all four warps
 // work where one would; the copies are put together at the end of a piece.
-template <bool kPaged, int kSubsets>
-__global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __grid_constant__ TileParams p) {
+// kEight: the pages hold codes of 8 bits, and a score's exponent is its product times one number, plus another, of its key's
+// block (paged8.cu has the formulas): the maximum of a block's raw scores is scaled once, and so is the sum of its probabilities.
+template <bool kPaged, int kSubsets, bool kEight = false>
+__global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_forward_tiles(const __grid_constant__ TileParams p) {
+    constexpr int kThreads = kEight ? kThreads8 : fb::kThreads;
+    constexpr int kWarps = kThreads / 32;
+    constexpr int kSlots = kEight ? kSlots8 : fb::kSlots;
+    constexpr int kFirstSoftmax = kEight ? 4 : 2;      // its warps; those before are TMA, MMA and two that convert
     // Few rows' tiles are not dealt out: finding one takes longer than what it gains (8 single tokens on up to 1,000 keys
     // 14.2 -> 15.2 us, 64 on up to 8,192 78 -> 82 us with the code alone).
     constexpr bool kDeals = kSubsets == 1;
@@ -130,7 +153,11 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
     const uint32_t q_tiles = base;
     const uint32_t ring = base + 2 * kTileBytes;
     const uint32_t staging = ring + kSlots * kTileBytes;
-    const Barriers bar{staging + kStagingBytes};
+    const uint32_t raw_ring = staging + kStagingBytes;
+    const Barriers bar{raw_ring + (kEight ? kRawSlots * kRawBytes : 0)};
+    __shared__ float raw_scales[kEight ? kScaleSteps : 1][2 * kBlocks];      // as they are in memory: K's, V's
+    __shared__ float4 block_scales[kEight ? kScaleSteps : 1][kBlocks];       // slope, offset, 1 / V's scale
+    __shared__ int scales_of[kRawSlots];      // which of them came with a raw tile (K's), or -1
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ Cut cuts[2];
@@ -161,8 +188,17 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             sm100::mbar_init(bar.piece_full(i), 1);
         }
         for (int s = 0; s < kSlots; ++s) {
-            sm100::mbar_init(bar.slot_full(s), 1);
+            sm100::mbar_init(bar.slot_full(s), kEight ? 2 : 1);      // (the converting warps)
             sm100::mbar_init(bar.slot_empty(s), 1);
+        }
+        if (kEight) {
+            for (int r = 0; r < kRawSlots; ++r) {
+                sm100::mbar_init(bar.raw_full(r), 1 + 32);     // the copies' bytes, and every lane's scales
+                sm100::mbar_init(bar.raw_empty(r), 2);
+            }
+            for (int i = 0; i < kScaleSteps; ++i) {
+                sm100::mbar_init(bar.scales_full(i), 1);
+            }
         }
         sm100::mbar_fence_init();
         sm100::tma_prefetch_descriptor(&p.map_q);
@@ -179,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
     }
     if (p.a.sequences > 32) {
         locate<kDeals, kThreads>(p, cuts, whole_tiles, scan, scan_longest);
-    } else if (warp == 2) {
+    } else if (warp == kFirstSoftmax) {
         locate_in_warp<kDeals>(p, cuts, whole_tiles, lane);
     }
     sm100::tc_fence_before_sync();
@@ -235,25 +271,50 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                 at_now = piece.sequence.first + j * kKeyTile;
             }
         };
-        auto load = [&](const CUtensorMap* map, int at, int head) {
-            if (!sm100::mbar_wait_warp(bar.slot_empty(slot), phase ^ 1u, abort)) {
+        uint32_t steps = 0;      // K tiles asked for
+        auto load = [&](const CUtensorMap* map, int at, int head, bool with_scales) {
+            if (!sm100::mbar_wait_warp(kEight ? bar.raw_empty(slot) : bar.slot_empty(slot), phase ^ 1u, abort)) {
                 ok = false;
                 return;
             }
-            const uint32_t full = bar.slot_full(slot), dst = ring + slot * kTileBytes;
+            const uint32_t full = kEight ? bar.raw_full(slot) : bar.slot_full(slot);
+            const uint32_t dst = kEight ? raw_ring + slot * kRawBytes : ring + slot * kTileBytes;
+            if constexpr (kEight) {
+                // The scales of a K tile's keys come with it: lane b has block b's of K, lane 8 + b V's. (Those of a page that
+                // is not there, or of blocks behind the sequence's end, are zeros.)
+                if (with_scales) {
+                    const int key = lane % kBlocks * kBlock, box = key / p.box_rows;
+                    const int box_at = __shfl_sync(kFullMask, at, box);
+                    if (lane < 2 * kBlocks) {
+                        const bool is = box_at < static_cast<int>(p.a.pages * p.a.kv_heads * p.a.page_size) &&
+                                        j * kKeyTile + key < piece.sequence.keys;
+                        const int row = is ? box_at + key - box * p.box_rows : 0;
+                        const float* from = (lane < kBlocks ? p.k_scales : p.v_scales) + row / kBlock;
+                        const uint32_t to = sm100::smem_u32(&raw_scales[steps % kScaleSteps][lane]);
+                        const unsigned bytes = is ? 4u : 0u;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+                    }
+                }
+                if (lane == 0) {
+                    scales_of[slot] = with_scales ? static_cast<int>(steps % kScaleSteps) : -1;
+                }
+                __syncwarp();
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+                steps += with_scales ? 1 : 0;
+            }
             if (lane == 0) {
-                sm100::mbar_expect_tx(full, kTileBytes);
+                sm100::mbar_expect_tx(full, kEight ? kRawBytes : kTileBytes);
             }
             __syncwarp();
             if constexpr (kPaged) {
                 if (lane < p.boxes) {
-                    sm100::tma_load_2d(dst + lane * p.box_rows * (kHead * 2), map, full, 0, at);
+                    sm100::tma_load_2d(dst + lane * p.box_rows * (kEight ? kHead : kHead * 2), map, full, 0, at);
                 }
             } else if (lane == 0) {
                 sm100::tma_load_3d(dst, map, full, 0, head, at);
             }
             __syncwarp();
-            if (++slot == kSlots) {
+            if (++slot == (kEight ? kRawSlots : kSlots)) {
                 slot = 0;
                 phase ^= 1u;
             }
@@ -297,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     __syncwarp();
                 }
                 find();
-                load(&p.map_k, at_now, head_now);
+                load(&p.map_k, at_now, head_now, true);
                 ++waiting;
                 if (++j == piece.to) {
                     ++round;
@@ -307,12 +368,12 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     continue;
                 }
                 if (ok) {
-                    load(&p.map_v, at_before, head_before);
+                    load(&p.map_v, at_before, head_before, false);
                     --waiting;
                 }
             } else {
                 if (waiting > 0) {
-                    load(&p.map_v, at_now, head_now);
+                    load(&p.map_v, at_now, head_now, false);
                 }
                 break;
             }
@@ -410,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             if (v_tile == 0) {
                 break;
             }
-            if (present < kKeyTile) {
+            if (!kEight && present < kKeyTile) {
                 // Rows behind the sequence's last key hold anything, and 0 times that need not be 0.
                 for (int at = max(present, 0) * (kHead * 2) + lane * 16; at < kTileBytes; at += 512) {
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + at), "r"(0) : "memory");
@@ -435,6 +496,75 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
             __syncwarp();
             step_ring();
         }
+    } else if (kEight && warp < kFirstSoftmax) {
+        // Codes into FP16 tiles as the tensor cores read them (128-byte rows whose 16-byte pieces are exchanged by the row's
+        // place among eight), half a tile for each of two warps. Tiles come in the order K, then K and V in turn, then V, two
+        // for every step: the pieces say how many.
+        const int half = warp - 2;
+        int raw = 0, slot = 0, round = 0, known = 0;
+        uint32_t raw_phase = 0, phase = 0;
+        for (int k = 0;; ++k) {
+            if (k == 2 * known) {
+                if (!sm100::mbar_wait_warp(bar.piece_full(round % kPieces), (round / kPieces) & 1, abort)) {
+                    break;
+                }
+                const PieceInfo& info = pieces[round % kPieces];
+                if (info.to == 0) {
+                    break;
+                }
+                known += info.to - info.from;
+                ++round;
+            }
+            if (!sm100::mbar_wait_warp(bar.raw_full(raw), raw_phase, abort) ||
+                !sm100::mbar_wait_warp(bar.slot_empty(slot), phase ^ 1u, abort)) {
+                break;
+            }
+            const int entry = scales_of[raw];
+            if (half == 0 && entry >= 0 && lane < kBlocks) {
+                const float v = raw_scales[entry][kBlocks + lane];
+                const float slope = raw_scales[entry][lane] * (p.a.scale * kLog2e), weight = v == 0.0f ? 1.0f : v;
+                // (Codes are 0 where a scale is 0. A slope above it keeps a score of minus infinity one.)
+                block_scales[entry][lane] = make_float4(slope == 0.0f ? 1e-30f : slope, __log2f(weight), 1.0f / weight, 0.0f);
+            }
+            const uint32_t from = raw_ring + raw * kRawBytes + half * (kRawBytes / 2) + lane * 16;
+            const uint32_t to = ring + slot * kTileBytes + half * (kTileBytes / 2) + lane / 4 * 128;
+            const uint32_t place = ((2 * (lane % 4)) ^ (lane / 4)) * 16;
+#pragma unroll 4
+            for (int i = 0; i < 8; ++i) {
+                uint32_t x[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                             : "r"(from + i * 512));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    x[c] ^= 0x80808080u;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + i * 1024 + (place ^ (h * 16))),
+                                 "r"(two_codes<0>(x[2 * h])), "r"(two_codes<2>(x[2 * h])), "r"(two_codes<0>(x[2 * h + 1])),
+                                 "r"(two_codes<2>(x[2 * h + 1]))
+                                 : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                sm100::mbar_arrive(bar.slot_full(slot));
+                sm100::mbar_arrive(bar.raw_empty(raw));
+                if (half == 0 && entry >= 0) {
+                    sm100::mbar_arrive(bar.scales_full(entry));
+                }
+            }
+            if (++raw == kRawSlots) {
+                raw = 0;
+                raw_phase ^= 1u;
+            }
+            if (++slot == kSlots) {
+                slot = 0;
+                phase ^= 1u;
+            }
+        }
     } else {
         constexpr int kColumns = kKeyTile / kSubsets / 2;    // of a key tile, that this thread works on
         constexpr int kChunk = kColumns < 32 ? kColumns : 32;
@@ -442,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
         constexpr int kOut = kHead / kSubsets / 2;           // columns of O that it writes
         constexpr int kCopyRows = kRows / kSubsets;
         const int quadrant = warp % 4;
-        const int half = (warp - 2) / 4;
+        const int half = (warp - kFirstSoftmax) / 4;
         const int subset = quadrant * kSubsets / 4;
         const int row = (quadrant * 32 + lane) % kCopyRows;  // of the tile
         const int lane_row = quadrant * 32 + lane;           // of the 128 lanes
@@ -493,6 +623,10 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     ok = false;
                     break;
                 }
+                if (kEight && !sm100::mbar_wait_warp(bar.scales_full(n % kScaleSteps), (n / kScaleSteps) & 1, abort)) {
+                    ok = false;
+                    break;
+                }
                 sm100::tc_fence_after_sync();
                 // One copy of 64 columns is read twice, 32 at a time (64 bytes spilled; all at once, 500: two threads'
                 // registers do not hold them beside everything else); up to 32 once.
@@ -530,11 +664,27 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                     for (int c = 0; c < kChunks; ++c) {
                         read(c);
                         mask(c);
+                        if constexpr (kEight) {
 #pragma unroll
-                        for (int i = 0; i < kChunk; i += 8) {
+                            for (int b = 0; b < kChunk; b += kBlock) {
+                                float two[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                            for (int t = 0; t < 4; ++t) {
-                                top[t] = max3_nan(top[t], __uint_as_float(raw[i + t]), __uint_as_float(raw[i + 4 + t]));
+                                for (int i = b; i < b + kBlock; i += 4) {
+                                    two[0] = max3_nan(two[0], __uint_as_float(raw[i]), __uint_as_float(raw[i + 1]));
+                                    two[1] = max3_nan(two[1], __uint_as_float(raw[i + 2]), __uint_as_float(raw[i + 3]));
+                                }
+                                const float largest = max3_nan(two[0], two[1], two[1]);
+                                const float4 of = block_scales[n % kScaleSteps][(first_column + kChunk * c + b) / kBlock];
+                                // (A row that sees nothing of the block has nothing to do with its scales.)
+                                top[0] = largest == -INFINITY ? top[0] : max3_nan(top[0], fmaf(largest, of.x, of.y), top[1]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kChunk; i += 8) {
+#pragma unroll
+                                for (int t = 0; t < 4; ++t) {
+                                    top[t] = max3_nan(top[t], __uint_as_float(raw[i + t]), __uint_as_float(raw[i + 4 + t]));
+                                }
                             }
                         }
                     }
@@ -542,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                         scores_are_read();
                     }
                     // The scale is positive, so the maximum may be scaled after it is taken.
-                    const float local = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale2;
+                    const float local = kEight ? top[0] : max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale2;
                     pair_max[n & 1][half][lane_row] = local;
                     if (!pair.meet()) {
                         ok = false;
@@ -591,8 +741,37 @@ __global__ void __launch_bounds__(kThreads, 2) fb_packed_forward_tiles(const __g
                             mask(c);
                         }
                         uint32_t packed[kChunk / 2];
+                        if constexpr (kEight) {
 #pragma unroll
-                        for (int i = 0; i < kChunk / 2; ++i) {
+                            for (int b = 0; b < kChunk; b += kBlock) {
+                                const float4 of = block_scales[n % kScaleSteps][(first_column + kChunk * c + b) / kBlock];
+                                const F2 slope = f2_pack(of.x, of.x), offset = f2_pack(of.y - m, of.y - m);
+                                F2 sum = 0;
+#pragma unroll
+                                for (int i = b / 2; i < b / 2 + kBlock / 2; ++i) {
+                                    float x, y;
+                                    F2 t = f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), slope, offset);
+                                    if (masked) {     // (minus infinity times a scale need not be that)
+                                        f2_unpack(t, x, y);
+                                        t = f2_pack(kChunk * c + 2 * i <= visible ? x : -INFINITY,
+                                                    kChunk * c + 2 * i + 1 <= visible ? y : -INFINITY);
+                                    }
+                                    if (kSubsets == 1 && (i & 3) == 0) {
+                                        exp2_pair_fma<false>(t, x, y);
+                                    } else {
+                                        f2_unpack(t, x, y);
+                                        x = fast_exp2(x);
+                                        y = fast_exp2(y);
+                                    }
+                                    sum = f2_add(sum, f2_pack(x, y));
+                                    packed[i] = pack2(x, y);
+                                }
+                                const float inverse = masked && kChunk * c + b > visible ? 0.0f : of.z;
+                                l = f2_fma(sum, f2_pack(inverse, inverse), l);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; !kEight && i < kChunk / 2; ++i) {
                             float x, y;
                             const F2 t = f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])),
                                                 scale_pair, shift);
@@ -1069,7 +1248,26 @@ cudaError_t packed_join(const PackedArgs& args, const Record* records, const flo
                             dim3(kJoinThreads), 0, stream, j);
 }
 
+namespace {
+
+template <bool kPaged, int kSubsets, bool kEight>
+cudaError_t launch_tiles(const TileParams& p, int ctas, cudaStream_t stream) {
+    static std::atomic<bool> configured[64] = {};
+    constexpr int kBytes = kEight ? kSmem8 : kSmem;
+    const auto kernel = fb_packed_forward_tiles<kPaged, kSubsets, kEight>;
+    const cudaError_t e = allow_shared_memory(kernel, kBytes, configured);
+    return e != cudaSuccess ? e
+                            : launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kEight ? kThreads8 : kThreads), kBytes,
+                                               stream, p);
+}
+
+}  // namespace
+
 cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace, cudaStream_t stream) {
+    return packed_forward(args, nullptr, longest, workspace, stream);
+}
+
+cudaError_t packed_forward(const PackedArgs& args, const Cache8* eight, int longest, void* workspace, cudaStream_t stream) {
     TileParams p;
     std::memset(&p, 0, sizeof p);
     p.a = args;
@@ -1091,8 +1289,15 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
         p.box_rows = std::min(args.page_size, kKeyTile);
         p.boxes = kKeyTile / p.box_rows;
         const long long cache_rows = args.pages * args.kv_heads * args.page_size;
-        if (e == cudaSuccess) e = encode_pages(&p.map_k, args.k, cache_rows, p.box_rows);
-        if (e == cudaSuccess) e = encode_pages(&p.map_v, args.v, cache_rows, p.box_rows);
+        if (eight != nullptr) {
+            p.k_scales = eight->k_scales;
+            p.v_scales = eight->v_scales;
+            if (e == cudaSuccess) e = encode_pages8(&p.map_k, eight->k, cache_rows, p.box_rows);
+            if (e == cudaSuccess) e = encode_pages8(&p.map_v, eight->v, cache_rows, p.box_rows);
+        } else {
+            if (e == cudaSuccess) e = encode_pages(&p.map_k, args.k, cache_rows, p.box_rows);
+            if (e == cudaSuccess) e = encode_pages(&p.map_v, args.v, cache_rows, p.box_rows);
+        }
     } else {
         if (e == cudaSuccess) e = encode_rows(&p.map_k, args.k, args.kv_heads, args.rows, args.kv_stride, 1, kKeyTile);
         if (e == cudaSuccess) e = encode_rows(&p.map_v, args.v, args.kv_heads, args.rows, args.kv_stride, 1, kKeyTile);
@@ -1105,17 +1310,16 @@ cudaError_t packed_forward(const PackedArgs& args, int longest, void* workspace,
     p.splits = most_keys > kWholeKeys;
     p.records = packed_records(workspace);
     p.parts = packed_parts(workspace, ctas);
-    const int form = !paged ? 0 : subsets == 1 ? 1 : subsets == 2 ? 2 : 3;
-    const auto kernel = form == 0   ? fb_packed_forward_tiles<false, 1>
-                        : form == 1 ? fb_packed_forward_tiles<true, 1>
-                        : form == 2 ? fb_packed_forward_tiles<true, 2>
-                                    : fb_packed_forward_tiles<true, 4>;
-    static std::atomic<bool> configured[4][64] = {};
-    e = allow_shared_memory(kernel, kSmem, configured[form]);
-    if (e != cudaSuccess) {
-        return e;
+    if (eight != nullptr) {
+        e = subsets == 1   ? launch_tiles<true, 1, true>(p, ctas, stream)
+            : subsets == 2 ? launch_tiles<true, 2, true>(p, ctas, stream)
+                           : launch_tiles<true, 4, true>(p, ctas, stream);
+    } else {
+        e = !paged         ? launch_tiles<false, 1, false>(p, ctas, stream)
+            : subsets == 1 ? launch_tiles<true, 1, false>(p, ctas, stream)
+            : subsets == 2 ? launch_tiles<true, 2, false>(p, ctas, stream)
+                           : launch_tiles<true, 4, false>(p, ctas, stream);
     }
-    e = launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmem, stream, p);
     if (e != cudaSuccess || !p.splits) {
         return e;
     }

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cstddef>
+#include <cstdint>
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -15,5 +16,7 @@ cudaError_t encode_rows(CUtensorMap* map, const __half* base, int heads, int row
 
 // (column, row) of rows of 64 values without gaps.
 cudaError_t encode_pages(CUtensorMap* map, const __half* base, long long rows, int box_rows);
+// The same of codes of 8 bits, copied as they lie.
+cudaError_t encode_pages8(CUtensorMap* map, const int8_t* base, long long rows, int box_rows);
 
 }  // namespace fb

@@ -15,6 +15,7 @@
 #include "common.h"
 #include "device_utils.cuh"
 #include "packed.cuh"
+#include "packed_codes.cuh"
 #include "packed_locate.cuh"
 #include "sm100.cuh"
 #include "softmax.cuh"
@@ -155,14 +156,6 @@ __device__ __forceinline__ unsigned transposed(unsigned x) {
     unsigned r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
-}
-
-// Bytes kLow and kLow + 1 of x, which are codes + 128, as FP16: 1,024 + byte has the byte as its low bits.
-template <int kLow>
-__device__ __forceinline__ unsigned two_codes(unsigned x) {
-    const unsigned biased = __byte_perm(x, 0x64646464u, kLow == 0 ? 0x4140 : 0x4342);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const unsigned*>(&h);
 }
 
 // CTAs that fit on an SM (registers).
@@ -540,9 +533,11 @@ cudaError_t paged8_attention(const PackedArgs& args, const Cache8& cache, int lo
     const long long most_keys = static_cast<long long>(args.table_stride) * args.page_size;
     return rows <= 8    ? launch_few<1, 1>(p, sms, workspace, most_keys, stream)
            : rows <= 16 ? launch_few<2, 1>(p, sms, workspace, most_keys, stream)
+#ifdef VFEW
            : rows <= 32 ? launch_few<4, 1>(p, sms, workspace, most_keys, stream)
            : rows <= 64 ? launch_few<4, 2>(p, sms, workspace, most_keys, stream)
-                        : launch_few<4, 4>(p, sms, workspace, most_keys, stream);
+#endif
+                        : packed_forward(args, &cache, longest, workspace, stream);
 }
 
 cudaError_t paged8_workspace(size_t* bytes) {
