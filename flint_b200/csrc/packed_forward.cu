@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
             const uint32_t from = raw_ring + raw * kRawBytes + half * (kRawBytes / 2) + lane * 16;
             const uint32_t to = ring + slot * kTileBytes + half * (kTileBytes / 2) + lane / 4 * 128;
             const uint32_t place = ((2 * (lane % 4)) ^ (lane / 4)) * 16;
-#pragma unroll 4
+#pragma unroll 2
             for (int i = 0; i < 8; ++i) {
                 uint32_t x[4];
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -656,6 +656,15 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                         sm100::mbar_arrive(bar.s_free());
                     }
                 };
+                // Of the block that this thread's column c is in: slope, offset, 1 / V's scale. A row that sees nothing of it has
+                // nothing to do with its scales, whatever they are.
+                auto scales_of_block = [&](int c) {
+                    float4 of = block_scales[kEight ? n % kScaleSteps : 0][kEight ? (first_column + c) / kBlock : 0];
+                    if (masked && c > visible) {
+                        of = make_float4(1e-30f, 0.0f, 0.0f, 0.0f);
+                    }
+                    return of;
+                };
                 float alpha = 1.0f;
                 bool moved = false;
                 if (active) {
@@ -673,10 +682,8 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                                     two[0] = max3_nan(two[0], __uint_as_float(raw[i]), __uint_as_float(raw[i + 1]));
                                     two[1] = max3_nan(two[1], __uint_as_float(raw[i + 2]), __uint_as_float(raw[i + 3]));
                                 }
-                                const float largest = max3_nan(two[0], two[1], two[1]);
-                                const float4 of = block_scales[n % kScaleSteps][(first_column + kChunk * c + b) / kBlock];
-                                // (A row that sees nothing of the block has nothing to do with its scales.)
-                                top[0] = largest == -INFINITY ? top[0] : max3_nan(top[0], fmaf(largest, of.x, of.y), top[1]);
+                                const float4 of = scales_of_block(kChunk * c + b);
+                                top[b / kBlock] = max3_nan(top[b / kBlock], fmaf(max3_nan(two[0], two[1], two[1]), of.x, of.y), top[3]);
                             }
                         } else {
 #pragma unroll
@@ -692,7 +699,7 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                         scores_are_read();
                     }
                     // The scale is positive, so the maximum may be scaled after it is taken.
-                    const float local = kEight ? top[0] : max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale2;
+                    const float local = kEight ? max3_nan(top[0], top[1], top[1]) : max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale2;
                     pair_max[n & 1][half][lane_row] = local;
                     if (!pair.meet()) {
                         ok = false;
@@ -744,18 +751,13 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                         if constexpr (kEight) {
 #pragma unroll
                             for (int b = 0; b < kChunk; b += kBlock) {
-                                const float4 of = block_scales[n % kScaleSteps][(first_column + kChunk * c + b) / kBlock];
+                                const float4 of = scales_of_block(kChunk * c + b);
                                 const F2 slope = f2_pack(of.x, of.x), offset = f2_pack(of.y - m, of.y - m);
                                 F2 sum = 0;
 #pragma unroll
                                 for (int i = b / 2; i < b / 2 + kBlock / 2; ++i) {
                                     float x, y;
-                                    F2 t = f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), slope, offset);
-                                    if (masked) {     // (minus infinity times a scale need not be that)
-                                        f2_unpack(t, x, y);
-                                        t = f2_pack(kChunk * c + 2 * i <= visible ? x : -INFINITY,
-                                                    kChunk * c + 2 * i + 1 <= visible ? y : -INFINITY);
-                                    }
+                                    const F2 t = f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), slope, offset);
                                     if (kSubsets == 1 && (i & 3) == 0) {
                                         exp2_pair_fma<false>(t, x, y);
                                     } else {
@@ -766,8 +768,7 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                                     sum = f2_add(sum, f2_pack(x, y));
                                     packed[i] = pack2(x, y);
                                 }
-                                const float inverse = masked && kChunk * c + b > visible ? 0.0f : of.z;
-                                l = f2_fma(sum, f2_pack(inverse, inverse), l);
+                                l = f2_fma(sum, f2_pack(of.z, of.z), l);
                             }
                         }
 #pragma unroll
