@@ -211,6 +211,61 @@ __device__ __forceinline__ void locate_in_warp(const P& p, Cut (&cuts)[2], int& 
     }
 }
 
+// The same for up to 32 kEach sequences, lane l having a run of them, where tiles are not dealt out.
+template <int kEach, typename P>
+__device__ __forceinline__ void locate_runs_in_warp(const P& p, Cut (&cuts)[2], int lane) {
+    const int each = (p.a.sequences + 31) / 32;
+    int before[kEach], tokens[kEach];
+    long long length[kEach], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        length[i] = length_of(p, i < each ? lane * each + i : p.a.sequences, before[i], tokens[i]);
+        mine += length[i] * p.a.kv_heads;
+    }
+    const long long upto = warp_prefix(mine, lane);
+    const long long total = __shfl_sync(kFullMask, upto, 31);
+    const Place place(p, total, lane & 1);
+    int owner[2], its_sequence[2], its_before[2], its_tokens[2];
+    long long its_length[2], its_begin[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const long long at = __shfl_sync(kFullMask, place.at, c);
+        const unsigned has = __ballot_sync(kFullMask, at >= upto - mine && at < upto);
+        owner[c] = has != 0 ? __ffs(has) - 1 : -1;
+        // This lane's sequence that it would be.
+        long long begin = upto - mine;
+        int k = 0;
+        its_before[c] = before[0];
+        its_tokens[c] = tokens[0];
+        its_length[c] = length[0];
+#pragma unroll
+        for (int i = 1; i < kEach; ++i) {
+            const long long next = begin + length[i - 1] * p.a.kv_heads;
+            if (k == i - 1 && at >= next) {
+                k = i;
+                begin = next;
+                its_before[c] = before[i];
+                its_tokens[c] = tokens[i];
+                its_length[c] = length[i];
+            }
+        }
+        const int from = max(owner[c], 0);
+        its_sequence[c] = __shfl_sync(kFullMask, lane * each + k, from);
+        its_before[c] = __shfl_sync(kFullMask, its_before[c], from);
+        its_tokens[c] = __shfl_sync(kFullMask, its_tokens[c], from);
+        its_length[c] = __shfl_sync(kFullMask, its_length[c], from);
+        its_begin[c] = __shfl_sync(kFullMask, begin, from);
+    }
+    if (lane < 2) {
+        const bool second = lane == 1;
+        cuts[lane] = (second ? owner[1] : owner[0]) < 0
+                         ? Cut{total, p.a.sequences, 0, 0, 0}
+                         : cut_at(place.at, place.at - (second ? its_begin[1] : its_begin[0]), second ? its_sequence[1] : its_sequence[0],
+                                  second ? its_before[1] : its_before[0], second ? its_tokens[1] : its_tokens[0], p.log_tokens,
+                                  second ? its_length[1] : its_length[0], place.tolerance);
+    }
+}
+
 // The same for any number: every thread of the block takes part.
 template <bool kDeals, int kThreads, typename P>
 __device__ __noinline__ void locate(const P& p, Cut (&cuts)[2], int& whole, long long (&scan)[kThreads / 32 + 1],

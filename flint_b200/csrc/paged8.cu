@@ -23,9 +23,6 @@
 namespace fb {
 namespace {
 
-#ifndef VPS
-#define VPS 3
-#endif
 constexpr int kHead = 64;
 constexpr int kBlock = 16;      // positions that share a scale
 constexpr float kLog2e = 1.4426950408889634f;
@@ -127,13 +124,12 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
 // that a lane has just turned into FP16 in its registers, where the tensor cores' larger instruction would want
 // them written to shared memory first. Keys are the products' rows and queries their columns, eight of them to a
 // product: S^T = K Q^T, O^T = V^T P^T. With 16 rows of queries instead, a group of four heads would leave three quarters of the
-// exponentials to nobody. A tile (packed_schedule.h) has up to 8 kTiles kSplit rows, of which a warp takes every kSplit-th eight, and
-// every (8 / kSplit)-th block of 16 keys, whose codes come to it alone through stages of asynchronous copies; the
-// warps' sums meet at the end of a piece.
+// exponentials to nobody. A tile (packed_schedule.h) has up to 8 kTiles rows; a warp takes every eighth unit of one or two blocks of 16
+// keys, whose codes come to it alone through stages of asynchronous copies, and the warps' sums meet at the end of a piece. (Two blocks
+// at a time where registers allow: one's products run under the other's conversions.)
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStages = 4;
-constexpr int kStageBytes = 2 * kBlock * kHead;       // K and V of a block
+constexpr int kBlockBytes = 2 * kBlock * kHead;       // K and V of a block
 constexpr int kMergeStride = kHead + 4;               // floats between rows that meet
 
 struct FewParams {
@@ -158,48 +154,52 @@ __device__ __forceinline__ unsigned transposed(unsigned x) {
     return r;
 }
 
-// CTAs that fit on an SM (registers).
-constexpr int few_per_sm(int tiles) { return tiles > 2 ? 1 : tiles == 2 ? 2 : VPS; }
-constexpr int kMostPerSm = VPS;
+constexpr int kFewPerSm = 2;     // CTAs on an SM (registers)
 
-template <int kTiles, int kSplit>
+template <int kTiles>
 struct FewMemory {
-    static constexpr int kRows = 8 * kTiles * kSplit;
-    static constexpr int kOf = 8 * kTiles;            // rows of a warp
+    static constexpr int kRows = 8 * kTiles;
+    static constexpr int kUnit = 2;        // blocks at a time
+    static constexpr int kStages = 3;
     union {
-        unsigned char ring[kWarps][kStages][kStageBytes];
-        float merge[kWarps][kOf][kMergeStride];       // (in the ring's place at the end of a piece)
+        unsigned char ring[kWarps][kStages][kUnit][kBlockBytes];
+        float merge[kWarps][kRows][kMergeStride];       // (in the ring's place at the end of a piece)
     };
-    uint4 queries[kTiles * kSplit][2][32];
+    uint4 queries[kTiles][2][32];
     int position[kRows];
-    float merge_max[kWarps][kOf], merge_sum[kWarps][kOf];
+    float merge_max[kWarps][kRows], merge_sum[kWarps][kRows];
     Cut cuts[2];
     long long scan[kWarps + 1];
     int scan_longest[kWarps];
     int whole_tiles;
 };
 
-template <int kTiles, int kSplit>
-__global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(const FewParams p) {
-    using Memory = FewMemory<kTiles, kSplit>;
-    constexpr int kApart = kWarps / kSplit;      // warps that share rows
+template <int kTiles>
+__global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewParams p) {
+    using Memory = FewMemory<kTiles>;
+    constexpr int kUnit = Memory::kUnit, kStages = Memory::kStages;
+    constexpr int kBatch = 32 / kUnit;           // units whose places the lanes hold
+    constexpr int kUnitKeys = kUnit * kBlock;
     extern __shared__ __align__(128) unsigned char memory[];
     Memory& shared = *reinterpret_cast<Memory*>(memory);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x / 32), 0), lane = threadIdx.x % 32;
     const int g = lane / 4, t = lane % 4;        // row and column of the products' fragments
     dependency_wait();
-    if (p.a.sequences > 32) {
+    if (p.a.sequences > 128) {
         locate<false, kThreads>(p, shared.cuts, shared.whole_tiles, shared.scan, shared.scan_longest);
     } else if (warp == 0) {
-        locate_in_warp<false>(p, shared.cuts, shared.whole_tiles, lane);
+        if (p.a.sequences > 32) {
+            locate_runs_in_warp<4>(p, shared.cuts, lane);
+        } else {
+            locate_in_warp<false>(p, shared.cuts, shared.whole_tiles, lane);
+        }
     }
     __syncthreads();
     dependency_release();
     if (threadIdx.x == 0) {
         p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, shared.cuts[0], shared.cuts[1]);
     }
-    const int split = warp % kSplit, share = warp / kSplit;
-    const unsigned char* stages = &shared.ring[warp][0][0];
+    const unsigned char* stages = &shared.ring[warp][0][0][0];
     const uint32_t stages_at = sm100::smem_u32(stages);
     const float scale2 = p.a.scale * kLog2e;
     Walk walk;
@@ -208,52 +208,55 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
     while (walk.next(SequenceOf{p.a}, p.a.sequences, p.a.kv_heads, p.log_tokens, piece)) {
         const int first_position = piece.position();
         const int first_block = piece.from * (kKeyTile / kBlock);
-        const int end_block = min(piece.to * (kKeyTile / kBlock), (piece.sequence.keys + kBlock - 1) / kBlock);
+        const int blocks = min(piece.to * (kKeyTile / kBlock), (piece.sequence.keys + kBlock - 1) / kBlock) - first_block;
         const int rows = piece.tokens * p.group;
-        const int tiles = (rows + 7) / 8;                          // of eight rows
-        const int mine = (tiles - split + kSplit - 1) / kSplit;    // of them this warp's, from `split` on
-        // This warp's blocks: first_block + share + i kApart.
-        const int count = mine <= 0 ? 0 : max(0, (end_block - first_block - share + kApart - 1) / kApart);
-        // Lane i has the place of block 32 batch + i (the row of its first key in the cache, -1 for none) and what its scales
-        // come to.
+        const int tiles = (rows + 7) / 8;        // of eight rows
+        // This warp's units: warp + 8 i.
+        const int count = max(0, ((blocks + kUnit - 1) / kUnit - warp + kWarps - 1) / kWarps);
+        // Lane i has the place of the i-th block of a batch (the row of its first key in the cache, -1 for none) and what its
+        // scales come to.
         auto place_of = [&](int i) {
-            if (i >= count) {
+            const int block = (warp + i / kUnit * kWarps) * kUnit + i % kUnit;
+            if (block >= blocks) {
                 return -1;
             }
-            const int key = (first_block + share + i * kApart) * kBlock;
+            const int key = (first_block + block) * kBlock;
             const long long page = page_of(p.a, piece.index, key);
             return page < 0 ? -1
                             : static_cast<int>((page * p.a.kv_heads + piece.head) << p.log_page) + (key & (p.a.page_size - 1));
         };
         int place_next = place_of(lane), place = -1;
         float k_next = 0.0f, v_next = 0.0f, slope_of = 0.0f, offset_of = 0.0f, inverse_of = 0.0f;
-        auto fetch = [&](int i) {
+        auto fetch = [&](int i, int stage) {
             if (i < count) {
-                if (i % 32 == 0) {
+                if (i % kBatch == 0) {
                     place = place_next;
                     k_next = v_next = 0.0f;
                     if (place >= 0) {
                         k_next = p.cache.k_scales[place / kBlock];
                         v_next = p.cache.v_scales[place / kBlock];
                     }
-                    place_next = place_of(i + 32 + lane);
+                    place_next = place_of(i * kUnit + 32 + lane);
                 }
-                const int from = __shfl_sync(kFullMask, place, i % 32);
-                const uint32_t to = stages_at + (i % kStages) * kStageBytes + lane * 16;
-                const unsigned bytes = from >= 0 ? 16u : 0u;       // zeros for a page that is not there
-                const long long at = static_cast<long long>(max(from, 0)) * kHead + lane * 16;
-                const int8_t* k = p.cache.k + at;
-                const int8_t* v = p.cache.v + at;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(k), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512), "l"(k + 512), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 1024), "l"(v), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 1536), "l"(v + 512), "r"(bytes) : "memory");
+#pragma unroll
+                for (int b = 0; b < kUnit; ++b) {
+                    const int from = __shfl_sync(kFullMask, place, i % kBatch * kUnit + b);
+                    const uint32_t to = stages_at + (stage * kUnit + b) * kBlockBytes + lane * 16;
+                    const unsigned bytes = from >= 0 ? 16u : 0u;       // zeros for a page that is not there
+                    const long long at = static_cast<long long>(max(from, 0)) * kHead + lane * 16;
+                    const int8_t* k = p.cache.k + at;
+                    const int8_t* v = p.cache.v + at;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(k), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512), "l"(k + 512), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 1024), "l"(v), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 1536), "l"(v + 512), "r"(bytes) : "memory");
+                }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) {
-            fetch(i);
+            fetch(i, i);
         }
         // Queries as they are multiplied: of eight rows, lane (g, t) has the 16 values from 16 t on of row g, four of
         // which are a product's term with the four codes that lie beside each other in a key.
@@ -282,8 +285,12 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
                 out[n][j][0] = out[n][j][1] = out[n][j][2] = out[n][j][3] = 0.0f;
             }
         }
+        // Of the products' rows the even ones are keys 0 to 3 and the odd ones 4 to 7, and so on: V's are then read four in
+        // a row at a time below.
+        const int low = (g & 1) * 4 + (g >> 1);      // key of the product's row g; 8 more for row g + 8
+        int stage = 0;
         for (int i = 0; i < count; ++i) {
-            if (i % 32 == 0) {
+            if (i % kBatch == 0) {
                 const float v = v_next == 0.0f ? 1.0f : v_next;      // (codes are 0 then)
                 slope_of = k_next * scale2;
                 offset_of = __log2f(v);
@@ -291,19 +298,21 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             __syncwarp();       // everybody's copies have landed, and the stage before is read
-            fetch(i + kStages - 1);
-            const unsigned char* stage = stages + (i % kStages) * kStageBytes;
-            const int key = (first_block + share + i * kApart) * kBlock;
-            const bool masked = key + kBlock - 1 > first_position;
-            const float slope = __shfl_sync(kFullMask, slope_of, i % 32), offset = __shfl_sync(kFullMask, offset_of, i % 32);
-            const float inverse = __shfl_sync(kFullMask, inverse_of, i % 32);
-            // Of the products' rows the even ones are keys 0 to 3 and the odd ones 4 to 7, and so on: V's are then read four in
-            // a row at a time below.
-            const int low = (g & 1) * 4 + (g >> 1);      // key of the product's row g; 8 more for row g + 8
-            float scores[kTiles][4];
-            {
-                const uint4 first = *reinterpret_cast<const uint4*>(stage + low * kHead + 16 * t);
-                const uint4 second = *reinterpret_cast<const uint4*>(stage + (8 + low) * kHead + 16 * t);
+            fetch(i + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+            const unsigned char* codes = stages + stage * (kUnit * kBlockBytes);
+            const int key = first_block * kBlock + (warp + i * kWarps) * kUnitKeys;
+            const bool masked = key + kUnitKeys - 1 > first_position;
+            float slope[kUnit], offset[kUnit], inverse[kUnit];
+            float scores[kTiles][kUnit][4];
+#pragma unroll
+            for (int b = 0; b < kUnit; ++b) {
+                const int of = i % kBatch * kUnit + b;
+                slope[b] = __shfl_sync(kFullMask, slope_of, of);
+                offset[b] = __shfl_sync(kFullMask, offset_of, of);
+                inverse[b] = __shfl_sync(kFullMask, inverse_of, of);
+                const unsigned char* k = codes + b * kBlockBytes;
+                const uint4 first = *reinterpret_cast<const uint4*>(k + low * kHead + 16 * t);
+                const uint4 second = *reinterpret_cast<const uint4*>(k + (8 + low) * kHead + 16 * t);
                 const unsigned x[4] = {first.x ^ 0x80808080u, first.y ^ 0x80808080u, first.z ^ 0x80808080u, first.w ^ 0x80808080u};
                 const unsigned y[4] = {second.x ^ 0x80808080u, second.y ^ 0x80808080u, second.z ^ 0x80808080u,
                                        second.w ^ 0x80808080u};
@@ -317,22 +326,23 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
                 }
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n) {
-                    scores[n][0] = scores[n][1] = scores[n][2] = scores[n][3] = 0.0f;
-                    if (kTiles == 1 || n < mine) {
-                        const uint4 q0 = shared.queries[n * kSplit + split][0][lane], q1 = shared.queries[n * kSplit + split][1][lane];
-                        mma_16816(scores[n], keys[0], q0.x, q0.y);
-                        mma_16816(scores[n], keys[1], q0.z, q0.w);
-                        mma_16816(scores[n], keys[2], q1.x, q1.y);
-                        mma_16816(scores[n], keys[3], q1.z, q1.w);
+                    scores[n][b][0] = scores[n][b][1] = scores[n][b][2] = scores[n][b][3] = 0.0f;
+                    if (kTiles == 1 || n < tiles) {
+                        const uint4 q0 = shared.queries[n][0][lane], q1 = shared.queries[n][1][lane];
+                        mma_16816(scores[n][b], keys[0], q0.x, q0.y);
+                        mma_16816(scores[n][b], keys[1], q0.z, q0.w);
+                        mma_16816(scores[n][b], keys[2], q1.x, q1.y);
+                        mma_16816(scores[n][b], keys[3], q1.z, q1.w);
                     }
                 }
             }
-            unsigned values[4][4];       // of the products with V: rows g and g + 8 are columns 8 g + 2 j and 8 g + 2 j + 1
-            {
-                uint2 read[4];           // keys t, t + 4, t + 8 and t + 12
+            unsigned values[kUnit][4][4];    // of the products with V: rows g and g + 8 are columns 8 g + 2 j and 8 g + 2 j + 1
+#pragma unroll
+            for (int b = 0; b < kUnit; ++b) {
+                uint2 read[4];               // keys t, t + 4, t + 8 and t + 12
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    read[k] = *reinterpret_cast<const uint2*>(stage + kBlock * kHead + (4 * k + t) * kHead + 8 * g);
+                    read[k] = *reinterpret_cast<const uint2*>(codes + b * kBlockBytes + kBlock * kHead + (4 * k + t) * kHead + 8 * g);
                     read[k].x ^= 0x80808080u;
                     read[k].y ^= 0x80808080u;
                 }
@@ -343,31 +353,37 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
                                                  : __byte_perm(read[0].y, read[1].y, j % 2 == 0 ? 0x5140 : 0x7362);
                     const unsigned second = j < 2 ? __byte_perm(read[2].x, read[3].x, j % 2 == 0 ? 0x5140 : 0x7362)
                                                   : __byte_perm(read[2].y, read[3].y, j % 2 == 0 ? 0x5140 : 0x7362);
-                    values[j][0] = two_codes<0>(first);
-                    values[j][1] = two_codes<2>(first);
-                    values[j][2] = two_codes<0>(second);
-                    values[j][3] = two_codes<2>(second);
+                    values[b][j][0] = two_codes<0>(first);
+                    values[b][j][1] = two_codes<2>(first);
+                    values[b][j][2] = two_codes<0>(second);
+                    values[b][j][3] = two_codes<2>(second);
                 }
             }
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
-                if (kTiles > 1 && n >= mine) {
+                if (kTiles > 1 && n >= tiles) {
                     break;
                 }
-                // Lane (g, t) has keys `low` and low + 8 of rows 2 t and 2 t + 1.
-                float (&x)[4] = scores[n];
+                // Lane (g, t) has keys `low` and low + 8 of each block, of rows 2 t and 2 t + 1.
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    x[c] = fmaf(x[c], slope, offset);
+                for (int b = 0; b < kUnit; ++b) {
+                    float (&x)[4] = scores[n][b];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        x[c] = fmaf(x[c], slope[b], offset[b]);
+                    }
+                    if (masked) {
+                        const int2 position = *reinterpret_cast<const int2*>(&shared.position[n * 8 + 2 * t]);
+                        const int here = key + b * kBlock + low;
+                        x[0] = here <= position.x ? x[0] : -INFINITY;
+                        x[1] = here <= position.y ? x[1] : -INFINITY;
+                        x[2] = here + 8 <= position.x ? x[2] : -INFINITY;
+                        x[3] = here + 8 <= position.y ? x[3] : -INFINITY;
+                    }
+                    top[0] = max_nan(top[0], max_nan(x[0], x[2]));
+                    top[1] = max_nan(top[1], max_nan(x[1], x[3]));
                 }
-                if (masked) {
-                    const int2 position = *reinterpret_cast<const int2*>(&shared.position[(n * kSplit + split) * 8 + 2 * t]);
-                    x[0] = key + low <= position.x ? x[0] : -INFINITY;
-                    x[1] = key + low <= position.y ? x[1] : -INFINITY;
-                    x[2] = key + low + 8 <= position.x ? x[2] : -INFINITY;
-                    x[3] = key + low + 8 <= position.y ? x[3] : -INFINITY;
-                }
-                float top[2] = {max_nan(x[0], x[2]), max_nan(x[1], x[3])};
                 if (__any_sync(kFullMask, !(top[0] - m[n][0] <= kLazyShift) || !(top[1] - m[n][1] <= kLazyShift))) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -386,32 +402,33 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    x[c] = fast_exp2(x[c] - m[n][c % 2]);
-                }
-                if (masked) {
-                    // (A row that sees nothing of the block has nothing to do with its scale, whatever that is.)
-                    l[n][0] = fmaf(x[0] + x[2], x[0] + x[2] == 0.0f ? 0.0f : inverse, l[n][0]);
-                    l[n][1] = fmaf(x[1] + x[3], x[1] + x[3] == 0.0f ? 0.0f : inverse, l[n][1]);
-                } else {
-                    l[n][0] = fmaf(x[0] + x[2], inverse, l[n][0]);
-                    l[n][1] = fmaf(x[1] + x[3], inverse, l[n][1]);
-                }
-                const unsigned b0 = transposed(pack2(x[0], x[1])), b1 = transposed(pack2(x[2], x[3]));
+                for (int b = 0; b < kUnit; ++b) {
+                    float (&x)[4] = scores[n][b];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    mma_16816(out[n][j], values[j], b0, b1);
+                    for (int c = 0; c < 4; ++c) {
+                        x[c] = fast_exp2(x[c] - m[n][c % 2]);
+                    }
+                    const float sum0 = x[0] + x[2], sum1 = x[1] + x[3];
+                    // (A row that sees nothing of the block has nothing to do with its scale, whatever that is.)
+                    l[n][0] = fmaf(sum0, masked && sum0 == 0.0f ? 0.0f : inverse[b], l[n][0]);
+                    l[n][1] = fmaf(sum1, masked && sum1 == 0.0f ? 0.0f : inverse[b], l[n][1]);
+                    const unsigned b0 = transposed(pack2(x[0], x[1])), b1 = transposed(pack2(x[2], x[3]));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        mma_16816(out[n][j], values[b][j], b0, b1);
+                    }
                 }
             }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();       // the ring is everybody's from here on
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
-            if (n < mine) {
+            if (n < tiles) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const int row = 8 * n + 2 * t + c;      // of this warp's
+                    const int row = 8 * n + 2 * t + c;
                     l[n][c] += __shfl_xor_sync(kFullMask, l[n][c], 4);
                     l[n][c] += __shfl_xor_sync(kFullMask, l[n][c], 8);
                     l[n][c] += __shfl_xor_sync(kFullMask, l[n][c], 16);
@@ -430,21 +447,19 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
         const bool whole = piece.from == 0 && piece.to == piece.tiles;
         for (int row = threadIdx.x / 16; row < rows; row += kThreads / 16) {
             const int column = threadIdx.x % 16 * 4;
-            const int its_split = row / 8 % kSplit, its_row = row / (8 * kSplit) * 8 + row % 8;
             float all = kNoKey;
 #pragma unroll
-            for (int w = 0; w < kApart; ++w) {
-                all = max_nan(all, shared.merge_max[w * kSplit + its_split][its_row]);
+            for (int w = 0; w < kWarps; ++w) {
+                all = max_nan(all, shared.merge_max[w][row]);
             }
             float total = 0.0f;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kApart; ++w) {
-                const int its = w * kSplit + its_split;
-                const float top = shared.merge_max[its][its_row], factor = fast_exp2(top - all);
-                const float4 x = *reinterpret_cast<const float4*>(&shared.merge[its][its_row][column]);
+            for (int w = 0; w < kWarps; ++w) {
+                const float top = shared.merge_max[w][row], factor = fast_exp2(top - all);
+                const float4 x = *reinterpret_cast<const float4*>(&shared.merge[w][row][column]);
                 if (top != kNoKey) {
-                    total = fmaf(shared.merge_sum[its][its_row], factor, total);
+                    total = fmaf(shared.merge_sum[w][row], factor, total);
                     sum.x = fmaf(x.x, factor, sum.x);
                     sum.y = fmaf(x.y, factor, sum.y);
                     sum.z = fmaf(x.z, factor, sum.z);
@@ -475,20 +490,20 @@ __global__ void __launch_bounds__(kThreads, few_per_sm(kTiles)) fb_paged8_few(co
     }
 }
 
-template <int kTiles, int kSplit>
+template <int kTiles>
 cudaError_t launch_few(FewParams p, int sms, void* workspace, long long most_keys, cudaStream_t stream) {
-    const int ctas = std::min(few_per_sm(kTiles) * sms, kMostPackedCtas);
+    const int ctas = std::min(kFewPerSm * sms, kMostPackedCtas);
     p.records = packed_records(workspace);
     p.parts = packed_parts(workspace, ctas);
     p.splits = most_keys > 1024;
-    constexpr int kBytes = sizeof(FewMemory<kTiles, kSplit>);
-    while ((2 << p.log_tokens) * p.group <= FewMemory<kTiles, kSplit>::kRows) {
+    constexpr int kBytes = sizeof(FewMemory<kTiles>);
+    while ((2 << p.log_tokens) * p.group <= FewMemory<kTiles>::kRows) {
         ++p.log_tokens;
     }
     static std::atomic<bool> configured[64] = {};
-    cudaError_t e = allow_shared_memory(fb_paged8_few<kTiles, kSplit>, kBytes, configured);
+    cudaError_t e = allow_shared_memory(fb_paged8_few<kTiles>, kBytes, configured);
     if (e == cudaSuccess) {
-        e = launch_dependent(fb_paged8_few<kTiles, kSplit>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kBytes, stream, p);
+        e = launch_dependent(fb_paged8_few<kTiles>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kBytes, stream, p);
     }
     if (e != cudaSuccess || !p.splits) {
         return e;
@@ -531,19 +546,15 @@ cudaError_t paged8_attention(const PackedArgs& args, const Cache8& cache, int lo
         return e;
     }
     const long long most_keys = static_cast<long long>(args.table_stride) * args.page_size;
-    return rows <= 8    ? launch_few<1, 1>(p, sms, workspace, most_keys, stream)
-           : rows <= 16 ? launch_few<2, 1>(p, sms, workspace, most_keys, stream)
-#ifdef VFEW
-           : rows <= 32 ? launch_few<4, 1>(p, sms, workspace, most_keys, stream)
-           : rows <= 64 ? launch_few<4, 2>(p, sms, workspace, most_keys, stream)
-#endif
+    return rows <= 8    ? launch_few<1>(p, sms, workspace, most_keys, stream)
+           : rows <= 16 ? launch_few<2>(p, sms, workspace, most_keys, stream)
                         : packed_forward(args, &cache, longest, workspace, stream);
 }
 
 cudaError_t paged8_workspace(size_t* bytes) {
     int sms = 148;
     const cudaError_t e = sm_count(&sms);
-    *bytes = packed_workspace(std::min(kMostPerSm * sms, kMostPackedCtas));
+    *bytes = packed_workspace(std::min(kFewPerSm * sms, kMostPackedCtas));
     return e;
 }
 
