@@ -159,14 +159,12 @@ constexpr int kFewPerSm = 2;     // CTAs on an SM (registers)
 template <int kTiles>
 struct FewMemory {
     static constexpr int kRows = 8 * kTiles;
-    static constexpr int kUnit = 2;        // blocks at a time
-    static constexpr int kStages = 3;
-    union {
-        unsigned char ring[kWarps][kStages][kUnit][kBlockBytes];
-        float merge[kWarps][kRows][kMergeStride];       // (in the ring's place at the end of a piece)
-    };
-    uint4 queries[kTiles][2][32];
-    int position[kRows];
+    static constexpr int kUnit = kTiles == 1 ? 2 : 1;        // blocks at a time
+    static constexpr int kStages = kUnit == 2 ? 3 : 5;
+    union {      // a warp's
+        unsigned char ring[kStages][kUnit][kBlockBytes];
+        float merge[kRows][kMergeStride];       // (at the end of a piece)
+    } of[kWarps];
     float merge_max[kWarps][kRows], merge_sum[kWarps][kRows];
     Cut cuts[2];
     long long scan[kWarps + 1];
@@ -175,7 +173,7 @@ struct FewMemory {
 };
 
 template <int kTiles>
-__global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewParams p) {
+__global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const __grid_constant__ FewParams p) {
     using Memory = FewMemory<kTiles>;
     constexpr int kUnit = Memory::kUnit, kStages = Memory::kStages;
     constexpr int kBatch = 32 / kUnit;           // units whose places the lanes hold
@@ -199,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
     if (threadIdx.x == 0) {
         p.records[blockIdx.x] = make_record(SequenceOf{p.a}, p.log_tokens, shared.cuts[0], shared.cuts[1]);
     }
-    const unsigned char* stages = &shared.ring[warp][0][0][0];
+    const unsigned char* stages = &shared.of[warp].ring[0][0][0];
     const uint32_t stages_at = sm100::smem_u32(stages);
     const float scale2 = p.a.scale * kLog2e;
     Walk walk;
@@ -259,21 +257,25 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
             fetch(i, i);
         }
         // Queries as they are multiplied: of eight rows, lane (g, t) has the 16 values from 16 t on of row g, four of
-        // which are a product's term with the four codes that lie beside each other in a key.
-        for (int i = threadIdx.x; i < tiles * 64; i += kThreads) {
-            const int row = i / 64 * 8 + i % 32 / 4, token = row / p.group;
-            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        // which are a product's term with the four codes that lie beside each other in a key. Its scores are of rows 2 t and
+        // 2 t + 1, whose positions it has.
+        uint4 query[kTiles][2];
+        int position[kTiles][2];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            const int row = 8 * n + g, token = row / p.group;
+            query[n][0] = query[n][1] = make_uint4(0u, 0u, 0u, 0u);
             if (row < rows) {
                 const __half* from = p.a.q + (static_cast<long long>(piece.sequence.first) + piece.first_token + token) * p.a.q_stride +
-                                     (piece.head * p.group + row - token * p.group) * kHead + 16 * (i % 4);
-                q = reinterpret_cast<const uint4*>(from)[i / 32 % 2];
+                                     (piece.head * p.group + row - token * p.group) * kHead + 16 * t;
+                query[n][0] = reinterpret_cast<const uint4*>(from)[0];
+                query[n][1] = reinterpret_cast<const uint4*>(from)[1];
             }
-            shared.queries[i / 64][i / 32 % 2][i % 32] = q;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                position[n][c] = 8 * n + 2 * t + c < rows ? first_position + (8 * n + 2 * t + c) / p.group : -1;
+            }
         }
-        for (int row = threadIdx.x; row < tiles * 8; row += kThreads) {
-            shared.position[row] = row < rows ? first_position + row / p.group : -1;
-        }
-        __syncthreads();
         float m[kTiles][2], l[kTiles][2];
         float out[kTiles][4][4];
 #pragma unroll
@@ -328,11 +330,10 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
                 for (int n = 0; n < kTiles; ++n) {
                     scores[n][b][0] = scores[n][b][1] = scores[n][b][2] = scores[n][b][3] = 0.0f;
                     if (kTiles == 1 || n < tiles) {
-                        const uint4 q0 = shared.queries[n][0][lane], q1 = shared.queries[n][1][lane];
-                        mma_16816(scores[n][b], keys[0], q0.x, q0.y);
-                        mma_16816(scores[n][b], keys[1], q0.z, q0.w);
-                        mma_16816(scores[n][b], keys[2], q1.x, q1.y);
-                        mma_16816(scores[n][b], keys[3], q1.z, q1.w);
+                        mma_16816(scores[n][b], keys[0], query[n][0].x, query[n][0].y);
+                        mma_16816(scores[n][b], keys[1], query[n][0].z, query[n][0].w);
+                        mma_16816(scores[n][b], keys[2], query[n][1].x, query[n][1].y);
+                        mma_16816(scores[n][b], keys[3], query[n][1].z, query[n][1].w);
                     }
                 }
             }
@@ -374,12 +375,11 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
                         x[c] = fmaf(x[c], slope[b], offset[b]);
                     }
                     if (masked) {
-                        const int2 position = *reinterpret_cast<const int2*>(&shared.position[n * 8 + 2 * t]);
                         const int here = key + b * kBlock + low;
-                        x[0] = here <= position.x ? x[0] : -INFINITY;
-                        x[1] = here <= position.y ? x[1] : -INFINITY;
-                        x[2] = here + 8 <= position.x ? x[2] : -INFINITY;
-                        x[3] = here + 8 <= position.y ? x[3] : -INFINITY;
+                        x[0] = here <= position[n][0] ? x[0] : -INFINITY;
+                        x[1] = here <= position[n][1] ? x[1] : -INFINITY;
+                        x[2] = here + 8 <= position[n][0] ? x[2] : -INFINITY;
+                        x[3] = here + 8 <= position[n][1] ? x[3] : -INFINITY;
                     }
                     top[0] = max_nan(top[0], max_nan(x[0], x[2]));
                     top[1] = max_nan(top[1], max_nan(x[1], x[3]));
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();       // the ring is everybody's from here on
+        __syncwarp();          // this warp's part of the ring is read
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
             if (n < tiles) {
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
                         shared.merge_sum[warp][row] = l[n][c];
                     }
                     // Column 8 g + 2 j of the row is out[j][c], column 8 g + 2 j + 1 out[j][2 + c].
-                    float4* to = reinterpret_cast<float4*>(&shared.merge[warp][row][8 * g]);
+                    float4* to = reinterpret_cast<float4*>(&shared.of[warp].merge[row][8 * g]);
                     to[0] = make_float4(out[n][0][c], out[n][0][2 + c], out[n][1][c], out[n][1][2 + c]);
                     to[1] = make_float4(out[n][2][c], out[n][2][2 + c], out[n][3][c], out[n][3][2 + c]);
                 }
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float top = shared.merge_max[w][row], factor = fast_exp2(top - all);
-                const float4 x = *reinterpret_cast<const float4*>(&shared.merge[w][row][column]);
+                const float4 x = *reinterpret_cast<const float4*>(&shared.of[w].merge[row][column]);
                 if (top != kNoKey) {
                     total = fmaf(shared.merge_sum[w][row], factor, total);
                     sum.x = fmaf(x.x, factor, sum.x);
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const FewPa
                 }
             }
         }
-        __syncthreads();       // the ring is the copies' again
+        __syncthreads();       // the rings are the copies' again
     }
 }
 
