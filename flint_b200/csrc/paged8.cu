@@ -46,16 +46,10 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
             const int which = static_cast<int>(item % 2);
             const int head = static_cast<int>(item / 2 % p.kv_heads);
             const int key = (low + static_cast<int>(item / 2 / p.kv_heads)) * kBlock;      // the block's first
-            const long long page = page_of(p, s, key);
-            if (page < 0) {
-                continue;
-            }
             const __half* from = (which == 0 ? p.k : p.v) + head * kHead;
-            const long long row = (page * p.kv_heads + head) * p.page_size + key % p.page_size;
-            int8_t* codes = (which == 0 ? cache.k : cache.v) + row * kHead;
-            float* scale_at = (which == 0 ? cache.k_scales : cache.v_scales) + row / kBlock;
+            // What the steps below need is asked for at once: the new rows beside the page's number, what the block holds
+            // beside its scale.
             uint4 held[4];
-            float largest = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = key + 4 * r + of_four - begins;      // of the new tokens
@@ -63,6 +57,27 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
                 if (i >= 0 && i < q.count) {
                     held[r] = reinterpret_cast<const uint4*>(from + (q.first + static_cast<long long>(i)) * p.kv_stride)[piece];
                 }
+            }
+            const long long page = page_of(p, s, key);
+            if (page < 0) {
+                continue;
+            }
+            const long long row = (page * p.kv_heads + head) * p.page_size + key % p.page_size;
+            int8_t* codes = (which == 0 ? cache.k : cache.v) + row * kHead;
+            float* scale_at = (which == 0 ? cache.k_scales : cache.v_scales) + row / kBlock;
+            const bool kept = begins > key;
+            const float before = kept ? *scale_at : 0.0f;
+            uint2 old[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                old[r] = make_uint2(0u, 0u);
+                if (key + 4 * r + of_four < begins) {
+                    old[r] = reinterpret_cast<const uint2*>(codes + (4 * r + of_four) * kHead)[piece];
+                }
+            }
+            float largest = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
                 float v[8];
                 unpack8(v, held[r]);
 #pragma unroll
@@ -76,12 +91,8 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
             }
             // (An infinity counts as NaN.)
             float scale = largest <= 65504.0f ? __fdiv_rn(largest, 127.0f) : __int_as_float(0x7fffffff);
-            float before = 0.0f;
-            if (begins > key) {
-                before = *scale_at;
-                scale = max_nan(before, scale);
-            }
-            const bool grows = begins > key && scale != before;     // (a NaN grows: codes of it are 0)
+            scale = kept ? max_nan(before, scale) : scale;
+            const bool grows = kept && scale != before;     // (a NaN grows: codes of it are 0)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = key + 4 * r + of_four - begins;
@@ -94,8 +105,7 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
                 if (fresh) {
                     unpack8(v, held[r]);
                 } else {
-                    const uint2 old = *to;
-                    const unsigned w[2] = {old.x, old.y};
+                    const unsigned w[2] = {old[r].x, old[r].y};
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         v[c] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[c / 4] >> (8 * (c % 4)))), before);

@@ -23,6 +23,7 @@ constexpr int kChunkBytes = 8192;      // that a block copies at a time
 // Up to which pools and tables are small (their kernels' comments).
 constexpr int kSmallPages = 32768;
 constexpr int kSmallEntries = 8 * 8192;
+constexpr int kNone = INT_MIN;         // no entry
 
 __device__ int g_pages_error = 0;
 
@@ -33,14 +34,14 @@ struct Pool {
 // Numbers out of range are passed over and reported.
 __device__ __forceinline__ void report() { atomicExch(&g_pages_error, 1); }
 
-__device__ __forceinline__ int length_of(const Pool& pool, const int* lengths, int s) {
-    const int given = lengths[s];
+__device__ __forceinline__ int in_range(const Pool& pool, int given) {
     const int length = min(max(given, 0), pool.stride << pool.log_size);
     if (length != given) {
         report();
     }
     return length;
 }
+__device__ __forceinline__ int length_of(const Pool& pool, const int* lengths, int s) { return in_range(pool, lengths[s]); }
 __device__ __forceinline__ int entries_of(const Pool& pool, int length) {
     return (length + pool.size - 1) >> pool.log_size;
 }
@@ -187,33 +188,60 @@ __global__ void __launch_bounds__(kThreads) fb_pages_fork_small(const ForkArgs p
         p.next_references[page] = p.references[page];
     }
     constexpr int kEach = kSmallEntries / (kRanks * kThreads);
-    int had[kEach], gets[kEach];      // the page that an entry had, and the one that it gets; -1 for none
+    // An entry's place in its row, its parent and both lengths, then the page that it had and the one that it gets: each step's
+    // loads together, ahead of the first store, which they would otherwise have to wait for.
+    int place[kEach], parent[kEach], had[kEach], gets[kEach];
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-        const int i = first + k * kRanks * kThreads;
         had[k] = gets[k] = -1;
+        if (k * kRanks * kThreads >= entries) {
+            continue;
+        }
+        const int i = first + k * kRanks * kThreads;
+        const int t = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride));
+        place[k] = i - t * p.pool.stride;
+        parent[k] = i < entries ? p.parents[t] : -1;
+        had[k] = i < entries ? p.lengths[t] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (k * kRanks * kThreads >= entries) {
+            continue;
+        }
+        const bool has = parent[k] >= 0 && parent[k] < p.pool.sequences;
+        if (!has && parent[k] != -1) {
+            report();
+        }
+        parent[k] = has ? parent[k] : -1;
+        gets[k] = has ? p.lengths[parent[k]] : 0;
+    }
+    int length[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (k * kRanks * kThreads >= entries) {
+            continue;
+        }
+        const int i = first + k * kRanks * kThreads;
+        length[k] = in_range(p.pool, gets[k]);
+        const bool old = i < entries && place[k] < entries_of(p.pool, in_range(p.pool, had[k]));
+        const bool now = i < entries && place[k] < entries_of(p.pool, length[k]);
+        had[k] = old ? p.table[i] : kNone;
+        gets[k] = now ? p.table[parent[k] * p.pool.stride + place[k]] : kNone;
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (k * kRanks * kThreads >= entries) {
+            continue;
+        }
+        const int i = first + k * kRanks * kThreads;
         if (i < entries) {
-            const int t = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride));
-            const int e = i - t * p.pool.stride, parent = p.parents[t];
-            const bool has = parent >= 0 && parent < p.pool.sequences;
-            if (!has && parent != -1) {
-                report();
-            }
-            const int length = has ? length_of(p.pool, p.lengths, parent) : 0;
-            int page = -1;
-            if (e < entries_of(p.pool, length)) {
-                page = p.table[parent * p.pool.stride + e];
-                gets[k] = is_page(p.pool, page) ? page : -1;
-            }
-            p.next_table[i] = page;
-            if (e == 0) {
-                p.next_lengths[t] = length;
-            }
-            if (e < entries_of(p.pool, length_of(p.pool, p.lengths, t))) {
-                page = p.table[i];
-                had[k] = is_page(p.pool, page) ? page : -1;
+            p.next_table[i] = gets[k] == kNone ? -1 : gets[k];
+            if (place[k] == 0) {
+                p.next_lengths[static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride)] = length[k];
             }
         }
+        had[k] = had[k] != kNone && is_page(p.pool, had[k]) ? had[k] : -1;
+        gets[k] = gets[k] != kNone && is_page(p.pool, gets[k]) ? gets[k] : -1;
     }
     meet();
 #pragma unroll
@@ -665,7 +693,8 @@ struct CopyArgs {
     unsigned char* base[kMostArrays];
 };
 
-// Blocks take chunks of 8 KB, of one array and move each: bound by HBM.
+// Blocks take chunks of 8 KB, of one array and move each: bound by HBM. Neither end is read again soon, which the loads and stores
+// say (1,150 moves of 397 KB 189 us with the compaction, 179 so; chunks of 16 KB 181).
 __global__ void __launch_bounds__(256) fb_pages_copy(const __grid_constant__ CopyArgs p) {
     fb::dependency_wait();
     fb::dependency_release();
@@ -694,19 +723,20 @@ __global__ void __launch_bounds__(256) fb_pages_copy(const __grid_constant__ Cop
         const unsigned char* source = p.base[low] + static_cast<size_t>(from) * bytes + begin;
         unsigned char* target = p.base[low] + static_cast<size_t>(to) * bytes + begin;
         if (bytes % 16 == 0) {
-            uint4 held[2];
+            constexpr int kWords = kChunkBytes / (256 * 16);
+            uint4 held[kWords];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kWords; ++i) {
                 const unsigned at = (i * 256 + threadIdx.x) * 16;
                 if (at < here) {
-                    held[i] = *reinterpret_cast<const uint4*>(source + at);
+                    held[i] = __ldcs(reinterpret_cast<const uint4*>(source + at));
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kWords; ++i) {
                 const unsigned at = (i * 256 + threadIdx.x) * 16;
                 if (at < here) {
-                    *reinterpret_cast<uint4*>(target + at) = held[i];
+                    __stcs(reinterpret_cast<uint4*>(target + at), held[i]);
                 }
             }
         } else {
