@@ -186,7 +186,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs p) {
     using R = Row<T>;
     __shared__ Key lists[kWarps][kCandidates];
-    __shared__ float group_max[kWarps][kGroups][32];
+    __shared__ T group_max[kWarps][kGroups][32];      // (a maximum of FP16 values is one)
     __shared__ int claimed;
     const int lane = static_cast<int>(threadIdx.x) % 32, warp = __shfl_sync(fb::kFullMask, static_cast<int>(threadIdx.x) / 32, 0);
     const int all_words = (p.vocab + R::kValues - 1) / R::kValues;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
                 }
             }
             const float mx = running.value();
-            group_max[warp][group++][lane] = mx;
+            group_max[warp][group++][lane] = static_cast<T>(mx);
             second_group = fmaxf(second_group, fminf(best_group, mx));
             best_group = fmaxf(best_group, mx);
         }
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs 
         unsigned mask = 0;
 #pragma unroll 4
         for (int g = 0; g < group; ++g) {
-            mask |= group_max[warp][g][lane] >= bound ? 1u << g : 0u;
+            mask |= static_cast<float>(group_max[warp][g][lane]) >= bound ? 1u << g : 0u;
         }
         int count = 0;
         bool overflow = false;
@@ -438,11 +438,10 @@ __device__ __forceinline__ Key order_total(double v) {
 
 constexpr int kBins = 64;
 constexpr int kMostEntries = 4096;   // of a group's lists
-constexpr int kFewEntries = 512, kSomeEntries = 1024;
 
 // The bound leaves entries of at most `beams` bins, each with those of its threads.
-__host__ __device__ constexpr int most_left(int entries, int beams) {
-    return beams * (kThreads / kBins) * ((entries + kThreads - 1) / kThreads);
+__host__ __device__ constexpr int most_left(int entries, int beams, int threads) {
+    return beams * (threads / kBins) * ((entries + threads - 1) / threads);
 }
 
 struct Candidate {
@@ -492,8 +491,10 @@ struct Beams {
 };
 
 // kHeldEntries: of a group's lists, per thread.
-template <int kHeldEntries>
-__global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_groups(const GroupArgs p) {
+// (Blocks of 128 threads for few entries: 1,000 groups of 5 beams are on the GPU at once then, XX us where 256 threads take 13.6.)
+template <int kThreads, int kHeldEntries>
+__global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThreads) fb_beam_groups(const GroupArgs p) {
+    constexpr int kWarps = kThreads / 32;
     extern __shared__ __align__(16) unsigned char left_memory[];
     __shared__ Beams of;
     __shared__ float2 stats[kMostLists];
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_gr
     fb::dependency_release();
     const long long first = static_cast<long long>(blockIdx.x) * p.beams;
     const int lists = p.beams * p.parts, entries = lists * p.beams, of_beam = p.parts * p.beams;
-    const int most = most_left(entries, p.beams);
+    const int most = most_left(entries, p.beams, kThreads);
     Key* left_rank = reinterpret_cast<Key*>(left_memory);
     double* left_total = reinterpret_cast<double*>(left_rank + most);
     unsigned* left_place = reinterpret_cast<unsigned*>(left_total + most);
@@ -517,8 +518,8 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_gr
     for (int i = 0; i < kHeldEntries; ++i) {
         held[i] = tid + i * kThreads < entries ? keys[tid + i * kThreads] : 0;
     }
-    if (tid < lists) {
-        stats[tid] = p.stats[first * p.parts + tid];
+    for (int i = tid; i < lists; i += kThreads) {
+        stats[i] = p.stats[first * p.parts + i];
     }
     // A warp takes the beams' lengths while others wait for statistics.
     if (warp == kWarps - 1 && lane < p.beams) {
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_gr
             const double grown = of.over[lane] != 0 ? max(of.length[lane], 1) : static_cast<double>(of.length[lane]) + 1.0;
             of.weight[lane] = p.power == 0.0f ? 1.0 : weight_of(grown, static_cast<double>(p.power));
         }
-    } else if (warp < kMostBeams * kLanes / 32) {
+    } else if (warp * (32 / kLanes) < p.beams) {
         float m = kLowest, sum = 0.0f;
         const int its = min(beam, p.beams - 1) * p.parts;
         for (int i = tid % kLanes; i < p.parts; i += kLanes) {
@@ -693,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 5) fb_beam_gr
     }
 }
 
-// Parts of a row: those with which the warps are done soonest, each part costing four chunks more than it has; never so many that
+// Parts of a row: those with which the warps are done soonest, each part costing three chunks more than it has; never so many that
 // a group has more than kMostLists or kMostEntries, or the GPU more than kMostRounds parts per warp on their account.
 constexpr int kMostRounds = 8;
 unsigned warps_of(int sms) { return static_cast<unsigned>(sms * kBlocks * kWarps); }
@@ -705,10 +706,10 @@ int parts_of(int words, size_t rows, int beams, int sms) {
     unsigned best = 1;
     float least = 0.0f;
     for (unsigned parts = 1; parts == 1 || (parts <= most && words / parts >= 32); ++parts) {
-        // (A block's warps are done at about the same time, half a part apart.)
+        // (A block's warps are done about a part apart: 5,000 rows 102.6 us so, 106.1 with half a part.)
         const float items = static_cast<float>(rows) * parts / static_cast<float>(warps);
         const unsigned chunks = ((words + parts - 1) / parts + kChunk - 1) / kChunk;
-        const float cost = (items <= 1.0f ? 1.0f : items + 0.5f) * static_cast<float>(chunks + 4);
+        const float cost = (items <= 1.0f ? 1.0f : items + 1.0f) * static_cast<float>(chunks + 3);
         if (parts == 1 || cost < least) {
             best = parts;
             least = cost;
@@ -727,6 +728,18 @@ cudaError_t launch_rows(RowArgs p, size_t rows, int sms, cudaStream_t stream) {
     p.items = static_cast<unsigned>(rows * p.parts);
     const size_t blocks = std::min<size_t>(p.items, static_cast<size_t>(kBlocks) * sms);
     return fb::launch_dependent(fb_beam_rows<T>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
+}
+
+template <int kThreads, int kHeldEntries>
+cudaError_t launch_groups(const GroupArgs& g, size_t groups, int entries, cudaStream_t stream) {
+    constexpr size_t kEach = sizeof(Key) + sizeof(double) + sizeof(unsigned);
+    constexpr int kMostSmem = static_cast<int>(most_left(kThreads * kHeldEntries, kMostBeams, kThreads) * kEach);
+    static std::atomic<bool> configured[64] = {};
+    const auto kernel = fb_beam_groups<kThreads, kHeldEntries>;
+    const cudaError_t e = fb::allow_shared_memory(kernel, kMostSmem, configured);
+    return e != cudaSuccess ? e
+                            : fb::launch_dependent(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads),
+                                                   most_left(entries, g.beams, kThreads) * kEach, stream, g);
 }
 
 constexpr flint_status kBad = FLINT_ERROR_INVALID_ARGUMENT;
@@ -875,15 +888,10 @@ flint_status flint_b200_beam_select(void* next_scores, void* parents, void* toke
     g.power = length_power;
     FB_CUDA(fp32_logits != 0 ? launch_rows<float>(p, rows, sms, stream) : launch_rows<__half>(p, rows, sms, stream));
     const int entries = p.parts * p.beams * p.beams;
-    const size_t smem = static_cast<size_t>(most_left(entries, p.beams)) * (sizeof(Key) + sizeof(double) + sizeof(unsigned));
-    const int form = entries <= kFewEntries ? 0 : entries <= kSomeEntries ? 1 : 2;
-    static std::atomic<bool> configured[3][64] = {};
-    const auto kernel = form == 0   ? fb_beam_groups<kFewEntries / kThreads>
-                        : form == 1 ? fb_beam_groups<kSomeEntries / kThreads>
-                                    : fb_beam_groups<kMostEntries / kThreads>;
-    constexpr int kMostSmem = most_left(kMostEntries, kMostBeams) * (sizeof(Key) + sizeof(double) + sizeof(unsigned));
-    FB_CUDA(fb::allow_shared_memory(kernel, kMostSmem, configured[form]));
-    FB_CUDA(fb::launch_dependent(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), smem, stream, g));
+    FB_CUDA(entries <= 256    ? (launch_groups<128, 2>(g, groups, entries, stream))
+            : entries <= 512  ? (launch_groups<256, 2>(g, groups, entries, stream))
+            : entries <= 1024 ? (launch_groups<256, 4>(g, groups, entries, stream))
+                              : (launch_groups<256, kMostEntries / 256>(g, groups, entries, stream)));
     return FLINT_OK;
 }
 
