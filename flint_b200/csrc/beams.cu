@@ -29,6 +29,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kHeld = 4;             // 16-byte words that a lane has on their way
 constexpr int kBlocks = 4;           // per SM
+static_assert(kHeld * 8 <= 32, "a lane's values of a chunk have a bit each");
 constexpr int kChunk = 32 * kHeld;   // words that a warp works on at a time
 constexpr int kCandidates = 128;     // of a warp
 constexpr int kMany = 96;            // from which on the bound rises
@@ -490,6 +491,44 @@ struct Beams {
     int over[kMostBeams], length[kMostBeams];
 };
 
+// Histories of a warp's new beams, kBeams of them at a time. (Loads first: to the compiler a store may change what is
+// loaded next, and each would wait for the one before.)
+template <int kWarps, int kBeams, int kAtOnce>
+__device__ __forceinline__ void copy_histories(const GroupArgs& p, long long first, const Beams& of,
+                                               const unsigned (&chosen)[kMostBeams], int warp, int lane) {
+    for (int t0 = warp; t0 < p.beams; t0 += kBeams * kWarps) {
+        const uint16_t* from[kBeams];
+        int lengths[kBeams], longest = 0;
+#pragma unroll
+        for (int b = 0; b < kBeams; ++b) {
+            const int t = t0 + b * kWarps;
+            const int parent = t >= p.beams ? 0 : chosen[t] == ~0u ? t : static_cast<int>(chosen[t] >> 16);
+            from[b] = p.histories + (first + parent) * p.history_stride;
+            lengths[b] = t < p.beams ? of.length[parent] : 0;
+            longest = max(longest, lengths[b]);
+        }
+        for (int c = lane; c < longest; c += 32 * kAtOnce) {
+            uint16_t some[kBeams][kAtOnce];
+#pragma unroll
+            for (int b = 0; b < kBeams; ++b) {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    some[b][i] = c + 32 * i < lengths[b] ? from[b][c + 32 * i] : 0;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < kBeams; ++b) {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (c + 32 * i < lengths[b]) {
+                        p.next_histories[(first + t0 + b * kWarps) * p.history_stride + c + 32 * i] = some[b][i];
+                    }
+                }
+            }
+        }
+    }
+}
+
 // kHeldEntries: of a group's lists, per thread.
 // (Blocks of 128 threads for few entries: 1,000 groups of 5 beams are on the GPU at once then, XX us where 256 threads take 13.6.)
 template <int kThreads, int kHeldEntries>
@@ -647,49 +686,38 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         }
     }
     __syncthreads();
-    // A warp per beam: its numbers, and its history.
-    for (int t = warp; t < p.beams; t += kWarps) {
+    // The new beams, a warp each in turn: their histories, and their numbers.
+    if (p.next_histories != nullptr) {
+        if (p.beams <= kWarps) {
+            copy_histories<kWarps, 1, 16>(p, first, of, chosen, warp, lane);
+        } else {
+            copy_histories<kWarps, 4, 4>(p, first, of, chosen, warp, lane);
+        }
+    }
+    if (tid < p.beams) {
+        const int t = tid;
         const bool none = chosen[t] == ~0u;
         const int parent = none ? t : static_cast<int>(chosen[t] >> 16);
         const bool over = of.over[parent] != 0;
         const int token = none ? (over ? max(p.end_token, 0) : 0) : static_cast<int>(chosen[t] & 0xffffu);
         int length = of.length[parent];
         const long long row = first + t;
-        if (p.next_histories != nullptr) {
-            const uint16_t* from = p.histories + (first + parent) * p.history_stride;
-            uint16_t* to = p.next_histories + row * p.history_stride;
-            // (Loads first: to the compiler a store may change what is loaded next, and each would wait for the one before.)
-            constexpr int kAtOnce = 16;
-            for (int c = lane; c < length; c += 32 * kAtOnce) {
-                uint16_t some[kAtOnce];
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    some[i] = c + 32 * i < length ? from[c + 32 * i] : 0;
-                }
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    if (c + 32 * i < length) {
-                        to[c + 32 * i] = some[i];
-                    }
-                }
-            }
-            if (!over && length == p.history_stride) {
+        if (!over && p.next_histories != nullptr) {
+            if (length == p.history_stride) {
                 atomicExch(&g_beams_error, 1);
                 --length;      // (stays as long as it is, and keeps its last token)
-            } else if (!over && lane == 0) {
-                to[length] = static_cast<uint16_t>(token);
+            } else {
+                p.next_histories[row * p.history_stride + length] = static_cast<uint16_t>(token);
             }
         }
-        if (lane == 0) {
-            p.next_scores[row] = none ? -INFINITY : static_cast<float>(chosen_total[t]);
-            p.parents[row] = static_cast<int>(first) + parent;
-            p.tokens[row] = static_cast<uint16_t>(token);
-            if (p.next_finished != nullptr) {
-                p.next_finished[row] = over || token == p.end_token ? 1 : 0;
-            }
-            if (p.next_lengths != nullptr) {
-                p.next_lengths[row] = over ? length : length + 1;
-            }
+        p.next_scores[row] = none ? -INFINITY : static_cast<float>(chosen_total[t]);
+        p.parents[row] = static_cast<int>(first) + parent;
+        p.tokens[row] = static_cast<uint16_t>(token);
+        if (p.next_finished != nullptr) {
+            p.next_finished[row] = over || token == p.end_token ? 1 : 0;
+        }
+        if (p.next_lengths != nullptr) {
+            p.next_lengths[row] = over ? length : length + 1;
         }
     }
 }
