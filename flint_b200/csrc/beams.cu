@@ -10,6 +10,7 @@
 // continuations can be closer than FP32 tells apart; a tie goes to the lower beam, then the lower token.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -466,6 +467,7 @@ __device__ __forceinline__ double log_of(float x) {
 
 // n^-power to about 2^-40, from log n = e log 2 + 2 artanh((f - 1) / (f + 1)) with f from 3/4 to 3/2, and the exponential's series.
 // (Weights that were off by FP32's roundings would move totals past each other; FP64's own power takes 5 us.)
+constexpr float kMostPower = 16.0f;
 __device__ __forceinline__ double weight_of(double n, double power) {
     const long long bits = __double_as_longlong(n);
     const int e = static_cast<int>((bits - 0x3fe8000000000000LL) >> 52);
@@ -474,10 +476,7 @@ __device__ __forceinline__ double weight_of(double n, double power) {
     r = r * (2.0 - (f + 1.0) * r);
     const double s = (f - 1.0) * r, z = s * s, z2 = z * z;
     const double tail = (1.0 / 3 + z * (1.0 / 5)) + z2 * ((1.0 / 7 + z * (1.0 / 9)) + z2 * (1.0 / 11 + z * (1.0 / 13)));
-    const double y = -power * (e * 0.69314718055994531 + 2.0 * s * (1.0 + z * tail));
-    if (!(y > -600.0)) {
-        return pow(n, -power);
-    }
+    const double y = -power * (e * 0.69314718055994531 + 2.0 * s * (1.0 + z * tail));      // above -350: n is below 2^31
     const int k = __double2int_rn(y * 1.4426950408889634);
     const double x = y - k * 0.69314718055994531, x2 = x * x, x4 = x2 * x2;
     const double series = (1.0 + x) + x2 * (1.0 / 2 + x * (1.0 / 6)) +
@@ -564,9 +563,10 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
     if (warp == kWarps - 1 && lane < p.beams) {
         const int over = p.finished != nullptr && p.finished[first + lane] != 0 ? 1 : 0;
         int length = p.lengths != nullptr ? p.lengths[first + lane] : 0;
-        if (length < 0 || (p.histories != nullptr && length > p.history_stride)) {
+        const int most = p.histories != nullptr ? static_cast<int>(p.history_stride) : INT_MAX - 1;
+        if (length < 0 || length > most) {
             atomicExch(&g_beams_error, 1);
-            length = length < 0 ? 0 : static_cast<int>(p.history_stride);
+            length = min(max(length, 0), most);
         }
         const float score = p.scores[first + lane];
         of.over[lane] = over;
@@ -831,9 +831,9 @@ flint_status flint_b200_beam_select(void* next_scores, void* parents, void* toke
     if (end_token < -1 || (end_token >= 0 && static_cast<size_t>(end_token) >= vocab)) {
         return fb::fail(kBad, "%s: end_token (%d) must be -1 or below vocab (%zu)", name, end_token, vocab);
     }
-    if (!std::isfinite(length_power) || length_power < 0.0f) {
-        return fb::fail(kBad, "%s: length_power (%g) must be finite and not negative", name,
-                        static_cast<double>(length_power));
+    if (!(length_power >= 0.0f && length_power <= kMostPower)) {
+        return fb::fail(kBad, "%s: length_power (%g) must be from 0 to %g", name, static_cast<double>(length_power),
+                        static_cast<double>(kMostPower));
     }
     const struct {
         const char* names;

@@ -798,6 +798,12 @@ size_t table_bytes(const Pool& pool) { return static_cast<size_t>(pool.sequences
 size_t row_bytes(const Pool& pool) { return static_cast<size_t>(pool.sequences) * 4; }
 size_t page_numbers(const Pool& pool) { return static_cast<size_t>(pool.pages) * 4; }
 
+// No sequences, or one page, leave nothing in some of the lists: those may be null, and stand as something that overlaps
+// nothing.
+fb::Span list(const char* what, const void* pointer, size_t bytes, const void* instead) {
+    return bytes != 0 ? fb::Span{what, pointer, bytes} : fb::Span{what, instead, 0};
+}
+
 // A warp per sequence, or a thread per page, up to eight blocks on every SM.
 cudaError_t row_grid(long long warps, long long threads, dim3* grid) {
     int sms = 148;
@@ -841,17 +847,14 @@ flint_status flint_b200_pages_fork(void* next_table, void* next_lengths, void* n
     constexpr const char* name = "flint_b200_pages_fork";
     Pool pool;
     FB_TRY(check_pool(name, shape, &pool));
-    if (pool.sequences == 0) {
-        return FLINT_OK;
-    }
     const fb::Span spans[] = {
-        {"next_table", next_table, table_bytes(pool)},
-        {"next_lengths", next_lengths, row_bytes(pool)},
+        list("next_table", next_table, table_bytes(pool), references),
+        list("next_lengths", next_lengths, row_bytes(pool), references),
         {"next_references", next_references, page_numbers(pool)},
-        {"page_table", page_table, table_bytes(pool)},
-        {"lengths", lengths, row_bytes(pool)},
+        list("page_table", page_table, table_bytes(pool), references),
+        list("lengths", lengths, row_bytes(pool), references),
         {"references", references, page_numbers(pool)},
-        {"parents", parents, row_bytes(pool)},
+        list("parents", parents, row_bytes(pool), references),
     };
     FB_TRY(fb::check_spans(name, spans, 3));
     const ForkArgs p = {pool,
@@ -869,8 +872,10 @@ flint_status flint_b200_pages_fork(void* next_table, void* next_lengths, void* n
     dim3 grid;
     FB_CUDA(row_grid(pool.sequences, pool.pages, &grid));
     FB_CUDA(fb::launch_dependent(fb_pages_fork_tables, grid, dim3(256), 0, stream, p));
-    FB_CUDA(row_grid(2LL * pool.sequences, 0, &grid));
-    FB_CUDA(fb::launch_dependent(fb_pages_fork_references, grid, dim3(256), 0, stream, p));
+    if (pool.sequences > 0) {
+        FB_CUDA(row_grid(2LL * pool.sequences, 0, &grid));
+        FB_CUDA(fb::launch_dependent(fb_pages_fork_references, grid, dim3(256), 0, stream, p));
+    }
     return FLINT_OK;
 }
 
@@ -880,18 +885,15 @@ flint_status flint_b200_pages_reserve(void* page_table, void* lengths, void* ref
     constexpr const char* name = "flint_b200_pages_reserve";
     Pool pool;
     FB_TRY(check_pool(name, shape, &pool));
-    if (pool.sequences == 0) {
-        return FLINT_OK;
-    }
     FB_TRY(check_workspace(name, pool, workspace_bytes));
     const fb::Span spans[] = {
-        {"page_table", page_table, table_bytes(pool)},
-        {"lengths", lengths, row_bytes(pool)},
+        list("page_table", page_table, table_bytes(pool), references),
+        list("lengths", lengths, row_bytes(pool), references),
         {"references", references, page_numbers(pool)},
-        {"moves", moves, 2 * row_bytes(pool)},
+        list("moves", moves, 2 * row_bytes(pool), references),
         {"counts", counts, 8},
         {"workspace", workspace, workspace_bytes_of(pool)},
-        {"added", added, row_bytes(pool)},
+        list("added", added, row_bytes(pool), references),
     };
     FB_TRY(fb::check_spans(name, spans, 6));
     int* space = static_cast<int*>(workspace);
@@ -946,18 +948,14 @@ flint_status flint_b200_pages_compact(void* next_table, void* next_references, v
     Pool pool;
     FB_TRY(check_pool(name, shape, &pool));
     FB_TRY(check_workspace(name, pool, workspace_bytes));
-    // (No sequences, or one page, leave nothing in some of the lists: those may be null.)
-    auto list = [&](const char* what, const void* pointer, size_t bytes) {
-        return bytes != 0 ? fb::Span{what, pointer, bytes} : fb::Span{what, references, 0};
-    };
     const fb::Span spans[] = {
-        list("next_table", next_table, table_bytes(pool)),
+        list("next_table", next_table, table_bytes(pool), references),
         {"next_references", next_references, page_numbers(pool)},
-        list("moves", moves, static_cast<size_t>(pool.pages / 2) * 8),
+        list("moves", moves, static_cast<size_t>(pool.pages / 2) * 8, references),
         {"counts", counts, 8},
         {"workspace", workspace, workspace_bytes_of(pool)},
-        list("page_table", page_table, table_bytes(pool)),
-        list("lengths", lengths, row_bytes(pool)),
+        list("page_table", page_table, table_bytes(pool), references),
+        list("lengths", lengths, row_bytes(pool), references),
         {"references", references, page_numbers(pool)},
     };
     FB_TRY(fb::check_spans(name, spans, 5));

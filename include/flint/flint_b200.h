@@ -16,8 +16,8 @@ extern "C" {
 #endif
 
 /* 1 if a kernel (GEMM, attention, column sums, cross-entropy, log-probabilities) gave up on a
- * bounded barrier wait since the last call, or one that reads starts, lengths or page numbers
- * met one out of range (the flag is cleared), 0 otherwise.
+ * bounded barrier wait since the last call, or one that reads starts, lengths, parents or page numbers
+ * met one out of range, or beam search a full history (the flag is cleared), 0 otherwise.
  * Synchronises the device; meant for tests. */
 FLINT_API flint_status flint_b200_kernel_fault(int* raised);
 
@@ -333,7 +333,8 @@ FLINT_API flint_status flint_b200_paged_attention(void* o, void* lse, const void
  * that and the scale it had otherwise; the codes of earlier positions become rint((q * s_before) / s), and the new ones
  * rint(x / s), ties to even, every step rounded to FP32 (0 where s is 0). A block that grows token by token is thus rounded anew
  * whenever a token exceeds what was there: up to half a step of the scale of that time, each time. A new value that is
- * not finite makes its block's scale NaN, until the block's first position is written again. */
+ * not finite makes its block's scale NaN, until the block's first position is written again. Two sequences that store into
+ * one block race; sequences may share pages that they only read. */
 FLINT_API flint_status flint_b200_paged8_store(void* k_pages, void* v_pages, void* k_scales, void* v_scales,
                                                const void* k, const void* v, const void* starts,
                                                const void* lengths, const void* page_table,
@@ -459,7 +460,8 @@ FLINT_API flint_status flint_b200_token_log_probs_backward(
  * Totals are compared in FP64, with log-sum-exps to FP32's accuracy.
  * end_token is -1 for none (beams that are finished all the same go on by token 0): finished and next_finished may then be null. lengths and next_lengths may be null
  * where histories (with next_histories) are and length_power is 0. cols is a multiple of 8 from 8 to 65,536,
- * groups * beams up to 2^20, length_power finite and not negative, history_stride up to 2^24. */
+ * groups * beams up to 2^20, length_power from 0 to 16, history_stride up to 2^24, lengths from 0 to 2^31 - 2 and to
+ * history_stride. */
 FLINT_API flint_status flint_b200_beam_select_workspace(size_t groups, size_t beams, size_t* bytes);
 
 FLINT_API flint_status flint_b200_beam_select(void* next_scores, void* parents, void* tokens,

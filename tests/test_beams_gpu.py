@@ -214,6 +214,23 @@ def test_logits_far_from_zero(flint, fp32):
         assert abs(out[0][row].item() - total) <= 2.0 ** -22 * (abs(total) + 20)
 
 
+@pytest.mark.parametrize("power", [3.0, 16.0])
+def test_long_lengths_and_large_powers(flint, power):
+    step = Step(3, 4, 300, end=5, power=power)
+    step.lengths[:] = torch.tensor([0, 1, 2, 3, 1000, 999, 1001, 1 << 20, (1 << 31) - 2, (1 << 31) - 3, 1, 0])
+    step.finished[:] = 0
+    step.finished[[0, 7]] = 1
+    flint.kernel_fault()
+    out = step.call(flint)
+    assert not flint.kernel_fault()
+    for row, (total, parent, token, _) in enumerate(step.want()):
+        assert (out[1][row].item() % 4, out[2].to(torch.int32)[row].item()) == (parent, token), row
+    assert out[4].to(torch.int64).min().item() >= 0
+    step.lengths[8] = (1 << 31) - 1
+    step.call(flint)
+    assert flint.kernel_fault()
+
+
 def test_full_histories_are_reported(flint):
     step = Step(2, 3, 100, end=5, history=6)
     step.lengths[:] = torch.tensor([6, 2, 5, 6, 6, 0])

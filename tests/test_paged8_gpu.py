@@ -291,6 +291,20 @@ def test_many_sequences(flint, count, new):
     cache.check_attention(*cache.attend(flint))
 
 
+@pytest.mark.parametrize("count", [33, 90, 128, 200])
+@pytest.mark.parametrize("longest", [1, 64])
+def test_many_sequences_without_tokens_among_them(flint, count, longest):
+    g = torch.Generator().manual_seed(count)
+    total = [int(t) if t > 0 else 0 for t in torch.randint(-300, 1200, (count,), generator=g)]
+    total[count // 2] = 5000
+    new = [0 if i % 3 == 1 else min(t, 1 + i % 2) for i, t in enumerate(total)]
+    cache = Cache(new, total, 8, 2, 32, longest=longest)
+    cache.store(flint)
+    cache.append()
+    cache.check_attention(*cache.attend(flint))
+    assert not flint.kernel_fault()
+
+
 @pytest.mark.parametrize("longest", [1, 64])
 @pytest.mark.parametrize("page", [-1, 1 << 30])
 def test_page_numbers_out_of_range_are_reported(flint, longest, page):

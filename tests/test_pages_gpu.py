@@ -230,6 +230,24 @@ def test_compact(flint, sequences, pages, size, stride, longest):
     assert not flint.kernel_fault()
 
 
+@pytest.mark.parametrize("pages", [1, 5, 40000])
+def test_no_sequences(flint, pages):
+    """References stand as they are, and counts say that nothing is to be copied."""
+    pool = PagePool(0, 3, pages, 16)
+    references = torch.randint(0, 3, (pages,), dtype=torch.int32, device=DEV)
+    after, counts = empty(pages), empty(2)
+    workspace = torch.empty(flint.pages_workspace(pool), dtype=torch.uint8, device=DEV)
+    flint.pages_fork(None, None, after, None, None, references, None, pool)
+    assert torch.equal(after, references)
+    flint.pages_reserve(None, None, after, None, counts, None, pool, workspace)
+    assert counts.tolist() == [0, 0] and torch.equal(after, references)
+    moves = empty(max(1, pages // 2), 2)
+    flint.pages_compact(None, after, moves if pages > 1 else None, counts, None, None, references, pool, workspace)
+    used = references > 0
+    assert counts[1].item() == used.sum().item() and torch.equal((after > 0).int().cumprod(0).sum(), used.sum())
+    assert torch.equal(after.sort().values, references.sort().values)
+
+
 @pytest.mark.parametrize("widths", [[64], [4, 8192, 12, 8196, 24580], [1 << 20, 16]])
 @pytest.mark.parametrize("count", [0, 1, 5])
 def test_copy(flint, widths, count):

@@ -43,8 +43,6 @@ def test_nothing_to_do(flint):
     flint.paged8_store(*[None] * 9, paged(rows=0), stream=0)
     flint.paged8_attention(*[None] * 10, paged(sequences=0), 0.125, stream=0)
     none = PagePool(0, 4, 10, 16)
-    flint.pages_fork(*[None] * 7, none, stream=0)
-    flint.pages_reserve(*[None] * 6, none, stream=0)
     flint.pages_truncate(*[None] * 4, none, stream=0)
     flint.pages_copy(PageArrays([]), None, None, 5, stream=0)
     flint.beam_select(*[None] * 11, True, 0, 4, 100, 104, stream=0)
@@ -151,7 +149,8 @@ def select(flint, fp32=True, groups=2, beams=3, vocab=100, cols=104, stride=20, 
     (dict(vocab=105), "vocab (105) must be"),
     (dict(end=100), "end_token (100) must be -1 or below vocab (100)"),
     (dict(end=-2), "end_token (-2) must be"),
-    (dict(power=-0.5), "length_power (-0.5) must be finite and not negative"),
+    (dict(power=-0.5), "length_power (-0.5) must be from 0 to 16"),
+    (dict(power=16.5), "length_power (16.5) must be"),
     (dict(power=float("nan")), "length_power (nan) must be"),
     (dict(power=float("inf")), "length_power (inf) must be"),
     (dict(finished=None), "finished and next_finished go together"),
