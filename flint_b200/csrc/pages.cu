@@ -20,10 +20,8 @@ namespace {
 
 constexpr int kMostArrays = 128;
 constexpr int kChunkBytes = 8192;      // that a block copies at a time
-// Up to which pools and tables are small (their kernels' comments).
+// Up to which pools are small (their kernels' comments).
 constexpr int kSmallPages = 32768;
-constexpr int kSmallEntries = 8 * 8192;
-constexpr int kNone = INT_MIN;         // no entry
 
 __device__ int g_pages_error = 0;
 
@@ -177,82 +175,41 @@ __global__ void __launch_bounds__(256) fb_pages_fork_references(const ForkArgs p
     }
 }
 
-// The same in one launch, for pools that a cluster's threads take a few entries each of: 512 sequences of 66 entries on 3,500
-// pages XX us against YY in two.
+// The same in one launch, a thread of a cluster per entry: 8 sequences of 22 entries 15.9 us with what follows, 18.0 in two launches.
+// (With several entries per thread the cluster is the slower one: 512 sequences of 66 entries 37.3 us, 35.4 in two launches.)
 __global__ void __launch_bounds__(kThreads) fb_pages_fork_small(const ForkArgs p) {
     fb::dependency_wait();
     fb::dependency_release();
-    const int first = static_cast<int>(sm100::cluster_cta_rank()) * kThreads + static_cast<int>(threadIdx.x);
-    const int entries = p.pool.sequences * p.pool.stride;
-    for (int page = first; page < p.pool.pages; page += kRanks * kThreads) {
+    const int i = static_cast<int>(sm100::cluster_cta_rank()) * kThreads + static_cast<int>(threadIdx.x);
+    for (int page = i; page < p.pool.pages; page += kRanks * kThreads) {
         p.next_references[page] = p.references[page];
     }
-    constexpr int kEach = kSmallEntries / (kRanks * kThreads);
-    // An entry's place in its row, its parent and both lengths, then the page that it had and the one that it gets: each step's
-    // loads together, ahead of the first store, which they would otherwise have to wait for.
-    int place[kEach], parent[kEach], had[kEach], gets[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        had[k] = gets[k] = -1;
-        if (k * kRanks * kThreads >= entries) {
-            continue;
-        }
-        const int i = first + k * kRanks * kThreads;
-        const int t = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride));
-        place[k] = i - t * p.pool.stride;
-        parent[k] = i < entries ? p.parents[t] : -1;
-        had[k] = i < entries ? p.lengths[t] : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        if (k * kRanks * kThreads >= entries) {
-            continue;
-        }
-        const bool has = parent[k] >= 0 && parent[k] < p.pool.sequences;
-        if (!has && parent[k] != -1) {
+    int had = -1, gets = -1;      // the page that the entry had, and the one that it gets; -1 for none
+    if (i < p.pool.sequences * p.pool.stride) {
+        const int t = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride)), e = i - t * p.pool.stride;
+        const int parent = p.parents[t];
+        const bool has = parent >= 0 && parent < p.pool.sequences;
+        if (!has && parent != -1) {
             report();
         }
-        parent[k] = has ? parent[k] : -1;
-        gets[k] = has ? p.lengths[parent[k]] : 0;
-    }
-    int length[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        if (k * kRanks * kThreads >= entries) {
-            continue;
+        const int before = length_of(p.pool, p.lengths, t), length = has ? length_of(p.pool, p.lengths, parent) : 0;
+        const bool old = e < entries_of(p.pool, before), now = e < entries_of(p.pool, length);
+        had = old ? p.table[i] : -1;
+        gets = now ? p.table[parent * p.pool.stride + e] : -1;
+        p.next_table[i] = gets;
+        if (e == 0) {
+            p.next_lengths[t] = length;
         }
-        const int i = first + k * kRanks * kThreads;
-        length[k] = in_range(p.pool, gets[k]);
-        const bool old = i < entries && place[k] < entries_of(p.pool, in_range(p.pool, had[k]));
-        const bool now = i < entries && place[k] < entries_of(p.pool, length[k]);
-        had[k] = old ? p.table[i] : kNone;
-        gets[k] = now ? p.table[parent[k] * p.pool.stride + place[k]] : kNone;
-    }
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        if (k * kRanks * kThreads >= entries) {
-            continue;
-        }
-        const int i = first + k * kRanks * kThreads;
-        if (i < entries) {
-            p.next_table[i] = gets[k] == kNone ? -1 : gets[k];
-            if (place[k] == 0) {
-                p.next_lengths[static_cast<unsigned>(i) / static_cast<unsigned>(p.pool.stride)] = length[k];
-            }
-        }
-        had[k] = had[k] != kNone && is_page(p.pool, had[k]) ? had[k] : -1;
-        gets[k] = gets[k] != kNone && is_page(p.pool, gets[k]) ? gets[k] : -1;
+        had = old && is_page(p.pool, had) ? had : -1;
+        gets = now && is_page(p.pool, gets) ? gets : -1;
     }
     meet();
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        if (had[k] != gets[k]) {
-            if (gets[k] >= 0) {
-                atomicAdd(p.next_references + gets[k], 1);
-            }
-            if (had[k] >= 0) {
-                atomicAdd(p.next_references + had[k], -1);
-            }
+    if (had != gets) {
+        if (gets >= 0) {
+            atomicAdd(p.next_references + gets, 1);
+        }
+        if (had >= 0) {
+            atomicAdd(p.next_references + had, -1);
         }
     }
 }
@@ -451,7 +408,8 @@ __global__ void __launch_bounds__(kThreads) fb_pages_reserve(const ReserveArgs p
     }
 }
 
-// The same for up to a thread per sequence and pools that are read soon: one block, whose barriers take a tenth of a cluster's.
+// The same for up to a thread per sequence and pools that are read soon: one block, whose barriers take a tenth of a cluster's (512
+// sequences on 3,500 pages 37.3 us with what else a step does, 47.9 with the cluster; 8 sequences 15.9 and 19.3).
 // Sequences that write into the same page meet in a table of pages in shared memory.
 constexpr int kSlots = 2048;
 constexpr int kListed = 4096;      // free pages that shared memory holds
@@ -865,7 +823,7 @@ flint_status flint_b200_pages_fork(void* next_table, void* next_lengths, void* n
                         static_cast<const int*>(lengths),
                         static_cast<const int*>(references),
                         static_cast<const int*>(parents)};
-    if (static_cast<long long>(pool.sequences) * pool.stride <= kSmallEntries && pool.pages <= kSmallPages) {
+    if (static_cast<long long>(pool.sequences) * pool.stride <= kRanks * kThreads && pool.pages <= kSmallPages) {
         FB_CUDA(fb::launch_dependent_cluster(fb_pages_fork_small, dim3(kRanks), dim3(kThreads), kRanks, 0, stream, p));
         return FLINT_OK;
     }

@@ -121,6 +121,25 @@ def test_sizes(flint, fp32, groups, beams, vocab, cols):
     assert not flint.kernel_fault()
 
 
+@pytest.mark.parametrize("fp32, vocab", [(False, 36000), (True, 20000)])
+def test_many_rows_in_one_part_each(flint, fp32, vocab):
+    """20,000 rows: a warp has a whole one, whose maxima are noted for two chunks together. Some groups are checked."""
+    groups, beams = 10000, 2
+    g = torch.Generator(device=DEV).manual_seed(5)
+    logits = torch.empty(groups * beams, vocab, dtype=torch.float32 if fp32 else torch.half, device=DEV)
+    for part in logits.split(1000):
+        part.copy_(torch.randn(part.shape, generator=g, device=DEV) * 3)
+    scores = torch.rand(groups * beams, generator=g, device=DEV) * -5
+    whole = Step(1, 2, 8)
+    whole.groups, whole.rows, whole.vocab, whole.cols, whole.fp32 = groups, groups * beams, vocab, vocab, fp32
+    out = whole.call(flint, given=[logits, scores, None, None, None])
+    for at in [0, 1, 4999, 9998, 9999, *range(37, 10000, 997)]:
+        rows = slice(at * beams, (at + 1) * beams)
+        one = Step(1, beams, vocab, vocab, fp32)
+        one.logits, one.scores = logits[rows].cpu(), scores[rows].cpu()
+        one.check([out[0][rows], out[1][rows] - at * beams, out[2][rows], None, None, None])
+
+
 @pytest.mark.parametrize("fp32", [False, True])
 @pytest.mark.parametrize("power", [0.0, 0.6, 1.0, 2.5])
 @pytest.mark.parametrize("groups, beams, vocab", [(9, 4, 3000), (3, 20, 12007)])
