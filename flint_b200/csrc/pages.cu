@@ -657,9 +657,12 @@ __global__ void __launch_bounds__(256) fb_pages_copy(const __grid_constant__ Cop
     fb::dependency_wait();
     fb::dependency_release();
     const long long moves = min(static_cast<long long>(max(p.counts[0], 0)), p.most_moves);
-    for (long long item = blockIdx.x; item < moves * p.chunks; item += gridDim.x) {
-        const long long move = item / p.chunks;
-        const int chunk = static_cast<int>(item - move * p.chunks);
+    // Items blockIdx + k gridDim, in moves and chunks of them (one division where every item would take a long one).
+    const int more_moves = static_cast<int>(gridDim.x) / p.chunks, more_chunks = static_cast<int>(gridDim.x) - more_moves * p.chunks;
+    long long move = static_cast<int>(blockIdx.x) / p.chunks;
+    int chunk = static_cast<int>(blockIdx.x) - static_cast<int>(move) * p.chunks;
+    for (; move < moves; move += more_moves, chunk += more_chunks, move += chunk >= p.chunks ? 1 : 0,
+                         chunk -= chunk >= p.chunks ? p.chunks : 0) {
         const int from = p.moves[2 * move], to = p.moves[2 * move + 1];
         if (from < 0 || from >= p.pages || to < 0 || to >= p.pages) {
             if (from != -1 || to != -1) {
