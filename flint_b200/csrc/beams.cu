@@ -28,10 +28,12 @@ namespace {
 constexpr int kMostBeams = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kHeld = 4;             // 16-byte words that a lane has on their way
-constexpr int kBlocks = 4;           // per SM
-static_assert(kHeld * 8 <= 32, "a lane's values of a chunk have a bit each");
-constexpr int kChunk = 32 * kHeld;   // words that a warp works on at a time
+// Of rows of values of 16 / `values` bytes: 16-byte words that a lane has on their way (its values have a bit each), words that a
+// warp works on at a time, and blocks per SM.
+struct Form {
+    int held, chunk, blocks;
+};
+__host__ __device__ constexpr Form form_of(int values) { return Form{32 / values, 32 * 32 / values, values == 4 ? 3 : 4}; }
 constexpr int kCandidates = 128;     // of a warp
 constexpr int kMany = 96;            // from which on the bound rises
 constexpr int kGroups = 32;          // of a lane's words, whose maxima are noted
@@ -185,8 +187,9 @@ __device__ __noinline__ int keep_largest(Key* list, int count, int k, float& bou
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, kBlocks) fb_beam_rows(const RowArgs p) {
+__global__ void __launch_bounds__(kThreads, form_of(Row<T>::kValues).blocks) fb_beam_rows(const RowArgs p) {
     using R = Row<T>;
+    constexpr int kHeld = form_of(R::kValues).held, kChunk = form_of(R::kValues).chunk;
     __shared__ Key lists[kWarps][kCandidates];
     __shared__ T group_max[kWarps][kGroups][32];      // (a maximum of FP16 values is one)
     __shared__ int claimed;
@@ -725,10 +728,10 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
 // Parts of a row: those with which the warps are done soonest, each part costing three chunks more than it has; never so many that
 // a group has more than kMostLists or kMostEntries, or the GPU more than kMostRounds parts per warp on their account.
 constexpr int kMostRounds = 8;
-unsigned warps_of(int sms) { return static_cast<unsigned>(sms * kBlocks * kWarps); }
+unsigned warps_of(const Form& form, int sms) { return static_cast<unsigned>(sms * form.blocks * kWarps); }
 
-int parts_of(int words, size_t rows, int beams, int sms) {
-    const unsigned warps = warps_of(sms);
+int parts_of(const Form& form, int words, size_t rows, int beams, int sms) {
+    const unsigned warps = warps_of(form, sms), chunk = static_cast<unsigned>(form.chunk);
     const size_t most = std::min<size_t>(std::min(kMostLists / beams, kMostEntries / (beams * beams)),
                                          kMostRounds * static_cast<size_t>(warps) / std::max<size_t>(rows, 1));
     unsigned best = 1;
@@ -736,7 +739,7 @@ int parts_of(int words, size_t rows, int beams, int sms) {
     for (unsigned parts = 1; parts == 1 || (parts <= most && words / parts >= 32); ++parts) {
         // (A block's warps are done about a part apart: 5,000 rows 102.6 us so, 106.1 with half a part.)
         const float items = static_cast<float>(rows) * parts / static_cast<float>(warps);
-        const unsigned chunks = ((words + parts - 1) / parts + kChunk - 1) / kChunk;
+        const unsigned chunks = ((words + parts - 1) / parts + chunk - 1) / chunk;
         const float cost = (items <= 1.0f ? 1.0f : items + 1.0f) * static_cast<float>(chunks + 3);
         if (parts == 1 || cost < least) {
             best = parts;
@@ -745,7 +748,7 @@ int parts_of(int words, size_t rows, int beams, int sms) {
     }
     return static_cast<int>(best);
 }
-size_t most_lists(size_t rows, int sms) { return rows + kMostRounds * static_cast<size_t>(warps_of(sms)); }
+size_t most_lists(size_t rows, int sms) { return rows + kMostRounds * static_cast<size_t>(warps_of(form_of(8), sms)); }
 
 size_t stats_bytes(size_t lists) { return (lists * sizeof(float2) + 255) / 256 * 256; }
 
@@ -754,7 +757,7 @@ cudaError_t launch_rows(RowArgs p, size_t rows, int sms, cudaStream_t stream) {
     const int words = (p.vocab + Row<T>::kValues - 1) / Row<T>::kValues;
     p.slice = (words + p.parts - 1) / p.parts;
     p.items = static_cast<unsigned>(rows * p.parts);
-    const size_t blocks = std::min<size_t>(p.items, static_cast<size_t>(kBlocks) * sms);
+    const size_t blocks = std::min<size_t>(p.items, static_cast<size_t>(form_of(Row<T>::kValues).blocks) * sms);
     return fb::launch_dependent(fb_beam_rows<T>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
 }
 
@@ -911,7 +914,7 @@ flint_status flint_b200_beam_select(void* next_scores, void* parents, void* toke
     g.history_stride = static_cast<long long>(history_stride);
     g.beams = p.beams;
     const int values = fp32_logits != 0 ? Row<float>::kValues : Row<__half>::kValues;
-    g.parts = p.parts = parts_of((p.vocab + values - 1) / values, rows, p.beams, sms);
+    g.parts = p.parts = parts_of(form_of(values), (p.vocab + values - 1) / values, rows, p.beams, sms);
     g.end_token = end_token;
     g.power = length_power;
     FB_CUDA(fp32_logits != 0 ? launch_rows<float>(p, rows, sms, stream) : launch_rows<__half>(p, rows, sms, stream));
