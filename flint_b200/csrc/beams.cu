@@ -457,36 +457,6 @@ struct Candidate {
     }
 };
 
-// log x to about 2^-25 absolute, the accuracy of a sum of FP32 exponentials: x = 2^e f with f from 3/4 to 3/2, whose logarithm
-// is at most 0.41. (FP64's own takes microseconds for what is one number per beam.)
-__device__ __forceinline__ double log_of(float x) {
-    if (!(x > 0.0f && x < INFINITY)) {
-        return logf(x);
-    }
-    const int e = ((__float_as_int(x) - 0x3f400000) >> 23);
-    const float f = __int_as_float(__float_as_int(x) - (e << 23));
-    return e * 0.69314718055994531 + static_cast<double>(log1pf(f - 1.0f));
-}
-
-// n^-power to about 2^-40, from log n = e log 2 + 2 artanh((f - 1) / (f + 1)) with f from 3/4 to 3/2, and the exponential's series.
-// (Weights that were off by FP32's roundings would move totals past each other; FP64's own power takes 5 us.)
-constexpr float kMostPower = 16.0f;
-__device__ __forceinline__ double weight_of(double n, double power) {
-    const long long bits = __double_as_longlong(n);
-    const int e = static_cast<int>((bits - 0x3fe8000000000000LL) >> 52);
-    const double f = __longlong_as_double(bits - (static_cast<long long>(e) << 52));
-    double r = 1.0f / (static_cast<float>(f) + 1.0f);
-    r = r * (2.0 - (f + 1.0) * r);
-    const double s = (f - 1.0) * r, z = s * s, z2 = z * z;
-    const double tail = (1.0 / 3 + z * (1.0 / 5)) + z2 * ((1.0 / 7 + z * (1.0 / 9)) + z2 * (1.0 / 11 + z * (1.0 / 13)));
-    const double y = -power * (e * 0.69314718055994531 + 2.0 * s * (1.0 + z * tail));      // above -350: n is below 2^31
-    const int k = __double2int_rn(y * 1.4426950408889634);
-    const double x = y - k * 0.69314718055994531, x2 = x * x, x4 = x2 * x2;
-    const double series = (1.0 + x) + x2 * (1.0 / 2 + x * (1.0 / 6)) +
-                          x4 * ((1.0 / 24 + x * (1.0 / 120)) + x2 * (1.0 / 720 + x * (1.0 / 5040)) + x4 * (1.0 / 40320 + x * (1.0 / 362880)));
-    return series * __longlong_as_double(static_cast<long long>(1023 + k) << 52);
-}
-
 // What is known of a group's beams.
 struct Beams {
     double score[kMostBeams], lse[kMostBeams], weight[kMostBeams];     // weight: length^-power
@@ -582,13 +552,14 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         bound = Candidate{1, ~0u};      // anything that is a continuation
     }
     __syncthreads();
-    // Four lanes take a beam's log-sum-exp, and a warp the weights of lengths meanwhile.
+    // Four lanes take a beam's log-sum-exp, and a warp the weights of lengths meanwhile. (FP64 throughout: weights that were off by
+    // FP32's roundings would move totals past each other.)
     constexpr int kLanes = 4;
     const int beam = tid / kLanes;
     if (warp == kWarps - 1) {
         if (lane < p.beams) {
             const double grown = of.over[lane] != 0 ? max(of.length[lane], 1) : static_cast<double>(of.length[lane]) + 1.0;
-            of.weight[lane] = p.power == 0.0f ? 1.0 : weight_of(grown, static_cast<double>(p.power));
+            of.weight[lane] = p.power == 0.0f ? 1.0 : pow(grown, -static_cast<double>(p.power));
         }
     } else if (warp * (32 / kLanes) < p.beams) {
         float m = kLowest, sum = 0.0f;
@@ -605,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         sum += __shfl_xor_sync(fb::kFullMask, sum, 1);
         sum += __shfl_xor_sync(fb::kFullMask, sum, 2);
         if (tid % kLanes == 0 && beam < p.beams) {
-            of.lse[beam] = static_cast<double>(m) + log_of(sum);
+            of.lse[beam] = static_cast<double>(m) + log(static_cast<double>(sum));
         }
     }
     __syncthreads();
