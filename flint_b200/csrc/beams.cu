@@ -38,6 +38,7 @@ constexpr int kCandidates = 128;     // of a warp
 constexpr int kMany = 96;            // from which on the bound rises
 constexpr int kGroups = 32;          // of a lane's words, whose maxima are noted
 constexpr int kMostLists = 256;      // of a group
+constexpr float kMostPower = 16.0f;  // of a length: its weights and their products with scores are FP64 numbers then
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int g_beams_error = 0;
