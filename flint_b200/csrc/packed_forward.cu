@@ -139,6 +139,9 @@ struct Meeting {
 // work where one would; the copies are put together at the end of a piece.
 // kEight: the pages hold codes of 8 bits, and a score's exponent is its product times one number, plus another, of its key's
 // block (paged8.cu has the formulas): the maximum of a block's raw scores is scaled once, and so is the sum of its probabilities.
+// Measured with the join: four chunks of 512 tokens and two single ones on up to 4,096 keys, 16 heads on 4, 49 us; 5 tokens each on 100,000 and 7,200 keys, 16 heads on 2, 30 us.
+// A CTA's ten or so key tiles are a chain of load, conversion, product, softmax and product, which two CTAs per SM only half cover: 39 % of
+// the issue slots are used, 18 % of the special-function unit and 12 % of the tensor pipe.
 template <bool kPaged, int kSubsets, bool kEight = false>
 __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_forward_tiles(const __grid_constant__ TileParams p) {
     constexpr int kThreads = kEight ? kThreads8 : fb::kThreads;
