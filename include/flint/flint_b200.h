@@ -449,8 +449,8 @@ FLINT_API flint_status flint_b200_token_log_probs_backward(
  * columns of logits [rows, cols] (FP16, or FP32 where fp32_logits is not 0) and scores (FP32 [rows], a beam's
  * log-probability so far; minus infinity for one that is not in use) every beam's continuations by a token get the
  * total score + log p(token); a beam that is finished (int32 [rows], not 0) goes on in one way, by end_token at
- * its score. The `beams` best of each group by total / length^length_power, length being the continuation's (at least 1), become the next beams
- * in descending order, equal ones by beam and token: next_scores (FP32, the totals), parents (int32, rows), tokens (uint16),
+ * its score. The `beams` best of each group by total / length^length_power, length being the continuation's (at
+ * least 1), become the next beams in descending order, equal ones by beam and token: next_scores (FP32, the totals), parents (int32, rows), tokens (uint16),
  * next_finished (parent finished, or token end_token), next_lengths (the parent's, one more unless it was finished) and
  * next_histories (uint16 [rows, history_stride]: the parent's first tokens, and the new one unless it was finished;
  * what lies behind is left as it is; a history that is full takes no more and is reported by flint_b200_kernel_fault).
@@ -459,8 +459,8 @@ FLINT_API flint_status flint_b200_token_log_probs_backward(
  * where that beam is finished) at a score of minus infinity.
  * Totals are compared in FP64, with log-sum-exps to FP32's accuracy.
  * end_token is -1 for none (beams that are finished all the same go on by token 0): finished and next_finished may then
- * be null. lengths and next_lengths may be null where histories (with next_histories) are and length_power is 0. cols is a multiple of 8 from 8 to 65,536,
- * groups * beams up to 2^20, length_power from 0 to 16, history_stride up to 2^24, lengths from 0 to 2^31 - 2 and to
+ * be null. lengths and next_lengths may be null where histories (with next_histories) are and length_power
+ * is 0. cols is a multiple of 8 from 8 to 65,536, groups * beams up to 2^20, length_power from 0 to 16, history_stride up to 2^24, lengths from 0 to 2^31 - 2 and to
  * history_stride. */
 FLINT_API flint_status flint_b200_beam_select_workspace(size_t groups, size_t beams, size_t* bytes);
 
