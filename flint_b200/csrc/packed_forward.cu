@@ -108,6 +108,15 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return r;
 }
 
+// What two FP16 numbers leave of x and y, as FP16. (The differences are exact.)
+__device__ __forceinline__ uint32_t rest_of(float x, float y, uint32_t first) {
+    float lo, hi;
+    asm("{\n.reg .f16 l, h;\nmov.b32 {l, h}, %4;\nadd.rn.f32.f16 %0, l, %2;\nadd.rn.f32.f16 %1, h, %3;\n}"
+        : "=f"(lo), "=f"(hi)
+        : "f"(x), "f"(y), "r"(first ^ 0x80008000u));
+    return pack2(lo, hi);
+}
+
 // A piece as the TMA warp hands it to the others; `to` of 0 ends the list.
 struct PieceInfo {
     int from, to, tiles;
@@ -139,6 +148,10 @@ struct Meeting {
 // work where one would; the copies are put together at the end of a piece.
 // kEight: the pages hold codes of 8 bits, and a score's exponent is its product times one number, plus another, of its key's
 // block (paged8.cu has the formulas): the maximum of a block's raw scores is scaled once, and so is the sum of its probabilities.
+// Probabilities go into the second product in two parts, FP16 and what that leaves: results are off by their own rounding only, as those of
+// fb_paged8_few (1.3 to 1.4 times it with the first alone). Tensor memory has no place for the second part but that of the scores that it
+// comes from, so that the next step's scores wait for the product with V: two products and their hand-overs longer a step
+// (chunks 58.8 -> 69.0 us with the store, 5 guessed tokens 37.2 -> 39.8).
 // Measured with the join: four chunks of 512 tokens and two single ones on up to 4,096 keys, 16 heads on 4, 49 us; 5 tokens each on 100,000 and 7,200 keys, 16 heads on 2, 30 us.
 // A CTA's ten or so key tiles are a chain of load, conversion, product, softmax and product, which two CTAs per SM only half cover: 39 % of
 // the issue slots are used, 18 % of the special-function unit and 12 % of the tensor pipe.
@@ -418,7 +431,11 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
         // Of the step whose scores were issued last: whether its piece begins with it, and the keys in its tile.
         bool begins_ahead = false;
         int present_ahead = 0;
-        auto issue_scores = [&]() {
+        // The next step's keys and queries, if there is one; 0 for none.
+        uint32_t k_tile = 0;
+        int k_slot = 0;
+        auto claim = [&]() {
+            k_tile = 0;
             if (ok && at_end) {
                 enter();
                 at_end = false;
@@ -431,15 +448,21 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                 ok = false;
                 return;
             }
-            const uint32_t k_tile = next_tile();
-            if (k_tile == 0) {
+            k_tile = next_tile();
+            k_slot = slot;
+            step_ring();
+        };
+        auto issue_scores = [&]() {
+            if (!ok || k_tile == 0) {
                 return;
             }
-            if (issued > 0 && !sm100::mbar_wait_warp(bar.s_free(), (issued - 1) & 1, abort)) {
+            // (Over codes a step's probabilities lie in the place of its scores until they have been used.)
+            if (issued > 0 && !sm100::mbar_wait_warp(kEight ? bar.pv_done() : bar.s_free(), (issued - 1) & 1, abort)) {
                 ok = false;
                 return;
             }
             sm100::tc_fence_after_sync();
+            const int b = round & 1;
             const uint64_t q_desc = desc_kmajor(q_tiles + b * kTileBytes, 0);
             const uint64_t k_desc = desc_kmajor(k_tile, 0);
             const bool last = j + 1 == to;
@@ -449,13 +472,12 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                 sm100::mma_f16_ss_at<1>(tmem_s, q_desc, 4, k_desc, 4, kIdescS);
                 sm100::mma_f16_ss_at<1>(tmem_s, q_desc, 6, k_desc, 6, kIdescS);
                 sm100::mma_commit(bar.s_full());
-                sm100::mma_commit(bar.slot_empty(slot));
+                sm100::mma_commit(bar.slot_empty(k_slot));
                 if (last) {
                     sm100::mma_commit(bar.q_empty(b));
                 }
             }
             __syncwarp();
-            step_ring();
             ++issued;
             begins_ahead = j == from;
             present_ahead = keys - j * kKeyTile;
@@ -465,11 +487,15 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                 at_end = true;
             }
         };
+        claim();
         issue_scores();
         for (uint32_t n = 0; ok && n < issued; ++n) {
             const bool begins = begins_ahead;
             const int present = present_ahead;
-            issue_scores();    // of the next step, as soon as this step's have been read
+            claim();
+            if (!kEight) {
+                issue_scores();    // of the next step, as soon as this step's have been read
+            }
             const uint32_t v_tile = ok ? next_tile() : 0u;
             if (v_tile == 0) {
                 break;
@@ -493,11 +519,20 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                 for (int ks = 1; ks < 8; ++ks) {
                     sm100::mma_f16_ts_at<1>(tmem_o, tmem_p + ks * 8, v_desc, ks * 128, kIdescPV);
                 }
+                if (kEight) {
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        sm100::mma_f16_ts_at<1>(tmem_o, tmem_s + ks / 2 * 32 + ks % 2 * 8, v_desc, ks * 128, kIdescPV);
+                    }
+                }
                 sm100::mma_commit(bar.pv_done());
                 sm100::mma_commit(bar.slot_empty(slot));
             }
             __syncwarp();
             step_ring();
+            if (kEight) {
+                issue_scores();
+            }
         }
     } else if (kEight && warp < kFirstSoftmax) {
         // Codes into FP16 tiles as the tensor cores read them (128-byte rows whose 16-byte pieces are exchanged by the row's
@@ -584,6 +619,8 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
         const uint32_t my_scores = tmem_s + lane_base + first_column;
         const uint32_t my_weights = tmem_p + lane_base + first_column / 2;
         const uint32_t my_output = tmem_o + lane_base;
+        // Over codes: what FP16 leaves of the probabilities of 32 keys, in the place of the first 16 of their scores.
+        const uint32_t my_rest = tmem_s + lane_base + first_column / 32 * 32 + first_column % 32 / 2;
         const uint32_t my_staging = staging + (half * 4 + quadrant) * kStaging;
         const int token = row / p.group;
         const int head_of_group = row - token * p.group;
@@ -653,6 +690,9 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                     }
                 };
                 auto scores_are_read = [&]() {     // the next step's may come
+                    if (kEight) {
+                        return;
+                    }
                     sm100::tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
@@ -740,6 +780,16 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                             sm100::tmem_st_32x16(my_output + 32 * half + c * 16, acc);
                         }
                     }
+                    if constexpr (kEight && kSubsets > 1) {
+                        // The other copies' keys. (Both threads of a row have read their scores: they have met.)
+                        const uint32_t zeros[8] = {};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (j * kSubsets / 4 != subset) {
+                                sm100::tmem_st_32x8(tmem_s + lane_base + 32 * j + 8 * half, zeros);
+                            }
+                        }
+                    }
                     const F2 shift = f2_pack(-m, -m);
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
@@ -750,10 +800,11 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                             }
                             mask(c);
                         }
-                        uint32_t packed[kChunk / 2];
+                        uint32_t packed[kEight ? 1 : kChunk / 2];
                         if constexpr (kEight) {
 #pragma unroll
                             for (int b = 0; b < kChunk; b += kBlock) {
+                                uint32_t first[kBlock / 2], rest[kBlock / 2];
                                 const float4 of = scales_of_block(kChunk * c + b);
                                 const F2 slope = f2_pack(of.x, of.x), offset = f2_pack(of.y - m, of.y - m);
                                 F2 sum = 0;
@@ -769,9 +820,12 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                                         y = fast_exp2(y);
                                     }
                                     sum = f2_add(sum, f2_pack(x, y));
-                                    packed[i] = pack2(x, y);
+                                    first[i - b / 2] = pack2(x, y);
+                                    rest[i - b / 2] = rest_of(x, y, first[i - b / 2]);
                                 }
                                 l = f2_fma(sum, f2_pack(of.z, of.z), l);
+                                sm100::tmem_st_32x8(my_weights + c * 16 + b / 2, first);
+                                sm100::tmem_st_32x8(my_rest + c * 32 + b / 2, rest);
                             }
                         }
 #pragma unroll
@@ -789,7 +843,8 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
                             l = f2_add(l, f2_pack(x, y));
                             packed[i] = pack2(x, y);
                         }
-                        if constexpr (kChunk == 32) {
+                        if constexpr (kEight) {
+                        } else if constexpr (kChunk == 32) {
                             sm100::tmem_st_32x16(my_weights + c * 16, packed);
                         } else {
                             sm100::tmem_st_32x8(my_weights, packed);
