@@ -41,9 +41,9 @@ flint_status check_spans(const char* function, const Span* spans, size_t count, 
         if (s.pointer == nullptr) {
             return fail(FLINT_ERROR_INVALID_ARGUMENT, "%s: %s is null", function, s.name);
         }
-        if (!aligned16(s.pointer)) {
-            return fail(FLINT_ERROR_INVALID_ARGUMENT, "%s: %s is not 16-byte aligned", function,
-                        s.name);
+        if (reinterpret_cast<uintptr_t>(s.pointer) % s.alignment != 0) {
+            return fail(FLINT_ERROR_INVALID_ARGUMENT, "%s: %s is not %zu-byte aligned", function,
+                        s.name, s.alignment);
         }
         if (!fits(s.pointer, s.bytes)) {
             return fail(FLINT_ERROR_INVALID_ARGUMENT,

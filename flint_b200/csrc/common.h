@@ -40,7 +40,12 @@ struct Span {
     const char* name;
     const void* pointer;
     size_t bytes;
+    size_t alignment = 16;
 };
+
+// Of arrays that can be one layer's part of a larger one: where a layer's size is no multiple of 16 bytes, layers
+// behind the first start between such boundaries.
+inline size_t layer_alignment(size_t bytes) { return bytes % 16 == 0 ? 16 : 4; }
 
 // In list order: null, then alignment, then address-space fit for every span;
 // only then each of the first `outputs` spans against every later span.

@@ -187,6 +187,7 @@ struct Rows {
     const char* name;
     const void* pointer;
     size_t rows, width, stride;
+    size_t alignment = 16;
     size_t bytes() const { return rows == 0 ? 0 : (rows - 1) * stride + width; }
 };
 
@@ -208,7 +209,7 @@ template <size_t N>
 flint_status check_all(const char* name, const Rows (&list)[N], size_t outputs) {
     fb::Span spans[N];
     for (size_t i = 0; i < N; ++i) {
-        spans[i] = fb::Span{list[i].name, list[i].pointer, list[i].bytes()};
+        spans[i] = fb::Span{list[i].name, list[i].pointer, list[i].bytes(), list[i].alignment};
     }
     FB_TRY(fb::check_spans(name, spans, N, 0));
     for (size_t i = 0; i < outputs; ++i) {
@@ -222,6 +223,11 @@ flint_status check_all(const char* name, const Rows (&list)[N], size_t outputs) 
 }
 
 Rows flat(const char* name, const void* pointer, size_t bytes) { return Rows{name, pointer, 1, bytes, bytes}; }
+
+// One layer's.
+Rows scale_rows(const char* name, const void* pointer, size_t bytes) {
+    return Rows{name, pointer, 1, bytes, bytes, fb::layer_alignment(bytes)};
+}
 
 Rows token_rows(const char* name, const void* pointer, size_t rows, size_t heads, size_t stride) {
     return Rows{name, pointer, rows, heads * 128, stride * 2};
@@ -503,8 +509,8 @@ flint_status flint_b200_paged8_store(void* k_pages, void* v_pages, void* k_scale
     const Rows list[] = {
         flat("k_pages", k_pages, cache_bytes(*shape) / 2),
         flat("v_pages", v_pages, cache_bytes(*shape) / 2),
-        flat("k_scales", k_scales, scale_bytes(*shape)),
-        flat("v_scales", v_scales, scale_bytes(*shape)),
+        scale_rows("k_scales", k_scales, scale_bytes(*shape)),
+        scale_rows("v_scales", v_scales, scale_bytes(*shape)),
         token_rows("k", k, shape->rows, shape->kv_heads, shape->kv_stride),
         token_rows("v", v, shape->rows, shape->kv_heads, shape->kv_stride),
         flat("starts", starts, (shape->sequences + 1) * 4),
@@ -553,8 +559,8 @@ flint_status flint_b200_paged8_attention(void* o, void* lse, const void* q, cons
         token_rows("q", q, shape->rows, shape->heads, shape->q_stride),
         flat("k_pages", k_pages, cache_bytes(*shape) / 2),
         flat("v_pages", v_pages, cache_bytes(*shape) / 2),
-        flat("k_scales", k_scales, scale_bytes(*shape)),
-        flat("v_scales", v_scales, scale_bytes(*shape)),
+        scale_rows("k_scales", k_scales, scale_bytes(*shape)),
+        scale_rows("v_scales", v_scales, scale_bytes(*shape)),
         flat("starts", starts, (shape->sequences + 1) * 4),
         flat("lengths", lengths, shape->sequences * 4),
         flat("page_table", page_table, shape->sequences * shape->table_stride * 4),

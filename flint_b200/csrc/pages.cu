@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(256) fb_pages_copy(const __grid_constant__ Cop
         const unsigned here = min(bytes - begin, static_cast<unsigned>(kChunkBytes));
         const unsigned char* source = p.base[low] + static_cast<size_t>(from) * bytes + begin;
         unsigned char* target = p.base[low] + static_cast<size_t>(to) * bytes + begin;
-        if (bytes % 16 == 0) {
+        if (bytes % 16 == 0) {      // (then the array begins on such a boundary: layer_alignment)
             constexpr int kWords = kChunkBytes / (256 * 16);
             uint4 held[kWords];
 #pragma unroll
@@ -975,7 +975,7 @@ flint_status flint_b200_pages_copy(void* const* arrays, const size_t* page_bytes
         p.bytes[i] = static_cast<unsigned>(page_bytes[i]);
         p.base[i] = static_cast<unsigned char*>(arrays[i]);
         chunks += static_cast<long long>((page_bytes[i] + kChunkBytes - 1) / kChunkBytes);
-        spans[i] = fb::Span{"an array", arrays[i], pages * page_bytes[i]};
+        spans[i] = fb::Span{"an array", arrays[i], pages * page_bytes[i], fb::layer_alignment(pages * page_bytes[i])};
     }
     p.first_chunk[count] = static_cast<int>(chunks);
     spans[count] = fb::Span{"moves", moves, most_moves * 8};

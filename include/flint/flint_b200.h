@@ -326,7 +326,8 @@ FLINT_API flint_status flint_b200_paged_attention(void* o, void* lse, const void
  *
  * Pages as above whose values are int8 codes: k_pages and v_pages are int8 [pages, kv_heads, page_size, 64], and
  * k_scales and v_scales FP32 [pages, kv_heads, page_size / 16], one for each block of 16 positions of a head; a code q
- * stands for q * scale. Half the memory of FP16 pages, and half of what attention reads.
+ * stands for q * scale. Half the memory of FP16 pages, and half of what attention reads. Arrays of scales whose size is not
+ * a multiple of 16 bytes (a layer's part of a tensor of all layers') may start at any multiple of 4.
  *
  * flint_b200_paged8_store writes the new tokens' keys and values, block by block. With a the largest |x| of the new
  * values in a block of a head, its scale becomes s = a / 127 if the call writes the block's first position, and the larger of
@@ -406,7 +407,8 @@ FLINT_API flint_status flint_b200_pages_compact(void* next_table, void* next_ref
                                                 flint_stream stream);
 
 /* Copies pages within each of `count` (up to 128) arrays: arrays[i] is [pages, page_bytes[i]] bytes on the device (the two
- * lists are on the host and are read during the call), page_bytes multiples of 4. moves and counts are as reserve and
+ * lists are on the host and are read during the call), page_bytes multiples of 4; one whose size is not a multiple of 16 bytes
+ * may start at any multiple of 4. moves and counts are as reserve and
  * compact leave them: the first counts[0] of up to most_moves rows; rows with a number that is not a page are passed over. No page may be
  * both copied from and to, or copied to twice. */
 FLINT_API flint_status flint_b200_pages_copy(void* const* arrays, const size_t* page_bytes, size_t count,
