@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_fo
             const int entry = scales_of[raw];
             if (half == 0 && entry >= 0 && lane < kBlocks) {
                 const float v = raw_scales[entry][kBlocks + lane];
-                const float slope = raw_scales[entry][lane] * (p.a.scale * kLog2e), weight = v == 0.0f ? 1.0f : v;
+                const float slope = raw_scales[entry][lane] * (p.a.scale * kLog2e), weight = v == 0.0f ? kWeightOfZeros : v;
                 // (Codes are 0 where a scale is 0. A slope above it keeps a score of minus infinity one.)
                 block_scales[entry][lane] = make_float4(slope == 0.0f ? 1e-30f : slope, __log2f(weight), 1.0f / weight, 0.0f);
             }

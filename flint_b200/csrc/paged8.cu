@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, kFewPerSm) fb_paged8_few(const __gri
         int stage = 0;
         for (int i = 0; i < count; ++i) {
             if (i % kBatch == 0) {
-                const float v = v_next == 0.0f ? 1.0f : v_next;      // (codes are 0 then)
+                const float v = v_next == 0.0f ? kWeightOfZeros : v_next;
                 slope_of = k_next * scale2;
                 offset_of = __log2f(v);
                 inverse_of = 1.0f / v;

@@ -45,3 +45,38 @@ def test_results_are_off_by_their_own_rounding(flint, new, count, total):
     cache.append()
     got, least = against_its_rounding(cache, cache.attend(flint)[0])
     assert got <= MOST * least, got / least
+
+
+def put(cache, s, which, block, codes, scale):
+    """Sets a block that the sequence has already, on the host and in the cache."""
+    blocks, size = cache.blocks[s][which], cache.size
+    positions = torch.arange(block * 16, block * 16 + 16)
+    blocks.codes[positions], blocks.scales[block] = codes, scale
+    page = cache.table[s].cpu().long()[positions // size].to(DEV)
+    cache.arrays[which][page, :, (positions % size).to(DEV)] = codes.to(torch.int8).to(DEV)
+    cache.arrays[2 + which][page[0], :, block * 16 % size // 16] = scale.to(DEV)
+
+
+@pytest.mark.parametrize("amplitude", [1e-3, 1e-2, 1.0])
+@pytest.mark.parametrize("new", [1, 4, 8, 16, 100])
+def test_zeros_cost_other_values_no_accuracy(flint, new, amplitude):
+    """Blocks of V that are 0 have no part in a result but their probabilities'. Their weight must not push the others' probabilities
+    below what FP16 holds: values of 10^-3 give scales near 2^-15, and products of both that are off by 2^-25 would be by a
+    thousandth of themselves and more. (Results near 10^-4 are FP16 numbers of their full precision above 2^-14, and off by 2^-25
+    below: both sides have that rounding.)"""
+    count = 12
+    cache = Cache([new] * count, [new + 48 + 3 * i for i in range(count)], 8, 2, 32, seed=new)
+    cache.qkv[:, (cache.heads + cache.kv_heads) * 64:] *= amplitude
+    for s in range(count):
+        blocks = cache.blocks[s][1]
+        for block in range(3):
+            put(cache, s, 1, block, blocks.codes[16 * block:16 * block + 16] * (block != 1), blocks.scales[block] * amplitude * (block != 1))
+        for block in range(3, blocks.scales.shape[0]):
+            blocks.scales[block] *= amplitude
+            at = block * 16
+            cache.v_scales[cache.table[s, at // 32].long(), :, at % 32 // 16] *= amplitude
+    cache.store(flint)
+    cache.append()
+    cache.check_stored()
+    got, least = against_its_rounding(cache, cache.attend(flint)[0])
+    assert got <= MOST * least, got / least
