@@ -42,7 +42,7 @@ constexpr int kCandidates = 128;     // of a warp
 constexpr int kMany = 96;            // from which on the bound rises
 constexpr int kGroups = 32;          // of a lane's words, whose maxima are noted
 constexpr int kMostLists = 256;      // of a group
-constexpr float kMostPower = 16.0f;  // of a length: its weights and their products with scores are FP64 numbers then
+constexpr float kMostPower = 16.0f;  // of a length: what scores are divided by, and the quotients, are FP64 numbers then
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int g_beams_error = 0;
@@ -446,6 +446,18 @@ __device__ __forceinline__ Key order_total(double v) {
     return (bits >> 63) != 0 ? ~bits : bits | (Key{1} << 63);
 }
 
+// length^power. Whole powers by products, which are exact up to 2^53: equal quotients of totals are equal numbers then.
+__device__ __forceinline__ double power_of(double length, float power) {
+    if (power != rintf(power)) {
+        return pow(length, static_cast<double>(power));
+    }
+    double product = 1.0;
+    for (int rest = static_cast<int>(power); rest != 0; rest >>= 1, length *= length) {
+        product *= (rest & 1) != 0 ? length : 1.0;
+    }
+    return product;
+}
+
 constexpr int kBins = 64;
 constexpr int kMostEntries = 4096;   // of a group's lists
 
@@ -464,7 +476,7 @@ struct Candidate {
 
 // What is known of a group's beams.
 struct Beams {
-    double score[kMostBeams], lse[kMostBeams], weight[kMostBeams];     // weight: length^-power
+    double score[kMostBeams], lse[kMostBeams], divisor[kMostBeams];     // divisor: length^power
     int over[kMostBeams], length[kMostBeams];
 };
 
@@ -557,14 +569,14 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         bound = Candidate{1, ~0u};      // anything that is a continuation
     }
     __syncthreads();
-    // Four lanes take a beam's log-sum-exp, and a warp the weights of lengths meanwhile. (FP64 throughout: weights that were off by
+    // Four lanes take a beam's log-sum-exp, and a warp the powers of lengths meanwhile. (FP64 throughout: powers that were off by
     // FP32's roundings would move totals past each other.)
     constexpr int kLanes = 4;
     const int beam = tid / kLanes;
     if (warp == kWarps - 1) {
         if (lane < p.beams) {
             const double grown = of.over[lane] != 0 ? max(of.length[lane], 1) : static_cast<double>(of.length[lane]) + 1.0;
-            of.weight[lane] = p.power == 0.0f ? 1.0 : pow(grown, -static_cast<double>(p.power));
+            of.divisor[lane] = power_of(grown, p.power);
         }
     } else if (warp * (32 / kLanes) < p.beams) {
         float m = kLowest, sum = 0.0f;
@@ -585,6 +597,8 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         }
     }
     __syncthreads();
+    // (A reciprocal in the quotient's place would be rounded once more, and equal quotients not be equal.)
+    auto rank_of = [&](double total, int its) { return order_total(p.power == 0.0f ? total : total / of.divisor[its]); };
     // Entry i, of beam i / of_beam.
     auto candidate_of = [&](int i, Key key, double& total) {
         const int its = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(of_beam));
@@ -592,12 +606,12 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         if (of.over[its] != 0) {
             // (A finished beam's row was not read; it has one continuation.)
             total = i == its * of_beam ? of.score[its] : -INFINITY;
-            return Candidate{order_total(total * of.weight[its]), high | static_cast<unsigned>(max(p.end_token, 0))};
+            return Candidate{rank_of(total, its), high | static_cast<unsigned>(max(p.end_token, 0))};
         }
         // (An lse that is not a number, or minus infinity, gives none.)
         total = key != 0 ? of.score[its] + (static_cast<double>(key_value(key)) - of.lse[its]) : -INFINITY;
         total = total < INFINITY ? total : -INFINITY;
-        return Candidate{order_total(total * of.weight[its]), high | static_cast<unsigned>(key_column(key) & 0xffff)};
+        return Candidate{rank_of(total, its), high | static_cast<unsigned>(key_column(key) & 0xffff)};
     };
     Candidate top = {0, ~0u};
     Key ranks[kHeldEntries];
