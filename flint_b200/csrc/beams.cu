@@ -476,7 +476,8 @@ struct Candidate {
 
 // What is known of a group's beams.
 struct Beams {
-    double score[kMostBeams], lse[kMostBeams], divisor[kMostBeams];     // divisor: length^power
+    // A row's log-sum-exp is top + log_sum, which stay apart: of the lowest FP32 number as the largest logit their sum would be the former.
+    double score[kMostBeams], top[kMostBeams], log_sum[kMostBeams], divisor[kMostBeams];     // divisor: length^power
     int over[kMostBeams], length[kMostBeams];
 };
 
@@ -593,7 +594,8 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         sum += __shfl_xor_sync(fb::kFullMask, sum, 1);
         sum += __shfl_xor_sync(fb::kFullMask, sum, 2);
         if (tid % kLanes == 0 && beam < p.beams) {
-            of.lse[beam] = static_cast<double>(m) + log(static_cast<double>(sum));
+            of.top[beam] = static_cast<double>(m);
+            of.log_sum[beam] = log(static_cast<double>(sum));
         }
     }
     __syncthreads();
@@ -608,8 +610,8 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
             total = i == its * of_beam ? of.score[its] : -INFINITY;
             return Candidate{rank_of(total, its), high | static_cast<unsigned>(max(p.end_token, 0))};
         }
-        // (An lse that is not a number, or minus infinity, gives none.)
-        total = key != 0 ? of.score[its] + (static_cast<double>(key_value(key)) - of.lse[its]) : -INFINITY;
+        // (A sum that is not a number gives none, nor does one of 0.)
+        total = key != 0 ? of.score[its] + (static_cast<double>(key_value(key)) - of.top[its] - of.log_sum[its]) : -INFINITY;
         total = total < INFINITY ? total : -INFINITY;
         return Candidate{rank_of(total, its), high | static_cast<unsigned>(key_column(key) & 0xffff)};
     };
