@@ -633,21 +633,23 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
         }
     }
     __syncthreads();
-    // (A reciprocal in the quotient's place would be rounded once more, and equal quotients not be equal.)
-    auto rank_of = [&](double total, int its) { return order_total(p.power == 0.0f ? total : total / of.divisor[its]); };
-    // Entry i, of beam i / of_beam.
-    auto candidate_of = [&](int i, Key key, double& total) {
+    // Entry i, of beam i / of_beam: its total, and its place.
+    auto total_of = [&](int i, Key key, unsigned& place) {
         const int its = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(of_beam));
         const unsigned high = static_cast<unsigned>(its) << 16;
         if (of.over[its] != 0) {
             // (A finished beam's row was not read; it has one continuation.)
-            total = i == its * of_beam ? of.score[its] : -INFINITY;
-            return Candidate{rank_of(total, its), high | static_cast<unsigned>(max(p.end_token, 0))};
+            place = high | static_cast<unsigned>(max(p.end_token, 0));
+            return i == its * of_beam ? of.score[its] : -INFINITY;
         }
+        place = high | static_cast<unsigned>(key_column(key) & 0xffff);
         // (A sum that is not a number gives none, nor does one of 0.)
-        total = key != 0 ? of.score[its] + (static_cast<double>(key_value(key)) - of.top[its] - of.log_sum[its]) : -INFINITY;
-        total = total < INFINITY ? total : -INFINITY;
-        return Candidate{rank_of(total, its), high | static_cast<unsigned>(key_column(key) & 0xffff)};
+        const double total = key != 0 ? of.score[its] + (static_cast<double>(key_value(key)) - of.top[its] - of.log_sum[its]) : -INFINITY;
+        return total < INFINITY ? total : -INFINITY;
+    };
+    // (A reciprocal in the quotient's place would be rounded once more, and equal quotients not be equal.)
+    auto rank_of = [&](double total, unsigned place) {
+        return order_total(p.power == 0.0f ? total : total / of.divisor[place >> 16]);
     };
     Candidate top = {0, ~0u};
     Key ranks[kHeldEntries];
@@ -655,8 +657,9 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
     for (int i = 0; i < kHeldEntries; ++i) {
         ranks[i] = 0;
         if (tid + i * kThreads < entries) {
-            double total;
-            const Candidate mine = candidate_of(tid + i * kThreads, held[i], total);
+            unsigned place;
+            const double total = total_of(tid + i * kThreads, held[i], place);
+            const Candidate mine = {rank_of(total, place), place};
             ranks[i] = mine.rank;
             top = mine.above(top) ? mine : top;
         }
@@ -686,8 +689,9 @@ __global__ void __launch_bounds__(kThreads, kHeldEntries > 4 ? 2 : 1280 / kThrea
 #pragma unroll
         for (int i = 0; i < kHeldEntries; ++i) {
             if (ranks[i] != 0 && ranks[i] >= bound.rank) {
-                double total;
-                const Candidate mine = candidate_of(tid + i * kThreads, held[i], total);
+                unsigned place;
+                const double total = total_of(tid + i * kThreads, held[i], place);
+                const Candidate mine = {ranks[i], place};
                 if (!bound.above(mine)) {
                     const int at = atomicAdd(&left_count, 1);
                     left_rank[at] = mine.rank;
