@@ -9,9 +9,10 @@
 // second launch has a block per group of beams and does the same with totals, in FP64, because two beams'
 // continuations can be closer than FP32 tells apart; a tie goes to the lower beam, then the lower token.
 //
-// 5,000 rows of 50,257 FP16 logits take 99 to 102 us (4.3 TB/s): an exponential per value keeps the special-function unit 57 % busy and what
-// there is to do per value 59 % of the issue slots, together what the SMs can do. 1,240 rows of 32,001 FP32 logits and 31 beams 48 us,
-// where a part's 31 candidates count as well; 512 rows 23.6 us and 4 rows 10.5 us, which are a warp's chain of loads and two launches' beginnings.
+// 5,000 rows of 50,257 FP16 logits take 99 to 102 us (4.3 TB/s): no unit is full (DRAM 57 %, special-function unit 57 %, issue slots 58 %); warps wait for
+// memory most, with one chunk on its way while they sum the one before and room for 42 % of an SM's warps. 1,240 rows of 32,001 FP32 logits and 31 beams 49 us,
+// where two parts of a row each leave 30 % of the warps without one, and a part's 31 candidates count as well; 512 rows 24 us and 4 rows 10.5 us,
+// which are a warp's chain of loads and two launches' beginnings.
 #include <algorithm>
 #include <atomic>
 #include <climits>

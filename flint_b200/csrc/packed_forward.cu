@@ -53,8 +53,8 @@ constexpr int kPieces = 8;      // ring of piece descriptions
 constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes + kStagingBytes + 256;
 
 // Pages of 8 bits: two more warps turn codes into the FP16 tiles that the products take, out of a ring of their own; one slot
-// less holds those. 384 threads twice on an SM have 80 registers each, which costs 96 bytes spilled. (Shares of 96 and 48, or 88 and 64, by
-// setmaxnreg: 6,800 and 3,400 bytes.)
+// less holds those. 384 threads twice on an SM have 80 registers each, which costs 64 bytes spilled. (Shares of 96 and 48, or 88 and 64, by
+// setmaxnreg: 6,800 and 3,400 bytes, before probabilities had two parts.)
 constexpr int kThreads8 = 384;
 constexpr int kSlots8 = 3;
 constexpr int kRawSlots = 2;
@@ -152,9 +152,10 @@ struct Meeting {
 // fb_paged8_few (1.3 to 1.4 times it with the first alone). Tensor memory has no place for the second part but that of the scores that it
 // comes from, so that the next step's scores wait for the product with V: two products and their hand-overs longer a step
 // (chunks 58.8 -> 69.0 us with the store, 5 guessed tokens 37.2 -> 39.8).
-// Measured with the join: four chunks of 512 tokens and two single ones on up to 4,096 keys, 16 heads on 4, 49 us; 5 tokens each on 100,000 and 7,200 keys, 16 heads on 2, 30 us.
-// A CTA's ten or so key tiles are a chain of load, conversion, product, softmax and product, which two CTAs per SM only half cover: 39 % of
-// the issue slots are used, 18 % of the special-function unit and 12 % of the tensor pipe.
+// Measured with the join, as part of a graph: four chunks of 512 tokens and two single ones on up to 4,096 keys, 16 heads on 4, 59 us (FP16 pages 43); 5 tokens each on
+// 100,000 and 7,200 keys, 16 heads on 2, 32 us (25).
+// A CTA's key tiles are a chain of load, conversion, product, softmax and product, which two CTAs per SM only half cover: 37 % of
+// the issue slots are used, 15 % of the special-function unit and 15 % of the tensor pipe.
 template <bool kPaged, int kSubsets, bool kEight = false>
 __global__ void __launch_bounds__(kEight ? kThreads8 : kThreads, 2) fb_packed_forward_tiles(const __grid_constant__ TileParams p) {
     constexpr int kThreads = kEight ? kThreads8 : fb::kThreads;

@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(256) fb_paged8_store(const PackedArgs p, const
 // keys, whose codes come to it alone through stages of asynchronous copies, and the warps' sums meet at the end of a piece. (Two blocks
 // at a time where registers allow: one's products run under the other's conversions.)
 // Measured with the join, as part of a graph: one sequence of 1,000 keys, 12 heads, 7.8 us; 64 sequences of up to 8,192, 32 heads on 8, 48 us (196 MB,
-// 4.1 TB/s), where issue slots are what is short: a fourth of the instructions turn codes into FP16.
+// 4.1 TB/s). There no pipe is full (47 % of the issue slots, DRAM 51 %, the tensor pipe 18 %): sixteen warps on an SM, each a chain
+// of copies, conversions and two products, and the pieces' uneven ends, at which the warps wait for each other.
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlockBytes = 2 * kBlock * kHead;       // K and V of a block
@@ -573,8 +574,10 @@ cudaError_t paged8_attention(const PackedArgs& args, const Cache8& cache, int lo
         return e;
     }
     const long long most_keys = static_cast<long long>(args.table_stride) * args.page_size;
-    // 64 single tokens, groups of four heads: 48 us here where the tensor cores' tiles of 128 rows take 107. Every eight
-    // rows more cost their products, exponentials and registers: from 17 rows on both take about as long.
+    // 64 sequences of up to 8,192 keys, 32 heads on 8, with 1, 2, 4, 5, 8 and 16 new tokens (4 to 64 rows): tiles of eight rows 47, 48, 80, 115, 150
+    // and 292 us; of 16 rows 52, 52, 66, 104, 116 and 220; the tensor cores' of 32 rows 105, 105, 105, 106, 106 and 190, of 64 rows 106 to 107
+    // and 119. Two sequences of 100,000 and 7,200, 16 heads on 2, with 8, 16, 24, 32 and 40 rows: 19, 23, 26, 30 and 36 us; 21, 23, 28, 29 and 34; 31 up to
+    // 32 rows and 42; 32 up to 32 rows and 34. From 17 rows on both take about as long.
     return rows <= 8    ? launch_few<1>(p, sms, workspace, most_keys, stream)
            : rows <= 16 ? launch_few<2>(p, sms, workspace, most_keys, stream)
                         : packed_forward(args, &cache, longest, workspace, stream);

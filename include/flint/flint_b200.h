@@ -326,16 +326,20 @@ FLINT_API flint_status flint_b200_paged_attention(void* o, void* lse, const void
  *
  * Pages as above whose values are int8 codes: k_pages and v_pages are int8 [pages, kv_heads, page_size, 64], and
  * k_scales and v_scales FP32 [pages, kv_heads, page_size / 16], one for each block of 16 positions of a head; a code q
- * stands for q * scale. Half the memory of FP16 pages, and half of what attention reads. Arrays of scales whose size is not
- * a multiple of 16 bytes (a layer's part of a tensor of all layers') may start at any multiple of 4.
+ * stands for q * scale. Half the memory of FP16 pages, and half of what attention reads; it is faster than FP16 pages' while the query heads of a
+ * K/V head and the new tokens of a sequence make up to 16 rows (64 single tokens on up to 8,192 keys 48 us, FP16 73), slower beyond
+ * (20 rows 106 and 74, chunks of 512 tokens 59 and 43). `longest` chooses one form for all sequences of a call: single
+ * tokens beside a prompt's chunk are done sooner in a call of their own (63 of them and a chunk of 512: 231 us together, 46 and 113 apart).
+ * Arrays of scales whose size is not a multiple of 16 bytes (a layer's part of a tensor of all layers') may start at any multiple of 4.
  *
  * flint_b200_paged8_store writes the new tokens' keys and values, block by block. With a the largest |x| of the new
  * values in a block of a head, its scale becomes s = a / 127 if the call writes the block's first position, and the larger of
  * that and the scale it had otherwise; the codes of earlier positions become rint((q * s_before) / s), and the new ones
  * rint(x / s), ties to even, every step rounded to FP32 (0 where s is 0). A block that grows token by token is thus rounded anew
  * whenever a token exceeds what was there: up to half a step of the scale of that time, each time. A new value that is
- * not finite makes its block's scale NaN, until the block's first position is written again. Two sequences that store into
- * one block race; sequences may share pages that they only read. */
+ * not finite makes its block's scale NaN, until the block's first position is written again; in the same way positions that
+ * are given back (guessed tokens that were wrong, by flint_b200_pages_truncate) leave their block the scale that they raised, and what stays
+ * in it, and what it takes next, as coarse. Two sequences that store into one block race; sequences may share pages that they only read. */
 FLINT_API flint_status flint_b200_paged8_store(void* k_pages, void* v_pages, void* k_scales, void* v_scales,
                                                const void* k, const void* v, const void* starts,
                                                const void* lengths, const void* page_table,
@@ -363,7 +367,8 @@ FLINT_API flint_status flint_b200_paged8_attention(void* o, void* lse, const voi
  * flint_b200_pages_copy carries out for every layer's arrays. Results do not depend on timing: free pages are taken in
  * ascending order by sequences in ascending order.
  * Limits: sequences up to 65,535, pages up to 2^24, page_size a power of two from 16 to 1,024, table_stride * page_size up
- * to 2^26. Numbers in device memory that are out of range are passed over and reported by flint_b200_kernel_fault. */
+ * to 2^26. Numbers in device memory that are out of range are reported by flint_b200_kernel_fault: pages and parents are passed over, lengths
+ * and numbers of tokens cut to what a row of the table holds. */
 typedef struct {
     size_t sequences;
     size_t table_stride;
@@ -459,7 +464,8 @@ FLINT_API flint_status flint_b200_token_log_probs_backward(
  * A total that is not finite is no continuation, nor is anything of a row of logits with a NaN or plus infinity; where
  * a group has fewer than `beams`, places left are filled by the beams of the same places, with token 0 (end_token
  * where that beam is finished) at a score of minus infinity.
- * Totals are compared in FP64, with log-sum-exps to FP32's accuracy.
+ * Totals are compared in FP64, with log-sum-exps to FP32's accuracy; a total beyond FP32's range (one masked by the lowest number twice)
+ * leaves its beam a score of minus infinity.
  * end_token is -1 for none (beams that are finished all the same go on by token 0): finished and next_finished may then
  * be null. lengths and next_lengths may be null where histories (with next_histories) are and length_power
  * is 0. cols is a multiple of 8 from 8 to 65,536, groups * beams up to 2^20, length_power from 0 to 16, history_stride up to 2^24, lengths from 0 to 2^31 - 2 and to
